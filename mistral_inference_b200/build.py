@@ -94,6 +94,37 @@ def build_hybrid(force: bool = False) -> Path:
     return HYBRID_LIB
 
 
+PAGED_SRC = CSRC / "paged"
+PAGED_LIB = PKG / "libmb200_paged.so"
+
+
+def build_paged(force: bool = False) -> Path:
+    """libmb200_paged.so: pages of 8-bit keys and values and the scores of tokens (csrc/paged/), built like libmb200_hybrid.so."""
+    headers = ["common.cuh", "device_info.cuh", "epilogue.cuh", "sigmoid.cuh", "gemm_tcgen05.cuh", "gemm_mma.cuh", "split_schedule.cuh", "decode_megakernel.cuh", "attn_decode.cuh",
+               "attn_prompt_tcgen05.cuh"]
+    files = sorted(PAGED_SRC.glob("*.cu")) + sorted(PAGED_SRC.glob("*.cuh")) + [CSRC / h for h in headers] + [PKG.parent / "include" / h for h in ("mistral_b200.h", "mistral_b200_paged.h")]
+    h = hashlib.sha256()
+    for f in files:
+        h.update(f.name.encode())
+        h.update(f.read_bytes())
+    h.update(" ".join(NVCC_FLAGS).encode())
+    digest = h.hexdigest()
+    stamp = PAGED_SRC / ".build_stamp"
+    if not force and PAGED_LIB.exists() and stamp.exists() and stamp.read_text().strip() == digest:
+        return PAGED_LIB
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    tmp = PKG / f".libmb200_paged.{os.getpid()}.so"
+    cmd = [nvcc, *NVCC_FLAGS, "-o", str(tmp)] + [str(f) for f in sorted(PAGED_SRC.glob("*.cu"))]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        sys.stderr.write(proc.stdout + proc.stderr)
+        raise RuntimeError(f"nvcc failed ({proc.returncode}): {' '.join(cmd)}")
+    os.replace(tmp, PAGED_LIB)
+    stamp.write_text(digest)
+    return PAGED_LIB
+
+
 if __name__ == "__main__":
+    print(build_paged(force="--force" in sys.argv))
     print(build_hybrid(force="--force" in sys.argv))
     print(build_library(force="--force" in sys.argv, verbose="--verbose" in sys.argv))

@@ -1,0 +1,213 @@
+// libmb200_paged.so -- the C ABI declared in include/mistral_b200_paged.h.  Argument checking + kernel dispatch only.
+#include "paged_attn.cuh"
+#include "paged_plan.cuh"
+#include "paged_write.cuh"
+#include "token_scores.cuh"
+
+namespace mb200 {
+thread_local char g_err[512] = "";
+
+static int run_plan(bool extend, PlanParams p, cudaStream_t st) {
+  const char* what = extend ? "pages_extend" : "pages_truncate";
+  MB_CHECK_ARG(p.table && p.lens && p.free && p.n_free && p.scratch && p.count && p.status, "%s: null pointer", what);
+  MB_CHECK_ARG(p.B >= 1 && p.B <= MBP_MAX_REQUESTS, "%s: %d requests (1 to %d)", what, p.B, MBP_MAX_REQUESTS);
+  const size_t smem = sizeof(int) * (3 * (size_t)p.B + 2);
+  if (extend) {
+    // one CTA fills a thousand places as fast as a launch of many starts
+    const int ctas = p.T <= PLAN_TOKENS_PER_CTA ? 1 : (ceil_div(p.T, PLAN_TOKENS_PER_CTA) < PLAN_MAX_CTAS ? ceil_div(p.T, PLAN_TOKENS_PER_CTA) : PLAN_MAX_CTAS);
+    MB_CHECK_CUDA(launch_pdl(page_extend_kernel, dim3((unsigned)ctas), dim3(PLAN_THREADS), smem, st, p));
+  } else {
+    MB_CHECK_CUDA(launch_pdl(page_truncate_kernel, dim3(1), dim3(1024), smem, st, p));
+  }
+  return MB200_OK;
+}
+
+static int plan_state(PlanParams& p, const char* what, int32_t* table, int32_t* lens, int32_t* free_pages, int32_t* n_free, int32_t* scratch, const int32_t* rows,
+                      const int32_t* count, int64_t B, int64_t R, int64_t P, int64_t n_pages, int32_t* status) {
+  MB_CHECK_ARG(R >= 1 && P >= 1 && n_pages >= 1 && R < (1 << 24) && P < (1 << 24) && n_pages <= 0x7fffffff / PG_TOKENS, "%s: %lld rows of %lld pages, %lld pages", what,
+               (long long)R, (long long)P, (long long)n_pages);
+  MB_CHECK_ARG(B >= 1 && B <= MBP_MAX_REQUESTS && (rows || B <= R), "%s: %lld requests (1 to %d, without a list of rows at most %lld)", what, (long long)B, MBP_MAX_REQUESTS,
+               (long long)R);
+  p = PlanParams{};
+  p.table = table;
+  p.lens = lens;
+  p.free = free_pages;
+  p.n_free = n_free;
+  p.scratch = scratch;
+  p.rows = rows;
+  p.count = count;
+  p.status = status;
+  p.B = (int)B;
+  p.R = (int)R;
+  p.P = (int)P;
+  p.N = (int)n_pages;
+  return MB200_OK;
+}
+}  // namespace mb200
+
+using namespace mb200;
+
+extern "C" {
+
+int mbp_abi_version(void) { return MBP_ABI_VERSION; }
+const char* mbp_last_error(void) { return g_err; }
+
+int mbp_pages_extend(int32_t* table, int32_t* lens, int32_t* free_pages, int32_t* n_free, int32_t* scratch, const int32_t* rows, const int32_t* add, int32_t* positions,
+                     int32_t* slots, int32_t* q_start, int32_t* seqpos, int32_t* status, int64_t B, int64_t T, int64_t R, int64_t P, int64_t n_pages, void* stream) {
+  PlanParams p;
+  int rc = plan_state(p, "pages_extend", table, lens, free_pages, n_free, scratch, rows, add, B, R, P, n_pages, status);
+  if (rc) return rc;
+  MB_CHECK_ARG(T >= 0 && T <= 0x7fffffff && (T == 0 || (positions && slots)) && q_start && seqpos, "pages_extend: room for %lld tokens", (long long)T);
+  p.positions = positions;
+  p.slots = slots;
+  p.q_start = q_start;
+  p.seqpos = seqpos;
+  p.T = (int)T;
+  return run_plan(true, p, (cudaStream_t)stream);
+}
+
+int mbp_pages_truncate(int32_t* table, int32_t* lens, int32_t* free_pages, int32_t* n_free, int32_t* scratch, const int32_t* rows, const int32_t* keep, int32_t* status,
+                       int64_t B, int64_t R, int64_t P, int64_t n_pages, void* stream) {
+  PlanParams p;
+  int rc = plan_state(p, "pages_truncate", table, lens, free_pages, n_free, scratch, rows, keep, B, R, P, n_pages, status);
+  if (rc) return rc;
+  return run_plan(false, p, (cudaStream_t)stream);
+}
+
+static int check_pool(const char* what, const void* kv, const void* scale, int64_t n_pages, int64_t KV) {
+  MB_CHECK_ARG(kv && scale, "%s: null pointer", what);
+  MB_CHECK_ARG((uintptr_t)kv % 16 == 0, "%s: the pool must be 16-byte aligned", what);
+  // rows of the pool and slots are counted in 32 bits; bytes are not
+  MB_CHECK_ARG(n_pages >= 1 && KV >= 1 && KV <= 65535 && n_pages <= 0x7fffffff / (2 * PG_TOKENS * KV), "%s: %lld pages of %lld heads", what, (long long)n_pages, (long long)KV);
+  return MB200_OK;
+}
+
+int mbp_pages_write(const void* k, int64_t ldk, const void* v, int64_t ldv, void* kv, float* scale, const int32_t* slots, const int32_t* q_start, const int32_t* seqpos,
+                    int64_t B, int64_t T, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages, void* stream) {
+  int rc = check_pool("pages_write", kv, scale, n_pages, n_kv_heads);
+  if (rc) return rc;
+  MB_CHECK_ARG(head_dim == kHeadDim, "pages_write: head_dim=%lld unsupported (128 only)", (long long)head_dim);
+  MB_CHECK_ARG(k && v && slots && q_start && seqpos, "pages_write: null pointer");
+  MB_CHECK_ARG(B >= 1 && B <= MBP_MAX_REQUESTS && T >= 0 && T <= 0x7fffffff - PG_TOKENS, "pages_write: %lld requests, %lld tokens", (long long)B, (long long)T);
+  MB_CHECK_ARG(((uintptr_t)k | (uintptr_t)v) % 16 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldk >= n_kv_heads * head_dim && ldv >= n_kv_heads * head_dim,
+               "pages_write: rows of keys and values must be 16-byte aligned and not overlap (%lld, %lld elements apart)", (long long)ldk, (long long)ldv);
+  if (T == 0) return MB200_OK;
+  PagedWriteParams p;
+  p.k = (const bf16*)k;
+  p.v = (const bf16*)v;
+  p.ldk = ldk;
+  p.ldv = ldv;
+  p.kv = (uint8_t*)kv;
+  p.scale = scale;
+  p.slots = slots;
+  p.q_start = q_start;
+  p.seqpos = seqpos;
+  p.B = (int)B;
+  p.T = (int)T;
+  p.KV = (int)n_kv_heads;
+  p.n_pages = (int)n_pages;
+  const dim3 grid((unsigned)(T / PG_TOKENS + 2 * B), (unsigned)n_kv_heads, 2);
+  MB_CHECK_CUDA(launch_pdl(page_write_kernel, grid, dim3(PW_THREADS), 0, (cudaStream_t)stream, p));
+  return MB200_OK;
+}
+
+int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scale, const int32_t* table, const int32_t* rows, const int32_t* q_start, const int32_t* seqpos,
+                   void* out, int32_t* status, int64_t B, int64_t T, int64_t longest, int64_t most, int64_t R, int64_t P, int64_t n_pages, int64_t n_heads, int64_t n_kv_heads,
+                   int64_t head_dim, int64_t window, float softmax_scale, void* stream) {
+  int rc = check_pool("attn_pages", kv, scale, n_pages, n_kv_heads);
+  if (rc) return rc;
+  MB_CHECK_ARG(head_dim == kHeadDim, "attn_pages: head_dim=%lld unsupported (128 only)", (long long)head_dim);
+  MB_CHECK_ARG(q && table && rows && q_start && seqpos && out, "attn_pages: null pointer");
+  MB_CHECK_ARG(n_heads >= 1 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= 32, "attn_pages: H=%lld KV=%lld (H a multiple of KV, at most 32 times it)",
+               (long long)n_heads, (long long)n_kv_heads);
+  MB_CHECK_ARG(B >= 1 && B <= MBP_MAX_REQUESTS && T >= 0 && T <= 0x7fffffff && longest >= 1 && R >= 1 && P >= 1 && P < (1 << 24) && window >= 0 && window <= 0x7fffffff,
+               "attn_pages: B=%lld T=%lld longest=%lld R=%lld P=%lld window=%lld", (long long)B, (long long)T, (long long)longest, (long long)R, (long long)P, (long long)window);
+  MB_CHECK_ARG(((uintptr_t)q) % 8 == 0 && ldq % 4 == 0 && ldq >= n_heads * head_dim, "attn_pages: rows of queries must be 8-byte aligned and not overlap (%lld elements apart)",
+               (long long)ldq);
+  MB_CHECK_ARG(softmax_scale > 0.f && softmax_scale < 3.4e38f, "attn_pages: scale %g", (double)softmax_scale);
+  if (T == 0) return MB200_OK;
+  const int rep = (int)(n_heads / n_kv_heads);
+  if (longest > T) longest = T;
+  // columns of a query tile: the fewest that hold a request's tokens, 32 at most
+  const int64_t want = longest * rep;
+  const int nq = want <= 8 ? 8 : want <= 16 ? 16 : 32;
+  const int tokens = nq / rep;
+  const int64_t q_tiles = (longest + tokens - 1) / tokens;
+  MB_CHECK_ARG(n_kv_heads * q_tiles <= 65535, "attn_pages: %lld tiles of queries", (long long)(n_kv_heads * q_tiles));
+  PagedAttnParams p;
+  p.q = (const bf16*)q;
+  p.ldq = ldq;
+  p.scale = scale;
+  p.table = table;
+  p.rows = rows;
+  p.q_start = q_start;
+  p.seqpos = seqpos;
+  p.out = (bf16*)out;
+  p.status = status;
+  p.T = (int)T;
+  p.B = (int)B;
+  p.R = (int)R;
+  p.P = (int)P;
+  p.n_pages = (int)n_pages;
+  p.H = (int)n_heads;
+  p.KV = (int)n_kv_heads;
+  p.window = (int)window;
+  p.tokens = tokens;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  CUtensorMap map;
+  rc = make_pool_map(&map, kv, n_pages, n_kv_heads);
+  if (rc) return rc;
+  // splits: as many as run at once, two tiles each at least
+  const int64_t pairs = B * n_kv_heads * q_tiles, room = (int64_t)device_info::sm_count() * (nq <= 16 ? 2 : 1);
+  int64_t keys = most > 0 && most < P * PG_TOKENS ? most : P * PG_TOKENS;
+  if (window > 0 && keys > window + longest) keys = window + longest;
+  int splits = 1;
+  while (splits < PA_MAX_SPLITS && pairs * splits * 2 <= room && keys >= (int64_t)splits * 4 * PA_KEYS) splits *= 2;
+  cudaStream_t st = (cudaStream_t)stream;
+  return nq == 8 ? launch_paged_attn<8>(p, map, q_tiles, splits, st) : nq == 16 ? launch_paged_attn<16>(p, map, q_tiles, splits, st) : launch_paged_attn<32>(p, map, q_tiles, splits, st);
+}
+
+int mbp_token_scores_sizes(int64_t T, int64_t vocab, int64_t top, int64_t* bytes) {
+  MB_CHECK_ARG(T >= 0 && vocab >= 1 && vocab <= MBP_MAX_VOCAB && top >= 0 && top <= TS_MAX_TOP && top <= vocab && bytes, "token_scores: T=%lld vocab=%lld top=%lld (at most %d)", (long long)T,
+               (long long)vocab, (long long)top, TS_MAX_TOP);
+  const int64_t slices = (vocab + TS_SLICE - 1) / TS_SLICE;
+  *bytes = T * slices * (8 * top + 12);
+  return MB200_OK;
+}
+
+int mbp_token_scores(const void* logits, int64_t ld, int dtype, const int64_t* target, float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs, int64_t T,
+                     int64_t vocab, int64_t top, void* scratch, void* stream) {
+  int64_t bytes = 0;
+  int rc = mbp_token_scores_sizes(T, vocab, top, &bytes);
+  if (rc) return rc;
+  MB_CHECK_ARG(logits && scratch && (uintptr_t)scratch % 8 == 0 && (logprob == nullptr || target) && (top == 0 || (top_ids && top_logprobs)), "token_scores: null pointer");
+  MB_CHECK_ARG(ld >= vocab && (dtype == 0 || dtype == 1), "token_scores: rows %lld elements apart of %lld, dtype %d", (long long)ld, (long long)vocab, dtype);
+  MB_CHECK_ARG(T <= 65535, "token_scores: %lld rows (at most 65535)", (long long)T);
+  if (T == 0) return MB200_OK;
+  TokenScoresParams p;
+  p.logits = logits;
+  p.ld = ld;
+  p.target = target;
+  p.T = (int)T;
+  p.V = (int)vocab;
+  p.slices = (int)((vocab + TS_SLICE - 1) / TS_SLICE);
+  p.top = (int)top;
+  p.best = (unsigned long long*)scratch;
+  p.sums = (float*)(p.best + T * p.slices * top);
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.top_ids = top_ids;
+  p.top_logprobs = top_logprobs;
+  const dim3 grid((unsigned)p.slices, (unsigned)T);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == 0) {
+    MB_CHECK_CUDA(launch_pdl(token_scores_slice_kernel<bf16>, grid, dim3(TS_THREADS), 0, st, p));
+    MB_CHECK_CUDA(launch_pdl(token_scores_join_kernel<bf16>, dim3((unsigned)ceil_div(T, TS_JOIN_ROWS)), dim3(TS_JOIN_ROWS * 32), 0, st, p));
+  } else {
+    MB_CHECK_CUDA(launch_pdl(token_scores_slice_kernel<float>, grid, dim3(TS_THREADS), 0, st, p));
+    MB_CHECK_CUDA(launch_pdl(token_scores_join_kernel<float>, dim3((unsigned)ceil_div(T, TS_JOIN_ROWS)), dim3(TS_JOIN_ROWS * 32), 0, st, p));
+  }
+  return MB200_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,483 @@
+// Causal attention of new tokens over pages of e4m3 keys and values, head size 128: decode steps, drafts of a few tokens, short portions.
+//
+//   o = softmax(scale * q K^T + mask) V with K, V = codes * page scales; a query at position p sees the positions (p - window, p] of its own request.
+//
+// The codes never leave 8 bits on their way to the tensor cores.  tcgen05 multiplies e4m3 by e4m3, so it is the QUERIES and the WEIGHTS that are given in
+// e4m3, each as two numbers: hi + lo / 16, hi = e4m3(x), lo = e4m3(16 (x - hi)).  The 8 significant bits of a bf16 query are held exactly that way (a row is
+// first scaled by a power of two to at most 448; entries below 2^-14 of the row's largest keep fewer bits, never worse than 2^-23 of that largest), a weight
+// to 2^-8 of itself, which is what bf16 weights have.  Scores, running maximum and sum, and the values' sums stay in fp32; the pages' scales multiply in fp32,
+// the keys' on the scores, the values' on each page's own accumulator.
+//
+// Keys are the MMA's 128 rows (S^T = K Q^T) and so are the values' dimensions (O^T = V^T P^T, V as it lies in the page: MN-major), the hi and lo parts of up to NQ
+// query columns (tokens x heads of one key/value head) its N = 2 NQ columns.  Memory bounds it: 256 bytes a key and key/value head, where converting them to 16 bits
+// on the way to mma.sync fragments would take more issue slots than the bytes take time.  CTA = (a range of pages, key/value head and tile of queries, request),
+// the ranges of one request's head are a cluster and are merged through distributed shared memory: one launch, no scratch, the same order every time.
+//   warp 4     TMA producer: tiles of two pages (8 KB of keys and of values each) into a ring of PA_STAGES x 32 KB
+//   warp 5     MMA issuer: S(0) S(1) | PV(t) S(t + 2) ...
+//   warps 0-3  a thread per key: its scores -> maximum (over the CTA) -> weights -> shared memory; then, a thread per dimension, the values' sums of the tile before
+#pragma once
+#include "paged_common.cuh"
+
+namespace mb200 {
+
+constexpr int PA_STAGES = 3, PA_KEYS = 2 * PG_TOKENS, PA_STAGE_BYTES = 4 * PG_BYTES;
+constexpr int PA_THREADS = 192, PA_SOFT = 128;
+constexpr int PA_MAX_SPLITS = 16;
+constexpr uint32_t PA_SPINS = 1u << 22;  // polls of a wait before it gives up (seconds)
+enum { PA_GAVE_UP = 16 };                // status: a wait ran out; the call's results are NaN
+
+struct PagedAttnParams {
+  const bf16* q;
+  int64_t ldq;  // elements between tokens
+  const float* scale;
+  const int32_t *table, *rows, *q_start, *seqpos;
+  bf16* out;  // [T, H * 128]
+  int32_t* status;
+  int T, B, R, P, n_pages, H, KV, window, tokens;  // tokens: of a query tile
+  float scale_log2;
+};
+
+template <int NQ>
+struct PaCfg {
+  static constexpr int kColBytes = 2 * NQ * 128;  // Q or one P tile: [2 NQ columns][128 bytes], 128B-swizzled
+  static constexpr int kRing = PA_STAGES * PA_STAGE_BYTES;
+  static constexpr int kMerge = NQ * (kHeadDim + 2) * 4;  // this split's result, over the ring once that is used up
+  static constexpr int kSmem = 1024 + kRing + 3 * kColBytes + 1024;
+  static constexpr int kTmemCols = 8 * NQ;  // two S tiles, the two pages' O
+  static_assert(kMerge <= kRing && kTmemCols <= 512, "fits");
+  // D = fp32, A = B = e4m3, N >> 3 at bit 17, M >> 4 at bit 24; values: A is MN-major (bit 15)
+  static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(2 * NQ >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  static constexpr uint32_t kIdescO = kIdescS | (1u << 15);
+};
+
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 da, db;\n"
+      "mov.b64 da, {%1, %5};\n"
+      "mov.b64 db, {%2, %5};\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(UMMA_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x16_nowait(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ float warp_max_sync(float v) {  // (NaN does not count)
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// false: the wait ran out, or another thread's has
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+  for (uint32_t i = 0; i < PA_SPINS; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 63u && *gave_up) return false;
+  }
+  *gave_up = 1;
+  return false;
+}
+// barrier of the PA_SOFT softmax threads; true if any of them says so
+__device__ __forceinline__ bool soft_sync_or(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"((uint32_t)v)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+// Columns go in groups of 8 queries: 8 columns of hi, 8 of lo.  Byte `k` of column (query q, part): its 128 bytes are one row of a 128B-swizzled K-major tile.
+__device__ __forceinline__ uint32_t pa_col(int q, int part, int k) {
+  const int r = q & 7;
+  return (uint32_t)((((q >> 3) * 2 + part) << 10) + (r << 7) + (((k >> 4) ^ r) << 4) + (k & 15));
+}
+
+template <int NQ>
+__global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kernel(const __grid_constant__ CUtensorMap map_kv, const PagedAttnParams p) {
+  using Cfg = PaCfg<NQ>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem + Cfg::kRing;
+  uint8_t* sP = sQ + Cfg::kColBytes;  // [2]
+  __shared__ uint64_t kv_full[PA_STAGES], kv_empty[PA_STAGES], q_full, s_full[2], p_full, o_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up;
+  __shared__ float page_scale[PA_STAGES][4];              // keys of page 0, 1, values of page 0, 1 of the stage's tile
+  __shared__ float q_scale[NQ];                           // a query row's scale, times the softmax scale, in log2 units
+  __shared__ __align__(16) float warp_most[2][NQ][4];     // by tile parity
+  __shared__ float sums[4][NQ];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int split = blockIdx.x, splits = gridDim.x, g = blockIdx.y % p.KV, qt = blockIdx.y / p.KV, b = blockIdx.z;
+  const int R = p.H / p.KV;
+  pdl_trigger();
+  if (tid == 0) {
+    for (int i = 0; i < PA_STAGES; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(&q_full, 4);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(&p_full, 4);
+    mbar_init(&o_full, 1);
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
+  }
+  if (warp == 5) tmem_alloc(&tmem_slot, Cfg::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+
+  const int t_first = p.q_start[b], n_all = p.q_start[b + 1] - t_first, past = p.seqpos[b];
+  const int i0 = qt * p.tokens;
+  const int n = t_first < 0 || n_all < 0 || n_all > p.T - t_first || past < 0 ? 0 : min(p.tokens, n_all - i0);  // tokens of this tile
+  if (n <= 0) {  // the whole cluster alike
+    __syncthreads();
+    if (warp == 5) tmem_dealloc(tmem, Cfg::kTmemCols);
+    return;
+  }
+  const int nq = n * R, tok0 = t_first + i0;
+  const int pos0 = past + i0, hi = pos0 + n;                                   // the tile's first position, one past its last
+  const int lo = p.window > 0 ? max(0, pos0 + 1 - p.window) : 0;               // the first position that any query sees
+  const int page_lo = lo / PG_TOKENS, n_pages = (hi + PG_TOKENS - 1) / PG_TOKENS - page_lo;
+  const int per = ((n_pages + 1) / 2 + splits - 1) / splits;                   // tiles of a split
+  const int first = page_lo + min(split * per * 2, n_pages), last = page_lo + min((split + 1) * per * 2, n_pages);  // this split's pages
+  const int tiles = (last - first + 1) / 2;
+
+  float o[NQ], m[NQ], l[NQ];
+  if (warp == 4) {
+    // ================= producer =================
+    const int row = p.rows[b];
+    const bool row_ok = row >= 0 && row < p.R;
+    int page = 0;
+    float ks = 0.f, vs = 0.f;
+    for (int t = 0; t < tiles; ++t) {
+      if ((t & 15) == 0) {  // the next 32 pages and their scales, one a lane
+        const int at = first + 2 * t + lane;
+        page = -1;
+        if (at < last && row_ok && at < p.P) page = p.table[(int64_t)row * p.P + at];
+        const bool ok = page >= 0 && page < p.n_pages;
+        if (!ok) page = 0;  // a page that is none: nothing is read out of bounds, and what it weighs is no number
+        const float* s = p.scale + ((int64_t)page * p.KV + g) * 2;
+        ks = ok ? s[0] : __int_as_float(0x7fffffff);
+        vs = ok ? s[1] : __int_as_float(0x7fffffff);
+      }
+      const int st = t % PA_STAGES, two = first + 2 * t + 1 < last, src = (2 * t) & 31;
+      const int page0 = __shfl_sync(0xffffffffu, page, src), page1 = __shfl_sync(0xffffffffu, page, src + 1);
+      const float ks0 = __shfl_sync(0xffffffffu, ks, src), ks1 = __shfl_sync(0xffffffffu, ks, src + 1);
+      const float vs0 = __shfl_sync(0xffffffffu, vs, src), vs1 = __shfl_sync(0xffffffffu, vs, src + 1);
+      if (!__all_sync(0xffffffffu, pa_wait(&kv_empty[st], ((t / PA_STAGES) & 1) ^ 1, &gave_up))) break;
+      if (lane == 0) {
+        page_scale[st][0] = ks0;
+        page_scale[st][1] = ks1;
+        page_scale[st][2] = vs0;
+        page_scale[st][3] = vs1;
+        mbar_arrive_expect_tx(&kv_full[st], (two ? 4 : 2) * PG_BYTES);
+        uint8_t* dst = smem + st * PA_STAGE_BYTES;
+        const int r0 = (page0 * p.KV + g) * 2 * PG_TOKENS, r1 = (page1 * p.KV + g) * 2 * PG_TOKENS;
+        tma_load_2d(dst, &map_kv, &kv_full[st], 0, r0);
+        if (two) tma_load_2d(dst + PG_BYTES, &map_kv, &kv_full[st], 0, r1);
+        tma_load_2d(dst + 2 * PG_BYTES, &map_kv, &kv_full[st], 0, r0 + PG_TOKENS);
+        if (two) tma_load_2d(dst + 3 * PG_BYTES, &map_kv, &kv_full[st], 0, r1 + PG_TOKENS);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 5) {
+    // ================= MMA issuer =================
+    bool ok = tiles == 0 || pa_wait(&q_full, 0, &gave_up);
+    const uint32_t q_desc = umma_desc_lo(smem_u32(sQ));
+    auto issue_s = [&](int t) {
+      const int st = t % PA_STAGES;
+      ok = ok && pa_wait(&kv_full[st], (t / PA_STAGES) & 1, &gave_up);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t k_desc = umma_desc_lo(smem_u32(smem + st * PA_STAGE_BYTES));
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_e4m3(tmem + (t & 1) * 2 * NQ, k_desc + k * 2, q_desc + k * 2, Cfg::kIdescS, k ? 1u : 0u);
+        umma_commit(&s_full[t & 1]);
+      }
+      __syncwarp();
+    };
+    if (tiles > 0) issue_s(0);
+    if (tiles > 1) issue_s(1);
+    for (int t = 0; t < tiles && ok; ++t) {
+      ok = pa_wait(&p_full, t & 1, &gave_up);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const int st = t % PA_STAGES;
+      const bool two = first + 2 * t + 1 < last;
+      const uint32_t v_desc = umma_desc_lo(smem_u32(smem + st * PA_STAGE_BYTES + 2 * PG_BYTES)), p_desc = umma_desc_lo(smem_u32(sP + (t & 1) * Cfg::kColBytes));
+      if (elect_one()) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          if (half == 0 || two) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)  // 32 keys each: 4 KB of values, 32 bytes of a weights' column
+              umma_e4m3(tmem + 4 * NQ + half * 2 * NQ, v_desc + ((half * PG_BYTES + k * 4096) >> 4), p_desc + half * 4 + k * 2, Cfg::kIdescO, k ? 1u : 0u);
+          }
+        umma_commit(&o_full);
+        umma_commit(&kv_empty[st]);
+      }
+      __syncwarp();
+      if (t + 2 < tiles) issue_s(t + 2);
+    }
+  } else {
+    // ================= softmax =================
+    // queries -> hi and lo parts, a warp per row
+    for (int q = warp; q < NQ; q += 4) {
+      uint2 u = make_uint2(0u, 0u);
+      if (q < nq) u = *reinterpret_cast<const uint2*>(p.q + (int64_t)(tok0 + q / R) * p.ldq + (int64_t)(g * R + q % R) * kHeadDim + lane * 4);
+      const float x[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
+      const int e = e4m3_exponent(warp_max(fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])))));
+      const float inv = pow2i(-e);
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = scaled(x[i], inv);
+      const uint32_t h0 = to_e4m3x2(y[0], y[1]), h1 = to_e4m3x2(y[2], y[3]);
+      const float2 f0 = from_e4m3x2(h0), f1 = from_e4m3x2(h1);
+      const uint32_t l0 = to_e4m3x2((y[0] - f0.x) * 16.f, (y[1] - f0.y) * 16.f), l1 = to_e4m3x2((y[2] - f1.x) * 16.f, (y[3] - f1.y) * 16.f);
+      *reinterpret_cast<uint32_t*>(sQ + pa_col(q, 0, lane * 4)) = h0 | h1 << 16;
+      *reinterpret_cast<uint32_t*>(sQ + pa_col(q, 1, lane * 4)) = l0 | l1 << 16;
+      if (lane == 0) q_scale[q] = pow2i(e) * p.scale_log2;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_full);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      o[q] = l[q] = 0.f;
+      m[q] = -INFINITY;
+    }
+    soft_sync_or(false);  // q_scale of all rows
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    float vs0 = 0.f, vs1 = 0.f;  // value scales of the tile before
+    bool two_before = false, ok = true;
+    auto add_values = [&](int t) {  // the sums of tile t, relative to m as it stood then
+      ok = ok && pa_wait(&o_full, t & 1, &gave_up);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < NQ / 8; ++c) {
+        uint32_t a[16], z[16];
+        tmem_ld_32x32b_x16_nowait(lanes + 4 * NQ + c * 16, a);
+        if (two_before) tmem_ld_32x32b_x16_nowait(lanes + 6 * NQ + c * 16, z);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[c * 8 + i] = fmaf(fmaf(__uint_as_float(a[8 + i]), 0.0625f, __uint_as_float(a[i])), vs0, o[c * 8 + i]);
+        if (two_before) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[c * 8 + i] = fmaf(fmaf(__uint_as_float(z[8 + i]), 0.0625f, __uint_as_float(z[i])), vs1, o[c * 8 + i]);
+        }
+      }
+    };
+    for (int t = 0; t < tiles; ++t) {
+      const int st = t % PA_STAGES;
+      const int half = tid >> 6, key = (first + 2 * t) * PG_TOKENS + tid;
+      const bool here = first + 2 * t + half < last;            // the tile's second page may be none
+      const bool seen = here && key >= lo && key < hi;          // by any query
+      float s[NQ];
+      ok = ok && pa_wait(&kv_full[st], (t / PA_STAGES) & 1, &gave_up) && pa_wait(&s_full[t & 1], (t >> 1) & 1, &gave_up);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tc_fence_after();
+        const float ks = page_scale[st][half];
+#pragma unroll
+        for (int c = 0; c < NQ / 8; ++c) {
+          uint32_t a[16];
+          tmem_ld_32x32b_x16_nowait(lanes + (t & 1) * 2 * NQ + c * 16, a);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int q = c * 8 + i;
+            const float x = fmaf(__uint_as_float(a[8 + i]), 0.0625f, __uint_as_float(a[i])) * (ks * q_scale[q]);
+            bool sees = seen;
+            if (n > 1) {  // (of one token every key in [lo, hi) is seen)
+              const int pos = pos0 + q / R;
+              sees = seen && key <= pos && (p.window <= 0 || key > pos - p.window);
+            }
+            s[q] = sees ? x : -INFINITY;
+          }
+        }
+      }
+      if (!seen && here) {  // what this row holds must not reach the sums: 0 * NaN is not 0
+        uint4* v = reinterpret_cast<uint4*>(smem + st * PA_STAGE_BYTES + 2 * PG_BYTES + tid * 128);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
+      }
+      if (ok) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const float w = warp_max_sync(s[q]);
+          if (lane == 0) warp_most[t & 1][q][warp] = w;
+        }
+      }
+      if (soft_sync_or(!ok)) {
+        ok = false;
+        break;
+      }
+      float alpha[NQ];
+      uint8_t* P = sP + (t & 1) * Cfg::kColBytes;
+#pragma unroll
+      for (int q = 0; q < NQ; q += 2) {
+        float e[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 w = *reinterpret_cast<const float4*>(warp_most[t & 1][q + i]);
+          const float top = fmaxf(fmaxf(m[q + i], fmaxf(w.x, w.y)), fmaxf(w.z, w.w));
+          const float ref = top == -INFINITY ? 0.f : top;  // (nothing seen yet weighs nothing)
+          alpha[q + i] = exp2_ftz(m[q + i] - ref);
+          m[q + i] = top;
+          e[i] = exp2_ftz(s[q + i] - ref + 8.f);  // weights times 256: the whole of e4m3's range
+          l[q + i] = fmaf(l[q + i], alpha[q + i], e[i]);
+        }
+        const uint32_t h = to_e4m3x2(e[0], e[1]);
+        const float2 f = from_e4m3x2(h);
+        const uint32_t r = to_e4m3x2((e[0] - f.x) * 16.f, (e[1] - f.y) * 16.f);
+        P[pa_col(q, 0, tid)] = (uint8_t)h;
+        P[pa_col(q + 1, 0, tid)] = (uint8_t)(h >> 8);
+        P[pa_col(q, 1, tid)] = (uint8_t)r;
+        P[pa_col(q + 1, 1, tid)] = (uint8_t)(r >> 8);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (t > 0) add_values(t - 1);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[q] *= alpha[q];
+      vs0 = page_scale[st][2];
+      vs1 = page_scale[st][3];
+      two_before = first + 2 * t + 1 < last;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0 && ok) mbar_arrive(&p_full);
+    }
+    if (tiles > 0 && ok) add_values(tiles - 1);
+    if (!__all_sync(0xffffffffu, ok)) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[q] = __int_as_float(0x7fffffff);
+      if (lane == 0 && p.status) atomicOr(p.status, PA_GAVE_UP);
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const float w = warp_sum(l[q]);
+      if (lane == 0) sums[warp][q] = w;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (gave_up && tid == 0) {  // copies of this CTA may still be in flight: they end before its shared memory does
+    for (int i = 0; i < PA_STAGES; ++i)
+      for (uint32_t k = 0; k < 2; ++k)
+        for (uint32_t spin = 0; spin < 4096 && !mbar_try_wait(&kv_full[i], k); ++spin) {}
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::kTmemCols);
+  }
+  // ================= merge the splits =================
+  // this split: [q][maximum, sum, 128 sums] over the ring, which is used up
+  float* mine = reinterpret_cast<float*>(smem);
+  if (warp < 4) {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      if (q < nq) {
+        mine[q * (kHeadDim + 2) + 2 + tid] = o[q];
+        if (tid == 0) {
+          mine[q * (kHeadDim + 2)] = m[q];
+          mine[q * (kHeadDim + 2) + 1] = sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q];
+        }
+      }
+    }
+  }
+  cluster_sync_all();
+  if (warp < 4) {
+    const uint32_t base = smem_u32(mine);
+    for (int q = split; q < nq; q += splits) {
+      const uint32_t at = base + q * (kHeadDim + 2) * 4;
+      float top = -INFINITY;
+      for (int r = 0; r < splits; ++r) top = fmaxf(top, ld_cluster_f32(map_to_rank(at, r)));
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, acc = 0.f;
+      for (int r = 0; r < splits; ++r) {
+        const uint32_t from = map_to_rank(at, r);
+        const float f = exp2_ftz(ld_cluster_f32(from) - ref);  // (a split without a key: 0)
+        sum = fmaf(f, ld_cluster_f32(from + 4), sum);
+        acc = fmaf(f, ld_cluster_f32(from + 8 + tid * 4), acc);
+      }
+      p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + tid] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
+    }
+  }
+  cluster_sync_all();  // nobody leaves while its results are read
+}
+
+// the pool as rows of 128 bytes; box = one head's keys or values of a page, 128-byte swizzle
+inline int make_pool_map(CUtensorMap* map, const void* kv, int64_t n_pages, int64_t KV) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (enc == nullptr) return fail(MB200_E_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  const cuuint64_t dims[2] = {(cuuint64_t)kHeadDim, (cuuint64_t)(n_pages * KV * 2 * PG_TOKENS)};
+  const cuuint64_t strides[1] = {(cuuint64_t)kHeadDim};
+  const cuuint32_t box[2] = {(cuuint32_t)kHeadDim, (cuuint32_t)PG_TOKENS};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(kv), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MB200_E_CUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", (int)r);
+  return MB200_OK;
+}
+
+template <int NQ>
+inline int launch_paged_attn(const PagedAttnParams& p, const CUtensorMap& map, int64_t q_tiles, int splits, cudaStream_t st) {
+  MB_CHECK_CUDA(device_info::allow_shared<paged_attn_kernel<NQ>>(PaCfg<NQ>::kSmem));
+  if (splits > 8) MB_CHECK_CUDA(cudaFuncSetAttribute(paged_attn_kernel<NQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)(p.KV * q_tiles), (unsigned)p.B);
+  cfg.blockDim = dim3(PA_THREADS);
+  cfg.dynamicSmemBytes = PaCfg<NQ>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  MB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_attn_kernel<NQ>, map, p));
+  return MB200_OK;
+}
+
+}  // namespace mb200

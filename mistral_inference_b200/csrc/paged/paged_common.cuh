@@ -1,0 +1,55 @@
+// Pages of 8-bit keys and values, shared by the kernels of libmb200_paged.so.
+//
+// Pool: kv [pages, KV, 2 (keys, values), 64 tokens, 128] e4m3, scale [pages, KV, 2] fp32; a number is its code times the scale of its (page, head, kind).
+// Scales are powers of two: an e4m3 code is a floating-point number, so a scale between two powers would gain no precision inside a page, only its
+// range matters; and a page's scale can grow by a power of two without changing any code but the few that fall below e4m3's normal numbers.
+#pragma once
+#include "../../../include/mistral_b200_paged.h"
+#include "../gemm_tcgen05.cuh"
+
+namespace mb200 {
+
+constexpr int PG_TOKENS = 64;                       // tokens of a page
+constexpr int PG_BYTES = PG_TOKENS * kHeadDim;      // one head's keys (or values) of a page: 8 KB, contiguous
+constexpr int PG_LOWEST_EXP = -100;                 // the scale of a page of zeros is 2^-100
+
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+// the smallest e with amax <= 448 * 2^e (448 = 1.75 * 2^8 is e4m3's largest number); amax finite
+__device__ __forceinline__ int e4m3_exponent(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  return max((int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0), PG_LOWEST_EXP);
+}
+__device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127; }
+__device__ __forceinline__ float finite_abs(float x) {  // |x|, 0 where x is no number or infinite
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;
+}
+// two numbers to two codes (lo in the low byte), to nearest even; |x| <= 448 or NaN
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {  // exact: every e4m3 number is an fp16 number
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)codes));
+  float2 f;
+  asm("{.reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.f32.f16 %0, l;\n cvt.f32.f16 %1, h;\n}" : "=f"(f.x), "=f"(f.y) : "r"(h));
+  return f;
+}
+// x times a power of two; not a number where x is infinite (e4m3 has no infinity, and the largest code would pass for a number)
+__device__ __forceinline__ float scaled(float x, float inv) { return fmaf(x, inv, x - x); }
+
+// largest i in [0, n) with start[i] <= x, start ascending, start[0] <= x
+template <typename F>
+__device__ __forceinline__ int last_not_above(int n, int x, F start) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start(mid) <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+}  // namespace mb200

@@ -1,0 +1,37 @@
+"""What a model thinks of tokens: log-probabilities of given ones, the entropy of their distribution and the most likely alternatives.
+
+The reference reports one log-probability a token (generate.py:101-117,134-135); here the same pass over a row of logits gives the row's entropy and its best tokens as well,
+in one kernel that reads the logits once (csrc/paged/token_scores.cuh)."""
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _abi_paged
+
+
+@dataclass
+class TokenScores:
+    logprob: Optional[torch.Tensor]   # [T] fp32: log-probability of each row's target, 0 where it has none (None without targets)
+    entropy: torch.Tensor             # [T] fp32, in nats
+    top_ids: torch.Tensor             # [T, top] int64, most likely first; of equal ones the lowest index
+    top_logprobs: torch.Tensor        # [T, top] fp32
+
+
+def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0) -> TokenScores:
+    """Scores of the rows of `logits` [T, V] (fp32 or bf16; rows may be part of wider ones).  targets [T] int64: a token of each row, or -1; a target past the vocabulary
+    scores NaN, as does a row that holds NaN or +infinity, or nothing but -infinity.  Other entries of -infinity (masked tokens) weigh nothing."""
+    assert logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16) and logits.shape[1] >= 1, f"logits [T, V], fp32 or bf16, got {tuple(logits.shape)} {logits.dtype}"
+    T, V = logits.shape
+    assert logits.stride(1) == 1 and (T <= 1 or logits.stride(0) >= V), "rows of logits are contiguous and do not overlap"
+    assert targets is None or (targets.dtype == torch.long and targets.shape == (T,)), "targets: one int64 a row"
+    assert 0 <= top <= min(_abi_paged.MAX_TOP, V), f"{top} alternatives (at most {_abi_paged.MAX_TOP}, and no more than tokens)"
+    new = dict(device=logits.device)
+    out = TokenScores(torch.zeros(T, dtype=torch.float32, **new) if targets is not None else None, torch.empty(T, dtype=torch.float32, **new),
+                      torch.empty(T, top, dtype=torch.long, **new), torch.empty(T, top, dtype=torch.float32, **new))
+    rows = 65535  # of a call
+    for r in range(0, T, rows):
+        cut = slice(r, r + rows)
+        part = [None if t is None else t[cut] for t in (targets, out.logprob, out.entropy, out.top_ids, out.top_logprobs)]
+        _abi_paged.token_scores(logits[cut], *part, top)
+    return out

@@ -1,0 +1,131 @@
+"""Scores of tokens on the GPU against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import mistral_inference_b200 as mi
+
+from . import paged_util as U
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def logits_of(T, V, seed, std=3.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, V, generator=g) * std).to(torch.bfloat16).to(dtype)  # equal values are common
+
+
+def check(x, targets, top):
+    s = mi.token_scores(x.to(DEV), None if targets is None else targets.to(DEV), top=top)
+    lp, ent, ids, lps = U.scores_ref(x, targets, top)
+    assert s.top_ids.cpu().tolist() == ids.tolist()
+    # x - m and its exponential in fp32: 2^-24 of the exponent and 2 ulp (2^-22) each, exponents up to 2^7 of those that count; sums of positive numbers by threads and in trees, at most
+    # 2^5 steps of 2^-24 each: 2^-17 of the sum, absolute in its logarithm; the difference with the target's logit rounds once (2^-24 of up to 2^8).  Entropies: the same of both sums.
+    for got, want in ((s.logprob, lp), (s.entropy, ent), (s.top_logprobs, lps)):
+        if want is None:
+            assert got is None
+            continue
+        got = got.cpu().double()
+        assert torch.equal(got.isnan(), want.isnan())
+        fin = want.isfinite()
+        assert torch.equal(got[~fin & ~want.isnan()], want[~fin & ~want.isnan()])
+        assert ((got - want).abs()[fin] <= 2.0 ** -17 + 2.0 ** -15 * want.abs()[fin].clamp(max=16)).all(), (got - want).abs()[fin].max()
+    return s
+
+
+@pytest.mark.parametrize("V", [1, 2, 31, 1000, 1003, 8192, 8193, 32000, 131072, 200001])
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores(V, T, dtype):
+    x = logits_of(T, V, V, dtype=dtype)
+    targets = torch.tensor([(7919 * i) % V if i % 3 != 1 else -1 for i in range(T)])
+    for top in sorted({0, 1, min(V, 5), min(V, 64)}):
+        check(x, targets, top)
+    check(x, None, min(V, 3))
+
+
+def test_many_rows():
+    x = logits_of(700, 1003, 3)
+    check(x, torch.randint(0, 1003, (700,)), 20)
+
+
+def test_masked_rows():
+    x = logits_of(6, 32000, 5)
+    allowed = torch.zeros_like(x, dtype=torch.bool)
+    for i, k in enumerate([1, 3, 19, 20, 500]):  # fewer tokens than alternatives: masked ones fill the list, lowest index first
+        allowed[i, torch.randperm(32000, generator=torch.Generator().manual_seed(i))[:k]] = True
+    x = x.masked_fill(~allowed, -math.inf)       # the last row: nothing is allowed
+    s = check(x, torch.tensor([0, 1, 2, 3, 4, 5]), 20)
+    assert s.entropy[0] == 0.0 and s.top_logprobs[0, 0] == 0.0 and s.entropy[5].isnan()
+
+
+def test_infinities_and_numbers_that_are_none():
+    x = logits_of(5, 9000, 6)
+    x[0, 8500] = math.nan
+    x[1, 17] = math.inf
+    x[2, 8999] = -math.nan
+    x[3] = -math.inf
+    check(x, torch.tensor([3, 17, 4, 5, 6]), 4)
+
+
+def test_equal_values():
+    x = torch.zeros(3, 20000)
+    x[0, ::2] = -0.0  # equal to 0
+    x[1, 15000:15010] = 1.0
+    x[2] = torch.arange(20000).float() * -1e-3  # sorted: all of the best in one place
+    check(x, torch.tensor([1, 15003, 19999]), 64)
+
+
+def test_lowest_values_of_the_type():
+    x = torch.full((2, 5000), torch.finfo(torch.float32).min)
+    x[0, 77] = 0.0
+    x[1, 4000:] = torch.finfo(torch.float32).max
+    check(x, torch.tensor([77, 4001]), 5)
+
+
+def test_peaked_rows_keep_their_digits():
+    """A token with almost all the probability: 1 - p, not p, sets the entropy and its own log-probability."""
+    x = torch.full((3, 40000), -30.0)
+    x[0, 5], x[1, 39999], x[2, 20000] = 0.0, 2.0, -11.0
+    targets = torch.tensor([5, 39999, 20000])
+    s = check(x, targets, 2)
+    lp, ent, _, _ = U.scores_ref(x, targets, 2)
+    # relative to themselves: exponents are exact to 2^-24 * 2^5, the exponential to 2^-22, sums to 2^-17
+    for got, want in ((s.logprob, lp), (s.entropy, ent)):
+        assert ((got.cpu().double() - want).abs() <= 2.0 ** -16 * want.abs()).all()
+
+
+def test_rows_of_wider_ones_and_targets_past_the_vocabulary():
+    wide = logits_of(4, 1100, 8)
+    x = wide.to(DEV)[:, 50:1050]
+    s = mi.token_scores(x, torch.tensor([0, 999, 1000, -5], device=DEV), top=3)
+    want = mi.token_scores(x.contiguous(), torch.tensor([0, 999, -1, -1], device=DEV), top=3)
+    assert torch.equal(s.top_ids, want.top_ids) and torch.equal(s.entropy, want.entropy)
+    assert torch.equal(s.logprob[:2], want.logprob[:2]) and s.logprob[2].isnan() and s.logprob[3] == 0
+
+
+def test_no_rows():
+    s = mi.token_scores(torch.empty(0, 100, device=DEV), torch.empty(0, dtype=torch.long, device=DEV), top=3)
+    assert s.logprob.shape == (0,) and s.top_ids.shape == (0, 3)
+
+
+def test_the_same_bits_alone_captured_and_on_another_stream():
+    x = logits_of(9, 50257, 9).to(DEV)
+    t = torch.arange(9, device=DEV)
+    a = mi.token_scores(x, t, top=7)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = mi.token_scores(x, t, top=7)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c = mi.token_scores(x, t, top=7)
+    g.replay()
+    one = mi.token_scores(x[4:5], t[4:5], top=7)
+    torch.cuda.synchronize()
+    for y in (b, c):
+        assert torch.equal(a.logprob, y.logprob) and torch.equal(a.entropy, y.entropy) and torch.equal(a.top_ids, y.top_ids) and torch.equal(a.top_logprobs, y.top_logprobs)
+    assert torch.equal(a.logprob[4:5], one.logprob) and torch.equal(a.top_ids[4:5], one.top_ids)

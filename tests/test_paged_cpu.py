@@ -1,0 +1,156 @@
+"""The paged library's boundary and refusals, without a GPU: everything here is turned away before a kernel is launched."""
+import ctypes
+import re
+import zlib
+from pathlib import Path
+
+import pytest
+import torch
+
+import mistral_inference_b200 as mi
+from mistral_inference_b200 import _abi_paged
+from mistral_inference_b200.build import build_paged
+
+from . import paged_util as U
+
+REPO = Path(__file__).resolve().parents[1]
+HEADER = REPO / "include" / "mistral_b200_paged.h"
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build_paged()
+    return _abi_paged.lib()
+
+
+def test_header_and_binding_name_the_same_symbols(lib):
+    declared = set(re.findall(r"\b(mbp_[a-z0-9_]+)\s*\(", HEADER.read_text()))
+    assert declared == set(_abi_paged._SIGNATURES)
+    assert lib.mbp_abi_version() == _abi_paged.ABI_VERSION == int(re.search(r"MBP_ABI_VERSION (\d+)", HEADER.read_text()).group(1))
+
+
+def test_constants_agree_with_the_header():
+    text = HEADER.read_text()
+    assert int(re.search(r"MBP_MAX_REQUESTS (\d+)", text).group(1)) == _abi_paged.MAX_REQUESTS
+    assert f"top <= {_abi_paged.MAX_TOP}" in text
+
+
+def last(lib):
+    return lib.mbp_last_error().decode()
+
+
+# Pointers that are never read: every call below is refused by its sizes.
+X = 4096
+
+
+def test_plans_are_refused(lib):
+    extend = lambda B=2, T=2, R=2, P=4, N=8, rows=None, table=X: lib.mbp_pages_extend(table, X, X, X, X, rows, X, X, X, X, X, X, B, T, R, P, N, None)  # noqa: E731
+    for kw, why in [(dict(table=None), "null"), (dict(B=0), "requests"), (dict(B=_abi_paged.MAX_REQUESTS + 1, R=5000), "requests"), (dict(B=3), "requests"), (dict(T=-1), "room"),
+                    (dict(R=0), "rows"), (dict(P=0), "pages"), (dict(N=0), "pages"), (dict(N=2 ** 31 // 64 + 1), "pages")]:
+        assert extend(**kw) == -1 and why in last(lib), (kw, last(lib))
+    truncate = lambda B=2, R=2, P=4, N=8, keep=X: lib.mbp_pages_truncate(X, X, X, X, X, None, keep, X, B, R, P, N, None)  # noqa: E731
+    for kw, why in [(dict(keep=None), "null"), (dict(B=3), "requests"), (dict(R=0), "rows")]:
+        assert truncate(**kw) == -1 and why in last(lib), (kw, last(lib))
+
+
+def test_writes_are_refused(lib):
+    def write(k=X, ldk=256, ldv=256, kv=X, B=1, T=1, KV=2, hd=128, N=4):
+        return lib.mbp_pages_write(k, ldk, X, ldv, kv, X, X, X, X, B, T, KV, hd, N, None)
+    for kw, why in [(dict(k=None), "null"), (dict(k=X + 8), "aligned"), (dict(ldk=128), "aligned"), (dict(ldv=260), "aligned"), (dict(kv=X + 4), "aligned"), (dict(hd=64), "128 only"),
+                    (dict(B=0), "requests"), (dict(T=-1), "tokens"), (dict(KV=0), "heads"), (dict(N=2 ** 31 // 256), "heads")]:
+        assert write(**kw) == -1 and why in last(lib), (kw, last(lib))
+    assert write(T=0) == 0
+
+
+def test_attention_is_refused(lib):
+    def attend(q=X, ldq=512, B=1, T=1, longest=1, H=4, KV=2, hd=128, P=4, N=4, window=0, scale=0.1):
+        return lib.mbp_attn_pages(q, ldq, X, X, X, X, X, X, X, None, B, T, longest, 0, 2, P, N, H, KV, hd, window, scale, None)
+    for kw, why in [(dict(q=None), "null"), (dict(q=X + 4), "aligned"), (dict(ldq=256), "overlap"), (dict(H=5), "multiple"), (dict(H=66, ldq=66 * 128), "32 times"), (dict(hd=64), "128 only"),
+                    (dict(longest=0), "longest"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(P=0), "P="), (dict(N=0), "pages")]:
+        assert attend(**kw) == -1 and why in last(lib), (kw, last(lib))
+    assert attend(T=0) == 0
+
+
+def test_scores_are_refused(lib):
+    need = ctypes.c_int64(0)
+
+    def score(logits=X, ld=100, dtype=1, target=X, logprob=X, T=2, V=100, top=3, scratch=X):
+        return lib.mbp_token_scores(logits, ld, dtype, target, logprob, X, X, X, T, V, top, scratch, None)
+    for kw, why in [(dict(logits=None), "null"), (dict(ld=99), "apart"), (dict(dtype=2), "dtype"), (dict(target=None), "null"), (dict(top=65), "top"), (dict(V=2, top=3), "top"), (dict(T=65536), "rows"),
+                    (dict(scratch=X + 4), "null"), (dict(V=0), "vocab")]:
+        assert score(**kw) == -1 and why in last(lib), (kw, last(lib))
+    assert score(T=0) == 0
+    assert lib.mbp_token_scores_sizes(2, 100, 3, ctypes.byref(need)) == 0 and need.value > 0
+
+
+def tables_cpu():
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    return i(2, 4), i(2), i(8), i(1)
+
+
+def test_python_refuses_what_it_cannot_take():
+    table, lens, free, n_free = tables_cpu()
+    with pytest.raises(AssertionError):
+        mi.PageTables(table.long(), lens, free, n_free)
+    with pytest.raises(AssertionError):
+        mi.PageTables(table, lens[:1], free, n_free)
+    with pytest.raises(AssertionError):
+        mi.PageTables(table[:, ::2], lens, free, n_free)
+    t = mi.PageTables(table, lens, free, n_free)
+    with pytest.raises(AssertionError):
+        t.extend(torch.ones(3, dtype=torch.int32), 3)  # more requests than rows
+    with pytest.raises(AssertionError):
+        t.extend(torch.ones(2), 2)
+    with pytest.raises(AssertionError):
+        t.truncate(torch.ones(2, dtype=torch.int32), rows=torch.ones(1, dtype=torch.int32))
+    with pytest.raises(AssertionError, match="CUDA"):  # no fallback
+        t.extend(torch.ones(2, dtype=torch.int32), 2)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    plan = mi.PagePlan(table, i(0), i(0, 1), i(0), i(0), i(0), 1)
+    kv, scale = torch.zeros(4, 2, 2, 64, 128, dtype=torch.uint8), torch.ones(4, 2, 2)
+    k, q = torch.zeros(1, 2, 128, dtype=torch.bfloat16), torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    for bad in (dict(kv=kv[:, :, :, :32]), dict(kv=kv.float()), dict(scale=scale.double()), dict(scale=scale[:, :1]), dict(k=k.float()), dict(k=k[:, :1]), dict(k=torch.cat([k, k]))):
+        a = {**dict(kv=kv, scale=scale, k=k), **bad}
+        with pytest.raises(AssertionError):
+            mi.write_pages(a["kv"], a["scale"], a["k"], a["k"], plan)
+    for bad in (dict(q=q[:, :3]), dict(q=q[0]), dict(q=q.half()), dict(out=torch.zeros(1, 512)), dict(q=torch.cat([q, q]))):
+        a = {**dict(q=q, out=None), **bad}
+        with pytest.raises(AssertionError):
+            mi.attend_pages(a["q"], kv, scale, plan, out=a["out"])
+    x = torch.zeros(2, 10)
+    for bad in (dict(x=x.half()), dict(x=x[0]), dict(x=x.t()), dict(t=torch.zeros(2, dtype=torch.int32)), dict(t=torch.zeros(3, dtype=torch.long)), dict(top=11), dict(top=-1)):
+        a = {**dict(x=x, t=None, top=1), **bad}
+        with pytest.raises(AssertionError):
+            mi.token_scores(a["x"], a["t"], top=a["top"])
+
+
+def test_status_says_why():
+    from mistral_inference_b200.paged import check_status
+    check_status(torch.zeros(1, dtype=torch.int32))
+    for code, word in ((1, "twice"), (2, "length"), (3, "room"), (4, "free"), (16, "wait")):
+        with pytest.raises(_abi_paged.Mb200Error, match=word):
+            check_status(torch.tensor([code], dtype=torch.int32))
+
+
+def test_the_restatement_rounds_like_torch():
+    """The oracle's e4m3 against torch's own conversion, over every binade and the middles between codes."""
+    g = torch.Generator().manual_seed(0)
+    x = (torch.randn(20000, generator=g) * torch.exp2(torch.randint(-12, 7, (20000,), generator=g).float())).clamp(-448, 448)
+    grid = U.e4m3_grid().float()
+    x = torch.cat([x, grid, -grid, (grid[1:] + grid[:-1]) / 2])
+    assert torch.equal(U.to_e4m3(x.double()).float(), x.to(U.E4M3).float())
+
+
+def test_host_tables_truncate_undoes_extend():
+    t = U.HostTables(3, 8, 20)
+    t.extend([100, 0, 65])
+    before = (str(t.table), list(t.lens), list(t.free), t.n_free)
+    t.extend([64, 1, 200])
+    t.truncate([100, 0, 65])
+    assert before == (str(t.table), t.lens, t.free, t.n_free)
+
+
+def test_declarations_of_this_abi_version():
+    """A change of the declarations takes a new version, so that a library built before it is refused."""
+    code = re.sub(r"/\*.*?\*/", " ", HEADER.read_text(), flags=re.S)
+    assert zlib.crc32(" ".join(code.split()).encode()) == 2367187686, "raise the ABI version with this change"
