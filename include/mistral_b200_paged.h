@@ -50,7 +50,7 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
                    int64_t head_dim, int64_t window, float softmax_scale, void* stream);
 
 /* Scores of the rows of logits [T, vocab] (dtype 0: bf16, 1: fp32; rows ld elements apart), each output NULL or
- *   logprob [T]: log_softmax(logits[t])[target[t]], rows with target[t] < 0 untouched, NaN for a target past the vocabulary
+ *   logprob [T]: log_softmax(logits[t])[target[t]], 0 where target[t] < 0, NaN for a target past the vocabulary
  *   entropy [T]: of softmax(logits[t]), in nats
  *   top_ids [T, top] int64, top_logprobs [T, top]: the largest logits, the lowest index first where they are equal, NaN before all, and their log-probabilities
  * all sums in fp32.  An entry of -infinity weighs nothing; a row of nothing else, or with NaN or +infinity, scores NaN.  top <= 64, T <= 65535.

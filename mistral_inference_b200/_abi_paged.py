@@ -5,6 +5,7 @@ in-tree by `build.build_paged()` (a fresh checkout has no binaries), a failing c
 """
 import contextlib
 import ctypes
+import functools
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 from typing import Optional, Tuple
 
@@ -18,6 +19,7 @@ PAGE = 64       # tokens of a page
 HEAD_DIM = 128
 MAX_REQUESTS = 4000
 MAX_TOP = 64
+MAX_SCORE_ROWS = 65535  # rows of a call
 _lib: Optional[ctypes.CDLL] = None
 
 P, I = c_void_p, c_int64
@@ -112,12 +114,17 @@ def attn_pages(q, kv, scale, plan, out, n_heads: int, window: int, softmax_scale
                                     _stream()), "mbp_attn_pages")
 
 
+@functools.lru_cache(maxsize=256)
+def _scores_scratch(T: int, V: int, top: int) -> int:
+    need = c_int64(0)
+    _check(lib().mbp_token_scores_sizes(T, V, top, ctypes.byref(need)), "mbp_token_scores_sizes")
+    return need.value
+
+
 def token_scores(logits, targets, logprob, entropy, top_ids, top_logprobs, top: int) -> None:
     T, V = logits.shape
     dev = logits.device
-    need = c_int64(0)
     with _on(dev):
-        _check(lib().mbp_token_scores_sizes(T, V, top, ctypes.byref(need)), "mbp_token_scores_sizes")
-        scratch = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        scratch = torch.empty(_scores_scratch(T, V, top), dtype=torch.uint8, device=dev)
         _check(lib().mbp_token_scores(logits.data_ptr(), logits.stride(0) if T > 1 else V, 1 if logits.dtype == torch.float32 else 0, _ptr(targets, dev), _ptr(logprob, dev), _ptr(entropy, dev),
                                       _ptr(top_ids, dev), _ptr(top_logprobs, dev), T, V, top, scratch.data_ptr(), _stream()), "mbp_token_scores")

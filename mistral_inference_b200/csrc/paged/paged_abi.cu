@@ -43,6 +43,42 @@ static int plan_state(PlanParams& p, const char* what, int32_t* table, int32_t* 
   p.N = (int)n_pages;
   return MB200_OK;
 }
+// Entries of a segment: a multiple of 16 bytes a thread, no more than shared memory holds, and of the numbers of segments a row the one whose rounds over the CTAs that run at once cost
+// least, a segment costing its entries and some 4096 more (251 rows of 50257: 5 segments, 20 us; the fewest, 4, leave a third round half empty: 28)
+static int64_t score_segment_length(int64_t T, int64_t vocab, int64_t size) {
+  const int64_t step = TS_THREADS * (16 / size), most = TS_BYTES / size, sms = device_info::sm_count(), room = (sms > 0 ? sms : 148) * TS_CTAS;
+  const int64_t fewest = (vocab + most - 1) / most;
+  int64_t best = most, least = 0;
+  for (int64_t n = fewest; n <= (fewest > TS_JOIN_SEGMENTS ? fewest : TS_JOIN_SEGMENTS); ++n) {
+    const int64_t length = ((vocab + n - 1) / n + step - 1) / step * step, cost = (T * ((vocab + length - 1) / length) + room - 1) / room * (length + 4096);
+    if (least == 0 || cost < least) {
+      least = cost;
+      best = length;
+    }
+  }
+  return best;
+}
+
+template <typename ST>
+static int launch_token_scores(const TokenScoresParams& p, cudaStream_t st) {
+  const int64_t items = (int64_t)p.T * p.segments, room = (int64_t)device_info::sm_count() * TS_CTAS;
+  const dim3 grid((unsigned)(items < room ? items : room));
+  const size_t smem = (size_t)p.length * sizeof(ST);
+  const uint64_t apart = (uintptr_t)p.logits | (p.T > 1 ? (uint64_t)p.ld * sizeof(ST) : 0);
+  auto go = [&](auto kernel, cudaError_t allowed) {
+    MB_CHECK_CUDA(allowed);
+    MB_CHECK_CUDA(launch_pdl(kernel, grid, dim3(TS_THREADS), smem, st, p));
+    return MB200_OK;
+  };
+  const int rc = apart % 16 == 0  ? go(token_scores_segment_kernel<ST, 16>, device_info::allow_shared<token_scores_segment_kernel<ST, 16>>(TS_BYTES))
+                 : apart % 4 == 0 ? go(token_scores_segment_kernel<ST, 4>, device_info::allow_shared<token_scores_segment_kernel<ST, 4>>(TS_BYTES))
+                                  : go(token_scores_segment_kernel<ST, 0>, device_info::allow_shared<token_scores_segment_kernel<ST, 0>>(TS_BYTES));
+  if (rc) return rc;
+  const size_t lists = p.segments <= TS_JOIN_SEGMENTS ? sizeof(unsigned long long) * (size_t)p.segments * p.top : 0;
+  MB_CHECK_CUDA(launch_pdl(token_scores_join_kernel<ST>, dim3((unsigned)p.T), dim3(32), lists, st, p));
+  return MB200_OK;
+}
+
 }  // namespace mb200
 
 using namespace mb200;
@@ -170,8 +206,8 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
 int mbp_token_scores_sizes(int64_t T, int64_t vocab, int64_t top, int64_t* bytes) {
   MB_CHECK_ARG(T >= 0 && vocab >= 1 && vocab <= MBP_MAX_VOCAB && top >= 0 && top <= TS_MAX_TOP && top <= vocab && bytes, "token_scores: T=%lld vocab=%lld top=%lld (at most %d)", (long long)T,
                (long long)vocab, (long long)top, TS_MAX_TOP);
-  const int64_t slices = (vocab + TS_SLICE - 1) / TS_SLICE;
-  *bytes = T * slices * (8 * top + 12);
+  const int64_t segments = vocab / (TS_BYTES / 4) + 1 > TS_JOIN_SEGMENTS + 1 ? vocab / (TS_BYTES / 4) + 1 : TS_JOIN_SEGMENTS + 1;  // at most
+  *bytes = T * segments * (8 * top + 12);
   return MB200_OK;
 }
 
@@ -181,6 +217,7 @@ int mbp_token_scores(const void* logits, int64_t ld, int dtype, const int64_t* t
   int rc = mbp_token_scores_sizes(T, vocab, top, &bytes);
   if (rc) return rc;
   MB_CHECK_ARG(logits && scratch && (uintptr_t)scratch % 8 == 0 && (logprob == nullptr || target) && (top == 0 || (top_ids && top_logprobs)), "token_scores: null pointer");
+  MB_CHECK_ARG((uintptr_t)logits % (dtype == 0 ? 2 : 4) == 0, "token_scores: logits that are not aligned to their type");
   MB_CHECK_ARG(ld >= vocab && (dtype == 0 || dtype == 1), "token_scores: rows %lld elements apart of %lld, dtype %d", (long long)ld, (long long)vocab, dtype);
   MB_CHECK_ARG(T <= 65535, "token_scores: %lld rows (at most 65535)", (long long)T);
   if (T == 0) return MB200_OK;
@@ -190,24 +227,17 @@ int mbp_token_scores(const void* logits, int64_t ld, int dtype, const int64_t* t
   p.target = target;
   p.T = (int)T;
   p.V = (int)vocab;
-  p.slices = (int)((vocab + TS_SLICE - 1) / TS_SLICE);
+  p.length = (int)score_segment_length(T, vocab, dtype == 0 ? 2 : 4);
+  p.segments = (int)((vocab + p.length - 1) / p.length);
   p.top = (int)top;
   p.best = (unsigned long long*)scratch;
-  p.sums = (float*)(p.best + T * p.slices * top);
+  p.sums = (float*)(p.best + T * p.segments * top);
   p.logprob = logprob;
   p.entropy = entropy;
   p.top_ids = top_ids;
   p.top_logprobs = top_logprobs;
-  const dim3 grid((unsigned)p.slices, (unsigned)T);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == 0) {
-    MB_CHECK_CUDA(launch_pdl(token_scores_slice_kernel<bf16>, grid, dim3(TS_THREADS), 0, st, p));
-    MB_CHECK_CUDA(launch_pdl(token_scores_join_kernel<bf16>, dim3((unsigned)ceil_div(T, TS_JOIN_ROWS)), dim3(TS_JOIN_ROWS * 32), 0, st, p));
-  } else {
-    MB_CHECK_CUDA(launch_pdl(token_scores_slice_kernel<float>, grid, dim3(TS_THREADS), 0, st, p));
-    MB_CHECK_CUDA(launch_pdl(token_scores_join_kernel<float>, dim3((unsigned)ceil_div(T, TS_JOIN_ROWS)), dim3(TS_JOIN_ROWS * 32), 0, st, p));
-  }
-  return MB200_OK;
+  return dtype == 0 ? launch_token_scores<bf16>(p, st) : launch_token_scores<float>(p, st);
 }
 
 }  // extern "C"

@@ -23,7 +23,6 @@ namespace mb200 {
 constexpr int PA_STAGES = 3, PA_KEYS = 2 * PG_TOKENS, PA_STAGE_BYTES = 4 * PG_BYTES;
 constexpr int PA_THREADS = 192, PA_SOFT = 128;
 constexpr int PA_MAX_SPLITS = 16;
-constexpr uint32_t PA_SPINS = 1u << 22;  // polls of a wait before it gives up (seconds)
 enum { PA_GAVE_UP = 16 };                // status: a wait ran out; the call's results are NaN
 
 struct PagedAttnParams {
@@ -69,25 +68,6 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16_nowait(uint32_t taddr, uint32
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
         "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
-}
-__device__ __forceinline__ float warp_max_sync(float v) {  // (NaN does not count)
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float exp2_ftz(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// false: the wait ran out, or another thread's has
-__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-  for (uint32_t i = 0; i < PA_SPINS; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 63u && *gave_up) return false;
-  }
-  *gave_up = 1;
-  return false;
 }
 // barrier of the PA_SOFT softmax threads; true if any of them says so
 __device__ __forceinline__ bool soft_sync_or(bool v) {
@@ -199,7 +179,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       const int page0 = __shfl_sync(0xffffffffu, page, src), page1 = __shfl_sync(0xffffffffu, page, src + 1);
       const float ks0 = __shfl_sync(0xffffffffu, ks, src), ks1 = __shfl_sync(0xffffffffu, ks, src + 1);
       const float vs0 = __shfl_sync(0xffffffffu, vs, src), vs1 = __shfl_sync(0xffffffffu, vs, src + 1);
-      if (!__all_sync(0xffffffffu, pa_wait(&kv_empty[st], ((t / PA_STAGES) & 1) ^ 1, &gave_up))) break;
+      if (!__all_sync(0xffffffffu, bounded_wait(&kv_empty[st], ((t / PA_STAGES) & 1) ^ 1, &gave_up))) break;
       if (lane == 0) {
         page_scale[st][0] = ks0;
         page_scale[st][1] = ks1;
@@ -217,11 +197,11 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
     }
   } else if (warp == 5) {
     // ================= MMA issuer =================
-    bool ok = tiles == 0 || pa_wait(&q_full, 0, &gave_up);
+    bool ok = tiles == 0 || bounded_wait(&q_full, 0, &gave_up);
     const uint32_t q_desc = umma_desc_lo(smem_u32(sQ));
     auto issue_s = [&](int t) {
       const int st = t % PA_STAGES;
-      ok = ok && pa_wait(&kv_full[st], (t / PA_STAGES) & 1, &gave_up);
+      ok = ok && bounded_wait(&kv_full[st], (t / PA_STAGES) & 1, &gave_up);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
@@ -236,7 +216,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
     if (tiles > 0) issue_s(0);
     if (tiles > 1) issue_s(1);
     for (int t = 0; t < tiles && ok; ++t) {
-      ok = pa_wait(&p_full, t & 1, &gave_up);
+      ok = bounded_wait(&p_full, t & 1, &gave_up);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -264,7 +244,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       uint2 u = make_uint2(0u, 0u);
       if (q < nq) u = *reinterpret_cast<const uint2*>(p.q + (int64_t)(tok0 + q / R) * p.ldq + (int64_t)(g * R + q % R) * kHeadDim + lane * 4);
       const float x[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
-      const int e = e4m3_exponent(warp_max(fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])))));
+      const int e = e4m3_exponent(warp_max_f32(fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])))));
       const float inv = pow2i(-e);
       float y[4];
 #pragma unroll
@@ -289,7 +269,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
     float vs0 = 0.f, vs1 = 0.f;  // value scales of the tile before
     bool two_before = false, ok = true;
     auto add_values = [&](int t) {  // the sums of tile t, relative to m as it stood then
-      ok = ok && pa_wait(&o_full, t & 1, &gave_up);
+      ok = ok && bounded_wait(&o_full, t & 1, &gave_up);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
@@ -313,7 +293,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       const bool here = first + 2 * t + half < last;            // the tile's second page may be none
       const bool seen = here && key >= lo && key < hi;          // by any query
       float s[NQ];
-      ok = ok && pa_wait(&kv_full[st], (t / PA_STAGES) & 1, &gave_up) && pa_wait(&s_full[t & 1], (t >> 1) & 1, &gave_up);
+      ok = ok && bounded_wait(&kv_full[st], (t / PA_STAGES) & 1, &gave_up) && bounded_wait(&s_full[t & 1], (t >> 1) & 1, &gave_up);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
@@ -344,7 +324,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       if (ok) {
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          const float w = warp_max_sync(s[q]);
+          const float w = warp_max_f32(s[q]);
           if (lane == 0) warp_most[t & 1][q][warp] = w;
         }
       }

@@ -40,6 +40,27 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {  // exact: every
 // x times a power of two; not a number where x is infinite (e4m3 has no infinity, and the largest code would pass for a number)
 __device__ __forceinline__ float scaled(float x, float inv) { return fmaf(x, inv, x - x); }
 
+__device__ __forceinline__ float warp_max_f32(float v) {  // (NaN does not count)
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr uint32_t PG_SPINS = 1u << 22;  // polls of a wait before it gives up (seconds)
+// false: the wait ran out, or another thread's has
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+  for (uint32_t i = 0; i < PG_SPINS; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 63u && *gave_up) return false;
+  }
+  *gave_up = 1;
+  return false;
+}
 // largest i in [0, n) with start[i] <= x, start ascending, start[0] <= x
 template <typename F>
 __device__ __forceinline__ int last_not_above(int n, int x, F start) {

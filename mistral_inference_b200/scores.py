@@ -26,12 +26,13 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, t
     assert logits.stride(1) == 1 and (T <= 1 or logits.stride(0) >= V), "rows of logits are contiguous and do not overlap"
     assert targets is None or (targets.dtype == torch.long and targets.shape == (T,)), "targets: one int64 a row"
     assert 0 <= top <= min(_abi_paged.MAX_TOP, V), f"{top} alternatives (at most {_abi_paged.MAX_TOP}, and no more than tokens)"
-    new = dict(device=logits.device)
-    out = TokenScores(torch.zeros(T, dtype=torch.float32, **new) if targets is not None else None, torch.empty(T, dtype=torch.float32, **new),
-                      torch.empty(T, top, dtype=torch.long, **new), torch.empty(T, top, dtype=torch.float32, **new))
-    rows = 65535  # of a call
-    for r in range(0, T, rows):
-        cut = slice(r, r + rows)
-        part = [None if t is None else t[cut] for t in (targets, out.logprob, out.entropy, out.top_ids, out.top_logprobs)]
-        _abi_paged.token_scores(logits[cut], *part, top)
+    dev = logits.device
+    out = TokenScores(torch.empty(T, dtype=torch.float32, device=dev) if targets is not None else None, torch.empty(T, dtype=torch.float32, device=dev),
+                      torch.empty(T, top, dtype=torch.long, device=dev), torch.empty(T, top, dtype=torch.float32, device=dev))
+    if 0 < T <= _abi_paged.MAX_SCORE_ROWS:
+        _abi_paged.token_scores(logits, targets, out.logprob, out.entropy, out.top_ids, out.top_logprobs, top)
+    else:
+        for r in range(0, T, _abi_paged.MAX_SCORE_ROWS):
+            cut = slice(r, r + _abi_paged.MAX_SCORE_ROWS)
+            _abi_paged.token_scores(logits[cut], *(None if t is None else t[cut] for t in (targets, out.logprob, out.entropy, out.top_ids, out.top_logprobs)), top)
     return out

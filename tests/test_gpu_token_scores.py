@@ -106,6 +106,19 @@ def test_rows_of_wider_ones_and_targets_past_the_vocabulary():
     assert torch.equal(s.logprob[:2], want.logprob[:2]) and s.logprob[2].isnan() and s.logprob[3] == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("first,pitch", [(0, 40008), (4, 40004), (1, 40008), (0, 40001), (2, 40002)])
+def test_rows_that_begin_anywhere(dtype, first, pitch):
+    """The same bits wherever a row lies: 16-byte copies, 4-byte copies, single entries."""
+    wide = logits_of(3, pitch, 8, dtype=dtype).to(DEV)
+    x = wide[:, first: first + 40000]
+    t = torch.tensor([5, 39999, 77], device=DEV)
+    s, want = mi.token_scores(x, t, top=20), mi.token_scores(x.contiguous(), t, top=20)
+    check(x.cpu(), t.cpu(), 20)
+    for a, b in zip((s.logprob, s.entropy, s.top_ids, s.top_logprobs), (want.logprob, want.entropy, want.top_ids, want.top_logprobs)):
+        assert torch.equal(a, b)
+
+
 def test_no_rows():
     s = mi.token_scores(torch.empty(0, 100, device=DEV), torch.empty(0, dtype=torch.long, device=DEV), top=3)
     assert s.logprob.shape == (0,) and s.top_ids.shape == (0, 3)
