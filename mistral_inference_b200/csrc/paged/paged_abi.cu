@@ -166,7 +166,7 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
   if (longest > T) longest = T;
   // columns of a query tile: the fewest that hold a request's tokens, 32 at most
   const int64_t want = longest * rep;
-  const int nq = want <= 8 ? 8 : want <= 16 ? 16 : 32;
+  const int nq = want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 ? 16 : 32;
   const int tokens = nq / rep;
   const int64_t q_tiles = (longest + tokens - 1) / tokens;
   MB_CHECK_ARG(n_kv_heads * q_tiles <= 65535, "attn_pages: %lld tiles of queries", (long long)(n_kv_heads * q_tiles));
@@ -200,7 +200,7 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
   int splits = 1;
   while (splits < PA_MAX_SPLITS && pairs * splits * 2 <= room && keys >= (int64_t)splits * 4 * PA_KEYS) splits *= 2;
   cudaStream_t st = (cudaStream_t)stream;
-  return nq == 8 ? launch_paged_attn<8>(p, map, q_tiles, splits, st) : nq == 16 ? launch_paged_attn<16>(p, map, q_tiles, splits, st) : launch_paged_attn<32>(p, map, q_tiles, splits, st);
+  return nq == 4 ? launch_paged_attn<4>(p, map, q_tiles, splits, st) : nq == 8 ? launch_paged_attn<8>(p, map, q_tiles, splits, st) : nq == 16 ? launch_paged_attn<16>(p, map, q_tiles, splits, st) : launch_paged_attn<32>(p, map, q_tiles, splits, st);
 }
 
 int mbp_token_scores_sizes(int64_t T, int64_t vocab, int64_t top, int64_t* bytes) {

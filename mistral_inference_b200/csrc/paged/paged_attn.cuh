@@ -9,20 +9,24 @@
 // the keys' on the scores, the values' on each page's own accumulator.
 //
 // Keys are the MMA's 128 rows (S^T = K Q^T) and so are the values' dimensions (O^T = V^T P^T, V as it lies in the page: MN-major), the hi and lo parts of up to NQ
-// query columns (tokens x heads of one key/value head) its N = 2 NQ columns.  Memory bounds it: 256 bytes a key and key/value head, where converting them to 16 bits
-// on the way to mma.sync fragments would take more issue slots than the bytes take time.  CTA = (a range of pages, key/value head and tile of queries, request),
-// the ranges of one request's head are a cluster and are merged through distributed shared memory: one launch, no scratch, the same order every time.
-//   warp 4     TMA producer: tiles of two pages (8 KB of keys and of values each) into a ring of PA_STAGES x 32 KB
-//   warp 5     MMA issuer: S(0) S(1) | PV(t) S(t + 2) ...
-//   warps 0-3  a thread per key: its scores -> maximum (over the CTA) -> weights -> shared memory; then, a thread per dimension, the values' sums of the tile before
+// query columns (tokens x heads of one key/value head) its columns.  Memory bounds it: 256 bytes a key and key/value head, where converting them to 16 bits on the way to
+// mma.sync fragments would take more issue slots than the bytes take time.  CTA = (a range of pages, key/value head and tile of queries, request); the ranges of one
+// request's head are a cluster and are merged through distributed shared memory: one launch, no scratch, the same order every time.
+//   warps 0-3, 4-7  half of the query columns each, a thread per key: scores -> maximum (over the four warps) -> weights -> shared memory; then, a thread per
+//                   dimension, the values' sums of the tile before
+//   warp 8          TMA producer: tiles of two pages (8 KB of keys and of values each) into a ring of PA_STAGES x 32 KB
+//   warp 9          MMA issuer: S(0) S(1) | PV(t) S(t + 2) ...
+// What a tile costs is the chain scores -> maximum -> weights -> sums of few warps, some 600 clocks where its bytes take 1200 of an SM.  (Four warps with eight columns each, half
+// of them empty for groups of four heads: 3200 clocks a tile, 32 requests of ~1100 tokens 21.0 us.)
 #pragma once
 #include "paged_common.cuh"
 
 namespace mb200 {
 
 constexpr int PA_STAGES = 3, PA_KEYS = 2 * PG_TOKENS, PA_STAGE_BYTES = 4 * PG_BYTES;
-constexpr int PA_THREADS = 192, PA_SOFT = 128;
+constexpr int PA_SOFT_WARPS = 8, PA_THREADS = 32 * (PA_SOFT_WARPS + 2);
 constexpr int PA_MAX_SPLITS = 16;
+constexpr float PA_NOTHING = -1.0e30f;   // the maximum of no score
 enum { PA_GAVE_UP = 16 };                // status: a wait ran out; the call's results are NaN
 
 struct PagedAttnParams {
@@ -36,16 +40,19 @@ struct PagedAttnParams {
   float scale_log2;
 };
 
+// NQ query columns, Q of them a half of the softmax warps; column c of the MMA: half h has hi parts at h * 2 Q, lo parts at h * 2 Q + Q
 template <int NQ>
 struct PaCfg {
-  static constexpr int kColBytes = 2 * NQ * 128;  // Q or one P tile: [2 NQ columns][128 bytes], 128B-swizzled
+  static constexpr int Q = NQ / 2;
+  static constexpr int N = 2 * NQ < 16 ? 16 : 2 * NQ;      // (16 at least; columns that nobody reads hold anything)
+  static constexpr int kColBytes = N * 128;                // Q or one P tile: [N columns][128 bytes], 128B-swizzled
   static constexpr int kRing = PA_STAGES * PA_STAGE_BYTES;
-  static constexpr int kMerge = NQ * (kHeadDim + 2) * 4;  // this split's result, over the ring once that is used up
-  static constexpr int kSmem = 1024 + kRing + 3 * kColBytes + 1024;
-  static constexpr int kTmemCols = 8 * NQ;  // two S tiles, the two pages' O
+  static constexpr int kMerge = NQ * (kHeadDim + 2) * 4;   // this split's result, over the ring once that is used up
+  static constexpr int kSmem = 1024 + kRing + 3 * kColBytes;
+  static constexpr int kTmemCols = 4 * N;                  // two S tiles, the two pages' O
   static_assert(kMerge <= kRing && kTmemCols <= 512, "fits");
   // D = fp32, A = B = e4m3, N >> 3 at bit 17, M >> 4 at bit 24; values: A is MN-major (bit 15)
-  static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(2 * NQ >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   static constexpr uint32_t kIdescO = kIdescS | (1u << 15);
 };
 
@@ -62,27 +69,53 @@ __device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint32_t a, uint32_t 
       "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(UMMA_DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_32x32b_x16_nowait(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
+// COLS consecutive columns of this warp's 32 lanes
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[COLS]) {
+  static_assert(COLS == 4 || COLS == 8 || COLS == 16 || COLS == 32, "");
+  if constexpr (COLS == 4)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(taddr));
+  else if constexpr (COLS == 8)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+  else if constexpr (COLS == 16)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+          "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+  else
+    tmem_ld_32x32b_x32_nowait(taddr, v);
 }
-// barrier of the PA_SOFT softmax threads; true if any of them says so
-__device__ __forceinline__ bool soft_sync_or(bool v) {
+// barrier of the 128 threads of a half; true if any of them says so
+__device__ __forceinline__ bool half_sync_or(int half, bool v) {
   uint32_t r;
   asm volatile(
       "{\n"
-      ".reg .pred p, q;\n"
+      ".reg .pred p, q, h;\n"
       "setp.ne.u32 p, %1, 0;\n"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n"
+      "setp.ne.u32 h, %2, 0;\n"
+      "@h barrier.cta.red.or.pred q, 2, 128, p;\n"
+      "@!h barrier.cta.red.or.pred q, 1, 128, p;\n"
       "selp.u32 %0, 1, 0, q;\n"
       "}\n"
       : "=r"(r)
-      : "r"((uint32_t)v)
+      : "r"((uint32_t)v), "r"(half)
       : "memory");
   return r != 0;
+}
+// two weights times 256 as codes: hi in the lower half-word, lo in the upper.  (Through fp16, whose 11 bits hold more than the two parts do.)
+__device__ __forceinline__ uint32_t weight_parts(float w0, float w1) {
+  uint32_t w, h, r;
+  uint16_t hi, lo;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(w1), "f"(w0));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(hi) : "r"(w));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(hi));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(h));
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0x4c004c00u));  // times 16
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(lo) : "r"(r));
+  return (uint32_t)hi | (uint32_t)lo << 16;
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
@@ -95,15 +128,13 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   return r;
 }
 
-// Columns go in groups of 8 queries: 8 columns of hi, 8 of lo.  Byte `k` of column (query q, part): its 128 bytes are one row of a 128B-swizzled K-major tile.
-__device__ __forceinline__ uint32_t pa_col(int q, int part, int k) {
-  const int r = q & 7;
-  return (uint32_t)((((q >> 3) * 2 + part) << 10) + (r << 7) + (((k >> 4) ^ r) << 4) + (k & 15));
-}
+// Byte k of column c: its 128 bytes are one row of a 128B-swizzled K-major tile
+__device__ __forceinline__ uint32_t pa_col(int c, int k) { return (uint32_t)(((c >> 3) << 10) + ((c & 7) << 7) + (((k >> 4) ^ (c & 7)) << 4) + (k & 15)); }
 
 template <int NQ>
 __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kernel(const __grid_constant__ CUtensorMap map_kv, const PagedAttnParams p) {
   using Cfg = PaCfg<NQ>;
+  constexpr int Q = Cfg::Q, N = Cfg::N;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem + Cfg::kRing;
@@ -122,31 +153,31 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
   pdl_trigger();
   if (tid == 0) {
     for (int i = 0; i < PA_STAGES; ++i) {
-      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_full[i], 2);  // the copies' arrival and the scales'
       mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(&q_full, 4);
+    mbar_init(&q_full, PA_SOFT_WARPS);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
-    mbar_init(&p_full, 4);
+    mbar_init(&p_full, PA_SOFT_WARPS);
     mbar_init(&o_full, 1);
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
   }
-  if (warp == 5) tmem_alloc(&tmem_slot, Cfg::kTmemCols);
+  if (warp == PA_SOFT_WARPS + 1) tmem_alloc(&tmem_slot, Cfg::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_wait();
 
-  const int t_first = p.q_start[b], n_all = p.q_start[b + 1] - t_first, past = p.seqpos[b];
+  const int t_first = p.q_start[b], n_all = p.q_start[b + 1] - t_first, past = p.seqpos[b], row = p.rows[b];
   const int i0 = qt * p.tokens;
   const int n = t_first < 0 || n_all < 0 || n_all > p.T - t_first || past < 0 ? 0 : min(p.tokens, n_all - i0);  // tokens of this tile
   if (n <= 0) {  // the whole cluster alike
     __syncthreads();
-    if (warp == 5) tmem_dealloc(tmem, Cfg::kTmemCols);
+    if (warp == PA_SOFT_WARPS + 1) tmem_dealloc(tmem, Cfg::kTmemCols);
     return;
   }
   const int nq = n * R, tok0 = t_first + i0;
@@ -157,15 +188,15 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
   const int first = page_lo + min(split * per * 2, n_pages), last = page_lo + min((split + 1) * per * 2, n_pages);  // this split's pages
   const int tiles = (last - first + 1) / 2;
 
-  float o[NQ], m[NQ], l[NQ];
-  if (warp == 4) {
+  float o[Q], m[Q], l[Q];
+  const int half = warp >> 2, key_at = tid & 127;  // of the softmax threads
+  if (warp == PA_SOFT_WARPS) {
     // ================= producer =================
-    const int row = p.rows[b];
     const bool row_ok = row >= 0 && row < p.R;
     int page = 0;
     float ks = 0.f, vs = 0.f;
     for (int t = 0; t < tiles; ++t) {
-      if ((t & 15) == 0) {  // the next 32 pages and their scales, one a lane
+      if ((t & 15) == 0) {  // the next 32 pages, one a lane; their scales arrive while the first tile's bytes do
         const int at = first + 2 * t + lane;
         page = -1;
         if (at < last && row_ok && at < p.P) page = p.table[(int64_t)row * p.P + at];
@@ -177,14 +208,8 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       }
       const int st = t % PA_STAGES, two = first + 2 * t + 1 < last, src = (2 * t) & 31;
       const int page0 = __shfl_sync(0xffffffffu, page, src), page1 = __shfl_sync(0xffffffffu, page, src + 1);
-      const float ks0 = __shfl_sync(0xffffffffu, ks, src), ks1 = __shfl_sync(0xffffffffu, ks, src + 1);
-      const float vs0 = __shfl_sync(0xffffffffu, vs, src), vs1 = __shfl_sync(0xffffffffu, vs, src + 1);
       if (!__all_sync(0xffffffffu, bounded_wait(&kv_empty[st], ((t / PA_STAGES) & 1) ^ 1, &gave_up))) break;
       if (lane == 0) {
-        page_scale[st][0] = ks0;
-        page_scale[st][1] = ks1;
-        page_scale[st][2] = vs0;
-        page_scale[st][3] = vs1;
         mbar_arrive_expect_tx(&kv_full[st], (two ? 4 : 2) * PG_BYTES);
         uint8_t* dst = smem + st * PA_STAGE_BYTES;
         const int r0 = (page0 * p.KV + g) * 2 * PG_TOKENS, r1 = (page1 * p.KV + g) * 2 * PG_TOKENS;
@@ -193,9 +218,18 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
         tma_load_2d(dst + 2 * PG_BYTES, &map_kv, &kv_full[st], 0, r0 + PG_TOKENS);
         if (two) tma_load_2d(dst + 3 * PG_BYTES, &map_kv, &kv_full[st], 0, r1 + PG_TOKENS);
       }
+      const float ks0 = __shfl_sync(0xffffffffu, ks, src), ks1 = __shfl_sync(0xffffffffu, ks, src + 1);
+      const float vs0 = __shfl_sync(0xffffffffu, vs, src), vs1 = __shfl_sync(0xffffffffu, vs, src + 1);
+      if (lane == 0) {
+        page_scale[st][0] = ks0;
+        page_scale[st][1] = ks1;
+        page_scale[st][2] = vs0;
+        page_scale[st][3] = vs1;
+        mbar_arrive(&kv_full[st]);
+      }
       __syncwarp();
     }
-  } else if (warp == 5) {
+  } else if (warp == PA_SOFT_WARPS + 1) {
     // ================= MMA issuer =================
     bool ok = tiles == 0 || bounded_wait(&q_full, 0, &gave_up);
     const uint32_t q_desc = umma_desc_lo(smem_u32(sQ));
@@ -208,7 +242,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       const uint32_t k_desc = umma_desc_lo(smem_u32(smem + st * PA_STAGE_BYTES));
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_e4m3(tmem + (t & 1) * 2 * NQ, k_desc + k * 2, q_desc + k * 2, Cfg::kIdescS, k ? 1u : 0u);
+        for (int k = 0; k < 4; ++k) umma_e4m3(tmem + (t & 1) * N, k_desc + k * 2, q_desc + k * 2, Cfg::kIdescS, k ? 1u : 0u);
         umma_commit(&s_full[t & 1]);
       }
       __syncwarp();
@@ -225,11 +259,11 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       const uint32_t v_desc = umma_desc_lo(smem_u32(smem + st * PA_STAGE_BYTES + 2 * PG_BYTES)), p_desc = umma_desc_lo(smem_u32(sP + (t & 1) * Cfg::kColBytes));
       if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-          if (half == 0 || two) {
+        for (int h = 0; h < 2; ++h)
+          if (h == 0 || two) {
 #pragma unroll
             for (int k = 0; k < 2; ++k)  // 32 keys each: 4 KB of values, 32 bytes of a weights' column
-              umma_e4m3(tmem + 4 * NQ + half * 2 * NQ, v_desc + ((half * PG_BYTES + k * 4096) >> 4), p_desc + half * 4 + k * 2, Cfg::kIdescO, k ? 1u : 0u);
+              umma_e4m3(tmem + (2 + h) * N, v_desc + ((h * PG_BYTES + k * 4096) >> 4), p_desc + h * 4 + k * 2, Cfg::kIdescO, k ? 1u : 0u);
           }
         umma_commit(&o_full);
         umma_commit(&kv_empty[st]);
@@ -240,7 +274,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
   } else {
     // ================= softmax =================
     // queries -> hi and lo parts, a warp per row
-    for (int q = warp; q < NQ; q += 4) {
+    for (int q = warp; q < NQ; q += PA_SOFT_WARPS) {
       uint2 u = make_uint2(0u, 0u);
       if (q < nq) u = *reinterpret_cast<const uint2*>(p.q + (int64_t)(tok0 + q / R) * p.ldq + (int64_t)(g * R + q % R) * kHeadDim + lane * 4);
       const float x[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
@@ -252,116 +286,124 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       const uint32_t h0 = to_e4m3x2(y[0], y[1]), h1 = to_e4m3x2(y[2], y[3]);
       const float2 f0 = from_e4m3x2(h0), f1 = from_e4m3x2(h1);
       const uint32_t l0 = to_e4m3x2((y[0] - f0.x) * 16.f, (y[1] - f0.y) * 16.f), l1 = to_e4m3x2((y[2] - f1.x) * 16.f, (y[3] - f1.y) * 16.f);
-      *reinterpret_cast<uint32_t*>(sQ + pa_col(q, 0, lane * 4)) = h0 | h1 << 16;
-      *reinterpret_cast<uint32_t*>(sQ + pa_col(q, 1, lane * 4)) = l0 | l1 << 16;
+      const int c = q / Q * 2 * Q + q % Q;
+      *reinterpret_cast<uint32_t*>(sQ + pa_col(c, lane * 4)) = h0 | h1 << 16;
+      *reinterpret_cast<uint32_t*>(sQ + pa_col(c + Q, lane * 4)) = l0 | l1 << 16;
       if (lane == 0) q_scale[q] = pow2i(e) * p.scale_log2;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(&q_full);
+    bool ok = bounded_wait(&q_full, 0, &gave_up);  // q_scale of all rows
+    float qs[Q];
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      o[q] = l[q] = 0.f;
-      m[q] = -INFINITY;
+    for (int i = 0; i < Q; ++i) {
+      o[i] = l[i] = 0.f;
+      m[i] = PA_NOTHING;
+      qs[i] = q_scale[half * Q + i];
     }
-    soft_sync_or(false);  // q_scale of all rows
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 2 * Q;
     float vs0 = 0.f, vs1 = 0.f;  // value scales of the tile before
-    bool two_before = false, ok = true;
+    bool two_before = false;
     auto add_values = [&](int t) {  // the sums of tile t, relative to m as it stood then
       ok = ok && bounded_wait(&o_full, t & 1, &gave_up);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
+      uint32_t a[2 * Q], z[2 * Q];
+      tmem_ld_cols<2 * Q>(lanes + 2 * N, a);
+      if (two_before) tmem_ld_cols<2 * Q>(lanes + 3 * N, z);
+      tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < NQ / 8; ++c) {
-        uint32_t a[16], z[16];
-        tmem_ld_32x32b_x16_nowait(lanes + 4 * NQ + c * 16, a);
-        if (two_before) tmem_ld_32x32b_x16_nowait(lanes + 6 * NQ + c * 16, z);
-        tmem_wait_ld();
+      for (int i = 0; i < Q; ++i) o[i] = fmaf(fmaf(__uint_as_float(a[Q + i]), 0.0625f, __uint_as_float(a[i])), vs0, o[i]);
+      if (two_before) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[c * 8 + i] = fmaf(fmaf(__uint_as_float(a[8 + i]), 0.0625f, __uint_as_float(a[i])), vs0, o[c * 8 + i]);
-        if (two_before) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[c * 8 + i] = fmaf(fmaf(__uint_as_float(z[8 + i]), 0.0625f, __uint_as_float(z[i])), vs1, o[c * 8 + i]);
-        }
+        for (int i = 0; i < Q; ++i) o[i] = fmaf(fmaf(__uint_as_float(z[Q + i]), 0.0625f, __uint_as_float(z[i])), vs1, o[i]);
       }
     };
     for (int t = 0; t < tiles; ++t) {
       const int st = t % PA_STAGES;
-      const int half = tid >> 6, key = (first + 2 * t) * PG_TOKENS + tid;
-      const bool here = first + 2 * t + half < last;            // the tile's second page may be none
+      const int key0 = (first + 2 * t) * PG_TOKENS, key = key0 + key_at;
+      const bool here = first + 2 * t + (key_at >> 6) < last;   // the tile's second page may be none
       const bool seen = here && key >= lo && key < hi;          // by any query
-      float s[NQ];
+      const bool two = first + 2 * t + 1 < last;
+      const bool edge = !two || key0 + PA_KEYS > pos0 + 1 || (p.window > 0 && key0 < pos0 + n - p.window);  // (uniform) some query does not see some key
+      float s[Q];
       ok = ok && bounded_wait(&kv_full[st], (t / PA_STAGES) & 1, &gave_up) && bounded_wait(&s_full[t & 1], (t >> 1) & 1, &gave_up);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        const float ks = page_scale[st][half];
+        const float ks = page_scale[st][key_at >> 6];
+        uint32_t a[2 * Q];
+        tmem_ld_cols<2 * Q>(lanes + (t & 1) * N, a);
+        tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < NQ / 8; ++c) {
-          uint32_t a[16];
-          tmem_ld_32x32b_x16_nowait(lanes + (t & 1) * 2 * NQ + c * 16, a);
-          tmem_wait_ld();
+        for (int i = 0; i < Q; ++i) s[i] = fmaf(__uint_as_float(a[Q + i]), 0.0625f, __uint_as_float(a[i])) * (ks * qs[i]);
+        if (edge) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int q = c * 8 + i;
-            const float x = fmaf(__uint_as_float(a[8 + i]), 0.0625f, __uint_as_float(a[i])) * (ks * q_scale[q]);
+          for (int i = 0; i < Q; ++i) {
             bool sees = seen;
             if (n > 1) {  // (of one token every key in [lo, hi) is seen)
-              const int pos = pos0 + q / R;
+              const int pos = pos0 + (half * Q + i) / R;
               sees = seen && key <= pos && (p.window <= 0 || key > pos - p.window);
             }
-            s[q] = sees ? x : -INFINITY;
+            s[i] = sees ? s[i] : -INFINITY;
+          }
+          if (!seen && here && half == 0) {  // what this row holds must not reach the sums: 0 * NaN is not 0
+            uint4* v = reinterpret_cast<uint4*>(smem + st * PA_STAGE_BYTES + 2 * PG_BYTES + key_at * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
           }
         }
-      }
-      if (!seen && here) {  // what this row holds must not reach the sums: 0 * NaN is not 0
-        uint4* v = reinterpret_cast<uint4*>(smem + st * PA_STAGE_BYTES + 2 * PG_BYTES + tid * 128);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
-      }
-      if (ok) {
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          const float w = warp_max_f32(s[q]);
-          if (lane == 0) warp_most[t & 1][q][warp] = w;
+        for (int i = 0; i < Q; ++i) {
+          const float w = warp_max_f32(s[i]);
+          if (lane == 0) warp_most[t & 1][half * Q + i][warp & 3] = w;
         }
       }
-      if (soft_sync_or(!ok)) {
+      if (half_sync_or(half, !ok)) {
         ok = false;
         break;
       }
-      float alpha[NQ];
+      float top[Q];
+      bool grew = false;
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        const float4 w = *reinterpret_cast<const float4*>(warp_most[t & 1][half * Q + i]);
+        top[i] = fmaxf(fmaxf(m[i], fmaxf(w.x, w.y)), fmaxf(w.z, w.w));
+        grew |= top[i] > m[i];
+      }
+      float alpha[Q];
+      if (grew) {  // (the same in all threads of the half)
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          alpha[i] = exp2_ftz(m[i] - top[i]);
+          m[i] = top[i];
+          l[i] *= alpha[i];
+        }
+      }
       uint8_t* P = sP + (t & 1) * Cfg::kColBytes;
 #pragma unroll
-      for (int q = 0; q < NQ; q += 2) {
-        float e[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 w = *reinterpret_cast<const float4*>(warp_most[t & 1][q + i]);
-          const float top = fmaxf(fmaxf(m[q + i], fmaxf(w.x, w.y)), fmaxf(w.z, w.w));
-          const float ref = top == -INFINITY ? 0.f : top;  // (nothing seen yet weighs nothing)
-          alpha[q + i] = exp2_ftz(m[q + i] - ref);
-          m[q + i] = top;
-          e[i] = exp2_ftz(s[q + i] - ref + 8.f);  // weights times 256: the whole of e4m3's range
-          l[q + i] = fmaf(l[q + i], alpha[q + i], e[i]);
-        }
-        const uint32_t h = to_e4m3x2(e[0], e[1]);
-        const float2 f = from_e4m3x2(h);
-        const uint32_t r = to_e4m3x2((e[0] - f.x) * 16.f, (e[1] - f.y) * 16.f);
-        P[pa_col(q, 0, tid)] = (uint8_t)h;
-        P[pa_col(q + 1, 0, tid)] = (uint8_t)(h >> 8);
-        P[pa_col(q, 1, tid)] = (uint8_t)r;
-        P[pa_col(q + 1, 1, tid)] = (uint8_t)(r >> 8);
+      for (int i = 0; i < Q; i += 2) {
+        const float e0 = exp2_ftz(s[i] - m[i] + 8.f), e1 = exp2_ftz(s[i + 1] - m[i + 1] + 8.f);  // weights times 256: the whole of e4m3's range
+        l[i] += e0;
+        l[i + 1] += e1;
+        const uint32_t w = weight_parts(e0, e1);
+        const int c = half * 2 * Q + i;
+        P[pa_col(c, key_at)] = (uint8_t)w;
+        P[pa_col(c + 1, key_at)] = (uint8_t)(w >> 8);
+        P[pa_col(c + Q, key_at)] = (uint8_t)(w >> 16);
+        P[pa_col(c + Q + 1, key_at)] = (uint8_t)(w >> 24);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (t > 0) add_values(t - 1);
+      if (grew) {
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) o[q] *= alpha[q];
+        for (int i = 0; i < Q; ++i) o[i] *= alpha[i];
+      }
       vs0 = page_scale[st][2];
       vs1 = page_scale[st][3];
-      two_before = first + 2 * t + 1 < last;
+      two_before = two;
       tc_fence_before();
       __syncwarp();
       if (lane == 0 && ok) mbar_arrive(&p_full);
@@ -369,13 +411,13 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
     if (tiles > 0 && ok) add_values(tiles - 1);
     if (!__all_sync(0xffffffffu, ok)) {
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) o[q] = __int_as_float(0x7fffffff);
+      for (int i = 0; i < Q; ++i) o[i] = __int_as_float(0x7fffffff);
       if (lane == 0 && p.status) atomicOr(p.status, PA_GAVE_UP);
     }
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const float w = warp_sum(l[q]);
-      if (lane == 0) sums[warp][q] = w;
+    for (int i = 0; i < Q; ++i) {
+      const float w = warp_sum(l[i]);
+      if (lane == 0) sums[warp & 3][half * Q + i] = w;
     }
   }
   tc_fence_before();
@@ -385,41 +427,47 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       for (uint32_t k = 0; k < 2; ++k)
         for (uint32_t spin = 0; spin < 4096 && !mbar_try_wait(&kv_full[i], k); ++spin) {}
   }
-  if (warp == 5) {
+  if (warp == PA_SOFT_WARPS + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::kTmemCols);
   }
   // ================= merge the splits =================
   // this split: [q][maximum, sum, 128 sums] over the ring, which is used up
   float* mine = reinterpret_cast<float*>(smem);
-  if (warp < 4) {
+  if (warp < PA_SOFT_WARPS) {
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
+    for (int i = 0; i < Q; ++i) {
+      const int q = half * Q + i;
       if (q < nq) {
-        mine[q * (kHeadDim + 2) + 2 + tid] = o[q];
-        if (tid == 0) {
-          mine[q * (kHeadDim + 2)] = m[q];
-          mine[q * (kHeadDim + 2) + 1] = sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q];
+        const float sum = sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q];
+        if (splits == 1) {
+          p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + key_at] = __float2bfloat16_rn(sum == 0.f ? 0.f : o[i] / sum);
+        } else {
+          mine[q * (kHeadDim + 2) + 2 + key_at] = o[i];
+          if (key_at == 0) {
+            mine[q * (kHeadDim + 2)] = m[i];
+            mine[q * (kHeadDim + 2) + 1] = sum;
+          }
         }
       }
     }
   }
+  if (splits == 1) return;
   cluster_sync_all();
-  if (warp < 4) {
+  if (warp < PA_SOFT_WARPS) {
     const uint32_t base = smem_u32(mine);
-    for (int q = split; q < nq; q += splits) {
+    for (int q = split * 2 + half; q < nq; q += splits * 2) {
       const uint32_t at = base + q * (kHeadDim + 2) * 4;
-      float top = -INFINITY;
+      float top = PA_NOTHING;
       for (int r = 0; r < splits; ++r) top = fmaxf(top, ld_cluster_f32(map_to_rank(at, r)));
-      const float ref = top == -INFINITY ? 0.f : top;
       float sum = 0.f, acc = 0.f;
       for (int r = 0; r < splits; ++r) {
         const uint32_t from = map_to_rank(at, r);
-        const float f = exp2_ftz(ld_cluster_f32(from) - ref);  // (a split without a key: 0)
+        const float f = exp2_ftz(ld_cluster_f32(from) - top);  // (a split without a key: its sums are 0)
         sum = fmaf(f, ld_cluster_f32(from + 4), sum);
-        acc = fmaf(f, ld_cluster_f32(from + 8 + tid * 4), acc);
+        acc = fmaf(f, ld_cluster_f32(from + 8 + key_at * 4), acc);
       }
-      p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + tid] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
+      p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + key_at] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
     }
   }
   cluster_sync_all();  // nobody leaves while its results are read
