@@ -12,19 +12,19 @@
 // query columns (tokens x heads of one key/value head) its columns.  Memory bounds it: 256 bytes a key and key/value head, where converting them to 16 bits on the way to
 // mma.sync fragments would take more issue slots than the bytes take time.  CTA = (a range of pages, key/value head and tile of queries, request); the ranges of one
 // request's head are a cluster and are merged through distributed shared memory: one launch, no scratch, the same order every time.
-//   warps 0-3, 4-7  half of the query columns each, a thread per key: scores -> maximum (over the four warps) -> weights -> shared memory; then, a thread per
-//                   dimension, the values' sums of the tile before
-//   warp 8          TMA producer: tiles of two pages (8 KB of keys and of values each) into a ring of PA_STAGES x 32 KB
-//   warp 9          MMA issuer: S(0) S(1) | PV(t) S(t + 2) ...
+//   softmax   groups of four warps, a part of the query columns each, a thread per key: scores -> maximum (over the group) -> weights -> shared memory; then, a thread
+//             per dimension, the values' sums of the tile before
+//   producer  TMA: tiles of two pages (8 KB of keys and of values each) into a ring of PA_STAGES x 32 KB
+//   issuer    MMAs: S(0) S(1) | PV(t) S(t + 2) ...
 // What a tile costs is the chain scores -> maximum -> weights -> sums of few warps, some 600 clocks where its bytes take 1200 of an SM.  (Four warps with eight columns each, half
-// of them empty for groups of four heads: 3200 clocks a tile, 32 requests of ~1100 tokens 21.0 us.)
+// of them empty for groups of four heads: 3200 clocks a tile, 32 requests of ~1100 tokens 21.0 us.)  Keys and values in slots of their own, keys' freed after S(t): no faster
+// (44.8 us for 42.3 with four requests of 32500 tokens): what lies in flight is enough.
 #pragma once
 #include "paged_common.cuh"
 
 namespace mb200 {
 
 constexpr int PA_STAGES = 3, PA_KEYS = 2 * PG_TOKENS, PA_STAGE_BYTES = 4 * PG_BYTES;
-constexpr int PA_SOFT_WARPS = 8, PA_THREADS = 32 * (PA_SOFT_WARPS + 2);
 constexpr int PA_MAX_SPLITS = 16;
 constexpr float PA_NOTHING = -1.0e30f;   // the maximum of no score
 enum { PA_GAVE_UP = 16 };                // status: a wait ran out; the call's results are NaN
@@ -40,10 +40,11 @@ struct PagedAttnParams {
   float scale_log2;
 };
 
-// NQ query columns, Q of them a half of the softmax warps; column c of the MMA: half h has hi parts at h * 2 Q, lo parts at h * 2 Q + Q
+// NQ query columns, Q of them a group of softmax warps; column c of the MMA: group i has hi parts at i * 2 Q, lo parts at i * 2 Q + Q
 template <int NQ>
 struct PaCfg {
-  static constexpr int Q = NQ / 2;
+  static constexpr int G = NQ >= 32 ? 4 : 2, Q = NQ / G;   // (32 columns: two groups 31.1 us for the drafts of 8 requests, four 25.5)
+  static constexpr int kSoftWarps = 4 * G, kThreads = 32 * (kSoftWarps + 2), kResident = NQ >= 32 ? 1 : 2;
   static constexpr int N = 2 * NQ < 16 ? 16 : 2 * NQ;      // (16 at least; columns that nobody reads hold anything)
   static constexpr int kColBytes = N * 128;                // Q or one P tile: [N columns][128 bytes], 128B-swizzled
   static constexpr int kRing = PA_STAGES * PA_STAGE_BYTES;
@@ -88,22 +89,28 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[COLS]
   else
     tmem_ld_32x32b_x32_nowait(taddr, v);
 }
-// barrier of the 128 threads of a half; true if any of them says so
-__device__ __forceinline__ bool half_sync_or(int half, bool v) {
+// barrier of the 128 threads of a group; true if any of them says so
+template <int ID>
+__device__ __forceinline__ bool group_sync_or_id(bool v) {
   uint32_t r;
   asm volatile(
       "{\n"
-      ".reg .pred p, q, h;\n"
+      ".reg .pred p, q;\n"
       "setp.ne.u32 p, %1, 0;\n"
-      "setp.ne.u32 h, %2, 0;\n"
-      "@h barrier.cta.red.or.pred q, 2, 128, p;\n"
-      "@!h barrier.cta.red.or.pred q, 1, 128, p;\n"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n"
       "selp.u32 %0, 1, 0, q;\n"
       "}\n"
       : "=r"(r)
-      : "r"((uint32_t)v), "r"(half)
+      : "r"((uint32_t)v), "n"(ID)
       : "memory");
   return r != 0;
+}
+template <int G>
+__device__ __forceinline__ bool group_sync_or(int group, bool v) {
+  if (group == 0) return group_sync_or_id<1>(v);
+  if (G == 2 || group == 1) return group_sync_or_id<2>(v);
+  if (group == 2) return group_sync_or_id<3>(v);
+  return group_sync_or_id<4>(v);
 }
 // two weights times 256 as codes: hi in the lower half-word, lo in the upper.  (Through fp16, whose 11 bits hold more than the two parts do.)
 __device__ __forceinline__ uint32_t weight_parts(float w0, float w1) {
@@ -132,9 +139,9 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ uint32_t pa_col(int c, int k) { return (uint32_t)(((c >> 3) << 10) + ((c & 7) << 7) + (((k >> 4) ^ (c & 7)) << 4) + (k & 15)); }
 
 template <int NQ>
-__global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kernel(const __grid_constant__ CUtensorMap map_kv, const PagedAttnParams p) {
+__global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) paged_attn_kernel(const __grid_constant__ CUtensorMap map_kv, const PagedAttnParams p) {
   using Cfg = PaCfg<NQ>;
-  constexpr int Q = Cfg::Q, N = Cfg::N;
+  constexpr int Q = Cfg::Q, N = Cfg::N, SOFT = Cfg::kSoftWarps;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem + Cfg::kRing;
@@ -156,16 +163,16 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       mbar_init(&kv_full[i], 2);  // the copies' arrival and the scales'
       mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(&q_full, PA_SOFT_WARPS);
+    mbar_init(&q_full, SOFT);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
-    mbar_init(&p_full, PA_SOFT_WARPS);
+    mbar_init(&p_full, SOFT);
     mbar_init(&o_full, 1);
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
   }
-  if (warp == PA_SOFT_WARPS + 1) tmem_alloc(&tmem_slot, Cfg::kTmemCols);
+  if (warp == SOFT + 1) tmem_alloc(&tmem_slot, Cfg::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -177,20 +184,19 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
   const int n = t_first < 0 || n_all < 0 || n_all > p.T - t_first || past < 0 ? 0 : min(p.tokens, n_all - i0);  // tokens of this tile
   if (n <= 0) {  // the whole cluster alike
     __syncthreads();
-    if (warp == PA_SOFT_WARPS + 1) tmem_dealloc(tmem, Cfg::kTmemCols);
+    if (warp == SOFT + 1) tmem_dealloc(tmem, Cfg::kTmemCols);
     return;
   }
   const int nq = n * R, tok0 = t_first + i0;
   const int pos0 = past + i0, hi = pos0 + n;                                   // the tile's first position, one past its last
   const int lo = p.window > 0 ? max(0, pos0 + 1 - p.window) : 0;               // the first position that any query sees
   const int page_lo = lo / PG_TOKENS, n_pages = (hi + PG_TOKENS - 1) / PG_TOKENS - page_lo;
-  const int per = ((n_pages + 1) / 2 + splits - 1) / splits;                   // tiles of a split
-  const int first = page_lo + min(split * per * 2, n_pages), last = page_lo + min((split + 1) * per * 2, n_pages);  // this split's pages
+  const int first = page_lo + n_pages * split / splits, last = page_lo + n_pages * (split + 1) / splits;  // this split's pages (n_pages < 2^25)
   const int tiles = (last - first + 1) / 2;
 
   float o[Q], m[Q], l[Q];
-  const int half = warp >> 2, key_at = tid & 127;  // of the softmax threads
-  if (warp == PA_SOFT_WARPS) {
+  const int group = warp >> 2, key_at = tid & 127;  // of the softmax threads
+  if (warp == SOFT) {
     // ================= producer =================
     const bool row_ok = row >= 0 && row < p.R;
     int page = 0;
@@ -229,7 +235,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       }
       __syncwarp();
     }
-  } else if (warp == PA_SOFT_WARPS + 1) {
+  } else if (warp == SOFT + 1) {
     // ================= MMA issuer =================
     bool ok = tiles == 0 || bounded_wait(&q_full, 0, &gave_up);
     const uint32_t q_desc = umma_desc_lo(smem_u32(sQ));
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
   } else {
     // ================= softmax =================
     // queries -> hi and lo parts, a warp per row
-    for (int q = warp; q < NQ; q += PA_SOFT_WARPS) {
+    for (int q = warp; q < NQ; q += SOFT) {
       uint2 u = make_uint2(0u, 0u);
       if (q < nq) u = *reinterpret_cast<const uint2*>(p.q + (int64_t)(tok0 + q / R) * p.ldq + (int64_t)(g * R + q % R) * kHeadDim + lane * 4);
       const float x[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
@@ -300,9 +306,9 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
     for (int i = 0; i < Q; ++i) {
       o[i] = l[i] = 0.f;
       m[i] = PA_NOTHING;
-      qs[i] = q_scale[half * Q + i];
+      qs[i] = q_scale[group * Q + i];
     }
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 2 * Q;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + group * 2 * Q;
     float vs0 = 0.f, vs1 = 0.f;  // value scales of the tile before
     bool two_before = false;
     auto add_values = [&](int t) {  // the sums of tile t, relative to m as it stood then
@@ -344,12 +350,12 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
           for (int i = 0; i < Q; ++i) {
             bool sees = seen;
             if (n > 1) {  // (of one token every key in [lo, hi) is seen)
-              const int pos = pos0 + (half * Q + i) / R;
+              const int pos = pos0 + (group * Q + i) / R;
               sees = seen && key <= pos && (p.window <= 0 || key > pos - p.window);
             }
             s[i] = sees ? s[i] : -INFINITY;
           }
-          if (!seen && here && half == 0) {  // what this row holds must not reach the sums: 0 * NaN is not 0
+          if (!seen && here && group == 0) {  // what this row holds must not reach the sums: 0 * NaN is not 0
             uint4* v = reinterpret_cast<uint4*>(smem + st * PA_STAGE_BYTES + 2 * PG_BYTES + key_at * 128);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
@@ -358,10 +364,10 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
           const float w = warp_max_f32(s[i]);
-          if (lane == 0) warp_most[t & 1][half * Q + i][warp & 3] = w;
+          if (lane == 0) warp_most[t & 1][group * Q + i][warp & 3] = w;
         }
       }
-      if (half_sync_or(half, !ok)) {
+      if (group_sync_or<Cfg::G>(group, !ok)) {
         ok = false;
         break;
       }
@@ -369,12 +375,12 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       bool grew = false;
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
-        const float4 w = *reinterpret_cast<const float4*>(warp_most[t & 1][half * Q + i]);
+        const float4 w = *reinterpret_cast<const float4*>(warp_most[t & 1][group * Q + i]);
         top[i] = fmaxf(fmaxf(m[i], fmaxf(w.x, w.y)), fmaxf(w.z, w.w));
         grew |= top[i] > m[i];
       }
       float alpha[Q];
-      if (grew) {  // (the same in all threads of the half)
+      if (grew) {  // (the same in all threads of the group)
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
           alpha[i] = exp2_ftz(m[i] - top[i]);
@@ -389,7 +395,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
         l[i] += e0;
         l[i + 1] += e1;
         const uint32_t w = weight_parts(e0, e1);
-        const int c = half * 2 * Q + i;
+        const int c = group * 2 * Q + i;
         P[pa_col(c, key_at)] = (uint8_t)w;
         P[pa_col(c + 1, key_at)] = (uint8_t)(w >> 8);
         P[pa_col(c + Q, key_at)] = (uint8_t)(w >> 16);
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
       const float w = warp_sum(l[i]);
-      if (lane == 0) sums[warp & 3][half * Q + i] = w;
+      if (lane == 0) sums[warp & 3][group * Q + i] = w;
     }
   }
   tc_fence_before();
@@ -427,17 +433,17 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
       for (uint32_t k = 0; k < 2; ++k)
         for (uint32_t spin = 0; spin < 4096 && !mbar_try_wait(&kv_full[i], k); ++spin) {}
   }
-  if (warp == PA_SOFT_WARPS + 1) {
+  if (warp == SOFT + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::kTmemCols);
   }
   // ================= merge the splits =================
   // this split: [q][maximum, sum, 128 sums] over the ring, which is used up
   float* mine = reinterpret_cast<float*>(smem);
-  if (warp < PA_SOFT_WARPS) {
+  if (warp < SOFT) {
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
-      const int q = half * Q + i;
+      const int q = group * Q + i;
       if (q < nq) {
         const float sum = sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q];
         if (splits == 1) {
@@ -454,20 +460,24 @@ __global__ void __launch_bounds__(PA_THREADS, NQ <= 16 ? 2 : 1) paged_attn_kerne
   }
   if (splits == 1) return;
   cluster_sync_all();
-  if (warp < PA_SOFT_WARPS) {
+  // The results are dealt to all CTAs of the cluster, 32 to a warp.  Maxima and sums of all splits come by one load, a split a lane, and the loads of
+  // their sums of values do not wait for one another.  (A loop over the splits in every thread: 4500 clocks for 16 of them.)
+  if (warp < SOFT) {
     const uint32_t base = smem_u32(mine);
-    for (int q = split * 2 + half; q < nq; q += splits * 2) {
+    for (int part = split * SOFT + warp; part < nq * (kHeadDim / 32); part += splits * SOFT) {
+      const int q = part / (kHeadDim / 32), d = part % (kHeadDim / 32) * 32 + lane;
       const uint32_t at = base + q * (kHeadDim + 2) * 4;
-      float top = PA_NOTHING;
-      for (int r = 0; r < splits; ++r) top = fmaxf(top, ld_cluster_f32(map_to_rank(at, r)));
-      float sum = 0.f, acc = 0.f;
-      for (int r = 0; r < splits; ++r) {
-        const uint32_t from = map_to_rank(at, r);
-        const float f = exp2_ftz(ld_cluster_f32(from) - top);  // (a split without a key: its sums are 0)
-        sum = fmaf(f, ld_cluster_f32(from + 4), sum);
-        acc = fmaf(f, ld_cluster_f32(from + 8 + key_at * 4), acc);
-      }
-      p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + key_at] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
+      const uint32_t from = map_to_rank(at, lane < splits ? lane : 0);
+      const float mine_m = lane < splits ? ld_cluster_f32(from) : PA_NOTHING, mine_l = lane < splits ? ld_cluster_f32(from + 4) : 0.f;
+      float v[PA_MAX_SPLITS];
+#pragma unroll
+      for (int r = 0; r < PA_MAX_SPLITS; ++r) v[r] = r < splits ? ld_cluster_f32(map_to_rank(at + 8 + d * 4, r)) : 0.f;
+      const float f = exp2_ftz(mine_m - warp_max_f32(mine_m));  // (a split without a key: its sums are 0)
+      const float sum = warp_sum(f * mine_l);
+      float acc = 0.f;
+#pragma unroll
+      for (int r = 0; r < PA_MAX_SPLITS; ++r) acc = fmaf(__shfl_sync(0xffffffffu, f, r), v[r], acc);
+      p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
     }
   }
   cluster_sync_all();  // nobody leaves while its results are read
@@ -493,7 +503,7 @@ inline int launch_paged_attn(const PagedAttnParams& p, const CUtensorMap& map, i
   if (splits > 8) MB_CHECK_CUDA(cudaFuncSetAttribute(paged_attn_kernel<NQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)splits, (unsigned)(p.KV * q_tiles), (unsigned)p.B);
-  cfg.blockDim = dim3(PA_THREADS);
+  cfg.blockDim = dim3(PaCfg<NQ>::kThreads);
   cfg.dynamicSmemBytes = PaCfg<NQ>::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
