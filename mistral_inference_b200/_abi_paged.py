@@ -29,7 +29,8 @@ _SIGNATURES = {
     "mbp_pages_extend": (c_int, [P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P]),
     "mbp_pages_truncate": (c_int, [P, P, P, P, P, P, P, P, I, I, I, I, P]),
     "mbp_pages_write": (c_int, [P, I, P, I, P, P, P, P, P, I, I, I, I, I, P]),
-    "mbp_attn_pages": (c_int, [P, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, c_float, P]),
+    "mbp_attn_pages_scratch": (I, [I, I, I, I, I, I, I]),
+    "mbp_attn_pages": (c_int, [P, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, c_float, P, I, P]),
     "mbp_token_scores_sizes": (c_int, [I, I, I, P]),
     "mbp_token_scores": (c_int, [P, I, c_int, P, P, P, P, P, I, I, I, P, P]),
 }
@@ -104,14 +105,22 @@ def pages_write(kv, scale, k, v, plan) -> None:
                                      plan.slots.shape[0], KV, HEAD_DIM, kv.shape[0], _stream()), "mbp_pages_write")
 
 
+@functools.lru_cache(maxsize=256)
+def _attn_scratch(B: int, longest: int, most: int, width: int, n_heads: int, KV: int, window: int) -> int:
+    return lib().mbp_attn_pages_scratch(B, longest, most, width, n_heads, KV, window)
+
+
 def attn_pages(q, kv, scale, plan, out, n_heads: int, window: int, softmax_scale: float) -> None:
     dev, KV = kv.device, kv.shape[1]
     pq, ldq = _rows(q, n_heads, dev)
     R, width = plan.table.shape
+    B = plan.rows.shape[0]
+    need = _attn_scratch(B, plan.longest, plan.most, width, n_heads, KV, window)
     with _on(dev):
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _check(lib().mbp_attn_pages(pq, ldq, _ptr(kv, dev), _ptr(scale, dev), _ptr(plan.table, dev), _ptr(plan.rows, dev), _ptr(plan.q_start, dev), _ptr(plan.seqpos, dev), _ptr(out, dev),
-                                    _ptr(plan.status, dev), plan.rows.shape[0], q.shape[0], plan.longest, plan.most, R, width, kv.shape[0], n_heads, KV, HEAD_DIM, window, softmax_scale,
-                                    _stream()), "mbp_attn_pages")
+                                    _ptr(plan.status, dev), B, q.shape[0], plan.longest, plan.most, R, width, kv.shape[0], n_heads, KV, HEAD_DIM, window, softmax_scale,
+                                    None if scratch is None else scratch.data_ptr(), need, _stream()), "mbp_attn_pages")
 
 
 @functools.lru_cache(maxsize=256)

@@ -1,6 +1,7 @@
 // libmb200_paged.so -- the C ABI declared in include/mistral_b200_paged.h.  Argument checking + kernel dispatch only.
 #include "paged_attn.cuh"
 #include "paged_plan.cuh"
+#include "paged_prompt.cuh"
 #include "paged_write.cuh"
 #include "token_scores.cuh"
 
@@ -79,6 +80,44 @@ static int launch_token_scores(const TokenScoresParams& p, cudaStream_t st) {
   return MB200_OK;
 }
 
+// How a call's attention is cut: columns of a query tile (the fewest that hold a request's tokens, 32 at most), its tokens, tiles of queries, splits of the keys (as many as run
+// at once, four tiles of keys each at least), and whether its pages go through 16-bit rings.
+struct AttnCut {
+  int nq, tokens, splits;
+  int64_t q_tiles, keys;
+  bool rings;
+};
+static AttnCut attn_cut(int64_t B, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window) {
+  AttnCut c;
+  const int64_t rep = n_heads / n_kv_heads, want = longest * rep, sms = device_info::sm_count() > 0 ? device_info::sm_count() : 148;
+  c.nq = want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 ? 16 : 32;
+  c.tokens = c.nq / (int)rep;
+  c.q_tiles = (longest + c.tokens - 1) / c.tokens;
+  c.keys = most > 0 && most < P * PG_TOKENS ? most : P * PG_TOKENS;
+  if (window > 0 && c.keys > window + longest) c.keys = window + longest;
+  const int64_t pairs = B * n_kv_heads * c.q_tiles, room = sms * (c.nq < 32 ? 2 : 1);
+  c.splits = 1;
+  while (c.splits < PA_MAX_SPLITS && pairs * c.splits * 2 <= room && c.keys >= (int64_t)c.splits * 4 * PA_KEYS) c.splits *= 2;
+  // Time of both ways in us, tiles of 128 keys: 1.9 each on 32 query columns, 2.9 each in the prompt kernel (two heads x 128 tokens), and the conversion.  (nemo shape, measured
+  // direct and by rings: 1 x 17 tokens behind 8000 39, 186; 1 x 257 behind 2000 79, 58; 3 x 65 behind 2000 68, 65; 3 x 129 behind 8000 328, 204.)
+  c.rings = false;
+  if (c.q_tiles > 1) {
+    const double tiles = (double)(c.keys + PA_KEYS - 1) / PA_KEYS;
+    const int64_t ctas = B * n_heads / (rep % 2 == 0 ? 2 : 1) * ((longest + 127) / 128);
+    const double direct = (double)((pairs * c.splits + sms - 1) / sms) * (tiles / c.splits) * 1.9 + 6;
+    const double rings = (double)((ctas + sms - 1) / sms) * tiles * 2.9 + 11 + (double)B * (double)c.keys * (double)n_kv_heads * (kHeadDim * 2 * 3) / 4e6;
+    c.rings = rings < direct || n_kv_heads * c.q_tiles > 65535;
+  }
+  return c;
+}
+// Bytes of the rings.  group: requests that share them at a time (1 GB at most, but for one request alone)
+static int64_t ring_scratch(int64_t B, int64_t longest, int64_t most, int64_t P, int64_t KV, int64_t window, int64_t* group) {
+  const int64_t rows = paged_ring_rows(longest, most > 0 && most < P * PG_TOKENS ? most : P * PG_TOKENS, window), each = rows * KV * kHeadDim * 4;
+  int64_t n = ((int64_t)1 << 30) / each;
+  n = n < 1 ? 1 : n > B ? B : n;
+  *group = n;
+  return n * each;
+}
 }  // namespace mb200
 
 using namespace mb200;
@@ -147,9 +186,15 @@ int mbp_pages_write(const void* k, int64_t ldk, const void* v, int64_t ldv, void
   return MB200_OK;
 }
 
+int64_t mbp_attn_pages_scratch(int64_t B, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window) {
+  int64_t group;
+  if (B < 1 || longest < 1 || P < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || n_heads > 32 * n_kv_heads || n_heads % n_kv_heads || window < 0) return 0;
+  return attn_cut(B, longest, most, P, n_heads, n_kv_heads, window).rings ? ring_scratch(B, longest, most, P, n_kv_heads, window, &group) : 0;
+}
+
 int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scale, const int32_t* table, const int32_t* rows, const int32_t* q_start, const int32_t* seqpos,
                    void* out, int32_t* status, int64_t B, int64_t T, int64_t longest, int64_t most, int64_t R, int64_t P, int64_t n_pages, int64_t n_heads, int64_t n_kv_heads,
-                   int64_t head_dim, int64_t window, float softmax_scale, void* stream) {
+                   int64_t head_dim, int64_t window, float softmax_scale, void* scratch, int64_t scratch_bytes, void* stream) {
   int rc = check_pool("attn_pages", kv, scale, n_pages, n_kv_heads);
   if (rc) return rc;
   MB_CHECK_ARG(head_dim == kHeadDim, "attn_pages: head_dim=%lld unsupported (128 only)", (long long)head_dim);
@@ -162,14 +207,35 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
                (long long)ldq);
   MB_CHECK_ARG(softmax_scale > 0.f && softmax_scale < 3.4e38f, "attn_pages: scale %g", (double)softmax_scale);
   if (T == 0) return MB200_OK;
-  const int rep = (int)(n_heads / n_kv_heads);
-  if (longest > T) longest = T;
-  // columns of a query tile: the fewest that hold a request's tokens, 32 at most
-  const int64_t want = longest * rep;
-  const int nq = want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 ? 16 : 32;
-  const int tokens = nq / rep;
-  const int64_t q_tiles = (longest + tokens - 1) / tokens;
-  MB_CHECK_ARG(n_kv_heads * q_tiles <= 65535, "attn_pages: %lld tiles of queries", (long long)(n_kv_heads * q_tiles));
+  const AttnCut cut = attn_cut(B, longest, most, P, n_heads, n_kv_heads, window);
+  // (rows of queries that the copy engine cannot take stay with the kernel below)
+  if (cut.rings && (uintptr_t)q % 16 == 0 && ldq % 8 == 0 && (uintptr_t)out % 16 == 0) {
+    int64_t group = 0;
+    const int64_t need = ring_scratch(B, longest, most, P, n_kv_heads, window, &group);
+    if (scratch == nullptr || scratch_bytes < need || (uintptr_t)scratch % 256 != 0)
+      return fail(MB200_E_WORKSPACE, "attn_pages: scratch %lld < %lld, or not 256-byte aligned", (long long)scratch_bytes, (long long)need);
+    PagedRingParams p;
+    p.kv = (const uint8_t*)kv;
+    p.scale = scale;
+    p.table = table;
+    p.rows = rows;
+    p.q_start = q_start;
+    p.seqpos = seqpos;
+    p.status = status;
+    p.T = (int)T;
+    p.R = (int)R;
+    p.P = (int)P;
+    p.n_pages = (int)n_pages;
+    p.KV = (int)n_kv_heads;
+    p.window = (int)window;
+    p.W = (int)paged_ring_rows(longest, most > 0 && most < P * PG_TOKENS ? most : P * PG_TOKENS, window);
+    for (int64_t b0 = 0; b0 < B; b0 += group) {
+      rc = launch_paged_prompt(p, q, ldq, (bf16*)out, b0, B - b0 < group ? B - b0 : group, longest, (int)n_heads, softmax_scale * 1.4426950408889634f, scratch, (cudaStream_t)stream);
+      if (rc) return rc;
+    }
+    return MB200_OK;
+  }
+  MB_CHECK_ARG(n_kv_heads * cut.q_tiles <= 65535, "attn_pages: %lld tiles of queries", (long long)(n_kv_heads * cut.q_tiles));
   PagedAttnParams p;
   p.q = (const bf16*)q;
   p.ldq = ldq;
@@ -188,19 +254,18 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
   p.H = (int)n_heads;
   p.KV = (int)n_kv_heads;
   p.window = (int)window;
-  p.tokens = tokens;
+  p.tokens = cut.tokens;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   CUtensorMap map;
   rc = make_pool_map(&map, kv, n_pages, n_kv_heads);
   if (rc) return rc;
-  // splits: as many as run at once, two tiles each at least
-  const int64_t pairs = B * n_kv_heads * q_tiles, room = (int64_t)device_info::sm_count() * (nq <= 16 ? 2 : 1);
-  int64_t keys = most > 0 && most < P * PG_TOKENS ? most : P * PG_TOKENS;
-  if (window > 0 && keys > window + longest) keys = window + longest;
-  int splits = 1;
-  while (splits < PA_MAX_SPLITS && pairs * splits * 2 <= room && keys >= (int64_t)splits * 4 * PA_KEYS) splits *= 2;
   cudaStream_t st = (cudaStream_t)stream;
-  return nq == 4 ? launch_paged_attn<4>(p, map, q_tiles, splits, st) : nq == 8 ? launch_paged_attn<8>(p, map, q_tiles, splits, st) : nq == 16 ? launch_paged_attn<16>(p, map, q_tiles, splits, st) : launch_paged_attn<32>(p, map, q_tiles, splits, st);
+  switch (cut.nq) {
+    case 4: return launch_paged_attn<4>(p, map, cut.q_tiles, cut.splits, st);
+    case 8: return launch_paged_attn<8>(p, map, cut.q_tiles, cut.splits, st);
+    case 16: return launch_paged_attn<16>(p, map, cut.q_tiles, cut.splits, st);
+    default: return launch_paged_attn<32>(p, map, cut.q_tiles, cut.splits, st);
+  }
 }
 
 int mbp_token_scores_sizes(int64_t T, int64_t vocab, int64_t top, int64_t* bytes) {

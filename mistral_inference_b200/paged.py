@@ -18,7 +18,7 @@ from ._abi import Mb200Error
 from ._abi_paged import HEAD_DIM, PAGE
 
 _REASONS = {1: "a row out of range, or named twice", 2: "a length that is negative or longer than a row of the block table", 3: "more tokens than the plan has room for",
-            4: "too few free pages", 16: "a wait inside attention ran out"}
+            4: "too few free pages", 16: "a wait inside attention ran out", 32: "a request of more tokens than the plan's `most`"}
 
 
 def pages_of(tokens: int) -> int:
@@ -29,7 +29,7 @@ def check_status(status: torch.Tensor) -> None:
     """Raises if a plan's or a truncation's status says that it was refused (waits for the GPU)."""
     code = int(status)
     if code:
-        raise Mb200Error("pages: " + "; ".join(v for k, v in _REASONS.items() if (code & 16 if k == 16 else code & 15 == k)))
+        raise Mb200Error("pages: " + "; ".join(v for k, v in _REASONS.items() if (code & k if k >= 16 else code & 15 == k)))
 
 
 @dataclass

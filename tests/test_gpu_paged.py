@@ -231,6 +231,72 @@ def test_attention_of_several_tokens(new, H, KV, window):
     check_attention(H, KV, [0, 100, 63, 200][: len(new)], new, window=window, seed=len(new))
 
 
+def by_rings(H, KV, past, new, window=0):
+    """Whether such a call's pages go through 16-bit rings."""
+    total = [p + n for p, n in zip(past, new)]
+    return _abi_paged.lib().mbp_attn_pages_scratch(len(past), max(new), max(total), U.cdiv(max(total), 64) + 1, H, KV, window) > 0
+
+
+@pytest.mark.parametrize("H,KV,past,new,window", [(32, 8, [0, 300], [300, 129], 0), (16, 16, [100, 0, 63], [257, 128, 0], 0), (24, 8, [700, 64], [200, 333], 150), (8, 1, [1000, 0, 5, 64], [400, 1, 130, 77], 65),
+                                                  (15, 5, [200, 100], [550, 460], 0), (32, 8, [1500, 3], [190, 333], 1000)])
+def test_attention_of_portions(H, KV, past, new, window):
+    assert by_rings(H, KV, past, new, window)
+    check_attention(H, KV, past, new, window=window, seed=len(new))
+
+
+def test_portions_of_one_request_at_a_time():
+    """Rings of a gigabyte at most: requests take turns, and a `most` of 0 stands for the whole row of the block table."""
+    plan, kv, scale, *_ = filled(8, [100, 30, 7], [250, 300, 200], 4)
+    q = numbers(750, 32, 128, seed=1, spread=0).to(DEV)
+    want = mi.attend_pages(q, kv, scale, plan)
+    wide = torch.full((plan.table.shape[0], 4200), -1, dtype=torch.int32, device=DEV)
+    wide[:, : plan.table.shape[1]] = plan.table
+    loose = mi.PagePlan(wide, plan.rows, plan.q_start, plan.seqpos, plan.positions, plan.slots, plan.longest)
+    assert _abi_paged.lib().mbp_attn_pages_scratch(3, 300, 0, 4200, 32, 8, 0) == 4200 * 64 * 8 * 128 * 4 > 1 << 30
+    assert torch.equal(mi.attend_pages(q, kv, scale, loose), want)
+
+
+def test_portions_longer_than_the_plan_says_are_no_numbers():
+    plan, kv, scale, *_ = filled(8, [900, 30], [250, 300], 4)
+    q = numbers(550, 32, 128, seed=1, spread=0).to(DEV)
+    want = mi.attend_pages(q, kv, scale, plan)
+    plan.check()
+    plan.most = 400
+    got = mi.attend_pages(q, kv, scale, plan)
+    assert got[:250].isnan().all() and torch.equal(got[250:], want[250:])
+    with pytest.raises(_abi_paged.Mb200Error, match="most"):
+        plan.check()
+
+
+def test_portions_of_pages_that_are_none_and_of_refused_plans():
+    plan, kv, scale, *_ = filled(8, [200, 30], [250, 300], 4)
+    q = numbers(550, 32, 128, seed=1, spread=0).to(DEV)
+    want = mi.attend_pages(q, kv, scale, plan)
+    for page in (-1, kv.shape[0], 2 ** 30):
+        table = plan.table.clone()
+        table[int(plan.rows[0]), 0] = page
+        got = mi.attend_pages(q, kv, scale, mi.PagePlan(table, plan.rows, plan.q_start, plan.seqpos, plan.positions, plan.slots, plan.longest, plan.most))
+        assert got[:250].isnan().all() and torch.equal(got[250:], want[250:])
+    t = mi.PageTables.empty(2, 8, 3, DEV)
+    refused = t.extend(ints([250, 300]), 550, longest=300, most=300)
+    out = torch.full((550, 32 * 128), 3.0, dtype=torch.bfloat16, device=DEV)
+    mi.attend_pages(q, kv, scale, refused, out=out)
+    mi.write_pages(kv.clone(), scale.clone(), q[:, :8].contiguous(), q[:, :8].contiguous(), refused)
+    assert (out == 3.0).all()
+
+
+def test_portions_out_of_a_wider_matrix():
+    plan, kv, scale, kv_h, scale_h, table, rows = filled(8, [200, 30], [250, 300], 4)
+    wide = numbers(550, 48 * 128, seed=1, spread=0).to(DEV)
+    for first in (0, 8, 1024):
+        x = wide[:, first: first + 32 * 128]
+        assert torch.equal(mi.attend_pages(x, kv, scale, plan), mi.attend_pages(x.contiguous(), kv, scale, plan))
+    x = numbers(550, 33 * 128 + 4, seed=1, spread=0).to(DEV)[:, 4: 4 + 32 * 128]  # rows that the copy engine cannot take
+    got = mi.attend_pages(x, kv, scale, plan).cpu().double().view(550, 32, 128)
+    want, mag = U.attend_ref(x.cpu().reshape(550, 32, 128), kv_h.double(), scale_h, table, rows, [0, 250, 550], [200, 30])
+    assert ((got - want).abs() <= U.attend_tolerance(want, mag, 450, float(448 * scale_h.max()))).all()
+
+
 @pytest.mark.parametrize("q_scale", [1e-3, 30.0])
 def test_attention_of_small_and_large_queries(q_scale):
     """Nearly even weights, and weights that one key has almost alone."""

@@ -63,12 +63,20 @@ def test_writes_are_refused(lib):
 
 
 def test_attention_is_refused(lib):
-    def attend(q=X, ldq=512, B=1, T=1, longest=1, H=4, KV=2, hd=128, P=4, N=4, window=0, scale=0.1):
-        return lib.mbp_attn_pages(q, ldq, X, X, X, X, X, X, X, None, B, T, longest, 0, 2, P, N, H, KV, hd, window, scale, None)
+    def attend(q=X, ldq=512, B=1, T=1, longest=1, most=0, H=4, KV=2, hd=128, P=4, N=4, window=0, scale=0.1, scratch=None, room=0):
+        return lib.mbp_attn_pages(q, ldq, X, X, X, X, X, X, X, None, B, T, longest, most, 2, P, N, H, KV, hd, window, scale, scratch, room, None)
     for kw, why in [(dict(q=None), "null"), (dict(q=X + 4), "aligned"), (dict(ldq=256), "overlap"), (dict(H=5), "multiple"), (dict(H=66, ldq=66 * 128), "32 times"), (dict(hd=64), "128 only"),
                     (dict(longest=0), "longest"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(P=0), "P="), (dict(N=0), "pages")]:
         assert attend(**kw) == -1 and why in last(lib), (kw, last(lib))
     assert attend(T=0) == 0
+    scratch = lambda B=4, longest=1000, most=0, P=64, H=32, KV=8, window=0: lib.mbp_attn_pages_scratch(B, longest, most, P, H, KV, window)  # noqa: E731
+    need = scratch()  # (sized for 148 SMs where there is no GPU)
+    assert need == 4 * 64 * 64 * 8 * 128 * 4 and scratch(longest=1) == 0
+    assert scratch(most=1500) < need and scratch(window=100) < need
+    assert scratch(B=0) == scratch(H=33) == scratch(KV=0) == scratch(window=-1) == 0
+    assert scratch(B=64, P=512) <= 1 << 30  # requests take turns
+    for kw in (dict(scratch=None, room=need), dict(scratch=X, room=need - 1), dict(scratch=X + 16, room=need)):  # a portion without room
+        assert attend(B=4, T=4000, longest=1000, P=64, H=32, KV=8, ldq=4096, **kw) == -2 and "scratch" in last(lib)
 
 
 def test_scores_are_refused(lib):
@@ -127,7 +135,7 @@ def test_python_refuses_what_it_cannot_take():
 def test_status_says_why():
     from mistral_inference_b200.paged import check_status
     check_status(torch.zeros(1, dtype=torch.int32))
-    for code, word in ((1, "twice"), (2, "length"), (3, "room"), (4, "free"), (16, "wait")):
+    for code, word in ((1, "twice"), (2, "length"), (3, "room"), (4, "free"), (16, "wait"), (32, "most")):
         with pytest.raises(_abi_paged.Mb200Error, match=word):
             check_status(torch.tensor([code], dtype=torch.int32))
 
@@ -153,4 +161,4 @@ def test_host_tables_truncate_undoes_extend():
 def test_declarations_of_this_abi_version():
     """A change of the declarations takes a new version, so that a library built before it is refused."""
     code = re.sub(r"/\*.*?\*/", " ", HEADER.read_text(), flags=re.S)
-    assert zlib.crc32(" ".join(code.split()).encode()) == 2367187686, "raise the ABI version with this change"
+    assert zlib.crc32(" ".join(code.split()).encode()) == 1661688504, "raise the ABI version with this change"
