@@ -3,7 +3,6 @@
 Same rules as `_abi`: the only place Python touches this library, and no fallback -- a missing library is built once
 in-tree by `build.build_paged()` (a fresh checkout has no binaries), a failing call raises.
 """
-import contextlib
 import ctypes
 import functools
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
@@ -55,54 +54,74 @@ def _check(rc: int, what: str) -> None:
         raise Mb200Error(f"{what} failed ({rc}): {msg.decode() if msg else '?'}")
 
 
-def _ptr(t: Optional[torch.Tensor], device: torch.device) -> Optional[int]:
+_lazy = {}  # name -> entry point, once the library is loaded
+
+
+def _fn(name: str):
+    fn = _lazy.get(name)
+    if fn is None:
+        fn = _lazy[name] = getattr(lib(), name)
+    return fn
+
+
+def index_of(t: torch.Tensor) -> int:
+    """The device that a call works on: its tensors' own, whatever the current one is."""
+    i = t.get_device()
+    assert i >= 0, f"libmb200_paged runs on CUDA only (got {t.device}); no fallback exists"
+    return i
+
+
+def _ptr(t: Optional[torch.Tensor], device: int) -> Optional[int]:
     if t is None:
         return None
-    assert t.device == device and t.is_contiguous(), f"libmb200_paged takes contiguous tensors of one device ({device}, got one on {t.device})"
+    assert t.get_device() == device and t.is_contiguous(), f"libmb200_paged takes contiguous tensors of one device (cuda:{device}, got one on {t.device})"
     return t.data_ptr()
 
 
-def _on(device: torch.device):
-    """The library works on the current device: make it the tensors' own."""
-    assert device.type == "cuda", f"libmb200_paged runs on CUDA only (got {device}); no fallback exists"
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _rows(x: torch.Tensor, heads: int, device: torch.device) -> Tuple[int, int]:
-    """(pointer, elements between tokens) of [T, heads, 128] or [T, heads * 128] bf16; tokens may be rows of a wider matrix."""
-    assert x.dtype == torch.bfloat16 and x.device == device, f"bf16 tokens on {device}, got {x.dtype} on {x.device}"
-    if x.dim() == 3:
-        assert x.shape[1:] == (heads, HEAD_DIM) and x.stride(2) == 1 and (heads == 1 or x.stride(1) == HEAD_DIM), f"[T, {heads}, {HEAD_DIM}] with contiguous heads, got {tuple(x.shape)}"
+def _call(name: str, device: int, *args) -> None:
+    fn = _fn(name)
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, _stream())
     else:
-        assert x.dim() == 2 and x.shape[1] == heads * HEAD_DIM and x.stride(1) == 1, f"[T, {heads * HEAD_DIM}] with contiguous rows, got {tuple(x.shape)}"
-    width = heads * HEAD_DIM
-    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else width
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream())
+    if rc != 0:
+        _check(rc, name)
 
 
-def pages_extend(tables, rows, add, positions, slots, q_start, seqpos, status, T: int) -> None:
-    dev = tables.table.device
+def _rows(x: torch.Tensor, heads: int, device: int) -> Tuple[int, int]:
+    """(pointer, elements between tokens) of [T, heads, 128] or [T, heads * 128] bf16; tokens may be rows of a wider matrix."""
+    assert x.dtype == torch.bfloat16 and x.get_device() == device, f"bf16 tokens on cuda:{device}, got {x.dtype} on {x.device}"
+    shape, stride = x.shape, x.stride()
+    if len(shape) == 3:
+        assert shape[1] == heads and shape[2] == HEAD_DIM and stride[2] == 1 and (heads == 1 or stride[1] == HEAD_DIM), f"[T, {heads}, {HEAD_DIM}] with contiguous heads, got {tuple(shape)}"
+    else:
+        assert len(shape) == 2 and shape[1] == heads * HEAD_DIM and stride[1] == 1, f"[T, {heads * HEAD_DIM}] with contiguous rows, got {tuple(shape)}"
+    return x.data_ptr(), stride[0] if shape[0] > 1 else heads * HEAD_DIM
+
+
+def _state(tables):
+    return tables.table.data_ptr(), tables.lens.data_ptr(), tables.free.data_ptr(), tables.n_free.data_ptr(), tables.scratch.data_ptr()
+
+
+def pages_extend(tables, rows, add, block, B: int, T: int) -> None:
+    """block: positions [T] | slots [T] | q_start [B + 1] | seqpos [B] | status [1]."""
+    at = block.data_ptr()
     R, width = tables.table.shape
-    with _on(dev):
-        _check(lib().mbp_pages_extend(_ptr(tables.table, dev), _ptr(tables.lens, dev), _ptr(tables.free, dev), _ptr(tables.n_free, dev), _ptr(tables.scratch, dev), _ptr(rows, dev),
-                                      _ptr(add, dev), _ptr(positions, dev), _ptr(slots, dev), _ptr(q_start, dev), _ptr(seqpos, dev), _ptr(status, dev), add.shape[0], T, R, width,
-                                      tables.free.shape[0], _stream()), "mbp_pages_extend")
+    _call("mbp_pages_extend", tables.device, *_state(tables), rows.data_ptr(), add.data_ptr(), at, at + 4 * T, at + 8 * T, at + 8 * T + 4 * (B + 1), at + 8 * T + 4 * (2 * B + 1), B, T, R,
+          width, tables.free.shape[0])
 
 
 def pages_truncate(tables, rows, keep, status) -> None:
-    dev = tables.table.device
     R, width = tables.table.shape
-    with _on(dev):
-        _check(lib().mbp_pages_truncate(_ptr(tables.table, dev), _ptr(tables.lens, dev), _ptr(tables.free, dev), _ptr(tables.n_free, dev), _ptr(tables.scratch, dev), _ptr(rows, dev),
-                                        _ptr(keep, dev), _ptr(status, dev), keep.shape[0], R, width, tables.free.shape[0], _stream()), "mbp_pages_truncate")
+    _call("mbp_pages_truncate", tables.device, *_state(tables), rows.data_ptr(), keep.data_ptr(), status.data_ptr(), keep.shape[0], R, width, tables.free.shape[0])
 
 
-def pages_write(kv, scale, k, v, plan) -> None:
-    dev, KV = kv.device, kv.shape[1]
+def pages_write(dev: int, kv, scale, k, v, plan, T: int, N: int, KV: int) -> None:
     pk, ldk = _rows(k, KV, dev)
     pv, ldv = _rows(v, KV, dev)
-    with _on(dev):
-        _check(lib().mbp_pages_write(pk, ldk, pv, ldv, _ptr(kv, dev), _ptr(scale, dev), _ptr(plan.slots, dev), _ptr(plan.q_start, dev), _ptr(plan.seqpos, dev), plan.rows.shape[0],
-                                     plan.slots.shape[0], KV, HEAD_DIM, kv.shape[0], _stream()), "mbp_pages_write")
+    _call("mbp_pages_write", dev, pk, ldk, pv, ldv, kv.data_ptr(), scale.data_ptr(), plan.slots.data_ptr(), plan.q_start.data_ptr(), plan.seqpos.data_ptr(), plan.rows.shape[0], T, KV,
+          HEAD_DIM, N)
 
 
 @functools.lru_cache(maxsize=256)
@@ -110,17 +129,13 @@ def _attn_scratch(B: int, longest: int, most: int, width: int, n_heads: int, KV:
     return lib().mbp_attn_pages_scratch(B, longest, most, width, n_heads, KV, window)
 
 
-def attn_pages(q, kv, scale, plan, out, n_heads: int, window: int, softmax_scale: float) -> None:
-    dev, KV = kv.device, kv.shape[1]
-    pq, ldq = _rows(q, n_heads, dev)
-    R, width = plan.table.shape
-    B = plan.rows.shape[0]
-    need = _attn_scratch(B, plan.longest, plan.most, width, n_heads, KV, window)
-    with _on(dev):
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _check(lib().mbp_attn_pages(pq, ldq, _ptr(kv, dev), _ptr(scale, dev), _ptr(plan.table, dev), _ptr(plan.rows, dev), _ptr(plan.q_start, dev), _ptr(plan.seqpos, dev), _ptr(out, dev),
-                                    _ptr(plan.status, dev), B, q.shape[0], plan.longest, plan.most, R, width, kv.shape[0], n_heads, KV, HEAD_DIM, window, softmax_scale,
-                                    None if scratch is None else scratch.data_ptr(), need, _stream()), "mbp_attn_pages")
+def attn_pages(dev: int, q, kv, scale, plan, out, T: int, N: int, KV: int, H: int, R: int, width: int, window: int, softmax_scale: float) -> None:
+    pq, ldq = _rows(q, H, dev)
+    B, status = plan.rows.shape[0], plan.status
+    need = _attn_scratch(B, plan.longest, plan.most, width, H, KV, window)
+    scratch = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
+    _call("mbp_attn_pages", dev, pq, ldq, kv.data_ptr(), scale.data_ptr(), plan.table.data_ptr(), plan.rows.data_ptr(), plan.q_start.data_ptr(), plan.seqpos.data_ptr(), out.data_ptr(),
+          None if status is None else _ptr(status, dev), B, T, plan.longest, plan.most, R, width, N, H, KV, HEAD_DIM, window, softmax_scale, None if scratch is None else scratch.data_ptr(), need)
 
 
 @functools.lru_cache(maxsize=256)
@@ -132,8 +147,7 @@ def _scores_scratch(T: int, V: int, top: int) -> int:
 
 def token_scores(logits, targets, logprob, entropy, top_ids, top_logprobs, top: int) -> None:
     T, V = logits.shape
-    dev = logits.device
-    with _on(dev):
-        scratch = torch.empty(_scores_scratch(T, V, top), dtype=torch.uint8, device=dev)
-        _check(lib().mbp_token_scores(logits.data_ptr(), logits.stride(0) if T > 1 else V, 1 if logits.dtype == torch.float32 else 0, _ptr(targets, dev), _ptr(logprob, dev), _ptr(entropy, dev),
-                                      _ptr(top_ids, dev), _ptr(top_logprobs, dev), T, V, top, scratch.data_ptr(), _stream()), "mbp_token_scores")
+    dev = index_of(logits)
+    scratch = torch.empty(_scores_scratch(T, V, top), dtype=torch.uint8, device=logits.device)
+    _call("mbp_token_scores", dev, logits.data_ptr(), logits.stride(0) if T > 1 else V, 1 if logits.dtype == torch.float32 else 0, _ptr(targets, dev), _ptr(logprob, dev), _ptr(entropy, dev),
+          _ptr(top_ids, dev), _ptr(top_logprobs, dev), T, V, top, scratch.data_ptr())

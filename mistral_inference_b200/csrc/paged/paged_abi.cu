@@ -60,20 +60,66 @@ static int64_t score_segment_length(int64_t T, int64_t vocab, int64_t size) {
   return best;
 }
 
-template <typename ST>
-static int launch_token_scores(const TokenScoresParams& p, cudaStream_t st) {
+// Few rows: segments of a row that can be a cluster (a power of two up to 16), all of them at once, one to an SM; 0: there are too many.  (32000 x 1: a launch less, 20.5 us of the
+// host's time 18.4; but 25 rows of 131072 as 400 CTAs in clusters of 16 20.5 us of the GPU's, as segments and a second kernel 13.2.)
+static int score_cluster(int64_t T, int64_t vocab, int64_t size) {
+  const int64_t step = TS_THREADS * (16 / size), room = device_info::sm_count();
+  int best = 0;
+  for (int64_t n = 1; n <= 16 && T * n <= room; n *= 2) {
+    const int64_t length = ((vocab + n - 1) / n + step - 1) / step * step;
+    if (length <= TS_BYTES / size && (n - 1) * length < vocab) best = (int)n;  // (no segment is empty)
+  }
+  return best;
+}
+
+template <typename ST, bool JOINS>
+static int launch_score_segments(const TokenScoresParams& p, cudaStream_t st) {
   const int64_t items = (int64_t)p.T * p.segments, room = (int64_t)device_info::sm_count() * TS_CTAS;
-  const dim3 grid((unsigned)(items < room ? items : room));
-  const size_t smem = (size_t)p.length * sizeof(ST);
+  const size_t lists = JOINS ? sizeof(unsigned long long) * (size_t)p.segments * p.top : 0, data = (size_t)p.length * sizeof(ST);
   const uint64_t apart = (uintptr_t)p.logits | (p.T > 1 ? (uint64_t)p.ld * sizeof(ST) : 0);
   auto go = [&](auto kernel, cudaError_t allowed) {
     MB_CHECK_CUDA(allowed);
-    MB_CHECK_CUDA(launch_pdl(kernel, grid, dim3(TS_THREADS), smem, st, p));
+    if (JOINS && p.segments > 8) MB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(JOINS || items < room ? items : room));
+    cfg.blockDim = dim3(TS_THREADS);
+    cfg.dynamicSmemBytes = data > lists ? data : lists;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (JOINS) {
+      at[n].id = cudaLaunchAttributeClusterDimension;
+      at[n].val.clusterDim.x = (unsigned)p.segments;
+      at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+      ++n;
+    }
+    if (pdl_enabled()) {
+      at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[n].val.programmaticStreamSerializationAllowed = 1;
+      ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    MB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return MB200_OK;
   };
-  const int rc = apart % 16 == 0  ? go(token_scores_segment_kernel<ST, 16>, device_info::allow_shared<token_scores_segment_kernel<ST, 16>>(TS_BYTES))
-                 : apart % 4 == 0 ? go(token_scores_segment_kernel<ST, 4>, device_info::allow_shared<token_scores_segment_kernel<ST, 4>>(TS_BYTES))
-                                  : go(token_scores_segment_kernel<ST, 0>, device_info::allow_shared<token_scores_segment_kernel<ST, 0>>(TS_BYTES));
+  return apart % 16 == 0  ? go(token_scores_segment_kernel<ST, 16, JOINS>, device_info::allow_shared<token_scores_segment_kernel<ST, 16, JOINS>>(TS_BYTES))
+         : apart % 4 == 0 ? go(token_scores_segment_kernel<ST, 4, JOINS>, device_info::allow_shared<token_scores_segment_kernel<ST, 4, JOINS>>(TS_BYTES))
+                          : go(token_scores_segment_kernel<ST, 0, JOINS>, device_info::allow_shared<token_scores_segment_kernel<ST, 0, JOINS>>(TS_BYTES));
+}
+
+template <typename ST>
+static int launch_token_scores(TokenScoresParams p, cudaStream_t st) {
+  const int cluster = score_cluster(p.T, p.V, sizeof(ST));
+  if (cluster > 0) {
+    const int step = TS_THREADS * (16 / (int)sizeof(ST));
+    p.length = ((p.V + cluster - 1) / cluster + step - 1) / step * step;
+    p.segments = cluster;
+    return launch_score_segments<ST, true>(p, st);
+  }
+  p.length = (int)score_segment_length(p.T, p.V, sizeof(ST));
+  p.segments = (int)((p.V + p.length - 1) / p.length);
+  const int rc = launch_score_segments<ST, false>(p, st);
   if (rc) return rc;
   const size_t lists = p.segments <= TS_JOIN_SEGMENTS ? sizeof(unsigned long long) * (size_t)p.segments * p.top : 0;
   MB_CHECK_CUDA(launch_pdl(token_scores_join_kernel<ST>, dim3((unsigned)p.T), dim3(32), lists, st, p));
@@ -286,17 +332,16 @@ int mbp_token_scores(const void* logits, int64_t ld, int dtype, const int64_t* t
   MB_CHECK_ARG(ld >= vocab && (dtype == 0 || dtype == 1), "token_scores: rows %lld elements apart of %lld, dtype %d", (long long)ld, (long long)vocab, dtype);
   MB_CHECK_ARG(T <= 65535, "token_scores: %lld rows (at most 65535)", (long long)T);
   if (T == 0) return MB200_OK;
-  TokenScoresParams p;
+  TokenScoresParams p = {};
   p.logits = logits;
   p.ld = ld;
   p.target = target;
   p.T = (int)T;
   p.V = (int)vocab;
-  p.length = (int)score_segment_length(T, vocab, dtype == 0 ? 2 : 4);
-  p.segments = (int)((vocab + p.length - 1) / p.length);
   p.top = (int)top;
+  const int64_t most = bytes / (T * (8 * top + 12));  // segments that there is room for
   p.best = (unsigned long long*)scratch;
-  p.sums = (float*)(p.best + T * p.segments * top);
+  p.sums = (float*)(p.best + T * most * top);
   p.logprob = logprob;
   p.entropy = entropy;
   p.top_ids = top_ids;

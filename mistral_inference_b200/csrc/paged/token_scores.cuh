@@ -9,7 +9,8 @@
 // the segment's maximum, in pairs (3.5 instructions an entry).  Every 16-byte piece is fetched, read and replaced by the next segment's by the same thread, so copies are in flight from
 // the middle of one segment to the beginning of the next and need no barrier.  The best are not sorted: a warp's r-th largest thread maximum, the least of them
 // over the warps, is a value that at least r * warps >= top entries reach, and few more; the threads that have some pick them out, and they are ranked by counting.  Two block
-// barriers a segment.  A second kernel, a warp a row, joins the segments.
+// barriers a segment.  A warp a row joins the segments, in a
+// second kernel or, where few rows leave room, behind a cluster's barrier.
 // 1000 x 131072 fp32, 8 alternatives: the largest taken off over and over 1540 us; entries in registers, a CTA for 8192 of them 141; longer walks with a list kept
 // up to date 205 (a barrier a slice, and more code than the instruction cache holds); whole segments by one bulk copy each, fetched behind the second barrier 107.
 #pragma once
@@ -113,9 +114,87 @@ __device__ __forceinline__ void ts_load16(const bf16* p, uint64_t* x) {
   for (int i = 0; i < 4; ++i) x[i] = pair(y[2 * i], y[2 * i + 1]);
 }
 
+// A warp joins the segments of row t.  lists: [segments][top] of shared memory, up to TS_JOIN_SEGMENTS
+template <typename ST>
+__device__ __forceinline__ void token_scores_join(const TokenScoresParams& p, int t, unsigned long long* lists) {
+  const int lane = threadIdx.x & 31;
+  const float* sums = p.sums + (int64_t)t * p.segments * 3;
+  const unsigned long long* best = p.best + (int64_t)t * p.segments * p.top;
+  const bool staged = p.segments <= TS_JOIN_SEGMENTS;
+  if (staged) {
+#pragma unroll 8
+    for (int i = lane; i < p.segments * p.top; i += 32) lists[i] = best[i];
+  }
+  const int64_t target = p.logprob ? p.target[t] : -1;
+  const float x = target >= 0 && target < p.V ? ts_load(static_cast<const ST*>(p.logits) + (int64_t)t * p.ld + target) : 0.f;
+  float M = -INFINITY;
+  bool bad = false;
+  for (int i = lane; i < p.segments; i += 32) {
+    M = fmaxf(M, sums[i * 3]);
+    bad |= sums[i * 3 + 2] != sums[i * 3 + 2];
+  }
+  M = warp_max_f32(M);
+  bad = __any_sync(0xffffffffu, bad) || !(fabsf(M) <= FLT_MAX);
+  int owner = 0x7fffffff;  // of the segments that hold the maximum, the one that leaves its 1 out
+  for (int i = lane; i < p.segments; i += 32)
+    if (sums[i * 3] == M) owner = min(owner, i);
+  owner = __reduce_min_sync(0xffffffffu, owner);
+  float S = 0.f, W = 0.f;
+  for (int i = lane; i < p.segments; i += 32) {
+    const float m = sums[i * 3];
+    if (m == -INFINITY) continue;
+    const float d = m - M, f = expf(d), s = sums[i * 3 + 1];
+    if (f == 0.f) continue;
+    S = fmaf(f, i == owner ? s : 1.f + s, S);
+    W = fmaf(f, fmaf(d, 1.f + s, sums[i * 3 + 2]), W);
+  }
+  S = warp_sum(S);
+  W = warp_sum(W);
+  const float none = __int_as_float(0x7fffffff), z = log1pf(S);
+  if (lane == 0) {
+    if (p.entropy) p.entropy[t] = bad ? none : z - W / (1.f + S);
+    if (p.logprob) p.logprob[t] = target < 0 ? 0.f : bad || target >= p.V ? none : (x - M) - z;
+  }
+  auto put = [&](int k, unsigned long long key) {
+    p.top_ids[(int64_t)t * p.top + k] = ts_index(key);
+    p.top_logprobs[(int64_t)t * p.top + k] = bad ? none : (ts_value(key) - M) - z;
+  };
+  if (staged) {  // lane i walks down the list of segment i: the largest of the heads, over and over
+    __syncwarp();
+    int at = 0;
+    unsigned long long head = lane < p.segments && p.top > 0 ? lists[lane * p.top] : 0ull, mine = 0ull;
+    for (int k = 0; k < p.top; ++k) {
+      const unsigned long long top = warp_max_key(head);
+      if (head == top) {
+        ++at;
+        head = at < p.top ? lists[lane * p.top + at] : 0ull;
+      }
+      if ((k & 31) == lane) mine = top;
+      if ((k & 31) == 31 || k + 1 == p.top)  // 32 results at a time
+        if ((k & ~31) + lane <= k) put((k & ~31) + lane, mine);
+    }
+    return;
+  }
+  unsigned long long below = ~0ull;  // lane i has the lists of segments i, i + 32, ...; keys differ
+  for (int k = 0; k < p.top; ++k) {
+    unsigned long long head = 0ull;
+    for (int i = lane; i < p.segments; i += 32)
+      for (int j = 0; j < p.top; ++j) {
+        const unsigned long long key = best[(int64_t)i * p.top + j];
+        if (key < below) {
+          head = max(head, key);
+          break;
+        }
+      }
+    below = warp_max_key(head);
+    if (lane == 0) put(k, below);
+  }
+}
+
 // BYTES: of a copy: 16, or 4 where rows begin on 4-byte boundaries only, or 0 (rows of 16-bit numbers that begin on odd ones are loaded entry by entry).  Entries go to the
 // same places in all three, so that a row's results do not depend on where it lies.  251 rows of 50257 fp32: 33.7 us loaded entry by entry, 28.0 by 4-byte copies.
-template <typename ST, int BYTES>
+// JOINS: the segments of a row are a cluster, a CTA each, whose first CTA joins them: one launch, for so few rows that all segments run at once.
+template <typename ST, int BYTES, bool JOINS>
 __global__ void __launch_bounds__(TS_THREADS, TS_CTAS) token_scores_segment_kernel(TokenScoresParams p) {
   constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
   constexpr bool COPIED = BYTES > 0;
@@ -181,7 +260,7 @@ __global__ void __launch_bounds__(TS_THREADS, TS_CTAS) token_scores_segment_kern
     }
     float v = most, reach = warp_max_f32(v);
     const float warp_most = reach;
-    const int warps = min(TS_WARPS, (count + 32 * VEC - 1) / (32 * VEC));  // those that have entries
+    const int warps = max(1, min(TS_WARPS, (count + 32 * VEC - 1) / (32 * VEC)));  // those that have entries
     for (int k = warps; k < top; k += warps) {  // the warp's next largest thread maximum
       if (lane == __ffs(__ballot_sync(0xffffffffu, v == reach)) - 1) v = -INFINITY;
       reach = warp_max_f32(v);
@@ -316,86 +395,18 @@ __global__ void __launch_bounds__(TS_THREADS, TS_CTAS) token_scores_segment_kern
       if (below == 0ull) below = 1ull;  // (none is left: the rest stays 0)
     }
   }
+  if (JOINS) {
+    cluster_sync_all();  // (what the other CTAs have written is seen behind it)
+    if (cluster_ctarank() == 0 && warp == 0) token_scores_join<ST>(p, blockIdx.x / p.segments, reinterpret_cast<unsigned long long*>(ts_data));
+  }
 }
 
-// A warp per row joins its segments.
 template <typename ST>
 __global__ void __launch_bounds__(32) token_scores_join_kernel(TokenScoresParams p) {
-  extern __shared__ unsigned long long lists[];  // [segments][top], up to TS_JOIN_SEGMENTS
+  extern __shared__ unsigned long long lists[];
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x, lane = threadIdx.x;
-  const float* sums = p.sums + (int64_t)t * p.segments * 3;
-  const unsigned long long* best = p.best + (int64_t)t * p.segments * p.top;
-  const bool staged = p.segments <= TS_JOIN_SEGMENTS;
-  if (staged) {
-#pragma unroll 8
-    for (int i = lane; i < p.segments * p.top; i += 32) lists[i] = best[i];
-  }
-  const int64_t target = p.logprob ? p.target[t] : -1;
-  const float x = target >= 0 && target < p.V ? ts_load(static_cast<const ST*>(p.logits) + (int64_t)t * p.ld + target) : 0.f;
-  float M = -INFINITY;
-  bool bad = false;
-  for (int i = lane; i < p.segments; i += 32) {
-    M = fmaxf(M, sums[i * 3]);
-    bad |= sums[i * 3 + 2] != sums[i * 3 + 2];
-  }
-  M = warp_max_f32(M);
-  bad = __any_sync(0xffffffffu, bad) || !(fabsf(M) <= FLT_MAX);
-  int owner = 0x7fffffff;  // of the segments that hold the maximum, the one that leaves its 1 out
-  for (int i = lane; i < p.segments; i += 32)
-    if (sums[i * 3] == M) owner = min(owner, i);
-  owner = __reduce_min_sync(0xffffffffu, owner);
-  float S = 0.f, W = 0.f;
-  for (int i = lane; i < p.segments; i += 32) {
-    const float m = sums[i * 3];
-    if (m == -INFINITY) continue;
-    const float d = m - M, f = expf(d), s = sums[i * 3 + 1];
-    if (f == 0.f) continue;
-    S = fmaf(f, i == owner ? s : 1.f + s, S);
-    W = fmaf(f, fmaf(d, 1.f + s, sums[i * 3 + 2]), W);
-  }
-  S = warp_sum(S);
-  W = warp_sum(W);
-  const float none = __int_as_float(0x7fffffff), z = log1pf(S);
-  if (lane == 0) {
-    if (p.entropy) p.entropy[t] = bad ? none : z - W / (1.f + S);
-    if (p.logprob) p.logprob[t] = target < 0 ? 0.f : bad || target >= p.V ? none : (x - M) - z;
-  }
-  auto put = [&](int k, unsigned long long key) {
-    p.top_ids[(int64_t)t * p.top + k] = ts_index(key);
-    p.top_logprobs[(int64_t)t * p.top + k] = bad ? none : (ts_value(key) - M) - z;
-  };
-  if (staged) {  // lane i walks down the list of segment i: the largest of the heads, over and over
-    __syncwarp();
-    int at = 0;
-    unsigned long long head = lane < p.segments && p.top > 0 ? lists[lane * p.top] : 0ull, mine = 0ull;
-    for (int k = 0; k < p.top; ++k) {
-      const unsigned long long top = warp_max_key(head);
-      if (head == top) {
-        ++at;
-        head = at < p.top ? lists[lane * p.top + at] : 0ull;
-      }
-      if ((k & 31) == lane) mine = top;
-      if ((k & 31) == 31 || k + 1 == p.top)  // 32 results at a time
-        if ((k & ~31) + lane <= k) put((k & ~31) + lane, mine);
-    }
-    return;
-  }
-  unsigned long long below = ~0ull;  // lane i has the lists of segments i, i + 32, ...; keys differ
-  for (int k = 0; k < p.top; ++k) {
-    unsigned long long head = 0ull;
-    for (int i = lane; i < p.segments; i += 32)
-      for (int j = 0; j < p.top; ++j) {
-        const unsigned long long key = best[(int64_t)i * p.top + j];
-        if (key < below) {
-          head = max(head, key);
-          break;
-        }
-      }
-    below = warp_max_key(head);
-    if (lane == 0) put(k, below);
-  }
+  token_scores_join<ST>(p, blockIdx.x, lists);
 }
 
 }  // namespace mb200

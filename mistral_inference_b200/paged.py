@@ -17,6 +17,7 @@ from . import _abi_paged
 from ._abi import Mb200Error
 from ._abi_paged import HEAD_DIM, PAGE
 
+SOFTMAX_SCALE = HEAD_DIM ** -0.5
 _REASONS = {1: "a row out of range, or named twice", 2: "a length that is negative or longer than a row of the block table", 3: "more tokens than the plan has room for",
             4: "too few free pages", 16: "a wait inside attention ran out", 32: "a request of more tokens than the plan's `most`"}
 
@@ -61,8 +62,10 @@ class PageTables:
             assert t.dtype == torch.int32 and t.is_contiguous() and t.device == table.device, "contiguous int32 tensors of one device"
         assert table.dim() == 2 and lens.shape == table.shape[:1] and free.dim() == 1 and n_free.shape == (1,), (table.shape, lens.shape, free.shape, n_free.shape)
         self.table, self.lens, self.free, self.n_free = table, lens, free, n_free
+        self.device = _abi_paged.index_of(table)
         self.scratch = torch.zeros(1 + table.shape[0], dtype=torch.int32, device=table.device)
         self._every = torch.arange(table.shape[0], dtype=torch.int32, device=table.device)
+        self._first = {}  # number of requests -> their rows, where they are the first ones
 
     @staticmethod
     def empty(rows: int, max_pages: int, n_pages: int, device) -> "PageTables":
@@ -71,11 +74,14 @@ class PageTables:
         return PageTables(torch.full((rows, max_pages), -1, **i32), torch.zeros(rows, **i32), torch.arange(n_pages - 1, -1, -1, **i32), torch.full((1,), n_pages, **i32))
 
     def _requests(self, count: torch.Tensor, rows: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-        assert count.dtype == torch.int32 and count.dim() == 1 and count.shape[0] >= 1, "one int32 a request"
+        assert count.dtype is torch.int32 and count.dim() == 1 and count.shape[0] >= 1 and count.is_contiguous() and count.get_device() == self.device, f"one int32 a request, on cuda:{self.device}"
         if rows is None:
-            assert count.shape[0] <= self.table.shape[0], f"{count.shape[0]} requests, {self.table.shape[0]} rows"
-            return count, self._every[: count.shape[0]]
-        assert rows.dtype == torch.int32 and rows.shape == count.shape, "rows: one int32 a request"
+            B = count.shape[0]
+            if B not in self._first:
+                assert B <= self.table.shape[0], f"{B} requests, {self.table.shape[0]} rows"
+                self._first[B] = self._every[:B]
+            return count, self._first[B]
+        assert rows.dtype is torch.int32 and rows.shape == count.shape and rows.is_contiguous() and rows.get_device() == self.device, "rows: one int32 a request"
         return count, rows
 
     def extend(self, add: torch.Tensor, n_tokens: int, rows: Optional[torch.Tensor] = None, longest: Optional[int] = None, most: int = 0) -> PagePlan:
@@ -83,13 +89,12 @@ class PageTables:
         request takes more than `longest`, none has more than `most` afterwards (both sizes of launches; unknown: n_tokens, a whole row).  A step that cannot be done changes nothing
         and leaves the reason in the plan's status: `plan.check()` raises it."""
         add, rows = self._requests(add, rows)
-        B, dev = add.shape[0], self.table.device
-        n_tokens = int(n_tokens)
-        assert n_tokens >= 0
-        block = torch.empty(2 * n_tokens + 2 * B + 2, dtype=torch.int32, device=dev)
-        positions, slots, q_start, seqpos, status = block.split([n_tokens, n_tokens, B + 1, B, 1])
-        _abi_paged.pages_extend(self, rows, add, positions, slots, q_start, seqpos, status, n_tokens)
-        return PagePlan(self.table, rows, q_start, seqpos, positions, slots, max(1, n_tokens if longest is None else int(longest)), int(most), status)
+        B, T = add.shape[0], int(n_tokens)
+        assert T >= 0
+        block = torch.empty(2 * T + 2 * B + 2, dtype=torch.int32, device=self.table.device)
+        positions, slots, q_start, seqpos, status = torch.split_with_sizes(block, (T, T, B + 1, B, 1))
+        _abi_paged.pages_extend(self, rows, add, block, B, T)
+        return PagePlan(self.table, rows, q_start, seqpos, positions, slots, max(1, T if longest is None else int(longest)), int(most), status)
 
     def truncate(self, keep: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Request b keeps its first keep[b] tokens (0: it has ended).  Returns the status (see `check_status`)."""
@@ -105,21 +110,30 @@ def empty_pool(n_pages: int, n_kv_heads: int, device) -> Tuple[torch.Tensor, tor
             torch.ones(n_pages, n_kv_heads, 2, dtype=torch.float32, device=device))
 
 
-def _check_pool(kv: torch.Tensor, scale: torch.Tensor, plan: PagePlan) -> None:
-    assert kv.dim() == 5 and kv.shape[2:] == (2, PAGE, HEAD_DIM) and kv.dtype in (torch.float8_e4m3fn, torch.uint8), f"pool [pages, heads, 2, {PAGE}, {HEAD_DIM}] of e4m3, got {tuple(kv.shape)} {kv.dtype}"
-    assert scale.shape == kv.shape[:3] and scale.dtype == torch.float32, f"one fp32 scale for each page, head and kind, got {tuple(scale.shape)} {scale.dtype}"
-    B, T = plan.rows.shape[0], plan.slots.shape[0]
-    assert plan.q_start.shape == (B + 1,) and plan.seqpos.shape == (B,) and plan.positions.shape == (T,) and plan.table.dim() == 2 and plan.longest >= 1, "a plan of PageTables.extend"
-    assert all(t.dtype == torch.int32 for t in (plan.table, plan.rows, plan.q_start, plan.seqpos, plan.slots)), "plans are int32"
+_I32, _CODES = torch.int32, (torch.float8_e4m3fn, torch.uint8)
+
+
+def _pool(kv: torch.Tensor, scale: torch.Tensor, plan: PagePlan) -> Tuple[int, int, int]:
+    """(device, pages, key/value heads) of a pool that a plan's tokens go into or attend over, all of it checked."""
+    N, KV, kinds, tokens, dim = kv.shape
+    dev = _abi_paged.index_of(kv)
+    assert kinds == 2 and tokens == PAGE and dim == HEAD_DIM and kv.dtype in _CODES and kv.is_contiguous(), f"pool [pages, heads, 2, {PAGE}, {HEAD_DIM}] of e4m3, got {tuple(kv.shape)} {kv.dtype}"
+    assert scale.shape == (N, KV, 2) and scale.dtype is torch.float32 and scale.is_contiguous() and scale.get_device() == dev, f"one fp32 scale for each page, head and kind, got {tuple(scale.shape)} {scale.dtype}"
+    B = plan.rows.shape[0]
+    assert plan.q_start.shape[0] == B + 1 and plan.seqpos.shape[0] == B and plan.longest >= 1, "a plan of PageTables.extend"
+    for t in (plan.rows, plan.q_start, plan.seqpos, plan.slots):
+        assert t.dtype is _I32 and t.get_device() == dev and t.is_contiguous(), f"plans are contiguous int32 tensors on cuda:{dev}, got {t.dtype} on {t.device}"
+    return dev, N, KV
 
 
 def write_pages(kv: torch.Tensor, scale: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PagePlan) -> None:
     """Keys and values [T, heads, 128] (or [T, heads * 128]; bf16) of the plan's tokens into the pool.  A page's scale for a head is the smallest power of two under which all
     of its tokens' numbers fit e4m3; it grows with later tokens.  Numbers that are not finite are kept as NaN."""
-    _check_pool(kv, scale, plan)
-    assert k.shape[0] == v.shape[0] == plan.slots.shape[0], f"{plan.slots.shape[0]} tokens planned, keys of {k.shape[0]}, values of {v.shape[0]}"
-    if k.shape[0]:
-        _abi_paged.pages_write(kv, scale, k, v, plan)
+    dev, N, KV = _pool(kv, scale, plan)
+    T = plan.slots.shape[0]
+    assert k.shape[0] == T and v.shape[0] == T, f"{T} tokens planned, keys of {k.shape[0]}, values of {v.shape[0]}"
+    if T:
+        _abi_paged.pages_write(dev, kv, scale, k, v, plan, T, N, KV)
 
 
 def attend_pages(q: torch.Tensor, kv: torch.Tensor, scale: torch.Tensor, plan: PagePlan, window: int = 0, softmax_scale: Optional[float] = None,
@@ -127,14 +141,17 @@ def attend_pages(q: torch.Tensor, kv: torch.Tensor, scale: torch.Tensor, plan: P
     """[T, H * 128] bf16: attention of the queries [T, H, 128] (or [T, H * 128]; bf16) of the plan's tokens, whose own keys and values have been written before.  A query sees the
     last `window` positions of its request up to its own (0: all).  H is a multiple of the pool's heads, at most 32 times as many.  Rows of `out` behind the plan's last
     token stay as they are."""
-    _check_pool(kv, scale, plan)
-    assert q.dim() in (2, 3) and q.shape[0] == plan.slots.shape[0], f"{plan.slots.shape[0]} tokens planned, queries {tuple(q.shape)}"
-    width = q.shape[1] * q.shape[2] if q.dim() == 3 else q.shape[1]
+    dev, N, KV = _pool(kv, scale, plan)
+    T, width = q.shape[0], q.shape[1] * q.shape[2] if q.dim() == 3 else q.shape[1]
+    assert T == plan.slots.shape[0], f"{plan.slots.shape[0]} tokens planned, queries {tuple(q.shape)}"
     H = width // HEAD_DIM
-    assert width == H * HEAD_DIM and H >= 1 and H % kv.shape[1] == 0, f"{width} columns of queries, {kv.shape[1]} key/value heads"
+    assert width == H * HEAD_DIM and H >= 1 and H % KV == 0, f"{width} columns of queries, {KV} key/value heads"
+    R, P = plan.table.shape
+    assert plan.table.dtype is _I32 and plan.table.is_contiguous() and plan.table.get_device() == dev, f"block table: contiguous int32 on cuda:{dev}"
     if out is None:
-        out = torch.empty(q.shape[0], width, dtype=torch.bfloat16, device=kv.device)
-    assert out.shape == (q.shape[0], width) and out.dtype == torch.bfloat16, f"out [T, {width}] bf16, got {tuple(out.shape)} {out.dtype}"
-    if q.shape[0]:
-        _abi_paged.attn_pages(q, kv, scale, plan, out, H, int(window), HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale))
+        out = torch.empty((T, width), dtype=torch.bfloat16, device=kv.device)
+    else:
+        assert out.shape == (T, width) and out.dtype is torch.bfloat16 and out.is_contiguous() and out.get_device() == dev, f"out [T, {width}] bf16, got {tuple(out.shape)} {out.dtype}"
+    if T:
+        _abi_paged.attn_pages(dev, q, kv, scale, plan, out, T, N, KV, H, R, P, int(window), SOFTMAX_SCALE if softmax_scale is None else float(softmax_scale))
     return out

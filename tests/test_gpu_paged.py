@@ -84,6 +84,23 @@ def test_steps_that_cannot_be_done_change_nothing():
         assert_same_state(t, h)
 
 
+def test_tables_refuse_what_they_cannot_take():
+    t = mi.PageTables.empty(2, 4, 8, DEV)
+    with pytest.raises(AssertionError):
+        t.extend(ints([1, 1, 1]), 3)  # more requests than rows
+    with pytest.raises(AssertionError):
+        t.extend(torch.ones(2, device=DEV), 2)
+    with pytest.raises(AssertionError):
+        t.extend(torch.ones(2, dtype=torch.int32), 2)
+    with pytest.raises(AssertionError):
+        t.extend(ints([1, 7, 1, 7])[::2], 2)
+    with pytest.raises(AssertionError):
+        t.truncate(ints([1, 1]), rows=ints([1]))
+    with pytest.raises(_abi_paged.Mb200Error, match="requests"):
+        big = mi.PageTables.empty(_abi_paged.MAX_REQUESTS + 1, 1, 8, DEV)
+        big.extend(torch.zeros(_abi_paged.MAX_REQUESTS + 1, dtype=torch.int32, device=DEV), 0)
+
+
 def test_many_requests_at_once():
     B = _abi_paged.MAX_REQUESTS
     t, h = mi.PageTables.empty(B, 2, 2 * B, DEV), U.HostTables(B, 2, 2 * B)

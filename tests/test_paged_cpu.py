@@ -104,15 +104,8 @@ def test_python_refuses_what_it_cannot_take():
         mi.PageTables(table, lens[:1], free, n_free)
     with pytest.raises(AssertionError):
         mi.PageTables(table[:, ::2], lens, free, n_free)
-    t = mi.PageTables(table, lens, free, n_free)
-    with pytest.raises(AssertionError):
-        t.extend(torch.ones(3, dtype=torch.int32), 3)  # more requests than rows
-    with pytest.raises(AssertionError):
-        t.extend(torch.ones(2), 2)
-    with pytest.raises(AssertionError):
-        t.truncate(torch.ones(2, dtype=torch.int32), rows=torch.ones(1, dtype=torch.int32))
     with pytest.raises(AssertionError, match="CUDA"):  # no fallback
-        t.extend(torch.ones(2, dtype=torch.int32), 2)
+        mi.PageTables(table, lens, free, n_free)
     i = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     plan = mi.PagePlan(table, i(0), i(0, 1), i(0), i(0), i(0), 1)
     kv, scale = torch.zeros(4, 2, 2, 64, 128, dtype=torch.uint8), torch.ones(4, 2, 2)
