@@ -11,5 +11,5 @@ from .generate import generate  # noqa: F401  (the function; the submodule stays
 from .transformer import Transformer  # noqa: F401
 from .layered import LayeredTransformer  # noqa: F401
 from .registry import load_model  # noqa: F401
-from .paged import PagePlan, PageTables, attend_pages, write_pages  # noqa: F401
+from .paged import PagedCache, PagePlan, PageTables, attend_pages, write_pages  # noqa: F401
 from .scores import TokenScores, token_scores  # noqa: F401

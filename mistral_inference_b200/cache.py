@@ -79,6 +79,7 @@ class CacheInputMetadata:
 
 class CacheView:
     """cache.py:70-137: one layer's ring plus the metadata of this forward."""
+    paged = False
 
     def __init__(self, cache_k: Optional[torch.Tensor], cache_v: Optional[torch.Tensor], metadata: CacheInputMetadata, kv_seqlens_host: List[int],
                  state: Optional[torch.Tensor] = None, conv: Optional[torch.Tensor] = None):
@@ -108,6 +109,7 @@ class CacheView:
 
 class BufferCache:
     """Rectangular rotating cache; constructor and methods as cache.py:140-195."""
+    paged = False  # (paged.PagedCache)
 
     def __init__(self, n_layers: int, max_batch_size: int, max_seq_len: int, n_kv_heads: int, head_dim: int,
                  sliding_window: SlidingWindow = None, layer_specs: Optional[List[LayerCacheSpec]] = None):

@@ -13,13 +13,17 @@ scalar per token back to the host (`.item()`), and in the decode loop it syncs t
   * the decode loop keeps tokens, log-probabilities and the eos flags on the device: pick (fused argmax of the decode kernel /
     `mb200_argmax_rows` / `mb200_sample_top_p`), `mb200_logprob_gather`, next step -- no host round trip per token; results
     come back with one copy at the end (with `eos_id` the flags are polled every EOS_POLL steps and the tail is dropped).
+Beyond the reference: `kv_cache="pages"` keeps keys and values in 8-bit pages that the sequences share (paged.py); `alternatives` asks, beside each log-probability, for the
+entropy of its distribution and the most likely tokens (scores.py).
 """
-from typing import List, Optional, Tuple
+from dataclasses import dataclass
+from typing import List, Optional, Tuple, Union
 
 import torch
 
 from . import _abi
 from .cache import BufferCache
+from .scores import TokenScores, empty_scores, token_scores
 from .transformer import Transformer
 
 TOP_P = 0.8     # generate.py:126
@@ -52,10 +56,23 @@ class _PromptPlan:
             self.chunks.append((flat, [len(x) for x in pieces], targets, where))
 
 
+@dataclass
+class TokenDetail:
+    """Beside a token's log-probability: the distribution that it was picked (or, in a prompt, scored) from."""
+    entropy: float         # nats
+    top_ids: List[int]     # the most likely tokens ...
+    top_logprobs: List[float]  # ... and their log-probabilities
+
+
+def _details(s: TokenScores) -> List[TokenDetail]:
+    return [TokenDetail(e, i, p) for e, i, p in zip(s.entropy.tolist(), s.top_ids.tolist(), s.top_logprobs.tolist())]
+
+
 @torch.inference_mode()
 def generate(encoded_prompts: List[List[int]], model: Transformer, images: List[List] = [], *, max_tokens: int,  # noqa: B006
-             temperature: float, chunk_size: Optional[int] = None, eos_id: Optional[int] = None
-             ) -> Tuple[List[List[int]], List[List[float]]]:
+             temperature: float, chunk_size: Optional[int] = None, eos_id: Optional[int] = None, kv_cache: str = "ring", alternatives: int = 0
+             ) -> Union[Tuple[List[List[int]], List[List[float]]], Tuple[List[List[int]], List[List[float]], List[List[TokenDetail]]]]:
+    """(tokens, logprobs) as above; with `alternatives` > 0 also a TokenDetail for each log-probability, with so many of the most likely tokens."""
     assert not images, "vision inputs are outside the accelerated hot path"
     model = model.eval()
     dev = model.device
@@ -63,15 +80,21 @@ def generate(encoded_prompts: List[List[int]], model: Transformer, images: List[
     B, V = plan.B, model.args.vocab_size
 
     # one ring per layer, sized like the reference's (generate.py:68-78)
-    cache = model.make_cache(model.args.max_batch_size, max(plan.lens) + max_tokens)
+    cache = model.make_cache(model.args.max_batch_size, max(plan.lens) + max_tokens, **({} if kv_cache == "ring" else {"kv_cache": kv_cache}))
 
     # ---- prompt: hidden states chunk by chunk, log-probabilities fused with the lm head ----
     prompt_lp: List[torch.Tensor] = []
+    prompt_scores: List[TokenScores] = []
     last_logits: Optional[torch.Tensor] = None
     for flat, seqlens, targets, _ in plan.chunks:
         ids = torch.tensor(flat, dtype=torch.long, device=dev)
         tgt = torch.tensor(targets, dtype=torch.long, device=dev)
-        lp, last_logits = model.forward_logprobs(ids, seqlens, cache, tgt)
+        if alternatives:
+            scores, last_logits = model.forward_scores(ids, seqlens, cache, tgt, alternatives)
+            prompt_scores.append(scores)
+            lp = scores.logprob
+        else:
+            lp, last_logits = model.forward_logprobs(ids, seqlens, cache, tgt)
         prompt_lp.append(lp)
     assert last_logits is not None and last_logits.shape == (B, V)
 
@@ -79,13 +102,17 @@ def generate(encoded_prompts: List[List[int]], model: Transformer, images: List[
     steps_run = 0
     gen_tok = torch.zeros(max(max_tokens, 1), B, dtype=torch.long, device=dev)       # [step, b]: each step's row is contiguous
     gen_lp = torch.zeros(max(max_tokens, 1), B, dtype=torch.float32, device=dev)
+    gen_scores = empty_scores(max(max_tokens, 1) * B, alternatives, True, dev) if alternatives else None
     all_done = torch.zeros(max(max_tokens, 1), dtype=torch.bool, device=dev)         # all_done[s]: every sequence finished at step s
     finished = torch.zeros(B, dtype=torch.bool, device=dev)
     stop_at = max_tokens
     for step in range(max_tokens):
         nxt = gen_tok[step]
         pick(last_logits, temperature, TOP_P, out=nxt, fused_argmax=model.last_argmax if model.last_argmax_valid_for(last_logits) else None)
-        _abi.logprob_gather(last_logits, nxt, out=gen_lp[step])
+        if gen_scores is not None:
+            token_scores(last_logits, nxt, top=alternatives, out=gen_scores.rows(step * B, step * B + B))
+        else:
+            _abi.logprob_gather(last_logits, nxt, out=gen_lp[step])
         if eos_id is not None:
             finished |= nxt == eos_id
             all_done[step] = finished.all()
@@ -102,6 +129,8 @@ def generate(encoded_prompts: List[List[int]], model: Transformer, images: List[
     else:
         stop_at = steps_run
     tokens: List[List[int]] = gen_tok[:stop_at].t().tolist() if stop_at > 0 else []
+    if gen_scores is not None:
+        gen_lp = gen_scores.logprob.view(-1, B)
     gen_lp_host = gen_lp[:stop_at].t().tolist() if stop_at > 0 else [[] for _ in range(B)]
     logprobs: List[List[float]] = [[] for _ in range(B)]
     for (_, _, targets, where), lp in zip(plan.chunks, prompt_lp):
@@ -110,7 +139,16 @@ def generate(encoded_prompts: List[List[int]], model: Transformer, images: List[
                 logprobs[b].append(v)
     for b in range(B):
         logprobs[b].extend(gen_lp_host[b])
-    return tokens, logprobs
+    if gen_scores is None:
+        return tokens, logprobs
+    details: List[List[TokenDetail]] = [[] for _ in range(B)]
+    for (_, _, targets, where), s in zip(plan.chunks, prompt_scores):
+        for (b, _), t, d in zip(where, targets, _details(s)):
+            if t >= 0:
+                details[b].append(d)
+    for i, d in enumerate(_details(gen_scores.rows(0, stop_at * B))):
+        details[i % B].append(d)
+    return tokens, logprobs, details
 
 
 def pick(logits: torch.Tensor, temperature: float, top_p: float, out: Optional[torch.Tensor] = None,

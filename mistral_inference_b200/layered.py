@@ -21,6 +21,7 @@ from torch import nn
 from . import _abi, _abi_hybrid as _h
 from .args import LayeredArgs
 from .cache import BufferCache, CacheInputMetadata
+from .scores import TokenScores, token_scores
 from .transformer_layers import FEED_FORWARDS, MIXERS, MIXERS_BY_ARGS, BiasedAttention, LayeredBlock, LightningMixer, Norm
 
 
@@ -66,10 +67,12 @@ class LayeredTransformer(nn.Module):
     def device(self) -> torch.device:
         return self.embed.device
 
-    def make_cache(self, max_batch_size: int, max_seq_len: int) -> BufferCache:
+    def make_cache(self, max_batch_size: int, max_seq_len: int, kv_cache: str = "ring") -> BufferCache:
         """The cache of this model, one entry per layer RUN (a layer that runs in several passes keeps each pass's keys apart): a
         whole-sequence ring per attention layer, an fp32 state per lightning layer.  A layer that reads another layer's keys and values
         shares the ring of that layer's latest run before its own."""
+        if kv_cache != "ring":
+            raise ValueError(f"kv_cache {kv_cache!r}: layered decoders keep rings and states")
         specs = [self.layers[i].mix.cache_spec() for i in self.runs]
         for r, sp in enumerate(specs):
             if sp.kind == "shared":  # the mixer names a layer; the cache wants its run
@@ -228,6 +231,13 @@ class LayeredTransformer(nn.Module):
         lp = _abi.logprob_gather(logits, targets)
         last_idx = torch.tensor(seqlens, device=input_ids.device).cumsum(0) - 1
         return lp, logits.index_select(0, last_idx)
+
+    @torch.inference_mode()
+    def forward_scores(self, input_ids: torch.Tensor, seqlens: List[int], cache: Optional[BufferCache], targets: torch.Tensor, top: int) -> Tuple[TokenScores, torch.Tensor]:
+        """`forward_logprobs` with the entropy of every token's distribution and its `top` most likely tokens (scores.py)."""
+        logits = self.forward(input_ids, seqlens, cache).float().contiguous()
+        last_idx = torch.tensor(seqlens, device=input_ids.device).cumsum(0) - 1
+        return token_scores(logits, targets, top=top), logits.index_select(0, last_idx)
 
     # ------------------------------------------------------------------ weights
     def _assign(self, k: str, v: torch.Tensor) -> None:

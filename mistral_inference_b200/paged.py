@@ -5,17 +5,19 @@ half of its 16-bit bytes to read.
                 of new tokens of each request), `truncate` takes tokens back.
   write_pages   keys and values of a plan's tokens into one layer's pool
   attend_pages  causal attention of a plan's tokens over that pool
+  PagedCache    pools of all layers with their block tables, in the place of a BufferCache: `Transformer.make_cache(..., kv_cache="pages")`
 
 A page holds 64 tokens of one request, for every key/value head: [2 (keys, values), 64, 128] e4m3 numbers and one power of two as scale for each head and kind.  All of
 it runs in libmb200_paged.so (include/mistral_b200_paged.h)."""
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
 from . import _abi_paged
 from ._abi import Mb200Error
 from ._abi_paged import HEAD_DIM, PAGE
+from .cache import SlidingWindow, get_cache_sizes, upload
 
 SOFTMAX_SCALE = HEAD_DIM ** -0.5
 _REASONS = {1: "a row out of range, or named twice", 2: "a length that is negative or longer than a row of the block table", 3: "more tokens than the plan has room for",
@@ -155,3 +157,193 @@ def attend_pages(q: torch.Tensor, kv: torch.Tensor, scale: torch.Tensor, plan: P
     if T:
         _abi_paged.attn_pages(dev, q, kv, scale, plan, out, T, N, KV, H, R, P, int(window), SOFTMAX_SCALE if softmax_scale is None else float(softmax_scale))
     return out
+
+
+class PageLedger:
+    """The host's account of a PagedCache: which row each live request has, its tokens, and how many pages are free.  It knows before a step is launched whether there is room."""
+
+    def __init__(self, rows: int, max_seq_len: int, n_pages: int):
+        self.max_seq_len, self.n_pages = max_seq_len, n_pages
+        self.free_rows = list(range(rows - 1, -1, -1))
+        self.rows: List[int] = []  # of the live requests, in batch order
+        self.lens: List[int] = []  # their tokens
+
+    @property
+    def free_pages(self) -> int:
+        return self.n_pages - sum(pages_of(n) for n in self.lens)
+
+    def admit(self, n: int) -> None:
+        if n > len(self.free_rows):
+            raise ValueError(f"{n} more requests in a cache with {len(self.free_rows)} free rows")
+        for _ in range(n):
+            self.rows.append(self.free_rows.pop())
+            self.lens.append(0)
+
+    def retire(self, indices: List[int]) -> None:
+        gone = set(indices)
+        assert all(0 <= i < len(self.rows) for i in gone), indices
+        self.free_rows += [self.rows[i] for i in sorted(gone, reverse=True)]
+        keep = [i for i in range(len(self.rows)) if i not in gone]
+        self.rows, self.lens = [self.rows[i] for i in keep], [self.lens[i] for i in keep]
+
+    def check(self, seqlens: List[int]) -> None:
+        """Raises if the live requests cannot take so many more tokens each."""
+        if len(seqlens) != len(self.rows):
+            raise ValueError(f"Batch size is {len(self.rows)}, got {len(seqlens)}, did you forget to reset cache?")
+        if min(seqlens) < 0 or sum(seqlens) < 1:
+            raise ValueError(f"new tokens of each request: {seqlens}")
+        if max(n + a for n, a in zip(self.lens, seqlens)) > self.max_seq_len:
+            raise ValueError(f"a request of more than {self.max_seq_len} tokens")
+        need = sum(pages_of(n + a) - pages_of(n) for n, a in zip(self.lens, seqlens))
+        if need > self.free_pages:
+            raise ValueError(f"{need} more pages needed, {self.free_pages} of {self.n_pages} free")
+
+
+@dataclass
+class PagedInputMetadata:
+    """What one layer's kernels need for this forward (CacheInputMetadata's part for pages)."""
+    plan: PagePlan
+    positions: torch.Tensor
+    q_start: torch.Tensor
+    seqpos: torch.Tensor
+    prefill: bool
+    first_prefill: bool  # nothing cached before for any request
+    seqlens: List[int]
+    max_seqlen: int
+    window: int          # positions that a query sees, itself included
+
+
+class PagedView:
+    """One layer's pool plus the metadata of this forward."""
+    paged = True
+
+    def __init__(self, kv: torch.Tensor, scale: torch.Tensor, metadata: PagedInputMetadata, windowed: bool):
+        self.kv, self.scale, self.metadata, self.windowed = kv, scale, metadata, windowed
+
+    def write(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        write_pages(self.kv, self.scale, k, v, self.metadata.plan)
+
+    def attend(self, q: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+        return attend_pages(q, self.kv, self.scale, self.metadata.plan, window=self.metadata.window if self.windowed else 0, out=out)
+
+
+class PagedCache:
+    """Keys and values of a running batch in 8-bit pages, with a BufferCache's methods for `Transformer.forward` and `generate()`.  Requests take pages as they grow and share
+    n_pages of them (by default as many as all rows of max_seq_len tokens need); they can be retired from a running batch and others admitted to it (`seqlens` of a
+    forward then has a 0 for those that bring nothing).  A request's pages are kept for its whole length, also behind a sliding window."""
+    paged = True
+
+    def __init__(self, n_layers: int, max_batch_size: int, max_seq_len: int, n_kv_heads: int, head_dim: int, sliding_window: SlidingWindow = None, n_pages: Optional[int] = None,
+                 device: torch.device = torch.device("cuda")):
+        assert head_dim == HEAD_DIM, f"pages hold heads of {HEAD_DIM} dimensions, got {head_dim}"
+        assert max_batch_size <= _abi_paged.MAX_REQUESTS, f"at most {_abi_paged.MAX_REQUESTS} requests"
+        self.n_layers, self.max_batch_size, self.max_seq_len, self.n_kv_heads, self.head_dim = n_layers, max_batch_size, max_seq_len, n_kv_heads, head_dim
+        self.cache_sizes = get_cache_sizes(n_layers, max_seq_len, sliding_window)
+        self.windowed = [w is not None for w in (sliding_window * (n_layers // len(sliding_window)) if isinstance(sliding_window, list) else [sliding_window] * n_layers)]
+        each = pages_of(max_seq_len)
+        self.n_pages = max_batch_size * each if n_pages is None else n_pages
+        self.tables = PageTables.empty(max_batch_size, each, self.n_pages, device)
+        self.pools = [empty_pool(self.n_pages, n_kv_heads, device) for _ in range(n_layers)]
+        self.reset()
+
+    # -- the batch ------------------------------------------------------------------------------
+    def reset(self) -> None:
+        """No requests: every page is free."""
+        t = self.tables
+        t.table.fill_(-1)
+        t.lens.zero_()
+        t.free.copy_(torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32))
+        t.n_free.fill_(self.n_pages)
+        self.ledger = PageLedger(self.max_batch_size, self.max_seq_len, self.n_pages)
+        self._on_device: List[int] = []  # tokens of the live requests in the block tables (a forward that failed may have left more than the ledger says)
+        self._rows_dev: Optional[torch.Tensor] = None
+        self._started = False
+        self.__dict__.pop("_mb200_decode_states", None)
+
+    def init_kvseqlens(self, batch_size: int) -> None:
+        assert not self._started, "a batch is running: reset() first, or admit() more requests"
+        self.admit(batch_size)
+
+    def _batch_changed(self) -> None:
+        self._rows_dev = None
+        self.__dict__.pop("_mb200_decode_states", None)  # captured decode graphs are per batch size and row set
+
+    def admit(self, n: int = 1) -> List[int]:
+        """n more requests, without tokens yet; their places in the batch order (the last ones)."""
+        self.ledger.admit(n)
+        self._on_device += [0] * n
+        self._started = True
+        self._batch_changed()
+        return list(range(len(self.ledger.rows) - n, len(self.ledger.rows)))
+
+    def retire(self, indices: List[int]) -> None:
+        """Requests `indices` (places in the batch order) have ended: their pages and rows are free, the others keep their order."""
+        gone = sorted(set(indices))
+        rows = [self.ledger.rows[i] for i in gone]
+        self.ledger.retire(gone)
+        if rows:
+            self.tables.truncate(self._ints([0] * len(rows)), self._ints(rows))
+        self._on_device = [n for i, n in enumerate(self._on_device) if i not in set(gone)]
+        self._batch_changed()
+
+    @property
+    def rows(self) -> List[int]:
+        return self.ledger.rows
+
+    @property
+    def _kv_seqlens_host(self) -> Optional[List[int]]:
+        return self.ledger.lens if self._started else None
+
+    @property
+    def kv_seqlens(self) -> Optional[torch.Tensor]:
+        return torch.tensor(self.ledger.lens, device=self.device, dtype=torch.long) if self._started else None
+
+    @property
+    def device(self) -> torch.device:
+        return self.tables.table.device
+
+    def update_seqlens(self, seqlens: List[int]) -> None:
+        """After a forward: its tokens count.  Negative numbers take (drafted) tokens back."""
+        lens = [n + a for n, a in zip(self.ledger.lens, seqlens)]
+        assert len(seqlens) == len(lens) and all(0 <= n <= d for n, d in zip(lens, self._on_device)), (self.ledger.lens, seqlens)
+        self.ledger.lens = lens
+
+    # -- metadata ---------------------------------------------------------------------------------
+    def _ints(self, values: List[int]) -> torch.Tensor:
+        return upload(torch.tensor(values, dtype=torch.int32), self.device)
+
+    def rows_on_device(self) -> torch.Tensor:
+        if self._rows_dev is None:
+            self._rows_dev = self._ints(self.ledger.rows)
+        return self._rows_dev
+
+    def settle(self) -> None:
+        """Tokens that the ledger does not count leave the block tables."""
+        if self._on_device != self.ledger.lens:
+            self.tables.truncate(self._ints(self.ledger.lens), self.rows_on_device())
+            self._on_device = list(self.ledger.lens)
+
+    def planned(self, seqlens: List[int]) -> None:
+        """The block tables hold `seqlens` more tokens of each request (planned here, or by a captured step)."""
+        self._on_device = [n + a for n, a in zip(self.ledger.lens, seqlens)]
+
+    def metadata_of(self, plan: PagePlan, seqlens: List[int]) -> List[PagedInputMetadata]:
+        """One per layer (shared by layers of one window)."""
+        first, longest = not any(self.ledger.lens), max(seqlens)
+        per_w = {w: PagedInputMetadata(plan, plan.positions, plan.q_start, plan.seqpos, first or longest > 1, first, list(seqlens), longest, w) for w in set(self.cache_sizes)}
+        return [per_w[w] for w in self.cache_sizes]
+
+    def get_input_metadata(self, seqlens: List[int]) -> List[PagedInputMetadata]:
+        seqlens = [int(n) for n in seqlens]
+        if not self._started:
+            self.init_kvseqlens(len(seqlens))
+        self.ledger.check(seqlens)
+        self.settle()
+        most = max(n + a for n, a in zip(self.ledger.lens, seqlens))
+        plan = self.tables.extend(self._ints(seqlens), sum(seqlens), self.rows_on_device(), longest=max(seqlens), most=most)
+        self.planned(seqlens)
+        return self.metadata_of(plan, seqlens)
+
+    def get_view(self, layer_id: int, metadata: PagedInputMetadata) -> PagedView:
+        kv, scale = self.pools[layer_id]
+        return PagedView(kv, scale, metadata, self.windowed[layer_id])

@@ -18,7 +18,9 @@ from torch import nn
 from . import _abi
 from .args import TransformerArgs
 from .cache import BufferCache, CacheInputMetadata, upload
+from .paged import PagedCache
 from .rope import precompute_freqs_cis
+from .scores import TokenScores, empty_scores, token_scores
 from .transformer_layers import RMSNorm, TransformerBlock
 
 ROPE_TABLE_LEN = 128_000  # transformer.py:116
@@ -136,8 +138,13 @@ class Transformer(nn.Module):
             self._ws_tokens = num_tokens
         return self._ws
 
-    def make_cache(self, max_batch_size: int, max_seq_len: int) -> BufferCache:
-        """The cache of this model on its device: one ring per local layer, sized like the reference's (generate.py:68-78)."""
+    def make_cache(self, max_batch_size: int, max_seq_len: int, kv_cache: str = "ring", n_pages: Optional[int] = None) -> Union[BufferCache, PagedCache]:
+        """The cache of this model on its device: one ring per local layer, sized like the reference's (generate.py:68-78), or kv_cache "pages": 8-bit pages that requests
+        take as they grow (n_pages of 64 tokens in all; paged.py)."""
+        if kv_cache == "pages":
+            return PagedCache(self.n_local_layers, max_batch_size, max_seq_len, self.args.n_kv_heads, self.args.head_dim, self.args.sliding_window, n_pages, self.device)
+        if kv_cache != "ring" or n_pages is not None:
+            raise ValueError(f"kv_cache {kv_cache!r} (ring, or pages with n_pages or without)")
         cache = BufferCache(self.n_local_layers, max_batch_size, max_seq_len, self.args.n_kv_heads, self.args.head_dim, self.args.sliding_window)
         cache.to(device=self.device, dtype=self.dtype)
         cache.reset()
@@ -337,7 +344,7 @@ class Transformer(nn.Module):
         round-1 design and a race).  Returns the STATIC fp32 logits buffer [B, V] (overwritten by the next step).  The first call
         per (cache, batch) runs eagerly (warm-up: loads modules, sets function attributes), the second captures."""
         B = tokens.shape[0]
-        if self._megakernel_ok(B):
+        if self._megakernel_ok(B) and not cache.paged:
             return self._decode_megakernel(tokens, cache)
         seqlens = [1] * B
         self.workspace(B)
@@ -354,14 +361,22 @@ class Transformer(nn.Module):
                        "meta": torch.zeros(3 * B + 1 + 2 * B * len(distinct), dtype=torch.int32, device=self.device),
                        "logits": torch.empty(B, self.vocab_size, dtype=torch.float32, device=self.device),
                        "next": torch.zeros(B, dtype=torch.long, device=self.device)})
-        if st["expected"] != host:  # another forward() advanced the cache since the last step (or this is the first one)
+            if cache.paged:
+                st.update({"one": torch.ones(B, dtype=torch.int32, device=self.device), "rows": cache.rows_on_device()})
+        if cache.paged:
+            cache.ledger.check(seqlens)  # (the captured plan finds its pages)
+            cache.settle()
+        elif st["expected"] != host:  # another forward() advanced the cache since the last step (or this is the first one)
             st["seqpos"].copy_(torch.tensor(host, dtype=torch.int32))  # pageable source: staged by the runtime, no reuse hazard
         st["tokens"].copy_(tokens, non_blocking=True)  # device source (previous pick): D2D; host source: staged by the runtime
         layout = {"T": B, "B": B, "prefill": False, "first_prefill": False, "max_seqlen": 1, "windows": distinct}
-        md = cache.metadata_from_block(st["meta"], layout, seqlens)
 
         def run() -> None:
-            _abi.decode_meta(st["seqpos"], st["meta"], distinct)
+            if cache.paged:  # block tables and slot map: a captured step takes its pages when it is replayed
+                md = cache.metadata_of(cache.tables.extend(st["one"], B, st["rows"], longest=1, most=cache.max_seq_len), seqlens)
+            else:
+                md = cache.metadata_from_block(st["meta"], layout, seqlens)
+                _abi.decode_meta(st["seqpos"], st["meta"], distinct)
             h = self._hidden_no_norm(st["tokens"], seqlens, cache, md)
             _abi.lm_head(h, self.norm.weight, self.output_weight, st["logits"], self.args.norm_eps, self.workspace(B))
             _abi.argmax_rows(st["logits"], st["next"])  # greedy pick on the device (generate.py:156): feeds the next step
@@ -377,6 +392,8 @@ class Transformer(nn.Module):
             g.replay()
         else:
             st["graph"].replay()
+        if cache.paged:
+            cache.planned(seqlens)
         cache.update_seqlens(seqlens)
         st["expected"] = list(cache._kv_seqlens_host)
         self.last_argmax = st["next"]
@@ -436,6 +453,36 @@ class Transformer(nn.Module):
         for r0, r1 in zip(bounds, bounds[1:]):
             _abi.lm_head_logprobs(h[r0:r1], self.norm.weight, self.output_weight, targets[r0:r1], keep[r0:r1], last_logits, lp[r0:r1], self.args.norm_eps, ws)
         return lp, last_logits
+
+    @torch.inference_mode()
+    def forward_scores(self, input_ids: torch.Tensor, seqlens: List[int], cache: Optional[Union[BufferCache, PagedCache]], targets: torch.Tensor, top: int
+                       ) -> Tuple[TokenScores, torch.Tensor]:
+        """`forward_logprobs` with the entropy of every token's distribution and its `top` most likely tokens (scores.py): the logits are written block by block."""
+        self._last_static_logits = 0
+        T, V = input_ids.shape[0], self.vocab_size
+        ends = list(itertools.accumulate(seqlens))
+        last_rows = torch.tensor([e - 1 for e in ends], device=input_ids.device)
+        if self.num_pipeline_ranks > 1:
+            logits = self.forward(input_ids, seqlens, cache).float().contiguous()
+            return token_scores(logits, targets, top=top), logits.index_select(0, last_rows)
+        self._check_runnable()
+        h = self._hidden_no_norm(input_ids, seqlens, cache)
+        if cache is not None:
+            cache.update_seqlens(seqlens)
+        assert self.norm is not None and self.output_weight is not None
+        ws = self.workspace(max(T, 1))
+        rows = max(128, (256 << 20) // (4 * V))
+        block = torch.empty(min(rows, T), V, dtype=torch.float32, device=h.device)
+        last_logits = torch.empty(len(ends), V, dtype=torch.float32, device=h.device)
+        out = empty_scores(T, top, True, h.device)
+        for r0 in range(0, T, rows):
+            r1 = min(T, r0 + rows)
+            _abi.lm_head(h[r0:r1], self.norm.weight, self.output_weight, block[: r1 - r0], self.args.norm_eps, ws)
+            token_scores(block[: r1 - r0], targets[r0:r1], top=top, out=out.rows(r0, r1))
+            for b, e in enumerate(ends):
+                if r0 < e <= r1:
+                    last_logits[b].copy_(block[e - 1 - r0])
+        return out, last_logits
 
     def _logprobs_of_written_logits(self, h: torch.Tensor, targets: torch.Tensor, ends: List[int], lp: torch.Tensor, ws: "_abi.Workspace"
                                     ) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -89,6 +89,15 @@ class Attention(nn.Module):
             _abi.attn_prefill(q, k, v, None, None, None, None, out, 1, T, 0, H, KV, hd, causal=False)
             return out
         md = cache.metadata
+        if cache.paged:
+            # write, THEN read the pages; a batch's first tokens attend over their own rows as they are
+            _abi.attn_qkv(x, norm_w, self.wqkv, rope, positions, q, k, v, None, None, None, H, KV, hd, eps, ws)
+            cache.write(k, v)
+            if md.first_prefill:
+                _abi.attn_prefill(q, k, v, k, v, md.q_start, md.seqpos, out, len(md.seqlens), md.max_seqlen, md.window, H, KV, hd, causal=True, first_prefill=True)
+            else:
+                cache.attend(q, out)
+            return out
         if md.prefill:
             # read the old ring, THEN write (transformer_layers.py:75-76)
             _abi.attn_qkv(x, norm_w, self.wqkv, rope, positions, q, k, v, None, None, None, H, KV, hd, eps, ws)

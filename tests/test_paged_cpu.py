@@ -151,6 +151,44 @@ def test_host_tables_truncate_undoes_extend():
     assert before == (str(t.table), t.lens, t.free, t.n_free)
 
 
+def test_ledger_knows_what_there_is_room_for():
+    from mistral_inference_b200.paged import PageLedger
+    g = PageLedger(rows=3, max_seq_len=200, n_pages=5)
+    g.admit(2)
+    assert g.rows == [0, 1] and g.lens == [0, 0] and g.free_pages == 5
+    g.check([130, 64])
+    with pytest.raises(ValueError, match="4 of 5|more pages"):
+        g.check([200, 130])
+    for bad, why in (([1], "Batch size"), ([-1, 5], "new tokens"), ([0, 0], "new tokens"), ([201, 0], "200")):
+        with pytest.raises(ValueError, match=why):
+            g.check(bad)
+    g.lens = [130, 64]
+    assert g.free_pages == 1
+    g.check([1, 1])  # one new page
+    g.admit(1)
+    with pytest.raises(ValueError, match="2 more pages needed, 1 of 5 free"):
+        g.check([0, 1, 1])
+    with pytest.raises(ValueError, match="free rows"):
+        g.admit(1)
+    g.retire([0])
+    assert g.rows == [1, 2] and g.lens == [64, 0] and g.free_pages == 4
+    g.admit(1)
+    assert g.rows == [1, 2, 0]
+
+
+def test_layered_decoders_keep_their_rings():
+    from mistral_inference_b200.layered import LayeredTransformer
+    with pytest.raises(ValueError, match="rings"):
+        LayeredTransformer.make_cache(object(), 1, 8, kv_cache="pages")
+
+
+def test_an_unknown_cache_is_refused():
+    from mistral_inference_b200.transformer import Transformer
+    for kw in (dict(kv_cache="paper"), dict(n_pages=3)):
+        with pytest.raises(ValueError, match="kv_cache"):
+            Transformer.make_cache(object(), 1, 8, **kw)
+
+
 def test_declarations_of_this_abi_version():
     """A change of the declarations takes a new version, so that a library built before it is refused."""
     code = re.sub(r"/\*.*?\*/", " ", HEADER.read_text(), flags=re.S)
