@@ -5,7 +5,7 @@
  *
  * Pages.  A page holds 64 tokens.  One layer's pool: kv [n_pages, KV, 2 (keys, values), 64, 128] e4m3 and scale [n_pages, KV, 2] fp32, powers of two; a number is its code
  * times the scale of its page, head and kind.  table [R, P] int32: row r names the pages of the request in it, in order, -1 behind the last.  lens [R] int32: its
- * tokens.  free_pages [n_pages] int32: a stack of n_free[0] page ids, the last one is taken first.  scratch [1 + R] int32: zero-filled once, this state's own.
+ * tokens.  free_pages [n_pages] int32: a stack of n_free[0] page ids, the last one is taken first.  scratch [1] int32: zero once, this state's own.
  * Calls on one state, and on pools that its pages name, are ordered on one stream (or by events).
  */
 #ifndef MISTRAL_B200_PAGED_H_
@@ -18,6 +18,7 @@ extern "C" {
 
 #define MBP_ABI_VERSION 1
 #define MBP_MAX_REQUESTS 4000 /* requests of a call */
+#define MBP_MAX_ROWS 131072   /* rows of a state */
 #define MBP_MAX_VOCAB (1 << 24)
 
 int mbp_abi_version(void);

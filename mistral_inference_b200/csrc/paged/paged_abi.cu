@@ -25,7 +25,7 @@ static int run_plan(bool extend, PlanParams p, cudaStream_t st) {
 
 static int plan_state(PlanParams& p, const char* what, int32_t* table, int32_t* lens, int32_t* free_pages, int32_t* n_free, int32_t* scratch, const int32_t* rows,
                       const int32_t* count, int64_t B, int64_t R, int64_t P, int64_t n_pages, int32_t* status) {
-  MB_CHECK_ARG(R >= 1 && P >= 1 && n_pages >= 1 && R < (1 << 24) && P < (1 << 24) && n_pages <= 0x7fffffff / PG_TOKENS, "%s: %lld rows of %lld pages, %lld pages", what,
+  MB_CHECK_ARG(R >= 1 && P >= 1 && n_pages >= 1 && R <= MBP_MAX_ROWS && P < (1 << 24) && n_pages <= 0x7fffffff / PG_TOKENS, "%s: %lld rows of %lld pages, %lld pages", what,
                (long long)R, (long long)P, (long long)n_pages);
   MB_CHECK_ARG(B >= 1 && B <= MBP_MAX_REQUESTS && (rows || B <= R), "%s: %lld requests (1 to %d, without a list of rows at most %lld)", what, (long long)B, MBP_MAX_REQUESTS,
                (long long)R);
@@ -178,7 +178,7 @@ int mbp_pages_extend(int32_t* table, int32_t* lens, int32_t* free_pages, int32_t
   PlanParams p;
   int rc = plan_state(p, "pages_extend", table, lens, free_pages, n_free, scratch, rows, add, B, R, P, n_pages, status);
   if (rc) return rc;
-  MB_CHECK_ARG(T >= 0 && T <= 0x7fffffff && (T == 0 || (positions && slots)) && q_start && seqpos, "pages_extend: room for %lld tokens", (long long)T);
+  MB_CHECK_ARG(T >= 0 && T <= (1 << 30) && (T == 0 || (positions && slots)) && q_start && seqpos, "pages_extend: room for %lld tokens", (long long)T);
   p.positions = positions;
   p.slots = slots;
   p.q_start = q_start;
@@ -199,7 +199,7 @@ static int check_pool(const char* what, const void* kv, const void* scale, int64
   MB_CHECK_ARG(kv && scale, "%s: null pointer", what);
   MB_CHECK_ARG((uintptr_t)kv % 16 == 0, "%s: the pool must be 16-byte aligned", what);
   // rows of the pool and slots are counted in 32 bits; bytes are not
-  MB_CHECK_ARG(n_pages >= 1 && KV >= 1 && KV <= 65535 && n_pages <= 0x7fffffff / (2 * PG_TOKENS * KV), "%s: %lld pages of %lld heads", what, (long long)n_pages, (long long)KV);
+  MB_CHECK_ARG(n_pages >= 1 && KV >= 1 && KV <= 32767 && n_pages <= 0x7fffffff / (2 * PG_TOKENS * KV), "%s: %lld pages of %lld heads", what, (long long)n_pages, (long long)KV);
   return MB200_OK;
 }
 
@@ -227,8 +227,14 @@ int mbp_pages_write(const void* k, int64_t ldk, const void* v, int64_t ldv, void
   p.T = (int)T;
   p.KV = (int)n_kv_heads;
   p.n_pages = (int)n_pages;
-  const dim3 grid((unsigned)(T / PG_TOKENS + 2 * B), (unsigned)n_kv_heads, 2);
-  MB_CHECK_CUDA(launch_pdl(page_write_kernel, grid, dim3(PW_THREADS), 0, (cudaStream_t)stream, p));
+  const int64_t items = T / PG_TOKENS + 2 * B, ctas = T <= PW_FEW * B ? items * ((2 * n_kv_heads + PW_WARPS - 1) / PW_WARPS) : items * 2 * n_kv_heads;
+  MB_CHECK_ARG(ctas <= 0x7fffffff, "pages_write: %lld tokens of %lld heads", (long long)T, (long long)n_kv_heads);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (T <= PW_FEW * B) {
+    MB_CHECK_CUDA(launch_pdl(page_write_kernel<32>, dim3((unsigned)ctas), dim3(PW_THREADS), 0, st, p));
+  } else {
+    MB_CHECK_CUDA(launch_pdl(page_write_kernel<PW_THREADS>, dim3((unsigned)ctas), dim3(PW_THREADS), 0, st, p));
+  }
   return MB200_OK;
 }
 

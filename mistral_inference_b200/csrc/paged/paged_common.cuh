@@ -73,4 +73,18 @@ __device__ __forceinline__ int last_not_above(int n, int x, F start) {
   return lo;
 }
 
+// the same by a whole warp, 32 places looked at in one trip to memory
+template <typename F>
+__device__ __forceinline__ int warp_last_not_above(int n, int x, F start) {
+  int lo = 0, len = n;  // the answer is in [lo, lo + len)
+  while (len > 1) {
+    const int step = (len + 31) / 32, at = lo + (int)(threadIdx.x & 31) * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < lo + len && start(at < lo + len ? at : lo) <= x);
+    const int last = below ? 31 - __clz(below) : 0;
+    len = min(step, lo + len - (lo + last * step));
+    lo += last * step;
+  }
+  return lo;
+}
+
 }  // namespace mb200

@@ -18,7 +18,7 @@ constexpr int PLAN_THREADS = 256, PLAN_TOKENS_PER_CTA = 1024, PLAN_MAX_CTAS = 14
 
 struct PlanParams {
   int32_t *table, *lens, *free, *n_free;
-  int32_t* scratch;     // [1 + R]: arrivals (zero between calls) | the request that names each row
+  int32_t* scratch;     // [1]: CTAs of an extend that are done (zero between calls)
   const int32_t* rows;  // [B] or null: request b is row b
   const int32_t* count; // [B] tokens to add, or to keep
   int32_t *positions, *slots, *q_start, *seqpos, *status;
@@ -51,7 +51,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* sums, lo
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + PG_TOKENS - 1) / PG_TOKENS; }
 
 // What both kernels begin with: lengths and prefix sums of all requests in shared memory.  Returns the status of the call, the same in every CTA.
-//   sm: first[B + 1] prefix sums of count | moved[B + 1] prefix sums of the pages that move | len[B] lengths before
+//   sm: len[B] lengths before | first[B + 1] prefix sums of count | moved[B + 1] prefix sums of the pages that move; a bit for each row first lies over the two
 template <bool EXTEND>
 __device__ __forceinline__ int plan_requests(const PlanParams& p, int* first, int* moved, int* len, int& n_free, int& n_moved) {
   __shared__ long long sums[32];
@@ -59,7 +59,9 @@ __device__ __forceinline__ int plan_requests(const PlanParams& p, int* first, in
   n_free = *p.n_free;
   int bad = 0;
   long long tokens = 0, pages = 0;
-  volatile int32_t* named = p.scratch + 1;
+  uint32_t* named = reinterpret_cast<uint32_t*>(first);
+  for (int i = threadIdx.x; i < (p.R + 31) / 32; i += blockDim.x) named[i] = 0;
+  __syncthreads();
   for (int b = b0; b < b1; ++b) {
     const int r = p.rows ? p.rows[b] : b, c = p.count[b];
     if (r < 0 || r >= p.R) {
@@ -67,7 +69,7 @@ __device__ __forceinline__ int plan_requests(const PlanParams& p, int* first, in
       len[b] = 0;
       continue;
     }
-    named[r] = b;  // (every CTA writes the same; of two requests that name one row at least one finds the other's number)
+    if (atomicOr(named + r / 32, 1u << (r & 31)) >> (r & 31) & 1) bad |= 1 << PLAN_BAD_ROW;  // (shared memory: the same answer in every CTA)
     const int l = p.lens[r];
     len[b] = l;
     const bool fits = EXTEND ? (c >= 0 && c <= p.P * PG_TOKENS - l) : (c >= 0 && c <= l);
@@ -77,11 +79,6 @@ __device__ __forceinline__ int plan_requests(const PlanParams& p, int* first, in
     }
     tokens += c;
     pages += EXTEND ? pages_of(l + c) - pages_of(l) : pages_of(l) - pages_of(c);
-  }
-  __syncthreads();
-  for (int b = b0; b < b1; ++b) {
-    const int r = p.rows ? p.rows[b] : b;
-    if (r >= 0 && r < p.R && named[r] != b) bad |= 1 << PLAN_BAD_ROW;
   }
   bad = (__syncthreads_or(bad & (1 << PLAN_BAD_ROW)) ? PLAN_BAD_ROW : 0) | (__syncthreads_or(bad & (1 << PLAN_BAD_LENGTH)) ? 16 : 0);
   if (bad) return bad & PLAN_BAD_ROW ? PLAN_BAD_ROW : PLAN_BAD_LENGTH;
@@ -107,7 +104,7 @@ __device__ __forceinline__ int plan_requests(const PlanParams& p, int* first, in
 
 __global__ void __launch_bounds__(PLAN_THREADS) page_extend_kernel(PlanParams p) {
   extern __shared__ int plan_sm[];
-  int *first = plan_sm, *moved = first + p.B + 1, *len = moved + p.B + 1;
+  int *len = plan_sm, *first = len + p.B, *moved = first + p.B + 1;
   pdl_trigger();
   pdl_wait();
   int n_free, n_new;
@@ -167,7 +164,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_extend_kernel(PlanParams p)
 // One CTA: what goes back is a few pages (drafted tokens) or a few hundred (a request that has ended).
 __global__ void __launch_bounds__(1024) page_truncate_kernel(PlanParams p) {
   extern __shared__ int plan_sm[];
-  int *first = plan_sm, *moved = first + p.B + 1, *len = moved + p.B + 1;
+  int *len = plan_sm, *first = len + p.B, *moved = first + p.B + 1;
   pdl_trigger();
   pdl_wait();
   int n_free, n_back;

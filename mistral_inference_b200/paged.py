@@ -65,7 +65,7 @@ class PageTables:
         assert table.dim() == 2 and lens.shape == table.shape[:1] and free.dim() == 1 and n_free.shape == (1,), (table.shape, lens.shape, free.shape, n_free.shape)
         self.table, self.lens, self.free, self.n_free = table, lens, free, n_free
         self.device = _abi_paged.index_of(table)
-        self.scratch = torch.zeros(1 + table.shape[0], dtype=torch.int32, device=table.device)
+        self.scratch = torch.zeros(1, dtype=torch.int32, device=table.device)
         self._every = torch.arange(table.shape[0], dtype=torch.int32, device=table.device)
         self._first = {}  # number of requests -> their rows, where they are the first ones
 

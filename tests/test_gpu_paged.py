@@ -84,6 +84,24 @@ def test_steps_that_cannot_be_done_change_nothing():
         assert_same_state(t, h)
 
 
+def test_a_row_named_twice_among_many_tokens():
+    """Every CTA of the call finds it, and the next call starts afresh."""
+    t, h = mi.PageTables.empty(40, 200, 8000, DEV), U.HostTables(40, 200, 8000)
+    rows = [(7 * i) % 40 for i in range(40)]
+    for i in range(10):
+        twice = list(rows)
+        twice[39] = rows[i]
+        plan = t.extend(ints([1000] * 40), 40000, ints(twice))
+        with pytest.raises(_abi_paged.Mb200Error, match="twice"):
+            plan.check()
+        assert plan.q_start.tolist() == [0] * 41 and (plan.slots == -1).all()
+        assert_same_state(t, h)
+        plan = t.extend(ints([900] * 40), 40000, ints(rows)).check()
+        _, slots, _, _ = h.extend([900] * 40, rows)
+        assert plan.slots.tolist() == slots + [-1] * 4000
+        assert_same_state(t, h)
+
+
 def test_tables_refuse_what_they_cannot_take():
     t = mi.PageTables.empty(2, 4, 8, DEV)
     with pytest.raises(AssertionError):
@@ -157,6 +175,17 @@ def test_write(KV, steps):
         pool.write(k, v, plan, slots)
         pool.assert_same()
         mi.write_pages(pool.kv, pool.scale, k, v, plan)  # the same step again
+        pool.assert_same()
+
+
+def test_write_of_a_portion_among_single_tokens():
+    """Few tokens a request on average, so a warp writes a page, whose rows it takes in turns; the earlier tokens' codes move to grown scales on the way."""
+    B, KV = 40, 3
+    t, h, pool = mi.PageTables.empty(B, 6, 3 * B, DEV), U.HostTables(B, 6, 3 * B), Pool(3 * B, KV)
+    for i, step in enumerate([[1] * 20 + [37] + [1] * 19, [i % 3 for i in range(39)] + [200], [63] + [0] * 18 + [17, 130] + [1] * 19]):
+        plan = t.extend(ints(step), sum(step)).check()
+        _, slots, _, _ = h.extend(step)
+        pool.write(numbers(sum(step), KV, 128, seed=i, spread=4 + 4 * i).to(DEV), numbers(sum(step), KV, 128, seed=50 + i, spread=4 + 4 * i).to(DEV), plan, slots)
         pool.assert_same()
 
 

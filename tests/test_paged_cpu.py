@@ -45,7 +45,7 @@ X = 4096
 
 def test_plans_are_refused(lib):
     extend = lambda B=2, T=2, R=2, P=4, N=8, rows=None, table=X: lib.mbp_pages_extend(table, X, X, X, X, rows, X, X, X, X, X, X, B, T, R, P, N, None)  # noqa: E731
-    for kw, why in [(dict(table=None), "null"), (dict(B=0), "requests"), (dict(B=_abi_paged.MAX_REQUESTS + 1, R=5000), "requests"), (dict(B=3), "requests"), (dict(T=-1), "room"),
+    for kw, why in [(dict(table=None), "null"), (dict(B=0), "requests"), (dict(B=_abi_paged.MAX_REQUESTS + 1, R=5000), "requests"), (dict(B=3), "requests"), (dict(T=-1), "room"), (dict(T=2 ** 30 + 1), "room"), (dict(R=131073), "rows"),
                     (dict(R=0), "rows"), (dict(P=0), "pages"), (dict(N=0), "pages"), (dict(N=2 ** 31 // 64 + 1), "pages")]:
         assert extend(**kw) == -1 and why in last(lib), (kw, last(lib))
     truncate = lambda B=2, R=2, P=4, N=8, keep=X: lib.mbp_pages_truncate(X, X, X, X, X, None, keep, X, B, R, P, N, None)  # noqa: E731
@@ -192,4 +192,4 @@ def test_an_unknown_cache_is_refused():
 def test_declarations_of_this_abi_version():
     """A change of the declarations takes a new version, so that a library built before it is refused."""
     code = re.sub(r"/\*.*?\*/", " ", HEADER.read_text(), flags=re.S)
-    assert zlib.crc32(" ".join(code.split()).encode()) == 1661688504, "raise the ABI version with this change"
+    assert zlib.crc32(" ".join(code.split()).encode()) == 2100840578, "raise the ABI version with this change"
