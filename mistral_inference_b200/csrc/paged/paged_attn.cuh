@@ -20,6 +20,8 @@
 // of them empty for groups of four heads: 3200 clocks a tile, 32 requests of ~1100 tokens 21.0 us.)  Keys and values in slots of their own, keys' freed after S(t): no faster
 // (44.8 us for 42.3 with four requests of 32500 tokens): what lies in flight is enough.
 #pragma once
+#include <type_traits>
+
 #include "paged_common.cuh"
 
 namespace mb200 {
@@ -112,17 +114,19 @@ __device__ __forceinline__ bool group_sync_or(int group, bool v) {
   if (group == 2) return group_sync_or_id<3>(v);
   return group_sync_or_id<4>(v);
 }
-// two weights times 256 as codes: hi in the lower half-word, lo in the upper.  (Through fp16, whose 11 bits hold more than the two parts do.)
-__device__ __forceinline__ uint32_t weight_parts(float w0, float w1) {
+// two weights times 256 as codes.  (Through fp16, whose 11 bits hold more than the two parts do.)
+__device__ __forceinline__ void weight_parts(float w0, float w1, uint16_t& hi, uint16_t& lo) {
   uint32_t w, h, r;
-  uint16_t hi, lo;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(w1), "f"(w0));
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(hi) : "r"(w));
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(hi));
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(h));
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0x4c004c00u));  // times 16
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(lo) : "r"(r));
-  return (uint32_t)hi | (uint32_t)lo << 16;
+}
+template <int AT>
+__device__ __forceinline__ void st_shared_u8(uint32_t addr, uint16_t v) {
+  asm volatile("st.shared.u8 [%0 + %2], %1;" ::"r"(addr), "h"(v), "n"(AT) : "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
@@ -133,6 +137,15 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
+}
+
+__device__ __forceinline__ uint64_t pair_of(uint32_t x, uint32_t y) { return pair(__uint_as_float(x), __uint_as_float(y)); }
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F f) {  // f(0) .. f(N - 1), constants
+  if constexpr (N > 0) {
+    unrolled<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
 }
 
 // Byte k of column c: its 128 bytes are one row of a 128B-swizzled K-major tile
@@ -151,7 +164,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   __shared__ int gave_up;
   __shared__ float page_scale[PA_STAGES][4];              // keys of page 0, 1, values of page 0, 1 of the stage's tile
   __shared__ float q_scale[NQ];                           // a query row's scale, times the softmax scale, in log2 units
-  __shared__ __align__(16) float warp_most[2][NQ][4];     // by tile parity
+  __shared__ float warp_most[2][NQ][4];                   // by tile parity
   __shared__ float sums[4][NQ];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
@@ -194,7 +207,8 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   const int first = page_lo + n_pages * split / splits, last = page_lo + n_pages * (split + 1) / splits;  // this split's pages (n_pages < 2^25)
   const int tiles = (last - first + 1) / 2;
 
-  float o[Q], m[Q], l[Q];
+  float m[Q];
+  uint64_t o[Q / 2], l[Q / 2];  // of two queries each
   const int group = warp >> 2, key_at = tid & 127;  // of the softmax threads
   if (warp == SOFT) {
     // ================= producer =================
@@ -301,13 +315,19 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
     __syncwarp();
     if (lane == 0) mbar_arrive(&q_full);
     bool ok = bounded_wait(&q_full, 0, &gave_up);  // q_scale of all rows
-    float qs[Q];
+    uint64_t qs[Q / 2], less[Q / 2];  // less: minus the maximum
 #pragma unroll
-    for (int i = 0; i < Q; ++i) {
-      o[i] = l[i] = 0.f;
-      m[i] = PA_NOTHING;
-      qs[i] = q_scale[group * Q + i];
+    for (int i = 0; i < Q; i += 2) {
+      m[i] = m[i + 1] = PA_NOTHING;
+      o[i / 2] = l[i / 2] = pair(0.f, 0.f);
+      less[i / 2] = pair(-PA_NOTHING, -PA_NOTHING);
+      qs[i / 2] = pair(q_scale[group * Q + i], q_scale[group * Q + i + 1]);
     }
+    const int most_at = lane % (4 * Q);  // the maximum that this lane looks at: column most_at / 4, warp most_at % 4
+    float most = PA_NOTHING;             // m[most_at / 4]
+    const uint64_t sixteenth = pair(0.0625f, 0.0625f), eight = pair(8.f, 8.f);
+    // Byte key_at of column j of the group: its 128 bytes are row j of a 128B-swizzled K-major tile, which pa_col(group * 2 Q + j, key_at) says in full
+    const uint32_t p_at = smem_u32(sP) + group * 2 * Q * 128 + (key_at ^ (Q == 2 ? group << 6 : 0));
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + group * 2 * Q;
     float vs0 = 0.f, vs1 = 0.f;  // value scales of the tile before
     bool two_before = false;
@@ -320,11 +340,12 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
       tmem_ld_cols<2 * Q>(lanes + 2 * N, a);
       if (two_before) tmem_ld_cols<2 * Q>(lanes + 3 * N, z);
       tmem_wait_ld();
+      const uint64_t by0 = pair(vs0, vs0), by1 = pair(vs1, vs1);
 #pragma unroll
-      for (int i = 0; i < Q; ++i) o[i] = fmaf(fmaf(__uint_as_float(a[Q + i]), 0.0625f, __uint_as_float(a[i])), vs0, o[i]);
+      for (int i = 0; i < Q; i += 2) o[i / 2] = fma_pair(fma_pair(pair_of(a[Q + i], a[Q + i + 1]), sixteenth, pair_of(a[i], a[i + 1])), by0, o[i / 2]);
       if (two_before) {
 #pragma unroll
-        for (int i = 0; i < Q; ++i) o[i] = fmaf(fmaf(__uint_as_float(z[Q + i]), 0.0625f, __uint_as_float(z[i])), vs1, o[i]);
+        for (int i = 0; i < Q; i += 2) o[i / 2] = fma_pair(fma_pair(pair_of(z[Q + i], z[Q + i + 1]), sixteenth, pair_of(z[i], z[i + 1])), by1, o[i / 2]);
       }
     };
     for (int t = 0; t < tiles; ++t) {
@@ -343,8 +364,13 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
         uint32_t a[2 * Q];
         tmem_ld_cols<2 * Q>(lanes + (t & 1) * N, a);
         tmem_wait_ld();
+        const uint64_t by = pair(ks, ks);
 #pragma unroll
-        for (int i = 0; i < Q; ++i) s[i] = fmaf(__uint_as_float(a[Q + i]), 0.0625f, __uint_as_float(a[i])) * (ks * qs[i]);
+        for (int i = 0; i < Q; i += 2) {
+          const float2 f = unpair(mul_pair(fma_pair(pair_of(a[Q + i], a[Q + i + 1]), sixteenth, pair_of(a[i], a[i + 1])), mul_pair(by, qs[i / 2])));
+          s[i] = f.x;
+          s[i + 1] = f.y;
+        }
         if (edge) {
 #pragma unroll
           for (int i = 0; i < Q; ++i) {
@@ -371,41 +397,42 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
         ok = false;
         break;
       }
-      float top[Q];
-      bool grew = false;
+      // The group's maxima, a column and warp a lane; broadcast only where one has grown.  (All of them by every thread: 40 instructions of some 350 a tile and thread.)
+      float top = warp_most[t & 1][group * Q + most_at / 4][most_at % 4];
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool grew = __any_sync(0xffffffffu, top > most);  // (the same in all threads of the group)
+      uint64_t alpha[Q / 2];
+      if (grew) {
+        most = fmaxf(most, top);
 #pragma unroll
-      for (int i = 0; i < Q; ++i) {
-        const float4 w = *reinterpret_cast<const float4*>(warp_most[t & 1][group * Q + i]);
-        top[i] = fmaxf(fmaxf(m[i], fmaxf(w.x, w.y)), fmaxf(w.z, w.w));
-        grew |= top[i] > m[i];
-      }
-      float alpha[Q];
-      if (grew) {  // (the same in all threads of the group)
-#pragma unroll
-        for (int i = 0; i < Q; ++i) {
-          alpha[i] = exp2_ftz(m[i] - top[i]);
-          m[i] = top[i];
-          l[i] *= alpha[i];
+        for (int i = 0; i < Q; i += 2) {
+          const float m0 = __shfl_sync(0xffffffffu, most, i * 4), m1 = __shfl_sync(0xffffffffu, most, i * 4 + 4);
+          alpha[i / 2] = pair(exp2_ftz(m[i] - m0), exp2_ftz(m[i + 1] - m1));
+          l[i / 2] = mul_pair(l[i / 2], alpha[i / 2]);
+          less[i / 2] = pair(-m0, -m1);
+          m[i] = m0;
+          m[i + 1] = m1;
         }
       }
-      uint8_t* P = sP + (t & 1) * Cfg::kColBytes;
-#pragma unroll
-      for (int i = 0; i < Q; i += 2) {
-        const float e0 = exp2_ftz(s[i] - m[i] + 8.f), e1 = exp2_ftz(s[i + 1] - m[i + 1] + 8.f);  // weights times 256: the whole of e4m3's range
-        l[i] += e0;
-        l[i + 1] += e1;
-        const uint32_t w = weight_parts(e0, e1);
-        const int c = group * 2 * Q + i;
-        P[pa_col(c, key_at)] = (uint8_t)w;
-        P[pa_col(c + 1, key_at)] = (uint8_t)(w >> 8);
-        P[pa_col(c + Q, key_at)] = (uint8_t)(w >> 16);
-        P[pa_col(c + Q + 1, key_at)] = (uint8_t)(w >> 24);
-      }
+      const uint32_t P = p_at + (t & 1) * Cfg::kColBytes;
+      unrolled<Q / 2>([&](auto at) {
+        constexpr int i = 2 * decltype(at)::value;
+        const float2 x = unpair(add_pair(add_pair(pair(s[i], s[i + 1]), less[i / 2]), eight));
+        const float e0 = exp2_ftz(x.x), e1 = exp2_ftz(x.y);  // weights times 256: the whole of e4m3's range
+        l[i / 2] = add_pair(l[i / 2], pair(e0, e1));
+        uint16_t hi, lo;
+        weight_parts(e0, e1, hi, lo);
+        st_shared_u8<i * 128>(P ^ ((i & 7) << 4), hi);
+        st_shared_u8<i * 128 + 128>(P ^ ((i + 1 & 7) << 4), hi >> 8);
+        st_shared_u8<(i + Q) * 128>(P ^ ((i + Q & 7) << 4), lo);
+        st_shared_u8<(i + Q) * 128 + 128>(P ^ ((i + Q + 1 & 7) << 4), lo >> 8);
+      });
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (t > 0) add_values(t - 1);
       if (grew) {
 #pragma unroll
-        for (int i = 0; i < Q; ++i) o[i] *= alpha[i];
+        for (int i = 0; i < Q / 2; ++i) o[i] = mul_pair(o[i], alpha[i]);
       }
       vs0 = page_scale[st][2];
       vs1 = page_scale[st][3];
@@ -417,12 +444,12 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
     if (tiles > 0 && ok) add_values(tiles - 1);
     if (!__all_sync(0xffffffffu, ok)) {
 #pragma unroll
-      for (int i = 0; i < Q; ++i) o[i] = __int_as_float(0x7fffffff);
+      for (int i = 0; i < Q / 2; ++i) o[i] = pair(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
       if (lane == 0 && p.status) atomicOr(p.status, PA_GAVE_UP);
     }
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
-      const float w = warp_sum(l[i]);
+      const float w = warp_sum(i & 1 ? unpair(l[i / 2]).y : unpair(l[i / 2]).x);
       if (lane == 0) sums[warp & 3][group * Q + i] = w;
     }
   }
@@ -445,11 +472,11 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
     for (int i = 0; i < Q; ++i) {
       const int q = group * Q + i;
       if (q < nq) {
-        const float sum = sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q];
+        const float sum = sums[0][q] + sums[1][q] + sums[2][q] + sums[3][q], mine_o = i & 1 ? unpair(o[i / 2]).y : unpair(o[i / 2]).x;
         if (splits == 1) {
-          p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + key_at] = __float2bfloat16_rn(sum == 0.f ? 0.f : o[i] / sum);
+          p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + key_at] = __float2bfloat16_rn(sum == 0.f ? 0.f : mine_o / sum);
         } else {
-          mine[q * (kHeadDim + 2) + 2 + key_at] = o[i];
+          mine[q * (kHeadDim + 2) + 2 + key_at] = mine_o;
           if (key_at == 0) {
             mine[q * (kHeadDim + 2)] = m[i];
             mine[q * (kHeadDim + 2) + 1] = sum;

@@ -62,26 +62,6 @@ __device__ __forceinline__ unsigned long long block_max_key(unsigned long long k
   __syncthreads();
   return warp_max_key(sm[threadIdx.x & (TS_WARPS - 1)]);
 }
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one is
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
