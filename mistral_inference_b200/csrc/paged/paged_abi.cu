@@ -257,6 +257,7 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
                "attn_pages: B=%lld T=%lld longest=%lld R=%lld P=%lld window=%lld", (long long)B, (long long)T, (long long)longest, (long long)R, (long long)P, (long long)window);
   MB_CHECK_ARG(((uintptr_t)q) % 8 == 0 && ldq % 4 == 0 && ldq >= n_heads * head_dim, "attn_pages: rows of queries must be 8-byte aligned and not overlap (%lld elements apart)",
                (long long)ldq);
+  MB_CHECK_ARG(((uintptr_t)out) % 8 == 0, "attn_pages: the output must be 8-byte aligned");
   MB_CHECK_ARG(softmax_scale > 0.f && softmax_scale < 3.4e38f, "attn_pages: scale %g", (double)softmax_scale);
   if (T == 0) return MB200_OK;
   const AttnCut cut = attn_cut(B, longest, most, P, n_heads, n_kv_heads, window);

@@ -28,6 +28,7 @@ namespace mb200 {
 
 constexpr int PA_STAGES = 3, PA_KEYS = 2 * PG_TOKENS, PA_STAGE_BYTES = 4 * PG_BYTES;
 constexpr int PA_MAX_SPLITS = 16;
+constexpr int PA_ROW = kHeadDim + 4;     // numbers of a split's result for one query: maximum, sum, -, -, the values' sums
 constexpr float PA_NOTHING = -1.0e30f;   // the maximum of no score
 enum { PA_GAVE_UP = 16 };                // status: a wait ran out; the call's results are NaN
 
@@ -50,7 +51,7 @@ struct PaCfg {
   static constexpr int N = 2 * NQ < 16 ? 16 : 2 * NQ;      // (16 at least; columns that nobody reads hold anything)
   static constexpr int kColBytes = N * 128;                // Q or one P tile: [N columns][128 bytes], 128B-swizzled
   static constexpr int kRing = PA_STAGES * PA_STAGE_BYTES;
-  static constexpr int kMerge = NQ * (kHeadDim + 2) * 4;   // this split's result, over the ring once that is used up
+  static constexpr int kMerge = NQ * PA_ROW * 4;            // this split's result, over the ring once that is used up
   static constexpr int kSmem = 1024 + kRing + 3 * kColBytes;
   static constexpr int kTmemCols = 4 * N;                  // two S tiles, the two pages' O
   static_assert(kMerge <= kRing && kTmemCols <= 512, "fits");
@@ -133,6 +134,11 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -199,6 +205,10 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
     __syncthreads();
     if (warp == SOFT + 1) tmem_dealloc(tmem, Cfg::kTmemCols);
     return;
+  }
+  if (i0 + p.tokens < n_all && blockIdx.y / p.KV == gridDim.y / p.KV - 1 && split == 0) {  // more tokens than there are tiles for
+    if (tid == 0 && p.status) atomicOr(p.status, PG_TOO_LONG);
+    no_numbers(p.out + (int64_t)t_first * p.H * kHeadDim + g * R * kHeadDim, i0 + p.tokens, n_all, p.H, R);
   }
   const int nq = n * R, tok0 = t_first + i0;
   const int pos0 = past + i0, hi = pos0 + n;                                   // the tile's first position, one past its last
@@ -465,7 +475,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
     tmem_dealloc(tmem, Cfg::kTmemCols);
   }
   // ================= merge the splits =================
-  // this split: [q][maximum, sum, 128 sums] over the ring, which is used up
+  // this split's results over the ring, which is used up
   float* mine = reinterpret_cast<float*>(smem);
   if (warp < SOFT) {
 #pragma unroll
@@ -476,10 +486,10 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
         if (splits == 1) {
           p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + key_at] = __float2bfloat16_rn(sum == 0.f ? 0.f : mine_o / sum);
         } else {
-          mine[q * (kHeadDim + 2) + 2 + key_at] = mine_o;
+          mine[q * PA_ROW + 4 + key_at] = mine_o;
           if (key_at == 0) {
-            mine[q * (kHeadDim + 2)] = m[i];
-            mine[q * (kHeadDim + 2) + 1] = sum;
+            mine[q * PA_ROW] = m[i];
+            mine[q * PA_ROW + 1] = sum;
           }
         }
       }
@@ -487,25 +497,48 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   }
   if (splits == 1) return;
   cluster_sync_all();
-  // The results are dealt to all CTAs of the cluster, 32 to a warp.  Maxima and sums of all splits come by one load, a split a lane, and the loads of
-  // their sums of values do not wait for one another.  (A loop over the splits in every thread: 4500 clocks for 16 of them.)
-  if (warp < SOFT) {
+  // The results are dealt to all warps of the cluster: a quarter of a query's to each where there are as many warps (one query of 4 heads, 16 splits: 7.9 us, 8.5
+  // by whole queries), else a query (drafts of 8 requests in 2 splits: 21.5 us, 23.0 by quarters, four to a warp).  Maxima and sums of all splits come by one
+  // load, a split a lane, and the loads of their sums of values do not wait for one another.  (A loop over the splits in every thread: 4500 clocks for 16 of them.)
+  auto merge = [&](auto wide) {
+    constexpr int D = decltype(wide)::value, PARTS = kHeadDim / (32 * D);  // D dimensions a lane
     const uint32_t base = smem_u32(mine);
-    for (int part = split * SOFT + warp; part < nq * (kHeadDim / 32); part += splits * SOFT) {
-      const int q = part / (kHeadDim / 32), d = part % (kHeadDim / 32) * 32 + lane;
-      const uint32_t at = base + q * (kHeadDim + 2) * 4;
+    for (int part = split * SOFT + warp; part < nq * PARTS; part += splits * SOFT) {
+      const int q = part / PARTS, d = (part % PARTS * 32 + lane) * D;
+      const uint32_t at = base + q * PA_ROW * 4;
       const uint32_t from = map_to_rank(at, lane < splits ? lane : 0);
       const float mine_m = lane < splits ? ld_cluster_f32(from) : PA_NOTHING, mine_l = lane < splits ? ld_cluster_f32(from + 4) : 0.f;
-      float v[PA_MAX_SPLITS];
+      float v[PA_MAX_SPLITS][D], acc[D];
 #pragma unroll
-      for (int r = 0; r < PA_MAX_SPLITS; ++r) v[r] = r < splits ? ld_cluster_f32(map_to_rank(at + 8 + d * 4, r)) : 0.f;
+      for (int r = 0; r < PA_MAX_SPLITS; ++r) {
+        const uint32_t src = map_to_rank(at + 16 + d * 4, r < splits ? r : 0);
+        if constexpr (D == 1) {
+          v[r][0] = r < splits ? ld_cluster_f32(src) : 0.f;
+        } else {
+          const float4 x = r < splits ? ld_cluster_f32x4(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[r][0] = x.x, v[r][1] = x.y, v[r][2] = x.z, v[r][3] = x.w;
+        }
+      }
       const float f = exp2_ftz(mine_m - warp_max_f32(mine_m));  // (a split without a key: its sums are 0)
-      const float sum = warp_sum(f * mine_l);
-      float acc = 0.f;
+      const float sum = warp_sum(f * mine_l), inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int r = 0; r < PA_MAX_SPLITS; ++r) acc = fmaf(__shfl_sync(0xffffffffu, f, r), v[r], acc);
-      p.out[((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
+      for (int i = 0; i < D; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int r = 0; r < PA_MAX_SPLITS; ++r) {
+        const float w = __shfl_sync(0xffffffffu, f, r);
+#pragma unroll
+        for (int i = 0; i < D; ++i) acc[i] = fmaf(w, v[r][i], acc[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < D; ++i) acc[i] = sum == 0.f ? 0.f : acc[i] * inv;
+      bf16* to = p.out + ((int64_t)(tok0 + q / R) * p.H + g * R + q % R) * kHeadDim + d;
+      if constexpr (D == 1) *to = __float2bfloat16_rn(acc[0]);
+      else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
     }
+  };
+  if (warp < SOFT) {
+    if (nq * 4 <= splits * SOFT) merge(std::integral_constant<int, 1>{});
+    else merge(std::integral_constant<int, 4>{});
   }
   cluster_sync_all();  // nobody leaves while its results are read
 }

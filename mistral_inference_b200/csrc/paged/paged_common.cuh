@@ -88,6 +88,15 @@ __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, vol
   *gave_up = 1;
   return false;
 }
+
+enum { PG_TOO_LONG = 32 };  // status of attention: a request has more tokens than the call was told
+// Rows first .. n - 1 of a request's results (its first row at `out`, H heads a row), which no tile of queries is there for: no numbers, for `heads` heads.  By a CTA.
+__device__ __forceinline__ void no_numbers(bf16* out, int first, int n, int H, int heads) {
+  for (int64_t i = (int64_t)first * heads * kHeadDim + threadIdx.x; i < (int64_t)n * heads * kHeadDim; i += blockDim.x) {
+    const int64_t t = i / (heads * kHeadDim), c = i % (heads * kHeadDim);
+    out[t * H * kHeadDim + c] = __ushort_as_bfloat16((unsigned short)0x7fff);
+  }
+}
 // largest i in [0, n) with start[i] <= x, start ascending, start[0] <= x
 template <typename F>
 __device__ __forceinline__ int last_not_above(int n, int x, F start) {

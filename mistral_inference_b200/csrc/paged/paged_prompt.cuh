@@ -10,7 +10,6 @@
 namespace mb200 {
 
 constexpr int PR_THREADS = 256;
-enum { PR_TOO_LONG = 32 };  // status: a request has more tokens than the call was told; its results are NaN
 
 struct PagedRingParams {
   const uint8_t* kv;
@@ -18,7 +17,8 @@ struct PagedRingParams {
   const int32_t *table, *rows, *q_start, *seqpos;
   bf16 *ring_k, *ring_v;  // [B, W, KV, 128], position p in row p % W
   int32_t* status;
-  int T, R, P, n_pages, KV, window, W;
+  bf16* out;
+  int T, R, P, n_pages, H, KV, window, W, longest;
 };
 
 // CTA = (page of a request, key/value head, request): 64 rows of keys and of values
@@ -29,8 +29,11 @@ __global__ void __launch_bounds__(PR_THREADS) paged_ring_kernel(PagedRingParams 
   if (t0 < 0 || n <= 0 || n > p.T - t0 || past < 0) return;
   const int lo = p.window > 0 ? max(0, past + 1 - p.window) : 0, end = past + n;
   const int page_at = lo / PG_TOKENS + blockIdx.x, from = max(lo, page_at * PG_TOKENS), to = min(end, (page_at + 1) * PG_TOKENS);
-  const bool fits = end - lo <= p.W;
-  if (!fits && blockIdx.x == 0 && g == 0 && threadIdx.x == 0 && p.status) atomicOr(p.status, PR_TOO_LONG);
+  const bool fits = end - lo <= p.W && n <= p.longest;
+  if (!fits && blockIdx.x == 0) {
+    if (g == 0 && threadIdx.x == 0 && p.status) atomicOr(p.status, PG_TOO_LONG);
+    no_numbers(p.out + (int64_t)t0 * p.H * kHeadDim + g * (p.H / p.KV) * kHeadDim, (p.longest + FA_BM - 1) / FA_BM * FA_BM, n, p.H, p.H / p.KV);
+  }
   if (from >= to) return;
   int page = row >= 0 && row < p.R && page_at < p.P ? p.table[(int64_t)row * p.P + page_at] : -1;
   const bool is = page >= 0 && page < p.n_pages && fits;  // (else nothing is read out of bounds, and what is attended to is no number)
@@ -79,6 +82,9 @@ inline int make_query_map(CUtensorMap* map, const void* q, int64_t T, int64_t co
 
 // p: the whole call's; requests b0 .. b0 + B - 1 of it through rings of W rows at `scratch`
 inline int launch_paged_prompt(PagedRingParams p, const void* q, int64_t ldq, bf16* out, int64_t b0, int64_t B, int64_t longest, int H, float scale_log2, void* scratch, cudaStream_t st) {
+  p.out = out;
+  p.H = H;
+  p.longest = (int)longest;
   p.rows += b0;
   p.q_start += b0;
   p.seqpos += b0;

@@ -314,6 +314,25 @@ def test_portions_longer_than_the_plan_says_are_no_numbers():
         plan.check()
 
 
+@pytest.mark.parametrize("past,new,longest", [([900, 30], [250, 300], 90), ([900, 30], [250, 300], 260), ([70, 30, 5], [1, 3, 2], 1), ([70, 30], [40, 12], 12)])
+def test_requests_that_bring_more_than_the_plan_says(past, new, longest):
+    """Both ways of attending: what there is no room for is no number, the other requests are right."""
+    plan, kv, scale, kv_h, scale_h, table, rows = filled(2, past, new, 4)
+    T = sum(new)
+    q = numbers(T, 8, 128, seed=1, spread=0)
+    plan.longest = longest
+    got = mi.attend_pages(q.to(DEV), kv, scale, plan, out=torch.full((T, 1024), 9.0, dtype=torch.bfloat16, device=DEV)).cpu().double().view(T, 8, 128)
+    starts = [sum(new[:i]) for i in range(len(new) + 1)]
+    want, mag = U.attend_ref(q, kv_h.double(), scale_h, table, rows, starts, past)
+    tol = U.attend_tolerance(want, mag, max(p + n for p, n in zip(past, new)), float(448 * scale_h.max()))
+    gone = got.isnan().all(2).all(1)
+    assert torch.equal(gone, got.isnan().any(2).any(1)) and ((got - want).abs() <= tol)[~gone].all()
+    for b, n in enumerate(new):
+        assert not gone[starts[b]: starts[b] + n].any() if n <= longest else gone[starts[b] + n - 1]
+    with pytest.raises(_abi_paged.Mb200Error, match="longest"):
+        plan.check()
+
+
 def test_portions_of_pages_that_are_none_and_of_refused_plans():
     plan, kv, scale, *_ = filled(8, [200, 30], [250, 300], 4)
     q = numbers(550, 32, 128, seed=1, spread=0).to(DEV)

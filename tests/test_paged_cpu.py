@@ -63,10 +63,10 @@ def test_writes_are_refused(lib):
 
 
 def test_attention_is_refused(lib):
-    def attend(q=X, ldq=512, B=1, T=1, longest=1, most=0, H=4, KV=2, hd=128, P=4, N=4, window=0, scale=0.1, scratch=None, room=0):
-        return lib.mbp_attn_pages(q, ldq, X, X, X, X, X, X, X, None, B, T, longest, most, 2, P, N, H, KV, hd, window, scale, scratch, room, None)
+    def attend(q=X, ldq=512, out=X, B=1, T=1, longest=1, most=0, H=4, KV=2, hd=128, P=4, N=4, window=0, scale=0.1, scratch=None, room=0):
+        return lib.mbp_attn_pages(q, ldq, X, X, X, X, X, X, out, None, B, T, longest, most, 2, P, N, H, KV, hd, window, scale, scratch, room, None)
     for kw, why in [(dict(q=None), "null"), (dict(q=X + 4), "aligned"), (dict(ldq=256), "overlap"), (dict(H=5), "multiple"), (dict(H=66, ldq=66 * 128), "32 times"), (dict(hd=64), "128 only"),
-                    (dict(longest=0), "longest"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(P=0), "P="), (dict(N=0), "pages")]:
+                    (dict(out=X + 4), "aligned"), (dict(longest=0), "longest"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(P=0), "P="), (dict(N=0), "pages")]:
         assert attend(**kw) == -1 and why in last(lib), (kw, last(lib))
     assert attend(T=0) == 0
     scratch = lambda B=4, longest=1000, most=0, P=64, H=32, KV=8, window=0: lib.mbp_attn_pages_scratch(B, longest, most, P, H, KV, window)  # noqa: E731
