@@ -72,40 +72,41 @@ static int score_cluster(int64_t T, int64_t vocab, int64_t size) {
   return best;
 }
 
+template <auto Kernel, bool JOINS>
+static int launch_score_segments(const TokenScoresParams& p, int size, cudaStream_t st) {
+  const int64_t items = (int64_t)p.T * p.segments, room = (int64_t)device_info::sm_count() * TS_CTAS;
+  const size_t lists = JOINS ? sizeof(unsigned long long) * (size_t)p.segments * p.top : 0, data = (size_t)p.length * size;
+  MB_CHECK_CUDA(device_info::allow_shared<Kernel>(TS_BYTES));
+  if (JOINS && p.segments > 8) MB_CHECK_CUDA(allow_wide_clusters<Kernel>());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(JOINS || items < room ? items : room));
+  cfg.blockDim = dim3(TS_THREADS);
+  cfg.dynamicSmemBytes = data > lists ? data : lists;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (JOINS) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)p.segments;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  MB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, Kernel, p));
+  return MB200_OK;
+}
 template <typename ST, bool JOINS>
 static int launch_score_segments(const TokenScoresParams& p, cudaStream_t st) {
-  const int64_t items = (int64_t)p.T * p.segments, room = (int64_t)device_info::sm_count() * TS_CTAS;
-  const size_t lists = JOINS ? sizeof(unsigned long long) * (size_t)p.segments * p.top : 0, data = (size_t)p.length * sizeof(ST);
   const uint64_t apart = (uintptr_t)p.logits | (p.T > 1 ? (uint64_t)p.ld * sizeof(ST) : 0);
-  auto go = [&](auto kernel, cudaError_t allowed) {
-    MB_CHECK_CUDA(allowed);
-    if (JOINS && p.segments > 8) MB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(JOINS || items < room ? items : room));
-    cfg.blockDim = dim3(TS_THREADS);
-    cfg.dynamicSmemBytes = data > lists ? data : lists;
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    int n = 0;
-    if (JOINS) {
-      at[n].id = cudaLaunchAttributeClusterDimension;
-      at[n].val.clusterDim.x = (unsigned)p.segments;
-      at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-      ++n;
-    }
-    if (pdl_enabled()) {
-      at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      at[n].val.programmaticStreamSerializationAllowed = 1;
-      ++n;
-    }
-    cfg.attrs = at;
-    cfg.numAttrs = n;
-    MB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-    return MB200_OK;
-  };
-  return apart % 16 == 0  ? go(token_scores_segment_kernel<ST, 16, JOINS>, device_info::allow_shared<token_scores_segment_kernel<ST, 16, JOINS>>(TS_BYTES))
-         : apart % 4 == 0 ? go(token_scores_segment_kernel<ST, 4, JOINS>, device_info::allow_shared<token_scores_segment_kernel<ST, 4, JOINS>>(TS_BYTES))
-                          : go(token_scores_segment_kernel<ST, 0, JOINS>, device_info::allow_shared<token_scores_segment_kernel<ST, 0, JOINS>>(TS_BYTES));
+  return apart % 16 == 0  ? launch_score_segments<token_scores_segment_kernel<ST, 16, JOINS>, JOINS>(p, sizeof(ST), st)
+         : apart % 4 == 0 ? launch_score_segments<token_scores_segment_kernel<ST, 4, JOINS>, JOINS>(p, sizeof(ST), st)
+                          : launch_score_segments<token_scores_segment_kernel<ST, 0, JOINS>, JOINS>(p, sizeof(ST), st);
 }
 
 template <typename ST>

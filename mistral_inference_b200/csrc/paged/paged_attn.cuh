@@ -560,7 +560,7 @@ inline int make_pool_map(CUtensorMap* map, const void* kv, int64_t n_pages, int6
 template <int NQ>
 inline int launch_paged_attn(const PagedAttnParams& p, const CUtensorMap& map, int64_t q_tiles, int splits, cudaStream_t st) {
   MB_CHECK_CUDA(device_info::allow_shared<paged_attn_kernel<NQ>>(PaCfg<NQ>::kSmem));
-  if (splits > 8) MB_CHECK_CUDA(cudaFuncSetAttribute(paged_attn_kernel<NQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (splits > 8) MB_CHECK_CUDA(allow_wide_clusters<paged_attn_kernel<NQ>>());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)splits, (unsigned)(p.KV * q_tiles), (unsigned)p.B);
   cfg.blockDim = dim3(PaCfg<NQ>::kThreads);

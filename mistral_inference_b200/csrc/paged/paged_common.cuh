@@ -78,6 +78,18 @@ __device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
   return r;
 }
 
+// Allows launches of Kernel in clusters of up to 16 on the current device
+template <auto Kernel>
+inline cudaError_t allow_wide_clusters() {
+  static std::atomic<uint64_t> done{0};
+  const int dev = device_info::current();
+  const uint64_t bit = dev >= 0 && dev < device_info::MAX_DEVICES ? (uint64_t)1 << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 constexpr uint32_t PG_SPINS = 1u << 22;  // polls of a wait before it gives up (seconds)
 // false: the wait ran out, or another thread's has
 __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
