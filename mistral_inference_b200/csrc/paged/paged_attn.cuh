@@ -16,9 +16,11 @@
 //             per dimension, the values' sums of the tile before
 //   producer  TMA: tiles of two pages (8 KB of keys and of values each) into a ring of PA_STAGES x 32 KB
 //   issuer    MMAs: S(0) S(1) | PV(t) S(t + 2) ...
-// What a tile costs is the chain scores -> maximum -> weights -> sums of few warps, some 600 clocks where its bytes take 1200 of an SM.  (Four warps with eight columns each, half
-// of them empty for groups of four heads: 3200 clocks a tile, 32 requests of ~1100 tokens 21.0 us.)  Keys and values in slots of their own, keys' freed after S(t): no faster
-// (44.8 us for 42.3 with four requests of 32500 tokens): what lies in flight is enough.
+// What it measured: single tokens of 4 requests with 32500 tokens each, 32 heads over 8: 42.3 us, 5.7 TB/s; of 32 with ~1000 each: 16.2 us, of which the bytes take 10 and launch,
+// the first loads and the merge 6.  A tile of a token's few columns takes 1700 clocks, the last 600 to 1000 of them waiting for the bytes.  (Four warps with eight columns
+// each, half of them empty for groups of four heads: 3200 clocks, 21.0 us.)  A tile of 32 columns takes 3600: scores and maximum 1050, weights 620, sums 470 by 16 warps, whose
+// instructions are the bound: drafts of 5 tokens x 6 heads for 8 requests behind 2100: 21.3 us for 4.9 of bytes.  Keys and values in slots of their own, keys' freed
+// after S(t): no faster (44.8 us for 42.3 with the four long requests): what lies in flight is enough.
 #pragma once
 #include <type_traits>
 
@@ -46,7 +48,7 @@ struct PagedAttnParams {
 // NQ query columns, Q of them a group of softmax warps; column c of the MMA: group i has hi parts at i * 2 Q, lo parts at i * 2 Q + Q
 template <int NQ>
 struct PaCfg {
-  static constexpr int G = NQ >= 32 ? 4 : 2, Q = NQ / G;   // (32 columns: two groups 31.1 us for the drafts of 8 requests, four 25.5)
+  static constexpr int G = NQ >= 32 ? 4 : 2, Q = NQ / G;   // (32 columns: two groups 31.1 us for drafts of 8 requests behind 2100, four 25.5; now 21.3)
   static constexpr int kSoftWarps = 4 * G, kThreads = 32 * (kSoftWarps + 2), kResident = NQ >= 32 ? 1 : 2;
   static constexpr int N = 2 * NQ < 16 ? 16 : 2 * NQ;      // (16 at least; columns that nobody reads hold anything)
   static constexpr int kColBytes = N * 128;                // Q or one P tile: [N columns][128 bytes], 128B-swizzled
@@ -154,6 +156,24 @@ __device__ __forceinline__ void unrolled(F f) {  // f(0) .. f(N - 1), constants
   }
 }
 
+// The warp's v[i] combined over its lanes, column i in lanes i * (32 / Q) and on.  Each step halves what is sent: Q + 4 - log2 Q shuffles.
+template <int Q, typename F>
+__device__ __forceinline__ float by_column(float (&v)[Q], int lane, F op) {
+  int o = 16;
+#pragma unroll
+  for (int w = Q / 2; w >= 1; w /= 2, o /= 2) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < w; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + w], o);
+      v[i] = op(upper ? v[i + w] : v[i], other);
+    }
+  }
+#pragma unroll
+  for (; o >= 1; o /= 2) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+  return v[0];
+}
+
 // Byte k of column c: its 128 bytes are one row of a 128B-swizzled K-major tile
 __device__ __forceinline__ uint32_t pa_col(int c, int k) { return (uint32_t)(((c >> 3) << 10) + ((c & 7) << 7) + (((k >> 4) ^ (c & 7)) << 4) + (k & 15)); }
 
@@ -217,8 +237,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   const int first = page_lo + n_pages * split / splits, last = page_lo + n_pages * (split + 1) / splits;  // this split's pages (n_pages < 2^25)
   const int tiles = (last - first + 1) / 2;
 
-  float m[Q];
-  uint64_t o[Q / 2], l[Q / 2];  // of two queries each
+  uint64_t o[Q / 2], l[Q / 2], less[Q / 2];  // of two queries each; less: minus the maximum
   const int group = warp >> 2, key_at = tid & 127;  // of the softmax threads
   if (warp == SOFT) {
     // ================= producer =================
@@ -304,15 +323,25 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   } else {
     // ================= softmax =================
     // queries -> hi and lo parts, a warp per row
-    for (int q = warp; q < NQ; q += SOFT) {
-      uint2 u = make_uint2(0u, 0u);
-      if (q < nq) u = *reinterpret_cast<const uint2*>(p.q + (int64_t)(tok0 + q / R) * p.ldq + (int64_t)(g * R + q % R) * kHeadDim + lane * 4);
+    constexpr int ROWS = (NQ + SOFT - 1) / SOFT;
+    uint2 raw[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int q = warp + i * SOFT;
+      raw[i] = make_uint2(0u, 0u);
+      if (q < nq) raw[i] = *reinterpret_cast<const uint2*>(p.q + (int64_t)(tok0 + q / R) * p.ldq + (int64_t)(g * R + q % R) * kHeadDim + lane * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int q = warp + i * SOFT;
+      if (q >= NQ) break;
+      const uint2 u = raw[i];
       const float x[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
       const int e = e4m3_exponent(warp_max_f32(fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])))));
       const float inv = pow2i(-e);
       float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = scaled(x[i], inv);
+      for (int j = 0; j < 4; ++j) y[j] = scaled(x[j], inv);
       const uint32_t h0 = to_e4m3x2(y[0], y[1]), h1 = to_e4m3x2(y[2], y[3]);
       const float2 f0 = from_e4m3x2(h0), f1 = from_e4m3x2(h1);
       const uint32_t l0 = to_e4m3x2((y[0] - f0.x) * 16.f, (y[1] - f0.y) * 16.f), l1 = to_e4m3x2((y[2] - f1.x) * 16.f, (y[3] - f1.y) * 16.f);
@@ -325,16 +354,15 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
     __syncwarp();
     if (lane == 0) mbar_arrive(&q_full);
     bool ok = bounded_wait(&q_full, 0, &gave_up);  // q_scale of all rows
-    uint64_t qs[Q / 2], less[Q / 2];  // less: minus the maximum
+    uint64_t qs[Q / 2];
 #pragma unroll
     for (int i = 0; i < Q; i += 2) {
-      m[i] = m[i + 1] = PA_NOTHING;
       o[i / 2] = l[i / 2] = pair(0.f, 0.f);
       less[i / 2] = pair(-PA_NOTHING, -PA_NOTHING);
       qs[i / 2] = pair(q_scale[group * Q + i], q_scale[group * Q + i + 1]);
     }
     const int most_at = lane % (4 * Q);  // the maximum that this lane looks at: column most_at / 4, warp most_at % 4
-    float most = PA_NOTHING;             // m[most_at / 4]
+    float most = PA_NOTHING;             // the maximum of column most_at / 4
     const uint64_t sixteenth = pair(0.0625f, 0.0625f), eight = pair(8.f, 8.f);
     // Byte key_at of column j of the group: its 128 bytes are row j of a 128B-swizzled K-major tile, which pa_col(group * 2 Q + j, key_at) says in full
     const uint32_t p_at = smem_u32(sP) + group * 2 * Q * 128 + (key_at ^ (Q == 2 ? group << 6 : 0));
@@ -397,10 +425,18 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
             for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
           }
         }
+        if constexpr (NQ == 16) {  // (2 tokens of 6 heads a group, 8 requests behind 8400: 35.7 us, 39.1 by the instruction below; 32 columns: 58.6 and 55.6)
+          float w[Q];
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-          const float w = warp_max_f32(s[i]);
-          if (lane == 0) warp_most[t & 1][group * Q + i][warp & 3] = w;
+          for (int i = 0; i < Q; ++i) w[i] = s[i];
+          const float most_here = by_column<Q>(w, lane, [](float x, float y) { return fmaxf(x, y); });
+          if (lane % (32 / Q) == 0) warp_most[t & 1][group * Q + lane / (32 / Q)][warp & 3] = most_here;
+        } else {
+#pragma unroll
+          for (int i = 0; i < Q; ++i) {
+            const float w = warp_max_f32(s[i]);
+            if (lane == 0) warp_most[t & 1][group * Q + i][warp & 3] = w;
+          }
         }
       }
       if (group_sync_or<Cfg::G>(group, !ok)) {
@@ -418,11 +454,10 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
 #pragma unroll
         for (int i = 0; i < Q; i += 2) {
           const float m0 = __shfl_sync(0xffffffffu, most, i * 4), m1 = __shfl_sync(0xffffffffu, most, i * 4 + 4);
-          alpha[i / 2] = pair(exp2_ftz(m[i] - m0), exp2_ftz(m[i + 1] - m1));
+          const float2 was = unpair(less[i / 2]);
+          alpha[i / 2] = pair(exp2_ftz(-was.x - m0), exp2_ftz(-was.y - m1));
           l[i / 2] = mul_pair(l[i / 2], alpha[i / 2]);
           less[i / 2] = pair(-m0, -m1);
-          m[i] = m0;
-          m[i + 1] = m1;
         }
       }
       const uint32_t P = p_at + (t & 1) * Cfg::kColBytes;
@@ -457,11 +492,15 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
       for (int i = 0; i < Q / 2; ++i) o[i] = pair(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
       if (lane == 0 && p.status) atomicOr(p.status, PA_GAVE_UP);
     }
+    float all[Q];
 #pragma unroll
-    for (int i = 0; i < Q; ++i) {
-      const float w = warp_sum(i & 1 ? unpair(l[i / 2]).y : unpair(l[i / 2]).x);
-      if (lane == 0) sums[warp & 3][group * Q + i] = w;
+    for (int i = 0; i < Q; i += 2) {
+      const float2 x = unpair(l[i / 2]);
+      all[i] = x.x;
+      all[i + 1] = x.y;
     }
+    const float sum = by_column<Q>(all, lane, [](float x, float y) { return x + y; });
+    if (lane % (32 / Q) == 0) sums[warp & 3][group * Q + lane / (32 / Q)] = sum;
   }
   tc_fence_before();
   __syncthreads();
@@ -488,7 +527,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
         } else {
           mine[q * PA_ROW + 4 + key_at] = mine_o;
           if (key_at == 0) {
-            mine[q * PA_ROW] = m[i];
+            mine[q * PA_ROW] = -(i & 1 ? unpair(less[i / 2]).y : unpair(less[i / 2]).x);
             mine[q * PA_ROW + 1] = sum;
           }
         }
