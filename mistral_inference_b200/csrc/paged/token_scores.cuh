@@ -9,10 +9,11 @@
 // the segment's maximum, in pairs (3.5 instructions an entry).  Every 16-byte piece is fetched, read and replaced by the next segment's by the same thread, so copies are in flight from
 // the middle of one segment to the beginning of the next and need no barrier.  The best are not sorted: a warp's r-th largest thread maximum, the least of them
 // over the warps, is a value that at least r * warps >= top entries reach, and few more; the threads that have some pick them out, and they are ranked by counting.  Two block
-// barriers a segment.  A warp a row joins the segments, in a
-// second kernel or, where few rows leave room, behind a cluster's barrier.
-// 1000 x 131072 fp32, 8 alternatives: the largest taken off over and over 1540 us; entries in registers, a CTA for 8192 of them 141; longer walks with a list kept
-// up to date 205 (a barrier a slice, and more code than the instruction cache holds); whole segments by one bulk copy each, fetched behind the second barrier 107.
+// barriers a segment.  A warp a row joins the segments, in a second kernel or, where few rows leave room, behind a cluster's barrier.
+// 1000 x 131072 fp32, 8 alternatives: 104 us, 5.0 TB/s (20 of them 118; bf16 79, whose entries take more of the bound by instructions).  Before: the largest taken off over and
+// over 1540 us; entries in registers, a CTA for 8192 of them 141; longer walks with a list kept up to date 205 (a barrier a slice, and more code than the instruction
+// cache holds); whole segments by one bulk copy each, fetched behind the second barrier 107.  32 rows, 20 alternatives: 14.4 us, 2.6 for the bytes, the rest two launches and
+// two segments' latency; 1 x 32000: 7.6.
 #pragma once
 #include <cfloat>
 
@@ -344,20 +345,16 @@ __global__ void __launch_bounds__(TS_THREADS, TS_CTAS) token_scores_segment_kern
     unsigned long long* best = p.best + (int64_t)item * top;
     const int have = n_list[turn];
     if (have <= TS_ROOM && !odd) {
-      if (have <= 64) {  // a warp an entry, or a thread (30 entries: 300 clocks sooner; 256: 10000 later)
-        for (int i = warp; i < have; i += TS_WARPS) {
-          const unsigned long long key = list[i];
-          const int rank = __popc(__ballot_sync(0xffffffffu, lane < have && list[lane] > key)) + __popc(__ballot_sync(0xffffffffu, lane + 32 < have && list[lane + 32] > key));
-          if (lane == 0 && rank < top) best[rank] = key;
-        }
-      } else {
-        for (int i = tid; i < have; i += TS_THREADS) {
-          const unsigned long long key = list[i];
-          int rank = 0;
+      // 2^g threads an entry.  (32 alternatives of 1500 x 32768: 56.6 us; a warp an entry up to 64 of them and one thread beyond 60.8)
+      const int g = have <= 32 ? 3 : have <= 64 ? 2 : have <= 128 ? 1 : 0;
+      for (int first = 0; first < have; first += TS_THREADS >> g) {
+        const int i = first + (tid >> g);
+        const unsigned long long key = i < have ? list[i] : ~0ull;
+        int rank = 0;
 #pragma unroll 4
-          for (int k = 0; k < have; ++k) rank += list[k] > key;
-          if (rank < top) best[rank] = key;
-        }
+        for (int k = tid & ((1 << g) - 1); k < have; k += 1 << g) rank += list[k] > key;
+        for (int o = 1; o < 1 << g; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (i < have && (tid & ((1 << g) - 1)) == 0 && rank < top) best[rank] = key;
       }
       for (int i = have + tid; i < top; i += TS_THREADS) best[i] = 0ull;  // (a segment of fewer entries)
       continue;
