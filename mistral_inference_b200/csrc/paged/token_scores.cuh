@@ -148,7 +148,7 @@ __device__ __forceinline__ void token_scores_join(const TokenScoresParams& p, in
       const unsigned long long top = warp_max_key(head);
       if (head == top) {
         ++at;
-        head = at < p.top ? lists[lane * p.top + at] : 0ull;
+        head = lane < p.segments && at < p.top ? lists[lane * p.top + at] : 0ull;
       }
       if ((k & 31) == lane) mine = top;
       if ((k & 31) == 31 || k + 1 == p.top)  // 32 results at a time

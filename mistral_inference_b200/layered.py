@@ -235,6 +235,7 @@ class LayeredTransformer(nn.Module):
     @torch.inference_mode()
     def forward_scores(self, input_ids: torch.Tensor, seqlens: List[int], cache: Optional[BufferCache], targets: torch.Tensor, top: int) -> Tuple[TokenScores, torch.Tensor]:
         """`forward_logprobs` with the entropy of every token's distribution and its `top` most likely tokens (scores.py)."""
+        assert min(seqlens) >= 1, "every sequence brings a token"
         logits = self.forward(input_ids, seqlens, cache).float().contiguous()
         last_idx = torch.tensor(seqlens, device=input_ids.device).cumsum(0) - 1
         return token_scores(logits, targets, top=top), logits.index_select(0, last_idx)

@@ -460,6 +460,7 @@ class Transformer(nn.Module):
         """`forward_logprobs` with the entropy of every token's distribution and its `top` most likely tokens (scores.py): the logits are written block by block."""
         self._last_static_logits = 0
         T, V = input_ids.shape[0], self.vocab_size
+        assert min(seqlens) >= 1, "every sequence brings a token"
         ends = list(itertools.accumulate(seqlens))
         last_rows = torch.tensor([e - 1 for e in ends], device=input_ids.device)
         if self.num_pipeline_ranks > 1:

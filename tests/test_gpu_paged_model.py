@@ -144,6 +144,24 @@ def test_requests_come_and_go():
     assert (got - want).abs().max() <= logit_tol(want, ULPS)
 
 
+def test_a_first_prompt_beside_requests_that_bring_nothing():
+    m, p = model_of(max_batch=3)
+    V = p["vocab_size"]
+    prompt = [(torch.arange(n) * 7 % V).cuda() for n in (90, 33)]
+    a, b = m.make_cache(3, 300, kv_cache="pages"), m.make_cache(3, 300, kv_cache="pages")
+    got = m.forward(prompt[0], [0, 90, 0], a)
+    got = torch.cat([got, m.forward(prompt[1], [33, 0, 0], a)])
+    step = m.forward(torch.tensor([4, 5], device="cuda"), [1, 1, 0], a)
+    want = m.forward(prompt[0], [90], b)
+    b.admit(1)
+    want = torch.cat([want, m.forward(prompt[1], [0, 33], b)])
+    assert (got[:90] - want[:90]).abs().max() <= logit_tol(want, ULPS) and (got[90:] - want[90:]).abs().max() <= logit_tol(want, ULPS)
+    want = m.forward(torch.tensor([5, 4], device="cuda"), [1, 1], b)
+    assert (step - want[[1, 0]]).abs().max() <= logit_tol(want, ULPS)
+    with pytest.raises(AssertionError, match="brings a token"):
+        m.forward_scores(prompt[0], [0, 90, 0], a, torch.zeros(90, dtype=torch.long, device="cuda"), 3)
+
+
 def test_a_step_that_fails_leaves_no_tokens_behind(monkeypatch):
     m, p = model_of(max_batch=2)
     cache = m.make_cache(2, 100, kv_cache="pages")
