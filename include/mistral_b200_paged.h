@@ -43,7 +43,7 @@ int mbp_pages_write(const void* k, int64_t ldk, const void* v, int64_t ldv, void
                     int64_t B, int64_t T, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages, void* stream);
 
 /* Bytes of scratch that mbp_attn_pages needs for these sizes (0: none): portions of prompts go through 16-bit rings. */
-int64_t mbp_attn_pages_scratch(int64_t B, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window);
+int64_t mbp_attn_pages_scratch(int64_t B, int64_t T, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window);
 /* Causal attention of a plan's tokens over one layer's pool, their own keys and values written before.  q [T, H * 128] bf16, rows ldq elements apart (8-byte aligned); out
  * [T, H * 128] bf16, 8-byte aligned.  The query at position p sees positions (p - window, p]; window 0: all.  longest: no request has more tokens in this plan; most: none has more in all
  * (0: unknown).  status [1] or NULL: 16 is set when a wait inside ran out, 32 when a request has more tokens than longest or most say: those it

@@ -28,7 +28,7 @@ _SIGNATURES = {
     "mbp_pages_extend": (c_int, [P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P]),
     "mbp_pages_truncate": (c_int, [P, P, P, P, P, P, P, P, I, I, I, I, P]),
     "mbp_pages_write": (c_int, [P, I, P, I, P, P, P, P, P, I, I, I, I, I, P]),
-    "mbp_attn_pages_scratch": (I, [I, I, I, I, I, I, I]),
+    "mbp_attn_pages_scratch": (I, [I, I, I, I, I, I, I, I]),
     "mbp_attn_pages": (c_int, [P, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, c_float, P, I, P]),
     "mbp_token_scores_sizes": (c_int, [I, I, I, P]),
     "mbp_token_scores": (c_int, [P, I, c_int, P, P, P, P, P, I, I, I, P, P]),
@@ -125,14 +125,14 @@ def pages_write(dev: int, kv, scale, k, v, plan, T: int, N: int, KV: int) -> Non
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_scratch(B: int, longest: int, most: int, width: int, n_heads: int, KV: int, window: int) -> int:
-    return lib().mbp_attn_pages_scratch(B, longest, most, width, n_heads, KV, window)
+def _attn_scratch(B: int, T: int, longest: int, most: int, width: int, n_heads: int, KV: int, window: int) -> int:
+    return lib().mbp_attn_pages_scratch(B, T, longest, most, width, n_heads, KV, window)
 
 
 def attn_pages(dev: int, q, kv, scale, plan, out, T: int, N: int, KV: int, H: int, R: int, width: int, window: int, softmax_scale: float) -> None:
     pq, ldq = _rows(q, H, dev)
     B, status = plan.rows.shape[0], plan.status
-    need = _attn_scratch(B, plan.longest, plan.most, width, H, KV, window)
+    need = _attn_scratch(B, T, plan.longest, plan.most, width, H, KV, window)
     scratch = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
     _call("mbp_attn_pages", dev, pq, ldq, kv.data_ptr(), scale.data_ptr(), plan.table.data_ptr(), plan.rows.data_ptr(), plan.q_start.data_ptr(), plan.seqpos.data_ptr(), out.data_ptr(),
           None if status is None else _ptr(status, dev), B, T, plan.longest, plan.most, R, width, N, H, KV, HEAD_DIM, window, softmax_scale, None if scratch is None else scratch.data_ptr(), need)

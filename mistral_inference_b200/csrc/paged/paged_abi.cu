@@ -125,7 +125,7 @@ struct AttnCut {
   int64_t q_tiles, keys;
   bool rings;
 };
-static AttnCut attn_cut(int64_t B, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window) {
+static AttnCut attn_cut(int64_t B, int64_t T, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window) {
   AttnCut c;
   const int64_t rep = n_heads / n_kv_heads, want = longest * rep, sms = device_info::sm_count() > 0 ? device_info::sm_count() : 148;
   c.nq = want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 ? 16 : 32;
@@ -133,17 +133,20 @@ static AttnCut attn_cut(int64_t B, int64_t longest, int64_t most, int64_t P, int
   c.q_tiles = (longest + c.tokens - 1) / c.tokens;
   c.keys = most > 0 && most < P * PG_TOKENS ? most : P * PG_TOKENS;
   if (window > 0 && c.keys > window + longest) c.keys = window + longest;
-  const int64_t pairs = B * n_kv_heads * c.q_tiles, room = sms * (c.nq < 32 ? 2 : 1);
+  // tiles of `rows` tokens that have any: the requests' lengths are not known here, but their sum is
+  auto used = [&](int64_t rows, int64_t most_tiles) { return T / rows + B < B * most_tiles ? T / rows + B : B * most_tiles; };
+  const int64_t pairs = n_kv_heads * used(c.tokens, c.q_tiles), room = sms * (c.nq < 32 ? 2 : 1);
   c.splits = 1;
   while (c.splits < PA_MAX_SPLITS && pairs * c.splits * 2 <= room && c.keys >= (int64_t)c.splits * 4 * PA_KEYS) c.splits *= 2;
-  // Time of both ways in us, tiles of 128 keys: 1.9 each on 32 query columns, 2.9 each in the prompt kernel (two heads x 128 tokens), and the conversion.  (nemo shape, measured
-  // direct and by rings: 1 x 17 tokens behind 8000 39, 186; 1 x 257 behind 2000 79, 58; 3 x 65 behind 2000 68, 65; 3 x 129 behind 8000 328, 204.)
+  // Time of both ways in us, tiles of 128 keys: 1.4 each on 32 query columns, 2.55 each in the prompt kernel (two heads x 128 tokens), and the conversion.  (nemo shape,
+  // measured direct and by rings: 1 x 17 tokens behind 8000 33, 186; 1 x 257 behind 2000 66, 58; 1 x 257 behind 300 28, 24; 3 x 65 behind 2000 57, 65; 3 x 129 behind
+  // 8000 268, 203; 16 heads over 4, 3 x 100 behind 20000 234, 464.)
   c.rings = false;
   if (c.q_tiles > 1) {
     const double tiles = (double)(c.keys + PA_KEYS - 1) / PA_KEYS;
-    const int64_t ctas = B * n_heads / (rep % 2 == 0 ? 2 : 1) * ((longest + 127) / 128);
-    const double direct = (double)((pairs * c.splits + sms - 1) / sms) * (tiles / c.splits) * 1.9 + 6;
-    const double rings = (double)((ctas + sms - 1) / sms) * tiles * 2.9 + 11 + (double)B * (double)c.keys * (double)n_kv_heads * (kHeadDim * 2 * 3) / 4e6;
+    const int64_t prompt = n_heads / (rep % 2 == 0 ? 2 : 1) * used(128, (longest + 127) / 128);
+    const double direct = (double)((pairs * c.splits + sms - 1) / sms) * (tiles / c.splits * 1.4 + 5) + 3;
+    const double rings = (double)((prompt + sms - 1) / sms) * tiles * 2.55 + 12 + (double)B * (double)c.keys * (double)n_kv_heads * (kHeadDim * 2 * 3) / 4e6;
     c.rings = rings < direct || n_kv_heads * c.q_tiles > 65535;
   }
   return c;
@@ -230,10 +233,10 @@ int mbp_pages_write(const void* k, int64_t ldk, const void* v, int64_t ldv, void
   return MB200_OK;
 }
 
-int64_t mbp_attn_pages_scratch(int64_t B, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window) {
+int64_t mbp_attn_pages_scratch(int64_t B, int64_t T, int64_t longest, int64_t most, int64_t P, int64_t n_heads, int64_t n_kv_heads, int64_t window) {
   int64_t group;
-  if (B < 1 || longest < 1 || P < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || n_heads > 32 * n_kv_heads || n_heads % n_kv_heads || window < 0) return 0;
-  return attn_cut(B, longest, most, P, n_heads, n_kv_heads, window).rings ? ring_scratch(B, longest, most, P, n_kv_heads, window, &group) : 0;
+  if (B < 1 || T < 1 || longest < 1 || P < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || n_heads > 32 * n_kv_heads || n_heads % n_kv_heads || window < 0) return 0;
+  return attn_cut(B, T, longest, most, P, n_heads, n_kv_heads, window).rings ? ring_scratch(B, longest, most, P, n_kv_heads, window, &group) : 0;
 }
 
 int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scale, const int32_t* table, const int32_t* rows, const int32_t* q_start, const int32_t* seqpos,
@@ -252,7 +255,7 @@ int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scal
   MB_CHECK_ARG(((uintptr_t)out) % 8 == 0, "attn_pages: the output must be 8-byte aligned");
   MB_CHECK_ARG(softmax_scale > 0.f && softmax_scale < 3.4e38f, "attn_pages: scale %g", (double)softmax_scale);
   if (T == 0) return MB200_OK;
-  const AttnCut cut = attn_cut(B, longest, most, P, n_heads, n_kv_heads, window);
+  const AttnCut cut = attn_cut(B, T, longest, most, P, n_heads, n_kv_heads, window);
   // (rows of queries that the copy engine cannot take stay with the kernel below)
   if (cut.rings && (uintptr_t)q % 16 == 0 && ldq % 8 == 0 && (uintptr_t)out % 16 == 0) {
     int64_t group = 0;

@@ -280,10 +280,10 @@ def test_attention_of_several_tokens(new, H, KV, window):
 def by_rings(H, KV, past, new, window=0):
     """Whether such a call's pages go through 16-bit rings."""
     total = [p + n for p, n in zip(past, new)]
-    return _abi_paged.lib().mbp_attn_pages_scratch(len(past), max(new), max(total), U.cdiv(max(total), 64) + 1, H, KV, window) > 0
+    return _abi_paged.lib().mbp_attn_pages_scratch(len(past), sum(new), max(new), max(total), U.cdiv(max(total), 64) + 1, H, KV, window) > 0
 
 
-@pytest.mark.parametrize("H,KV,past,new,window", [(32, 8, [0, 300], [300, 129], 0), (16, 16, [100, 0, 63], [257, 128, 0], 0), (24, 8, [700, 64], [200, 333], 150), (8, 1, [1000, 0, 5, 64], [400, 1, 130, 77], 65),
+@pytest.mark.parametrize("H,KV,past,new,window", [(32, 8, [0, 300], [300, 129], 0), (16, 16, [100, 0, 63], [500, 300, 0], 0), (24, 8, [700, 64], [200, 333], 150), (8, 1, [1000, 0, 5, 64], [400, 1, 130, 77], 65),
                                                   (15, 5, [200, 100], [550, 460], 0), (32, 8, [1500, 3], [190, 333], 1000)])
 def test_attention_of_portions(H, KV, past, new, window):
     assert by_rings(H, KV, past, new, window)
@@ -298,7 +298,7 @@ def test_portions_of_one_request_at_a_time():
     wide = torch.full((plan.table.shape[0], 4200), -1, dtype=torch.int32, device=DEV)
     wide[:, : plan.table.shape[1]] = plan.table
     loose = mi.PagePlan(wide, plan.rows, plan.q_start, plan.seqpos, plan.positions, plan.slots, plan.longest)
-    assert _abi_paged.lib().mbp_attn_pages_scratch(3, 300, 0, 4200, 32, 8, 0) == 4200 * 64 * 8 * 128 * 4 > 1 << 30
+    assert _abi_paged.lib().mbp_attn_pages_scratch(3, 900, 300, 0, 4200, 32, 8, 0) == 4200 * 64 * 8 * 128 * 4 > 1 << 30
     assert torch.equal(mi.attend_pages(q, kv, scale, loose), want)
 
 
@@ -314,14 +314,15 @@ def test_portions_longer_than_the_plan_says_are_no_numbers():
         plan.check()
 
 
-@pytest.mark.parametrize("past,new,longest", [([900, 30], [250, 300], 90), ([900, 30], [250, 300], 260), ([70, 30, 5], [1, 3, 2], 1), ([70, 30], [40, 12], 12)])
-def test_requests_that_bring_more_than_the_plan_says(past, new, longest):
+@pytest.mark.parametrize("KV,past,new,longest", [(8, [900, 30], [250, 300], 260), (8, [900, 30], [250, 300], 200), (2, [900, 30], [250, 300], 260), (2, [70, 30, 5], [1, 3, 2], 1),
+                                                 (2, [70, 30], [40, 12], 12)])
+def test_requests_that_bring_more_than_the_plan_says(KV, past, new, longest):
     """Both ways of attending: what there is no room for is no number, the other requests are right."""
-    plan, kv, scale, kv_h, scale_h, table, rows = filled(2, past, new, 4)
-    T = sum(new)
-    q = numbers(T, 8, 128, seed=1, spread=0)
+    plan, kv, scale, kv_h, scale_h, table, rows = filled(KV, past, new, 4)
+    T, H = sum(new), 4 * KV
+    q = numbers(T, H, 128, seed=1, spread=0)
     plan.longest = longest
-    got = mi.attend_pages(q.to(DEV), kv, scale, plan, out=torch.full((T, 1024), 9.0, dtype=torch.bfloat16, device=DEV)).cpu().double().view(T, 8, 128)
+    got = mi.attend_pages(q.to(DEV), kv, scale, plan, out=torch.full((T, H * 128), 9.0, dtype=torch.bfloat16, device=DEV)).cpu().double().view(T, H, 128)
     starts = [sum(new[:i]) for i in range(len(new) + 1)]
     want, mag = U.attend_ref(q, kv_h.double(), scale_h, table, rows, starts, past)
     tol = U.attend_tolerance(want, mag, max(p + n for p, n in zip(past, new)), float(448 * scale_h.max()))

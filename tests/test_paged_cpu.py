@@ -69,12 +69,12 @@ def test_attention_is_refused(lib):
                     (dict(out=X + 4), "aligned"), (dict(longest=0), "longest"), (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(P=0), "P="), (dict(N=0), "pages")]:
         assert attend(**kw) == -1 and why in last(lib), (kw, last(lib))
     assert attend(T=0) == 0
-    scratch = lambda B=4, longest=1000, most=0, P=64, H=32, KV=8, window=0: lib.mbp_attn_pages_scratch(B, longest, most, P, H, KV, window)  # noqa: E731
+    scratch = lambda B=4, T=4000, longest=1000, most=0, P=64, H=32, KV=8, window=0: lib.mbp_attn_pages_scratch(B, T, longest, most, P, H, KV, window)  # noqa: E731
     need = scratch()  # (sized for 148 SMs where there is no GPU)
-    assert need == 4 * 64 * 64 * 8 * 128 * 4 and scratch(longest=1) == 0
+    assert need == 4 * 64 * 64 * 8 * 128 * 4 and scratch(longest=1) == 0 and scratch(T=40) == 0
     assert scratch(most=1500) < need and scratch(window=100) < need
-    assert scratch(B=0) == scratch(H=33) == scratch(KV=0) == scratch(window=-1) == 0
-    assert scratch(B=64, P=512) <= 1 << 30  # requests take turns
+    assert scratch(B=0) == scratch(T=0) == scratch(H=33) == scratch(KV=0) == scratch(window=-1) == 0
+    assert 0 < scratch(B=64, T=64000, P=512) <= 1 << 30  # requests take turns
     for kw in (dict(scratch=None, room=need), dict(scratch=X, room=need - 1), dict(scratch=X + 16, room=need)):  # a portion without room
         assert attend(B=4, T=4000, longest=1000, P=64, H=32, KV=8, ldq=4096, **kw) == -2 and "scratch" in last(lib)
 
@@ -192,4 +192,4 @@ def test_an_unknown_cache_is_refused():
 def test_declarations_of_this_abi_version():
     """A change of the declarations takes a new version, so that a library built before it is refused."""
     code = re.sub(r"/\*.*?\*/", " ", HEADER.read_text(), flags=re.S)
-    assert zlib.crc32(" ".join(code.split()).encode()) == 2100840578, "raise the ABI version with this change"
+    assert zlib.crc32(" ".join(code.split()).encode()) == 1297119818, "raise the ABI version with this change"
