@@ -48,7 +48,8 @@ int64_t mbp_attn_pages_scratch(int64_t B, int64_t T, int64_t longest, int64_t mo
  * [T, H * 128] bf16, 8-byte aligned.  The query at position p sees positions (p - window, p]; window 0: all.  longest: no request has more tokens in this plan; most: none has more in all
  * (0: unknown).  status [1] or NULL: 16 is set when a wait inside ran out, 32 when a request has more tokens than longest or most say: those it
  * has no room for, or all of its results, are NaN.  scratch:
- * mbp_attn_pages_scratch bytes, 256-byte aligned, of any content and this call's own until it has run.  A page id out of range makes the results that need it NaN; rows of out behind
+ * mbp_attn_pages_scratch bytes, 256-byte aligned, of any content and this call's own until it has run.  A page id out of range makes the results that need it NaN.  So does a NaN among the
+ * values, in its column, of the queries that see it (by rings also of others up to 127 positions from those); rows of out behind
  * q_start[B] are left as they are. */
 int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scale, const int32_t* table, const int32_t* rows, const int32_t* q_start, const int32_t* seqpos,
                    void* out, int32_t* status, int64_t B, int64_t T, int64_t longest, int64_t most, int64_t R, int64_t P, int64_t n_pages, int64_t n_heads, int64_t n_kv_heads,

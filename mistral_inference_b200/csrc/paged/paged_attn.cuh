@@ -192,11 +192,15 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   __shared__ float q_scale[NQ];                           // a query row's scale, times the softmax scale, in log2 units
   __shared__ float warp_most[2][NQ][4];                   // by tile parity
   __shared__ float sums[4][NQ];
+  // Values that are no numbers, of keys that not all tokens of the tile see, are taken out (0 * NaN is not 0) and noted by dimension: a bit for each token of the tile behind
+  // its first, and for each place from the beginning of the first one's window on
+  __shared__ uint32_t nan_new[kHeadDim], nan_old[kHeadDim];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int split = blockIdx.x, splits = gridDim.x, g = blockIdx.y % p.KV, qt = blockIdx.y / p.KV, b = blockIdx.z;
   const int R = p.H / p.KV;
   pdl_trigger();
+  if (tid < kHeadDim) nan_new[tid] = nan_old[tid] = 0;
   if (tid == 0) {
     for (int i = 0; i < PA_STAGES; ++i) {
       mbar_init(&kv_full[i], 2);  // the copies' arrival and the scales'
@@ -296,9 +300,41 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
       }
       __syncwarp();
     };
+    // What values that a query does not see hold must not reach its sums: 0 * NaN is not 0.  Done while the softmax warps have the tile's scores.
+    auto hide_values = [&](int t) {
+      const int key0 = (first + 2 * t) * PG_TOKENS, end = min(hi, last * PG_TOKENS);
+      if (key0 >= lo && key0 + PA_KEYS <= pos0 + 1 && (p.window <= 0 || key0 >= pos0 + n - p.window)) return;  // every query sees every key
+      uint8_t* v = smem + t % PA_STAGES * PA_STAGE_BYTES + 2 * PG_BYTES;
+      for (int r = lane >> 3; r < PA_KEYS; r += 4)  // rows that no query sees, eight lanes each
+        if (key0 + r < lo || key0 + r >= end) *reinterpret_cast<uint4*>(v + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+      // rows that some queries see: later tokens of the tile, and what the later tokens' windows have left behind, a lane each
+      auto scan = [&](int key, uint32_t* whose) {
+        uint4* row = reinterpret_cast<uint4*>(v + (key - key0) * 128);
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const int chunk = (i + lane) & 7;
+          uint4 x = row[chunk];
+          const uint32_t bad[4] = {__vcmpeq4(x.x & 0x7f7f7f7fu, 0x7f7f7f7fu), __vcmpeq4(x.y & 0x7f7f7f7fu, 0x7f7f7f7fu), __vcmpeq4(x.z & 0x7f7f7f7fu, 0x7f7f7f7fu),
+                                   __vcmpeq4(x.w & 0x7f7f7f7fu, 0x7f7f7f7fu)};
+          if ((bad[0] | bad[1] | bad[2] | bad[3]) == 0) continue;
+          row[chunk] = make_uint4(x.x & ~bad[0], x.y & ~bad[1], x.z & ~bad[2], x.w & ~bad[3]);
+          for (int c = 0; c < 16; ++c)
+            if (bad[c >> 2] >> 8 * (c & 3) & 1) atomicOr(whose + (chunk ^ (key - key0 & 7)) * 16 + c, 1u << lane);
+        }
+      };
+      __syncwarp();
+      if (n > 1) {
+        const int later = pos0 + 1 + lane, left = pos0 + 1 - p.window + lane;
+        if (later < hi && later >= key0 && later < min(end, key0 + PA_KEYS)) scan(later, nan_new);
+        if (p.window > 0 && lane < n - 1 && left <= pos0 && left >= max(lo, key0) && left < min(end, key0 + PA_KEYS)) scan(left, nan_old);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
     if (tiles > 0) issue_s(0);
     if (tiles > 1) issue_s(1);
     for (int t = 0; t < tiles && ok; ++t) {
+      hide_values(t);
       ok = bounded_wait(&p_full, t & 1, &gave_up);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -419,11 +455,6 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
             }
             s[i] = sees ? s[i] : -INFINITY;
           }
-          if (!seen && here && group == 0) {  // what this row holds must not reach the sums: 0 * NaN is not 0
-            uint4* v = reinterpret_cast<uint4*>(smem + st * PA_STAGE_BYTES + 2 * PG_BYTES + key_at * 128);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
-          }
         }
         if constexpr (NQ == 16) {  // (2 tokens of 6 heads a group, 8 requests behind 8400: 35.7 us, 39.1 by the instruction below; 32 columns: 58.6 and 55.6)
           float w[Q];
@@ -517,6 +548,19 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   // this split's results over the ring, which is used up
   float* mine = reinterpret_cast<float*>(smem);
   if (warp < SOFT) {
+    const uint32_t in_new = nan_new[key_at], in_old = nan_old[key_at];
+    if (__any_sync(0xffffffffu, (in_new | in_old) != 0)) {
+      unrolled<Q / 2>([&](auto at) {
+        float2 x = unpair(o[decltype(at)::value]);
+        for (int half = 0; half < 2; ++half) {
+          const int i = (group * Q + 2 * decltype(at)::value + half) / R;  // token of the tile
+          uint32_t sees = (1u << i) - 1;  // the tokens before it but for the first, whose values every query sees or has left behind
+          if (p.window > 0 && i >= p.window) sees &= ~((1u << (i - p.window)) - 1);
+          if ((in_new & sees) != 0 || in_old >> i != 0) (half ? x.y : x.x) = __int_as_float(0x7fffffff);
+        }
+        o[decltype(at)::value] = pair(x.x, x.y);
+      });
+    }
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
       const int q = group * Q + i;

@@ -142,7 +142,8 @@ def attend_pages(q: torch.Tensor, kv: torch.Tensor, scale: torch.Tensor, plan: P
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[T, H * 128] bf16: attention of the queries [T, H, 128] (or [T, H * 128]; bf16) of the plan's tokens, whose own keys and values have been written before.  A query sees the
     last `window` positions of its request up to its own (0: all).  H is a multiple of the pool's heads, at most 32 times as many.  Rows of `out` behind the plan's last
-    token stay as they are."""
+    token stay as they are.  A NaN among the values makes its column NaN for the queries that see it; in a portion long enough to go through 16-bit rings also for
+    others of its block of 128 tokens, as in the prompt kernel."""
     dev, N, KV = _pool(kv, scale, plan)
     T, width = q.shape[0], q.shape[1] * q.shape[2] if q.dim() == 3 else q.shape[1]
     assert T == plan.slots.shape[0], f"{plan.slots.shape[0]} tokens planned, queries {tuple(q.shape)}"

@@ -410,6 +410,24 @@ def test_numbers_that_are_none_stay_with_the_queries_that_see_them():
     assert got[0, 4:].isnan().all() and got.isnan().sum() == 4 * 128
 
 
+@pytest.mark.parametrize("past,new,window", [(300, 5, 0), (60, 8, 0), (125, 8, 0), (300, 6, 40), (61, 7, 3), (2, 8, 20), (130, 8, 8), (190, 2, 64)])
+def test_values_that_are_none_stay_with_the_tokens_that_see_them(past, new, window):
+    """Several tokens at once: those before a NaN, and those whose window has left it behind, do not notice."""
+    plan, kv, scale, *_ = filled(2, [past, 40], [new, 1], 9)
+    q = numbers(new + 1, 8, 128, seed=2, spread=0).to(DEV)
+    clean = mi.attend_pages(q, kv, scale, plan, window=window).view(new + 1, 8, 128)
+    for at in sorted({past - 1, past, past + 1, past + new // 2, past + new - 1, max(0, past - window + 1), max(0, past - window + new // 2 + 1)}):
+        for code, dim in ((0x7F, 33), (0xFF, 126)):
+            bad = kv.view(torch.uint8).clone()
+            bad[int(plan.table[int(plan.rows[0]), at // 64]), 1, 1, at % 64, dim] = code
+            got = mi.attend_pages(q, bad.view(U.E4M3), scale, plan, window=window).view(new + 1, 8, 128)
+            want = torch.zeros_like(got, dtype=torch.bool)
+            for i in range(new):
+                want[i, 4:, dim] = at <= past + i and (window == 0 or at > past + i - window)
+            assert torch.equal(got.isnan(), want), (at, code)
+            assert torch.equal(got[~want], clean[~want])
+
+
 def test_pages_that_are_none_make_no_numbers():
     plan, kv, scale, *_ = filled(2, [300, 200], [1, 1], 9)
     q = numbers(2, 8, 128, seed=2, spread=0).to(DEV)
