@@ -2,7 +2,8 @@
 //
 // From some tokens on the tensor pipe bounds attention, not the pages' bytes: the 128 x 128 tiles of the prompt kernel use it four times as well as the few query columns of
 // paged_attn.cuh, and a page is converted once instead of once a tile of queries.  A number is code * scale, a power of two: exact in bf16.  Converting is memory-bound: 1 byte
-// read and 2 written a number, and read once more by the attention.
+// read and 2 written a number, and read once more by the attention.  Three portions of ~650 tokens behind ~2000, 32 heads over 8: 133 us, 597 TFLOP/s, of which converting takes 11.6
+// (4.4 TB/s).  The rest is 336 CTAs of the prompt kernel on 148 SMs, a third round of which is a quarter full.
 #pragma once
 #include "../attn_prompt_tcgen05.cuh"
 #include "paged_common.cuh"
@@ -41,13 +42,20 @@ __global__ void __launch_bounds__(PR_THREADS) paged_ring_kernel(PagedRingParams 
   const int64_t block = ((int64_t)page * p.KV + g) * 2;
   const float scale[2] = {is ? p.scale[block] : __int_as_float(0x7fffffff), is ? p.scale[block + 1] : __int_as_float(0x7fffffff)};
   const uint8_t* src = p.kv + block * PG_BYTES;
+  constexpr int STEPS = 2 * PG_BYTES / 16 / PR_THREADS;  // 16 codes a thread and step, all fetched before the first is used
+  uint4 v[STEPS];
+  auto pos_of = [&](int at) { return page_at * PG_TOKENS + at % (PG_BYTES / 16) / (kHeadDim / 16); };
 #pragma unroll
-  for (int i = 0; i < 2 * PG_BYTES / 16 / PR_THREADS; ++i) {  // 16 codes a thread and step
-    const int at = i * PR_THREADS + threadIdx.x, kind = at / (PG_BYTES / 16), key = at % (PG_BYTES / 16) / (kHeadDim / 16), col = at % (kHeadDim / 16) * 16;
-    const int pos = page_at * PG_TOKENS + key;
+  for (int i = 0; i < STEPS; ++i) {
+    const int at = i * PR_THREADS + threadIdx.x, pos = pos_of(at);
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (pos >= from && pos < to) v[i] = *reinterpret_cast<const uint4*>(src + (int64_t)at * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int at = i * PR_THREADS + threadIdx.x, kind = at / (PG_BYTES / 16), col = at % (kHeadDim / 16) * 16, pos = pos_of(at);
     if (pos < from || pos >= to) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(src + (int64_t)at * 16);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
     uint32_t out[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -111,7 +119,8 @@ inline int launch_paged_prompt(PagedRingParams p, const void* q, int64_t ldq, bf
   f.own = 0;
   f.n_tab = 0;
   f.scale_log2 = scale_log2;
-  const bool two = (H / p.KV) % 2 == 0;
+  // Two heads a CTA share every key and value tile, unless single ones all run at once.  (257 tokens of 32 heads behind 2000: 53 us, 58 by two; 3 x 700: 163 and 115.)
+  const bool two = (H / p.KV) % 2 == 0 && H * B * ceil_div(longest, FA_BM) > device_info::sm_count();
   const dim3 fgrid((unsigned)(H / (two ? 2 : 1)), (unsigned)ceil_div(longest, FA_BM), (unsigned)B);
   if (two) {
     MB_CHECK_CUDA((device_info::allow_shared<attn_prompt_tcgen05_kernel<2, false>>(FA_SMEM_BASE)));
