@@ -102,6 +102,15 @@ static int launch_score_segments(const TokenScoresParams& p, cudaStream_t st) {
 
 template <typename ST>
 static int launch_token_scores(TokenScoresParams p, cudaStream_t st) {
+  if (p.V <= TS_SHORT) {
+    const dim3 grid((unsigned)((p.T + TS_SHORT_WARPS - 1) / TS_SHORT_WARPS)), block(TS_SHORT_WARPS * 32);
+    if (p.V <= TS_SHORT / 2) {
+      MB_CHECK_CUDA(launch_pdl(token_scores_short_kernel<ST, TS_SHORT / 64>, grid, block, 0, st, p));
+    } else {
+      MB_CHECK_CUDA(launch_pdl(token_scores_short_kernel<ST, TS_SHORT / 32>, grid, block, 0, st, p));
+    }
+    return MB200_OK;
+  }
   const int cluster = score_cluster(p.T, p.V, sizeof(ST));
   if (cluster > 0) {
     const int step = TS_THREADS * (16 / (int)sizeof(ST));

@@ -46,6 +46,29 @@ def test_scores(V, T, dtype):
     check(x, None, min(V, 3))
 
 
+@pytest.mark.parametrize("V", [33, 64, 1024, 1025, 2047, 2048, 2049])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_short_rows(V, dtype):
+    """NaN, infinities, masked and equal entries where a warp holds a row."""
+    x = logits_of(12, V, V + 1, dtype=dtype)
+    x[1, 3] = math.nan
+    x[2, V - 1] = math.inf
+    x[3] = -math.inf
+    x[4, torch.randperm(V, generator=torch.Generator().manual_seed(V))[7:]] = -math.inf
+    x[5, 0], x[5, 1:] = 1.0, torch.finfo(dtype).min
+    x[6] = 0.0
+    x[6, ::2] = -0.0
+    x[7, 10:] = x[7, 0]
+    x[8] = torch.arange(V) * -2.0 ** -7
+    x[9] = -30.0
+    x[9, V // 2] = 1.0
+    x[10] = torch.finfo(dtype).max
+    targets = torch.tensor([(i * 5) % V for i in range(10)] + [-1, V])
+    for top in sorted({0, 1, 5, 20, 32, min(V, 33), min(V, 64)}):
+        check(x[:, :V], targets.clamp(max=V - 1), top)
+    assert mi.token_scores(x.to(DEV), targets.to(DEV), top=1).logprob[11].isnan()
+
+
 def test_many_rows():
     x = logits_of(700, 1003, 3)
     check(x, torch.randint(0, 1003, (700,)), 20)
