@@ -443,7 +443,7 @@ def test_pages_that_are_none_make_no_numbers():
     assert got[0].isnan().all() and torch.equal(got[1], clean[1])
 
 
-def test_the_same_bits_every_time_and_in_every_company():
+def test_the_same_bits_every_time():
     plan, kv, scale, *_ = filled(2, [3000, 100], [1, 1], 11)
     q = numbers(2, 8, 128, seed=2, spread=0).to(DEV)
     a = mi.attend_pages(q, kv, scale, plan)

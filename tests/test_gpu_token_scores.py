@@ -142,6 +142,11 @@ def test_rows_that_begin_anywhere(dtype, first, pitch):
         assert torch.equal(a, b)
 
 
+def test_more_rows_than_a_call_takes():
+    x = logits_of(3, 40, 4).repeat(22000, 1)
+    check(x, torch.arange(66000) % 40, 2)
+
+
 def test_no_rows():
     s = mi.token_scores(torch.empty(0, 100, device=DEV), torch.empty(0, dtype=torch.long, device=DEV), top=3)
     assert s.logprob.shape == (0,) and s.top_ids.shape == (0, 3)
