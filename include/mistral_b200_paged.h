@@ -38,7 +38,8 @@ int mbp_pages_truncate(int32_t* table, int32_t* lens, int32_t* free_pages, int32
 
 /* Keys and values of a plan's tokens into one layer's pool.  k, v [T, KV * 128] bf16, rows ldk, ldv elements apart (16-byte aligned).  scale = 2^e, e >= -100 the smallest with
  * max |x| <= 448 * 2^e over the page's new numbers, and no smaller than the page's scale where it holds earlier tokens, whose codes are rounded to a grown scale; codes are
- * rounded to nearest even.  Infinities and NaNs become NaN.  Tokens with slot -1 are left out.  The plan may be written again (the same result). */
+ * rounded to nearest even.  Infinities and NaNs become NaN.  Tokens with slot -1 are left out.  Plans are written in the order in
+ * which they were made; the last one may be written again (the same result). */
 int mbp_pages_write(const void* k, int64_t ldk, const void* v, int64_t ldv, void* kv, float* scale, const int32_t* slots, const int32_t* q_start, const int32_t* seqpos,
                     int64_t B, int64_t T, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages, void* stream);
 

@@ -130,7 +130,8 @@ def _pool(kv: torch.Tensor, scale: torch.Tensor, plan: PagePlan) -> Tuple[int, i
 
 def write_pages(kv: torch.Tensor, scale: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PagePlan) -> None:
     """Keys and values [T, heads, 128] (or [T, heads * 128]; bf16) of the plan's tokens into the pool.  A page's scale for a head is the smallest power of two under which all
-    of its tokens' numbers fit e4m3; it grows with later tokens.  Numbers that are not finite are kept as NaN."""
+    of its tokens' numbers fit e4m3; it grows with later tokens (and keeps that if they are taken back).  Numbers that are not finite are kept as NaN.  Plans are written in the
+    order in which they were made."""
     dev, N, KV = _pool(kv, scale, plan)
     T = plan.slots.shape[0]
     assert k.shape[0] == T and v.shape[0] == T, f"{T} tokens planned, keys of {k.shape[0]}, values of {v.shape[0]}"
