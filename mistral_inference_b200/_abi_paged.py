@@ -148,6 +148,6 @@ def _scores_scratch(T: int, V: int, top: int) -> int:
 def token_scores(logits, targets, logprob, entropy, top_ids, top_logprobs, top: int) -> None:
     T, V = logits.shape
     dev = index_of(logits)
-    scratch = torch.empty(_scores_scratch(T, V, top), dtype=torch.uint8, device=logits.device)
+    scratch = logits.new_empty(_scores_scratch(T, V, top) // 4 + 2, dtype=torch.float32)  # (of 8 bytes' alignment, as any)
     _call("mbp_token_scores", dev, logits.data_ptr(), logits.stride(0) if T > 1 else V, 1 if logits.dtype == torch.float32 else 0, _ptr(targets, dev), _ptr(logprob, dev), _ptr(entropy, dev),
           _ptr(top_ids, dev), _ptr(top_logprobs, dev), T, V, top, scratch.data_ptr())

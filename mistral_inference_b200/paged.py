@@ -93,15 +93,15 @@ class PageTables:
         add, rows = self._requests(add, rows)
         B, T = add.shape[0], int(n_tokens)
         assert T >= 0
-        block = torch.empty(2 * T + 2 * B + 2, dtype=torch.int32, device=self.table.device)
-        positions, slots, q_start, seqpos, status = torch.split_with_sizes(block, (T, T, B + 1, B, 1))
+        block = self.lens.new_empty(2 * T + 2 * B + 2)
+        positions, slots, q_start, seqpos, status = torch.unsafe_split_with_sizes(block, (T, T, B + 1, B, 1))
         _abi_paged.pages_extend(self, rows, add, block, B, T)
         return PagePlan(self.table, rows, q_start, seqpos, positions, slots, max(1, T if longest is None else int(longest)), int(most), status)
 
     def truncate(self, keep: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Request b keeps its first keep[b] tokens (0: it has ended).  Returns the status (see `check_status`)."""
         keep, rows = self._requests(keep, rows)
-        status = torch.empty(1, dtype=torch.int32, device=self.table.device)
+        status = self.lens.new_empty(1)
         _abi_paged.pages_truncate(self, rows, keep, status)
         return status
 
@@ -153,7 +153,7 @@ def attend_pages(q: torch.Tensor, kv: torch.Tensor, scale: torch.Tensor, plan: P
     R, P = plan.table.shape
     assert plan.table.dtype is _I32 and plan.table.is_contiguous() and plan.table.get_device() == dev, f"block table: contiguous int32 on cuda:{dev}"
     if out is None:
-        out = torch.empty((T, width), dtype=torch.bfloat16, device=kv.device)
+        out = q.new_empty(T, width)
     else:
         assert out.shape == (T, width) and out.dtype is torch.bfloat16 and out.is_contiguous() and out.get_device() == dev, f"out [T, {width}] bf16, got {tuple(out.shape)} {out.dtype}"
     if T:
