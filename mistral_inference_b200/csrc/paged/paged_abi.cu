@@ -128,7 +128,8 @@ static int launch_token_scores(TokenScoresParams p, cudaStream_t st) {
 }
 
 // How a call's attention is cut: columns of a query tile (the fewest that hold a request's tokens, 32 at most), its tokens, tiles of queries, splits of the keys (as many as run
-// at once, four tiles of keys each at least), and whether its pages go through 16-bit rings.
+// at once, two tiles of keys each at least; a cluster lies within one GPC, so fewer run than the SMs hold CTAs: powers of two by the SMs alone took 60 us for drafts of 5 x 48 heads
+// for 5 requests behind 9000, now 44, 41.7 for 9 single tokens behind 9000, now 30.8, and 18.4 for 2, now 12.1), and whether its pages go through 16-bit rings.
 struct AttnCut {
   int nq, tokens, splits;
   int64_t q_tiles, keys;
@@ -146,7 +147,14 @@ static AttnCut attn_cut(int64_t B, int64_t T, int64_t longest, int64_t most, int
   auto used = [&](int64_t rows, int64_t most_tiles) { return T / rows + B < B * most_tiles ? T / rows + B : B * most_tiles; };
   const int64_t pairs = n_kv_heads * used(c.tokens, c.q_tiles), room = sms * (c.nq < 32 ? 2 : 1);
   c.splits = 1;
-  while (c.splits < PA_MAX_SPLITS && pairs * c.splits * 2 <= room && c.keys >= (int64_t)c.splits * 4 * PA_KEYS) c.splits *= 2;
+  for (int s = PA_MAX_SPLITS; s > 1; --s) {
+    if (pairs * s > room || c.keys < (int64_t)s * 2 * PA_KEYS) continue;
+    const int fit = c.nq == 4 ? paged_attn_clusters<4>(s) : c.nq == 8 ? paged_attn_clusters<8>(s) : c.nq == 16 ? paged_attn_clusters<16>(s) : paged_attn_clusters<32>(s);
+    if (fit == 0 ? (s & (s - 1)) == 0 : pairs <= fit) {
+      c.splits = s;
+      break;
+    }
+  }
   // Time of both ways in us, tiles of 128 keys: 1.4 each on 32 query columns, 2.55 each in the prompt kernel (two heads x 128 tokens), and the conversion.  (nemo shape,
   // measured direct and by rings: 1 x 17 tokens behind 8000 33, 186; 1 x 257 behind 2000 66, 58; 1 x 257 behind 300 28, 24; 3 x 65 behind 2000 57, 65; 3 x 129 behind
   // 8000 268, 203; 16 heads over 4, 3 x 100 behind 20000 234, 464.)

@@ -640,6 +640,42 @@ inline int make_pool_map(CUtensorMap* map, const void* kv, int64_t n_pages, int6
   return MB200_OK;
 }
 
+// Clusters of `splits` CTAs that run at once on the current device where each CTA has an SM to itself; 0: unknown
+template <int NQ>
+inline int paged_attn_clusters_apart(int splits) {
+  static std::atomic<int> known[device_info::MAX_DEVICES][PA_MAX_SPLITS + 1];
+  const int dev = device_info::current();
+  if (dev < 0 || dev >= device_info::MAX_DEVICES || device_info::sm_count() == 0) return 0;
+  std::atomic<int>& here = known[dev][splits];
+  if (here.load(std::memory_order_relaxed) > 0) return here.load(std::memory_order_relaxed);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)splits);
+  cfg.blockDim = dim3(PaCfg<NQ>::kThreads);
+  cfg.dynamicSmemBytes = PaCfg<NQ>::kSmem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (device_info::allow_shared<paged_attn_kernel<NQ>>(PaCfg<NQ>::kSmem) != cudaSuccess || allow_wide_clusters<paged_attn_kernel<NQ>>() != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, paged_attn_kernel<NQ>, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // (not this call's: the caller has an estimate of its own)
+    return 0;
+  }
+  here.store(n, std::memory_order_relaxed);
+  return n;
+}
+// Clusters that run at once: where two CTAs share an SM, two layers of them, or clusters of half as many SMs (all but a few of those: 72 of 74 clusters of 4 did not, 32 of 33 of 8 did)
+template <int NQ>
+inline int paged_attn_clusters(int splits) {
+  const int apart = paged_attn_clusters_apart<NQ>(splits);
+  if (PaCfg<NQ>::kResident == 1) return apart;
+  const int half = splits % 2 == 0 && splits > 2 ? paged_attn_clusters_apart<NQ>(splits / 2) * 97 / 100 : 0;
+  return 2 * apart > half ? 2 * apart : half;
+}
+
 template <int NQ>
 inline int launch_paged_attn(const PagedAttnParams& p, const CUtensorMap& map, int64_t q_tiles, int splits, cudaStream_t st) {
   MB_CHECK_CUDA(device_info::allow_shared<paged_attn_kernel<NQ>>(PaCfg<NQ>::kSmem));
