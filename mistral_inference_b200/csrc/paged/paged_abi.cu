@@ -12,7 +12,7 @@ static int run_plan(bool extend, PlanParams p, cudaStream_t st) {
   const char* what = extend ? "pages_extend" : "pages_truncate";
   MB_CHECK_ARG(p.table && p.lens && p.free && p.n_free && p.scratch && p.count && p.status, "%s: null pointer", what);
   MB_CHECK_ARG(p.B >= 1 && p.B <= MBP_MAX_REQUESTS, "%s: %d requests (1 to %d)", what, p.B, MBP_MAX_REQUESTS);
-  const size_t smem = sizeof(int) * (3 * (size_t)p.B + 2);
+  const size_t smem = sizeof(int) * (size_t)plan_words(p.B, p.R);
   if (extend) {
     // one CTA fills a thousand places as fast as a launch of many starts
     const int ctas = p.T <= PLAN_TOKENS_PER_CTA ? 1 : (ceil_div(p.T, PLAN_TOKENS_PER_CTA) < PLAN_MAX_CTAS ? ceil_div(p.T, PLAN_TOKENS_PER_CTA) : PLAN_MAX_CTAS);

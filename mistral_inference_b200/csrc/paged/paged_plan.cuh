@@ -12,6 +12,7 @@
 // shared memory, reads only the state as it was, and the last CTA to be done commits.
 #pragma once
 #include "paged_common.cuh"
+#include "plan_layout.cuh"
 
 namespace mb200 {
 
@@ -52,16 +53,17 @@ __device__ __forceinline__ long long block_scan(long long v, long long* sums, lo
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + PG_TOKENS - 1) / PG_TOKENS; }
 
 // What both kernels begin with: lengths and prefix sums of all requests in shared memory.  Returns the status of the call, the same in every CTA.
-//   sm: len[B] lengths before | first[B + 1] prefix sums of count | moved[B + 1] prefix sums of the pages that move; a bit for each row first lies over the two
+// (plan_layout.cuh says what lies where)
 template <bool EXTEND>
-__device__ __forceinline__ int plan_requests(const PlanParams& p, int* first, int* moved, int* len, int& n_free, int& n_moved) {
+__device__ __forceinline__ int plan_requests(const PlanParams& p, int* sm, int& n_free, int& n_moved) {
+  int *len = sm, *first = sm + plan_first_at(p.B), *moved = sm + plan_moved_at(p.B);
   __shared__ long long sums[32];
   const int per = (p.B + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
   n_free = *p.n_free;
   int bad = 0;
   long long tokens = 0, pages = 0;
-  uint32_t* named = reinterpret_cast<uint32_t*>(first);
-  for (int i = threadIdx.x; i < (p.R + 31) / 32; i += blockDim.x) named[i] = 0;
+  uint32_t* named = reinterpret_cast<uint32_t*>(sm + plan_named_at(p.B));
+  for (int i = threadIdx.x; i < plan_named_words(p.R); i += blockDim.x) named[i] = 0;
   __syncthreads();
   for (int b = b0; b < b1; ++b) {
     const int r = p.rows ? p.rows[b] : b, c = p.count[b];
@@ -105,11 +107,11 @@ __device__ __forceinline__ int plan_requests(const PlanParams& p, int* first, in
 
 __global__ void __launch_bounds__(PLAN_THREADS) page_extend_kernel(PlanParams p) {
   extern __shared__ int plan_sm[];
-  int *len = plan_sm, *first = len + p.B, *moved = first + p.B + 1;
+  const int *len = plan_sm, *first = plan_sm + plan_first_at(p.B), *moved = plan_sm + plan_moved_at(p.B);
   pdl_trigger();
   pdl_wait();
   int n_free, n_new;
-  const int status = plan_requests<true>(p, first, moved, len, n_free, n_new);
+  const int status = plan_requests<true>(p, plan_sm, n_free, n_new);
   const int at = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
   if (status != PLAN_OK) {
     for (int i = at; i < p.T; i += step) {
@@ -165,11 +167,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_extend_kernel(PlanParams p)
 // One CTA: what goes back is a few pages (drafted tokens) or a few hundred (a request that has ended).
 __global__ void __launch_bounds__(1024) page_truncate_kernel(PlanParams p) {
   extern __shared__ int plan_sm[];
-  int *len = plan_sm, *first = len + p.B, *moved = first + p.B + 1;
+  const int *len = plan_sm, *first = plan_sm + plan_first_at(p.B), *moved = plan_sm + plan_moved_at(p.B);
   pdl_trigger();
   pdl_wait();
   int n_free, n_back;
-  const int status = plan_requests<false>(p, first, moved, len, n_free, n_back);
+  const int status = plan_requests<false>(p, plan_sm, n_free, n_back);
   if (threadIdx.x == 0) *p.status = status;
   if (status != PLAN_OK) return;
   for (int a = threadIdx.x; a < n_back; a += blockDim.x) {

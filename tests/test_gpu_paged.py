@@ -134,6 +134,44 @@ def test_many_requests_at_once():
     assert_same_state(t, h)
 
 
+@pytest.mark.parametrize("R", [129, 4000, 131072])
+def test_few_requests_of_states_with_many_rows(R):
+    """One or two requests of a state of many rows, the last ones among them: what marks a row as named has a place for every row."""
+    t, h = mi.PageTables.empty(R, 2, 64, DEV), U.HostTables(R, 2, 64)
+    def same():  # rows as tensors: a state of 131072 rows is slow as lists
+        assert torch.equal(t.table.cpu(), torch.tensor(h.table, dtype=torch.int32)) and t.lens.tolist() == h.lens and t.free.tolist() == h.free and t.n_free.item() == h.n_free
+    for add, rows in [([70], [R - 1]), ([3, 65], [R // 2, 0]), ([1], [R - 1]), ([5, 0], [R - 2, R - 1]), ([64], [127])]:
+        plan = t.extend(ints(add), sum(add), ints(rows)).check()
+        positions, slots, q_start, seqpos = h.extend(add, rows)
+        assert plan.positions.tolist() == positions and plan.slots.tolist() == slots and plan.q_start.tolist() == q_start and plan.seqpos.tolist() == seqpos
+        same()
+    for rows in ([R - 1, R - 1], [R, 0], [0, -1]):
+        with pytest.raises(_abi_paged.Mb200Error, match="row"):
+            t.extend(ints([1, 1]), 2, ints(rows)).check()
+        with pytest.raises(_abi_paged.Mb200Error, match="row"):
+            check_status(t.truncate(ints([0, 0]), ints(rows)))
+    for keep, rows in [([0], [R - 1]), ([2, 0], [R // 2, R - 2]), ([0], [127])]:
+        check_status(t.truncate(ints(keep), ints(rows)))
+        h.truncate(keep, rows)
+        same()
+
+
+def test_a_cache_of_many_rows_admits_and_retires_single_requests():
+    c = mi.PagedCache(1, 1000, 256, 1, 128, n_pages=40)
+    for i in range(6):
+        places = c.admit(1)
+        c.get_input_metadata([0] * places[0] + [10 + 30 * i])[0].plan.check()
+        c.update_seqlens([0] * places[0] + [10 + 30 * i])
+    c.retire([2])
+    c.retire([0, 4])
+    c.admit(2)
+    c.get_input_metadata([1, 0, 1, 64, 0])[0].plan.check()
+    c.update_seqlens([1, 0, 1, 64, 0])
+    lens = c.tables.lens.tolist()
+    assert [lens[r] for r in c.rows] == c.ledger.lens == [41, 100, 131, 64, 0] and sum(lens) == sum(c.ledger.lens)
+    assert int(c.tables.n_free) == c.ledger.free_pages
+
+
 # ---------------------------------------------------------------------------------------------------------------- writes
 def numbers(*shape, seed, spread=4, dtype=torch.bfloat16):
     """Normal numbers of magnitudes that differ by token and head."""

@@ -1,6 +1,7 @@
 """The paged library's boundary and refusals, without a GPU: everything here is turned away before a kernel is launched."""
 import ctypes
 import re
+import subprocess
 import zlib
 from pathlib import Path
 
@@ -193,3 +194,28 @@ def test_declarations_of_this_abi_version():
     """A change of the declarations takes a new version, so that a library built before it is refused."""
     code = re.sub(r"/\*.*?\*/", " ", HEADER.read_text(), flags=re.S)
     assert zlib.crc32(" ".join(code.split()).encode()) == 1297119818, "raise the ABI version with this change"
+
+
+LAYOUT = """
+#include "plan_layout.cuh"
+extern "C" void layout(int B, int R, int* out) {
+  out[0] = mb200::plan_first_at(B); out[1] = mb200::plan_moved_at(B); out[2] = mb200::plan_named_at(B); out[3] = mb200::plan_named_words(R); out[4] = mb200::plan_words(B, R);
+}
+"""
+
+
+def test_a_plans_shared_memory_holds_a_bit_for_every_row(tmp_path):
+    """States have many more rows than a call has requests: one request of a server of thousands."""
+    (tmp_path / "l.cc").write_text(LAYOUT)
+    csrc = REPO / "mistral_inference_b200" / "csrc" / "paged"
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", str(csrc), "-o", str(tmp_path / "l.so"), str(tmp_path / "l.cc")], check=True)
+    layout, out = ctypes.CDLL(str(tmp_path / "l.so")).layout, (ctypes.c_int * 5)()
+    for B in (1, 2, 3, 64, 1999, _abi_paged.MAX_REQUESTS):
+        for R in (1, 2, 31, 32, 33, 128, 129, 300, 4000, 131071, 131072):
+            layout(B, R, out)
+            first, moved, named, named_words, words = out
+            assert B <= first and first + B + 1 <= moved and moved + B + 1 <= words          # lengths, two prefix sums
+            assert B <= named and 32 * named_words >= R and named + named_words <= words      # bits, which must not lie over the lengths
+            assert 4 * words <= 48 * 1024 - 512                                               # beside the kernels' own few words
+    text = (csrc / "paged_plan.cuh").read_text() + (csrc / "paged_abi.cu").read_text()
+    assert "plan_words(p.B, p.R)" in text and text.count("plan_named_words(p.R)") == 1
