@@ -281,7 +281,9 @@ __global__ void __launch_bounds__(TS_THREADS, TS_CTAS) token_scores_segment_kern
       }
     }
     // t = log2(e) x - R, R = log2(e) M rounded: e^(x - M) = 2^t * 2^(R - log2(e) M), the second factor put right below
-    const bool none = M == -INFINITY, huge = fabsf(M) > 1e30f && !none;  // (R would not be finite, or not near enough)
+    // R is off by half a step at most: 64 up to |M| = 2^30 (masks of -1e9 among them), where 2^64 times the sums is still far inside fp32.  Beyond, the difference comes first.
+    // (M is a segment's maximum: that of one whose entries are all masked by a finite number is the mask's.)
+    const bool none = M == -INFINITY, huge = fabsf(M) > 1073741824.f && !none;
     const float R = huge || none ? 0.f : M * LOG2E;
     float s = 0.f, w = 0.f;
     int j = 0;

@@ -170,3 +170,43 @@ def test_the_same_bits_alone_captured_and_on_another_stream():
     for y in (b, c):
         assert torch.equal(a.logprob, y.logprob) and torch.equal(a.entropy, y.entropy) and torch.equal(a.top_ids, y.top_ids) and torch.equal(a.top_logprobs, y.top_logprobs)
     assert torch.equal(a.logprob[4:5], one.logprob) and torch.equal(a.top_ids[4:5], one.top_ids)
+
+
+def check_large(x, targets, top):
+    """As check(), for log-probabilities of any size: a difference of two numbers and of that and the logarithm, 2^-24 of itself each."""
+    s = mi.token_scores(x.to(DEV), targets.to(DEV), top=top)
+    lp, ent, ids, lps = U.scores_ref(x, targets, top)
+    assert s.top_ids.cpu().tolist() == ids.tolist()
+    for got, want in ((s.logprob, lp), (s.entropy, ent), (s.top_logprobs, lps)):
+        got = got.cpu().double()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        tol = 2.0 ** -17 + 2.0 ** -15 * want.abs().clamp(max=16) + 2.0 ** -23 * want.abs()
+        fin = want.isfinite()
+        assert ((got - want).abs() <= tol)[fin].all(), ((got - want).abs() / tol)[fin].max()
+
+
+FILLS = [-(2.0 ** 24), -1e8, -1e9, -(2.0 ** 30), -1.5e9, -1e10] + [-(10.0 ** e) for e in range(11, 31)] + [-3e38]
+
+
+@pytest.mark.parametrize("T,V", [(3, 5000), (160, 5000), (3, 40000), (160, 40000)])  # one segment or several, joined by a cluster or by a second launch
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("top", [0, 20])
+def test_masks_of_any_finite_number(T, V, dtype, top):
+    """A grammar that leaves tokens in one place only: the other segments of a row hold nothing but the mask's number."""
+    few = logits_of(len(FILLS), 100, 13, dtype=dtype)
+    rows = []
+    for i, fill in enumerate(FILLS):
+        row = torch.full((V,), fill).to(dtype)
+        at = (0, V - 100, V // 2)[i % 3]
+        row[at: at + 100] = few[i]
+        rows.append((row, at + 7))
+    for i, m in enumerate((1e10, -1e10, 3e9, 1e12)):  # rows whose own numbers are that large, a few steps of the type apart
+        row = torch.full((V,), -3e38 if i % 2 else 0.9 * m - abs(m)).to(dtype)
+        row[5: V: 977] = torch.tensor(m).to(dtype)
+        row[11: V: 1999] = (torch.tensor(m) - abs(m) * torch.finfo(dtype).eps).to(dtype)
+        rows.append((row, 5))
+    rows.append((torch.full((V,), -1e11).to(dtype), 3))  # nothing but the mask
+    n = len(rows)
+    for first in range(0, n, T):  # T rows a call; of many, a few different ones and the first over and over
+        take = [rows[i] for i in range(first, min(n, first + T))] + [rows[0]] * max(0, first + T - n)
+        check_large(torch.stack([r for r, _ in take]), torch.tensor([t for _, t in take]), top)
