@@ -326,7 +326,8 @@ class PagedCache:
             self._on_device = list(self.ledger.lens)
 
     def planned(self, seqlens: List[int]) -> None:
-        """The block tables hold `seqlens` more tokens of each request (planned here, or by a captured step)."""
+        """The block tables hold `seqlens` more tokens of each request, or are about to (planned here, or by a step that is run or replayed next): settle() takes back what a
+        failed step has left of them, and finds nothing to take back where it never came to its plan."""
         self._on_device = [n + a for n, a in zip(self.ledger.lens, seqlens)]
 
     def metadata_of(self, plan: PagePlan, seqlens: List[int]) -> List[PagedInputMetadata]:

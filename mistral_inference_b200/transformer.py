@@ -366,6 +366,7 @@ class Transformer(nn.Module):
         if cache.paged:
             cache.ledger.check(seqlens)  # (the captured plan finds its pages)
             cache.settle()
+            cache.planned(seqlens)  # before the step: one that fails behind its plan has its tokens taken back by the next settle()
         elif st["expected"] != host:  # another forward() advanced the cache since the last step (or this is the first one)
             st["seqpos"].copy_(torch.tensor(host, dtype=torch.int32))  # pageable source: staged by the runtime, no reuse hazard
         st["tokens"].copy_(tokens, non_blocking=True)  # device source (previous pick): D2D; host source: staged by the runtime
@@ -392,8 +393,6 @@ class Transformer(nn.Module):
             g.replay()
         else:
             st["graph"].replay()
-        if cache.paged:
-            cache.planned(seqlens)
         cache.update_seqlens(seqlens)
         st["expected"] = list(cache._kv_seqlens_host)
         self.last_argmax = st["next"]

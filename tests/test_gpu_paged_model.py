@@ -231,3 +231,36 @@ def test_layered_decoders_report_alternatives(tmp_path, dtype):
         assert [d.top_ids[0] for d in details[b][len(prompts[b]) - 1:]] == tokens[b] and max(abs(x - y) for x, y in zip(lps[b], lps2[b])) <= 2.0 ** -10
     with pytest.raises(ValueError, match="rings"):
         mi.generate(prompts, m, max_tokens=1, temperature=0.0, kv_cache="pages")
+
+
+@pytest.mark.parametrize("where", ["warm-up", "capture", "replay"])
+def test_a_decode_step_that_fails_leaves_no_tokens_behind(monkeypatch, where):
+    """A layer raises in a single-token step (run eagerly, or captured), or the replay does before anything is enqueued: the steps after it are those of a cache that never failed."""
+    monkeypatch.setenv("MB200_DECODE_GRAPH", "1")
+    m, p = model_of(max_batch=2)
+    runs = []
+    for fails in (False, True):
+        cache = m.make_cache(2, 200, kv_cache="pages")
+        m.forward(torch.arange(126).cuda(), [63, 63], cache)  # the next token but one of each begins a page
+        steps = 0
+        def step():
+            nonlocal steps
+            steps += 1
+            return m.forward(torch.tensor([steps, steps + 1], device="cuda"), [1, 1], cache).clone()
+        got = [step() for _ in range({"warm-up": 0, "capture": 1, "replay": 2}[where])]
+        if fails:
+            def broken(*a):
+                raise RuntimeError("lost")
+            with monkeypatch.context() as mp:
+                if where == "replay":
+                    mp.setattr(torch.cuda.CUDAGraph, "replay", broken)
+                else:
+                    mp.setattr(type(m.layers["1"]), "forward", broken)
+                with pytest.raises(RuntimeError, match="lost"):
+                    m.forward(torch.tensor([steps + 1, steps + 2], device="cuda"), [1, 1], cache)
+            assert cache.kv_seqlens.tolist() == [63 + steps] * 2
+        got += [step() for _ in range(5)]
+        runs.append((got, cache.tables.lens.tolist(), cache.ledger.lens, int(cache.tables.n_free)))
+    assert runs[0][1:] == runs[1][1:] and runs[0][1] == runs[0][2]
+    for a, b in zip(runs[0][0], runs[1][0]):
+        assert torch.equal(a, b)
