@@ -5,8 +5,11 @@
 // The codes never leave 8 bits on their way to the tensor cores.  tcgen05 multiplies e4m3 by e4m3, so it is the QUERIES and the WEIGHTS that are given in
 // e4m3, each as two numbers: hi + lo / 16, hi = e4m3(x), lo = e4m3(16 (x - hi)).  The 8 significant bits of a bf16 query are held exactly that way (a row is
 // first scaled by a power of two to at most 448; entries below 2^-14 of the row's largest keep fewer bits, never worse than 2^-23 of that largest), a weight
-// to 2^-8 of itself, which is what bf16 weights have.  Scores, running maximum and sum, and the values' sums stay in fp32; the pages' scales multiply in fp32,
-// the keys' on the scores, the values' on each page's own accumulator.
+// to 2^-8 of itself, as bf16 weights are, or to 2^-22 of the weight 1 where that is more.  That lets many small weights beside a large one vanish (30000 of 2^-22
+// are 0.7 % of it), so the score that has weight 1 is not the running maximum for good: it goes up with the maximum, and, after a CTA's first 2048 keys, down
+// to a tile's own maximum where that lies more than 8 binary places below.  A tile's weights are then off by 128 * 2^-22 * 2^8 = 2^-7 of its largest in all, those of the
+// first 2048 keys by 2^-11 of theirs.  Scores, maxima and sums, and the values' sums stay in fp32; the pages' scales multiply in fp32, the keys' on the scores, the values' on
+// each page's own accumulator.
 //
 // Keys are the MMA's 128 rows (S^T = K Q^T) and so are the values' dimensions (O^T = V^T P^T, V as it lies in the page: MN-major), the hi and lo parts of up to NQ
 // query columns (tokens x heads of one key/value head) its columns.  Memory bounds it: 256 bytes a key and key/value head, where converting them to 16 bits on the way to
@@ -30,8 +33,10 @@ namespace mb200 {
 
 constexpr int PA_STAGES = 3, PA_KEYS = 2 * PG_TOKENS, PA_STAGE_BYTES = 4 * PG_BYTES;
 constexpr int PA_MAX_SPLITS = 16;
-constexpr int PA_ROW = kHeadDim + 4;     // numbers of a split's result for one query: maximum, sum, -, -, the values' sums
+constexpr int PA_ROW = kHeadDim + 4;     // numbers of a split's result for one query: the score of weight 1, sum, -, -, the values' sums
 constexpr float PA_NOTHING = -1.0e30f;   // the maximum of no score
+constexpr int PA_NEAR_TILES = 16;        // tiles whose weights are held against the running maximum only
+constexpr float PA_FAR = 8.f, PA_DOWN = 16.f;  // log2 units: how far below a tile's maximum may lie, and how far weight 1 may at most (2^16 times the sums is far inside fp32)
 enum { PA_GAVE_UP = 16 };                // status: a wait ran out; the call's results are NaN
 
 struct PagedAttnParams {
@@ -241,7 +246,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   const int first = page_lo + n_pages * split / splits, last = page_lo + n_pages * (split + 1) / splits;  // this split's pages (n_pages < 2^25)
   const int tiles = (last - first + 1) / 2;
 
-  uint64_t o[Q / 2], l[Q / 2], less[Q / 2];  // of two queries each; less: minus the maximum
+  uint64_t o[Q / 2], l[Q / 2], less[Q / 2];  // of two queries each; less: minus the score that has weight 1
   const int group = warp >> 2, key_at = tid & 127;  // of the softmax threads
   if (warp == SOFT) {
     // ================= producer =================
@@ -398,7 +403,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
       qs[i / 2] = pair(q_scale[group * Q + i], q_scale[group * Q + i + 1]);
     }
     const int most_at = lane % (4 * Q);  // the maximum that this lane looks at: column most_at / 4, warp most_at % 4
-    float most = PA_NOTHING;             // the maximum of column most_at / 4
+    float most = PA_NOTHING, peak = PA_NOTHING;  // of column most_at / 4: the score that has weight 1 (times 256), the maximum
     const uint64_t sixteenth = pair(0.0625f, 0.0625f), eight = pair(8.f, 8.f);
     // Byte key_at of column j of the group: its 128 bytes are row j of a 128B-swizzled K-major tile, which pa_col(group * 2 Q + j, key_at) says in full
     const uint32_t p_at = smem_u32(sP) + group * 2 * Q * 128 + (key_at ^ (Q == 2 ? group << 6 : 0));
@@ -474,14 +479,21 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
         ok = false;
         break;
       }
-      // The group's maxima, a column and warp a lane; broadcast only where one has grown.  (All of them by every thread: 40 instructions of some 350 a tile and thread.)
+      // The group's maxima, a column and warp a lane; broadcast only where one has moved.  (All of them by every thread: 40 instructions of some 350 a tile and thread.)
       float top = warp_most[t & 1][group * Q + most_at / 4][most_at % 4];
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const bool grew = __any_sync(0xffffffffu, top > most);  // (the same in all threads of the group)
+      float to = top;
+      bool moves = top > most;
+      if (t >= PA_NEAR_TILES) {
+        to = fmaxf(top, peak - PA_DOWN);
+        moves |= top > PA_NOTHING && to < most - PA_FAR;
+      }
+      const bool moved = __any_sync(0xffffffffu, moves);  // (the same in all threads of the group)
       uint64_t alpha[Q / 2];
-      if (grew) {
-        most = fmaxf(most, top);
+      if (moved) {
+        if (moves) most = to;
+        peak = fmaxf(peak, most);
 #pragma unroll
         for (int i = 0; i < Q; i += 2) {
           const float m0 = __shfl_sync(0xffffffffu, most, i * 4), m1 = __shfl_sync(0xffffffffu, most, i * 4 + 4);
@@ -506,7 +518,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
       });
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (t > 0) add_values(t - 1);
-      if (grew) {
+      if (moved) {
 #pragma unroll
         for (int i = 0; i < Q / 2; ++i) o[i] = mul_pair(o[i], alpha[i]);
       }

@@ -489,6 +489,35 @@ def test_the_same_bits_every_time():
         assert torch.equal(a, mi.attend_pages(q, kv, scale, plan))
 
 
+@pytest.mark.parametrize("gap", [10.0, 16.0, 20.0, 21.5, 22.06, 22.5, 24.0, 60.0])
+@pytest.mark.parametrize("H,new,at", [(8, 1, 0), (8, 1, 20000), (32, 4, 100)])
+def test_many_small_weights_beside_a_large_one(gap, H, new, at):
+    """One key `gap` binary places above tens of thousands of equal ones whose values share a sign: each of those weighs next to nothing, all of them together do not.  Many requests, so that
+    one CTA walks over all keys of a request (they are one request's pages, named by all).  Weights: 2^-8 of themselves, or 2^-22 of the weight that they are held against: the largest
+    so far for a CTA's first 2048 keys (2^-11 of the values' largest in all), then one at most 2^8 above the largest of their tile, whose others here are as large: 2^-14 of themselves.
+    Scores and the result's rounding as in attend_tolerance."""
+    KV, keys = 2, 30000 + new
+    n = U.cdiv(keys, 64)
+    g = torch.Generator().manual_seed(3)
+    kv = torch.zeros(n, KV, 2, 64, 128)
+    kv[:, :, 1] = 1.0 + torch.randint(0, 8, (n, KV, 64, 128), generator=g) / 8  # values in [1, 2)
+    kv[at // 64, :, 0, at % 64, 0] = 1.0                                        # the large key, whose values are 0
+    kv[at // 64, :, 1, at % 64] = 0.0
+    kv, scale = kv.to(U.E4M3), torch.ones(n, KV, 2)
+    q = torch.zeros(new, H, 128)
+    q[:, :, 0] = gap / (128 ** -0.5 * math.log2(math.e))
+    q = q.to(torch.bfloat16)
+    B = 80
+    plan = mi.PagePlan(torch.arange(n, dtype=torch.int32, device=DEV)[None].contiguous(), ints([0] * B), ints([new * b for b in range(B + 1)]), ints([30000] * B), ints([0] * new * B), ints([0] * new * B),
+                       new, keys)
+    assert not by_rings(H, KV, [30000] * B, [new] * B)
+    got = mi.attend_pages(q.repeat(B, 1, 1).to(DEV), kv.to(DEV), scale.to(DEV), plan).cpu().double().view(B, new, H, 128)
+    want, mag = U.attend_ref(q, kv.double(), scale, [list(range(n))], [0], [0, new], [30000])
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -9 + 2.0 ** -14) * mag + 2.0 ** -11 * 2.0
+    worst = ((got - want).abs() / tol).max().item()
+    assert worst <= 1, f"{worst:.2f} times the tolerance"
+
+
 # ---------------------------------------------------------------------------------------------------------------- together
 def test_a_run_of_requests_together():
     """Prompts, decode steps, drafts taken back, a request that ends and another that takes its pages: attention over what was written, at each step against 64 bits."""
