@@ -79,6 +79,7 @@ def _ptr(t: Optional[torch.Tensor], device: int) -> Optional[int]:
 
 
 def _call(name: str, device: int, *args) -> None:
+    """The entry point on the current stream of `device`, whatever the current device is."""
     fn = _fn(name)
     if device == torch._C._cuda_getDevice():
         rc = fn(*args, _stream())
@@ -125,14 +126,16 @@ def pages_write(dev: int, kv, scale, k, v, plan, T: int, N: int, KV: int) -> Non
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_scratch(B: int, T: int, longest: int, most: int, width: int, n_heads: int, KV: int, window: int) -> int:
-    return lib().mbp_attn_pages_scratch(B, T, longest, most, width, n_heads, KV, window)
+def _attn_scratch(device: int, B: int, T: int, longest: int, most: int, width: int, n_heads: int, KV: int, window: int) -> int:
+    """How a call is cut goes by its device's SMs: the same device is asked that the call will run on."""
+    with torch.cuda.device(device):
+        return _fn("mbp_attn_pages_scratch")(B, T, longest, most, width, n_heads, KV, window)
 
 
 def attn_pages(dev: int, q, kv, scale, plan, out, T: int, N: int, KV: int, H: int, R: int, width: int, window: int, softmax_scale: float) -> None:
     pq, ldq = _rows(q, H, dev)
     B, status = plan.rows.shape[0], plan.status
-    need = _attn_scratch(B, T, plan.longest, plan.most, width, H, KV, window)
+    need = _attn_scratch(dev, B, T, plan.longest, plan.most, width, H, KV, window)
     scratch = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
     _call("mbp_attn_pages", dev, pq, ldq, kv.data_ptr(), scale.data_ptr(), plan.table.data_ptr(), plan.rows.data_ptr(), plan.q_start.data_ptr(), plan.seqpos.data_ptr(), out.data_ptr(),
           None if status is None else _ptr(status, dev), B, T, plan.longest, plan.most, R, width, N, H, KV, HEAD_DIM, window, softmax_scale, None if scratch is None else scratch.data_ptr(), need)

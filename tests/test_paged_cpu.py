@@ -196,6 +196,31 @@ def test_declarations_of_this_abi_version():
     assert zlib.crc32(" ".join(code.split()).encode()) == 1297119818, "raise the ABI version with this change"
 
 
+def test_scratch_is_sized_by_the_device_that_the_call_runs_on(monkeypatch):
+    """Devices of unlike size: what one of them needs is asked of it, and not taken from what another answered."""
+    import contextlib
+    current, asked = [0], []
+
+    @contextlib.contextmanager
+    def use(device):
+        before, current[0] = current[0], device
+        yield
+        current[0] = before
+
+    def sizes(*args):
+        asked.append((current[0], args))
+        return 1000 + current[0]
+
+    monkeypatch.setattr(torch.cuda, "device", use)
+    monkeypatch.setitem(_abi_paged._lazy, "mbp_attn_pages_scratch", sizes)
+    _abi_paged._attn_scratch.cache_clear()
+    try:
+        sizes_of = [_abi_paged._attn_scratch(d, 2, 600, 300, 900, 20, 32, 8, 0) for d in (1, 0, 1)]
+    finally:
+        _abi_paged._attn_scratch.cache_clear()
+    assert sizes_of == [1001, 1000, 1001] and [d for d, _ in asked] == [1, 0] and asked[0][1] == (2, 600, 300, 900, 20, 32, 8, 0)
+
+
 LAYOUT = """
 #include "plan_layout.cuh"
 extern "C" void layout(int B, int R, int* out) {
