@@ -46,6 +46,7 @@ struct FaParams {
   int own;                 // 1: keys from seqpos on are the call's own rows; 0: every key is in the ring
   int n_tab;
   float scale_log2;
+  int T = 0x7fffffff;      // rows of q and out: a sequence that reaches beyond them, or begins before position 0, is left out
 };
 
 constexpr uint32_t kIdescQK = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(FA_BN >> 3) << 17) | ((uint32_t)(FA_BM >> 4) << 24);
@@ -147,6 +148,7 @@ __global__ void __launch_bounds__(FA_THREADS, 1)
   const int i0 = qt * FA_BM;
   if (i0 >= s_len) return;
   const int seqpos = p.seqpos != nullptr ? p.seqpos[b] : 0;
+  if (tok0 < 0 || s_len > p.T - tok0 || seqpos < 0) return;
   const int q_first = seqpos + i0, q_last = seqpos + min(i0 + FA_BM, s_len) - 1;  // positions
   const FaRuns runs = fa_runs(p, seqpos, tok0, q_first, q_last);
   const int n_tiles = runs.first[3];

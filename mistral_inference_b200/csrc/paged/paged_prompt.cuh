@@ -119,6 +119,7 @@ inline int launch_paged_prompt(PagedRingParams p, const void* q, int64_t ldq, bf
   f.own = 0;
   f.n_tab = 0;
   f.scale_log2 = scale_log2;
+  f.T = p.T;
   // Two heads a CTA share every key and value tile, unless single ones all run at once.  (257 tokens of 32 heads behind 2000: 53 us, 58 by two; 3 x 700: 163 and 115.)
   const bool two = (H / p.KV) % 2 == 0 && H * B * ceil_div(longest, FA_BM) > device_info::sm_count();
   const dim3 fgrid((unsigned)(H / (two ? 2 : 1)), (unsigned)ceil_div(longest, FA_BM), (unsigned)B);

@@ -389,6 +389,20 @@ def test_portions_of_pages_that_are_none_and_of_refused_plans():
     assert (out == 3.0).all()
 
 
+@pytest.mark.parametrize("H,KV,rings", [(32, 8, True), (8, 2, False)])
+def test_plans_that_name_rows_that_are_not_there(H, KV, rings):
+    """Both ways of attending: a request whose tokens reach behind the queries, or that begins before position 0, is left out; nothing is written elsewhere."""
+    plan, kv, scale, *_ = filled(KV, [200, 30], [250, 300], 4)
+    assert by_rings(H, KV, [200, 30], [250, 300]) == rings
+    q = numbers(550, H, 128, seed=1, spread=0).to(DEV)
+    want = mi.attend_pages(q, kv, scale, plan)
+    for q_start, seqpos in (([0, 250, 551], [200, 30]), ([0, 250, 900], [200, 30]), ([0, 250, 550], [200, -1]), ([0, 250, 550], [200, -2 ** 31]), ([0, 250, 2 ** 31 - 1], [200, 30])):
+        room = torch.full((1200, H * 128), 3.0, dtype=torch.bfloat16, device=DEV)
+        odd = mi.PagePlan(plan.table, plan.rows, ints(q_start), ints(seqpos), plan.positions, plan.slots, plan.longest, plan.most)
+        mi.attend_pages(q, kv, scale, odd, out=room[:550])
+        assert torch.equal(room[:250], want[:250]) and (room[250:] == 3.0).all()
+
+
 def test_portions_out_of_a_wider_matrix():
     plan, kv, scale, kv_h, scale_h, table, rows = filled(8, [200, 30], [250, 300], 4)
     wide = numbers(550, 48 * 128, seed=1, spread=0).to(DEV)
