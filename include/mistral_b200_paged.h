@@ -28,7 +28,7 @@ const char* mbp_last_error(void);
  *   positions, slots [T]  of the new tokens, request after request: position in the request, and page * 64 + place in the page; places behind the last new token 0, -1
  *   q_start [B + 1]       prefix sums of add;  seqpos [B]: lengths before
  *   status [1]            0, or why nothing was changed: 1 a row out of range or named twice, 2 a length that is negative or longer than P pages,
- *                         3 more tokens than T, 4 too few free pages; then q_start is 0 and every slot -1: writes and attention by this plan do nothing. */
+ *                         3 more tokens than T, 4 too few free pages, or n_free is not within 0 .. n_pages; then q_start is 0 and every slot -1: writes and attention by this plan do nothing. */
 int mbp_pages_extend(int32_t* table, int32_t* lens, int32_t* free_pages, int32_t* n_free, int32_t* scratch, const int32_t* rows, const int32_t* add, int32_t* positions,
                      int32_t* slots, int32_t* q_start, int32_t* seqpos, int32_t* status, int64_t B, int64_t T, int64_t R, int64_t P, int64_t n_pages, void* stream);
 /* Request b keeps its first keep[b] tokens (at most what it has); pages that hold none of them go back on the stack, so that an extend by the same requests would take
@@ -49,7 +49,8 @@ int64_t mbp_attn_pages_scratch(int64_t B, int64_t T, int64_t longest, int64_t mo
  * [T, H * 128] bf16, 8-byte aligned.  The query at position p sees positions (p - window, p]; window 0: all.  longest: no request has more tokens in this plan; most: none has more in all
  * (0: unknown).  status [1] or NULL: 16 is set when a wait inside ran out, 32 when a request has more tokens than longest or most say: those it
  * has no room for, or all of its results, are NaN.  scratch:
- * mbp_attn_pages_scratch bytes, 256-byte aligned, of any content and this call's own until it has run.  A page id out of range makes the results that need it NaN.  So does a NaN among the
+ * mbp_attn_pages_scratch bytes, 256-byte aligned, of any content and this call's own until it has run.  A page id out of range makes the results that need it NaN (and
+ * perhaps those of a few tokens of its request ahead of it).  So does a NaN among the
  * values, in its column, of the queries that see it (by rings also of others up to 127 positions from those); rows of out behind
  * q_start[B] are left as they are. */
 int mbp_attn_pages(const void* q, int64_t ldq, const void* kv, const float* scale, const int32_t* table, const int32_t* rows, const int32_t* q_start, const int32_t* seqpos,

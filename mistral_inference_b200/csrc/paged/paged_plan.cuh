@@ -2,9 +2,9 @@
 //
 // State: table [R, P] page ids (-1 behind a row's last page), lens [R] tokens of each row, free [N] a stack of page ids, n_free [1].
 //   extend    request b (row r_b) takes add_b more tokens.  Pages are taken in request order: the a-th new page of the call is free[n_free - 1 - a], so the
-//             result is the same in every run.  Per token: its position, and its slot = page * 64 + place in the page.
+//             result is the same in every run.  Per token: its position, and its slot = page * 64 + place in the page (-1 where the stack held no page's id).
 //   truncate  request b keeps keep_b tokens; pages go back so that the next extend by the same requests finds them again: the exact inverse of extend.
-// A call that cannot be done (a row twice or out of range, a negative or too large length, too few free pages, more tokens than there is room for) changes
+// A call that cannot be done (a row twice or out of range, a negative or too large length, too few free pages or an n_free that no stack of N has, more tokens than there is room for) changes
 // nothing and says why in `status`.
 //
 // Nothing but latency bounds it: the lengths are a few hundred bytes, and each of the dependent steps (lengths -> prefix sums -> page -> slot) is one trip to L2.  So it is
@@ -88,7 +88,7 @@ __device__ __forceinline__ int plan_requests(const PlanParams& p, int* sm, int& 
   long long n_tokens, n_pages;
   long long t = block_scan(tokens, sums, n_tokens), a = block_scan(pages, sums, n_pages);
   if (EXTEND && n_tokens > p.T) return PLAN_NO_ROOM;
-  if (EXTEND ? n_pages > n_free : n_free + n_pages > p.N) return PLAN_NO_PAGES;
+  if (n_free < 0 || n_free > p.N || (EXTEND ? n_pages > n_free : n_free + n_pages > p.N)) return PLAN_NO_PAGES;
   for (int b = b0; b < b1; ++b) {
     const int c = p.count[b], l = len[b];
     first[b] = (int)t;
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_extend_kernel(PlanParams p)
       pos = len[b] + i - first[b];
       const int j = pos / PG_TOKENS, had = pages_of(len[b]);
       const int page = j < had ? p.table[row_of(b) + j] : p.free[n_free - 1 - (moved[b] + j - had)];
-      slot = page < 0 ? -1 : page * PG_TOKENS + pos % PG_TOKENS;
+      slot = page < 0 || page > 0x7fffffff / PG_TOKENS ? -1 : page * PG_TOKENS + pos % PG_TOKENS;  // (an id past that would wrap into another page's slots)
     }
     p.positions[i] = pos;
     p.slots[i] = slot;

@@ -21,7 +21,7 @@ from .cache import SlidingWindow, get_cache_sizes, upload
 
 SOFTMAX_SCALE = HEAD_DIM ** -0.5
 _REASONS = {1: "a row out of range, or named twice", 2: "a length that is negative or longer than a row of the block table", 3: "more tokens than the plan has room for",
-            4: "too few free pages", 16: "a wait inside attention ran out", 32: "a request of more tokens than the plan's `longest` or `most`"}
+            4: "too few free pages, or a number of them that the stack cannot have", 16: "a wait inside attention ran out", 32: "a request of more tokens than the plan's `longest` or `most`"}
 
 
 def pages_of(tokens: int) -> int:

@@ -252,6 +252,27 @@ def test_write_takes_rows_of_wider_matrices_and_leaves_empty_places_out():
     pool.assert_same()
 
 
+def test_stacks_that_are_none():
+    """A count of free pages that the stack cannot have is refused; an id that no pool has becomes no slot, and not another page's."""
+    for n_free in (9, 2 ** 31 - 1, -1, -2 ** 31):
+        t = mi.PageTables(torch.full((2, 4), -1, dtype=torch.int32, device=DEV), ints([0, 0]), ints(list(range(8))), ints([n_free]))
+        with pytest.raises(_abi_paged.Mb200Error, match="free"):
+            t.extend(ints([70, 1]), 71).check()
+        t.table[0, :2], t.lens[0] = ints([6, 7]), 100
+        with pytest.raises(_abi_paged.Mb200Error, match="free"):
+            check_status(t.truncate(ints([0, 0])))
+        assert t.lens.tolist() == [100, 0] and t.free.tolist() == list(range(8)) and t.n_free.item() == n_free
+    for page in (2 ** 25, 2 ** 25 + 1, 2 ** 31 - 1, -1):
+        t = mi.PageTables(torch.full((1, 4), -1, dtype=torch.int32, device=DEV), ints([0]), ints([page, 3]), ints([2]))
+        plan = t.extend(ints([70]), 70).check()
+        assert plan.slots.tolist() == list(range(192, 256)) + [-1] * 6 and t.table.tolist() == [[3, page, -1, -1]]
+        pool, k = Pool(4, 1), numbers(70, 1, 128, seed=1)
+        pool.write(k.to(DEV), k.to(DEV), plan, plan.slots.tolist())
+        pool.assert_same()
+        out = mi.attend_pages(k.to(DEV), pool.kv, pool.scale, plan)
+        assert out[:64].isfinite().all() and out[64:].isnan().all()
+
+
 # ---------------------------------------------------------------------------------------------------------------- attention
 def filled(KV, past, new, seed, extra_rows=0, kv_std=1.0):
     """(tables' plan of `new` tokens behind `past`, pool) with pages in a random order and random codes everywhere; what nobody has written is NaN."""
