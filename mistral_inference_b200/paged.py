@@ -306,8 +306,9 @@ class PagedCache:
 
     def update_seqlens(self, seqlens: List[int]) -> None:
         """After a forward: its tokens count.  Negative numbers take (drafted) tokens back."""
+        assert len(seqlens) == len(self.ledger.lens), f"{len(seqlens)} numbers of tokens, {len(self.ledger.lens)} requests"
         lens = [n + a for n, a in zip(self.ledger.lens, seqlens)]
-        assert len(seqlens) == len(lens) and all(0 <= n <= d for n, d in zip(lens, self._on_device)), (self.ledger.lens, seqlens)
+        assert all(0 <= n <= d for n, d in zip(lens, self._on_device)), (self.ledger.lens, seqlens)
         self.ledger.lens = lens
 
     # -- metadata ---------------------------------------------------------------------------------

@@ -221,6 +221,26 @@ def test_scratch_is_sized_by_the_device_that_the_call_runs_on(monkeypatch):
     assert sizes_of == [1001, 1000, 1001] and [d for d, _ in asked] == [1, 0] and asked[0][1] == (2, 600, 300, 900, 20, 32, 8, 0)
 
 
+def account(lens, on_device=None):
+    """A PagedCache's account on the host, without its tensors."""
+    from mistral_inference_b200.paged import PageLedger
+    c = mi.PagedCache.__new__(mi.PagedCache)
+    c.ledger = PageLedger(rows=4, max_seq_len=300, n_pages=20)
+    c.ledger.admit(len(lens))
+    c.ledger.lens, c._on_device, c.cache_sizes, c._started = list(lens), list(on_device or lens), [300, 300], True
+    return c
+
+
+def test_tokens_count_for_every_request_or_for_none():
+    c = account([10, 20, 30], [11, 22, 30])
+    for bad in ([1], [1, 2], [1, 2, 0, 0], [2, 0, 0], [-11, 0, 0]):
+        with pytest.raises(AssertionError):
+            c.update_seqlens(bad)
+        assert c.ledger.lens == [10, 20, 30]
+    c.update_seqlens([1, 1, -30])
+    assert c.ledger.lens == [11, 21, 0]
+
+
 LAYOUT = """
 #include "plan_layout.cuh"
 extern "C" void layout(int B, int R, int* out) {
