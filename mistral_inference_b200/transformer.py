@@ -424,6 +424,7 @@ class Transformer(nn.Module):
         per-token gathers (generate.py:97-118).  From 128 tokens on the lm head's epilogue reduces the logits where they are computed
         (blocks of up to SCORE_BLOCK_TOKENS rows) and keeps the rows of the sequences' last tokens; the [T, V] logits never exist.
         Fewer tokens: the logits of all rows, then the fused log-softmax + gather kernel."""
+        assert cache is None or not cache.paged or min(seqlens) >= 1, "every sequence brings a token"  # (requests on pages may bring none elsewhere)
         self._last_static_logits = 0
         T, V = input_ids.shape[0], self.vocab_size
         ends = list(itertools.accumulate(seqlens))

@@ -241,6 +241,16 @@ def test_tokens_count_for_every_request_or_for_none():
     assert c.ledger.lens == [11, 21, 0]
 
 
+def test_log_probabilities_of_requests_that_bring_nothing_are_refused():
+    """Their last tokens' logits were those of memory that nobody wrote."""
+    from types import SimpleNamespace
+    from mistral_inference_b200.transformer import Transformer
+    ids = torch.zeros(90, dtype=torch.long)
+    for seqlens in ([0, 90], [90, 0], [40, 0, 50]):
+        with pytest.raises(AssertionError, match="brings a token"):
+            Transformer.forward_logprobs(SimpleNamespace(vocab_size=8, num_pipeline_ranks=1), ids, seqlens, account([5] * len(seqlens)), ids)
+
+
 LAYOUT = """
 #include "plan_layout.cuh"
 extern "C" void layout(int B, int R, int* out) {
