@@ -23,7 +23,7 @@ import torch
 
 from . import _abi
 from .cache import BufferCache
-from .scores import TokenScores, empty_scores, token_scores
+from .scores import MAX_ALTERNATIVES, TokenScores, empty_scores, token_scores
 from .transformer import Transformer
 
 TOP_P = 0.8     # generate.py:126
@@ -78,6 +78,8 @@ def generate(encoded_prompts: List[List[int]], model: Transformer, images: List[
     dev = model.device
     plan = _PromptPlan(encoded_prompts, chunk_size)
     B, V = plan.B, model.args.vocab_size
+    if not 0 <= alternatives <= min(MAX_ALTERNATIVES, V):
+        raise ValueError(f"{alternatives} alternatives (0 to {MAX_ALTERNATIVES}, and no more than the {V} tokens)")
 
     # one ring per layer, sized like the reference's (generate.py:68-78)
     cache = model.make_cache(model.args.max_batch_size, max(plan.lens) + max_tokens, **({} if kv_cache == "ring" else {"kv_cache": kv_cache}))

@@ -9,6 +9,8 @@ import torch
 
 from . import _abi_paged
 
+MAX_ALTERNATIVES = _abi_paged.MAX_TOP
+
 
 @dataclass
 class TokenScores:
@@ -36,7 +38,7 @@ def token_scores(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, t
     T, V = logits.shape
     assert logits.stride(1) == 1 and (T <= 1 or logits.stride(0) >= V), "rows of logits are contiguous and do not overlap"
     assert targets is None or (targets.dtype == torch.long and targets.shape == (T,)), "targets: one int64 a row"
-    assert 0 <= top <= min(_abi_paged.MAX_TOP, V), f"{top} alternatives (at most {_abi_paged.MAX_TOP}, and no more than tokens)"
+    assert 0 <= top <= min(MAX_ALTERNATIVES, V), f"{top} alternatives (at most {MAX_ALTERNATIVES}, and no more than tokens)"
     if out is None:
         out = empty_scores(T, top, targets is not None, logits.device)
     else:

@@ -251,6 +251,21 @@ def test_log_probabilities_of_requests_that_bring_nothing_are_refused():
             Transformer.forward_logprobs(SimpleNamespace(vocab_size=8, num_pipeline_ranks=1), ids, seqlens, account([5] * len(seqlens)), ids)
 
 
+def test_numbers_of_alternatives_are_refused_before_the_prompt_runs():
+    from types import SimpleNamespace
+
+    def runs(*a, **kw):
+        raise RuntimeError("the prompt ran")
+    model = SimpleNamespace(device=torch.device("cpu"), args=SimpleNamespace(vocab_size=40, max_batch_size=1), make_cache=lambda *a, **kw: account([0]), forward_scores=runs, forward_logprobs=runs)
+    model.eval = lambda: model
+    for bad in (-1, 41, 65, 1000):
+        with pytest.raises(ValueError, match="alternatives"):
+            mi.generate([[1, 2]], model, max_tokens=1, temperature=0.0, alternatives=bad)
+    for good in (0, 1, 40):
+        with pytest.raises(RuntimeError, match="ran"):
+            mi.generate([[1, 2]], model, max_tokens=1, temperature=0.0, alternatives=good)
+
+
 LAYOUT = """
 #include "plan_layout.cuh"
 extern "C" void layout(int B, int R, int* out) {
