@@ -331,9 +331,10 @@ class PagedCache:
         failed step has left of them, and finds nothing to take back where it never came to its plan."""
         self._on_device = [n + a for n, a in zip(self.ledger.lens, seqlens)]
 
-    def metadata_of(self, plan: PagePlan, seqlens: List[int]) -> List[PagedInputMetadata]:
-        """One per layer (shared by layers of one window)."""
-        first, longest = not any(self.ledger.lens), max(seqlens)
+    def metadata_of(self, plan: PagePlan, seqlens: List[int], first: bool) -> List[PagedInputMetadata]:
+        """One per layer (shared by layers of one window).  first: no request has a token yet, and attention need not read pages; a step that is captured may be replayed when
+        they have some."""
+        longest = max(seqlens)
         per_w = {w: PagedInputMetadata(plan, plan.positions, plan.q_start, plan.seqpos, first or longest > 1, first, list(seqlens), longest, w) for w in set(self.cache_sizes)}
         return [per_w[w] for w in self.cache_sizes]
 
@@ -346,7 +347,7 @@ class PagedCache:
         most = max(n + a for n, a in zip(self.ledger.lens, seqlens))
         plan = self.tables.extend(self._ints(seqlens), sum(seqlens), self.rows_on_device(), longest=max(seqlens), most=most)
         self.planned(seqlens)
-        return self.metadata_of(plan, seqlens)
+        return self.metadata_of(plan, seqlens, first=not any(self.ledger.lens))
 
     def get_view(self, layer_id: int, metadata: PagedInputMetadata) -> PagedView:
         kv, scale = self.pools[layer_id]

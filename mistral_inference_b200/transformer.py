@@ -374,7 +374,7 @@ class Transformer(nn.Module):
 
         def run() -> None:
             if cache.paged:  # block tables and slot map: a captured step takes its pages when it is replayed
-                md = cache.metadata_of(cache.tables.extend(st["one"], B, st["rows"], longest=1, most=cache.max_seq_len), seqlens)
+                md = cache.metadata_of(cache.tables.extend(st["one"], B, st["rows"], longest=1, most=cache.max_seq_len), seqlens, first=False)
             else:
                 md = cache.metadata_from_block(st["meta"], layout, seqlens)
                 _abi.decode_meta(st["seqpos"], st["meta"], distinct)

@@ -264,3 +264,22 @@ def test_a_decode_step_that_fails_leaves_no_tokens_behind(monkeypatch, where):
     assert runs[0][1:] == runs[1][1:] and runs[0][1] == runs[0][2]
     for a, b in zip(runs[0][0], runs[1][0]):
         assert torch.equal(a, b)
+
+
+def test_a_decode_step_captured_without_tokens_sees_those_that_come():
+    """Requests that have given all their tokens back when the step is captured: its replays attend over what they have by then."""
+    m, p = model_of(max_batch=2)
+    steps = [torch.tensor(t, device="cuda") for t in ([5, 6], [7, 8], [9, 1], [2, 3])]
+    cache = m.make_cache(2, 100, kv_cache="pages")
+    cache.admit(2)
+    m.decode_static(steps[0], cache)
+    cache.update_seqlens([-1, -1])
+    got = [m.decode_static(t, cache).clone() for t in steps]
+    other = m.make_cache(2, 100, kv_cache="pages")
+    other.admit(2)
+    for i, t in enumerate(steps):
+        other.__dict__.pop("_mb200_decode_states", None)  # run, not captured
+        assert torch.equal(got[i], m.decode_static(t, other)), i
+    # the same tokens without the second: what came before a token matters
+    other.update_seqlens([-3, -3])
+    assert other.kv_seqlens.tolist() == [1, 1] and not torch.equal(got[2], m.decode_static(steps[2], other))
