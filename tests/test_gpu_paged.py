@@ -651,3 +651,26 @@ def test_a_pool_past_32_bit_offsets():
     assert torch.equal(got, mi.attend_pages(q, kv2, scale2, plan2))
     check = kv.view(torch.uint8)[plan2.slots.long()[:1] // 64]
     assert check is not None
+
+
+def test_writes_past_32_bit_offsets():
+    """The same tokens into pages behind the first 4 GB and into a small pool: the same codes and scales, and nothing in between."""
+    n, KV, ids = 40000, 8, [5, 39999, 33000, 39000]
+    kv = torch.zeros(n, KV, 2, 64, 128, dtype=torch.uint8, device=DEV)
+    scale = torch.ones(n, KV, 2, device=DEV)
+    t = mi.PageTables(torch.full((1, 4), -1, dtype=torch.int32, device=DEV), ints([0]), ints(ids), ints([4]))
+    small = mi.PageTables(torch.full((1, 4), -1, dtype=torch.int32, device=DEV), ints([0]), ints([0, 1, 2, 3]), ints([4]))
+    pool = Pool(4, KV)
+    pool.kv.view(torch.uint8).zero_()
+    pool.scale.fill_(1.0)
+    pool.ref_kv.zero_()
+    pool.ref_scale.fill_(1.0)
+    for i, count in enumerate((150, 1, 90)):
+        k, v = (numbers(count, KV, 128, seed=2 * i + j, spread=1 + i).to(DEV) for j in range(2))
+        mi.write_pages(kv, scale, k, v, t.extend(ints([count]), count).check())
+        plan = small.extend(ints([count]), count).check()
+        pool.write(k, v, plan, plan.slots.tolist())
+    pool.assert_same()
+    assert torch.equal(kv[ids], pool.kv.view(torch.uint8)) and torch.equal(scale[ids], pool.scale)
+    kv[ids], scale[ids] = 0, 1.0
+    assert int(kv.view(torch.int64).count_nonzero()) == 0 and (scale == 1.0).all()

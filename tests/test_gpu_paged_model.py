@@ -1,4 +1,6 @@
 """The Transformer on 8-bit pages: the whole path through forward and generate, its attention held against 64 bits over the same pages."""
+import re
+
 import pytest
 import torch
 
@@ -283,3 +285,26 @@ def test_a_decode_step_captured_without_tokens_sees_those_that_come():
     # the same tokens without the second: what came before a token matters
     other.update_seqlens([-3, -3])
     assert other.kv_seqlens.tolist() == [1, 1] and not torch.equal(got[2], m.decode_static(steps[2], other))
+
+
+def test_forward_of_a_mixture_on_pages(plain_attention):
+    """test_forward_on_pages for a model whose experts are all alike: whichever the router takes between two that are nearly equal, the numbers are the same."""
+    p = synth.shape("tiny-moe")
+    args = mi.TransformerArgs.from_dict(dict(p))
+    args.max_batch_size = 3
+    sd = synth.synth_state_dict(p, 1, torch.bfloat16, "cuda")
+    alike = {k: sd[re.sub(r"experts\.\d+\.", "experts.0.", k)] for k in sd}
+    assert any(alike[k] is not sd[k] for k in sd)
+    m = Transformer.empty(args, "cuda", torch.bfloat16)
+    m.load_state_dict(alike)
+    m.eval()
+    g = torch.Generator().manual_seed(3)
+    steps = [[70, 3, 129], [1, 1, 1], [20, 64, 1], [1, 1, 1]]
+    ids = [torch.randint(0, p["vocab_size"], (sum(s),), generator=g).cuda() for s in steps]
+    outs = []
+    for plain in (False, True):
+        plain_attention(plain)
+        cache = m.make_cache(3, 300, kv_cache="pages")
+        outs.append([m.forward(x, s, cache) for x, s in zip(ids, steps)])
+    for got, want in zip(*outs):
+        assert (got - want).abs().max() <= logit_tol(want, ULPS), (got - want).abs().max()
