@@ -64,34 +64,39 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
+def _build_small(src: Path, lib: Path, others, flags=(), force: bool = False) -> Path:
+    """A library of its own of the sources in `src` (and of `others`, which they include), so that who needs only it compiles only them (seconds).  Safe when several
+    processes start at once: the output is written under a private name and renamed."""
+    sources = sorted(src.glob("*.cu"))
+    h = hashlib.sha256()
+    for f in sources + sorted(src.glob("*.cuh")) + sorted(src.glob("*.h")) + list(others):
+        h.update(f.name.encode())
+        h.update(f.read_bytes())
+    h.update(" ".join(NVCC_FLAGS).encode())
+    digest = h.hexdigest()
+    stamp = src / ".build_stamp"
+    if not force and lib.exists() and stamp.exists() and stamp.read_text().strip() == digest:
+        return lib
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    tmp = PKG / f".{lib.stem}.{os.getpid()}.so"
+    cmd = [nvcc, *NVCC_FLAGS, *flags, "-o", str(tmp)] + [str(f) for f in sources]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        sys.stderr.write(proc.stdout + proc.stderr)
+        raise RuntimeError(f"nvcc failed ({proc.returncode}): {' '.join(cmd)}")
+    os.replace(tmp, lib)
+    stamp.write_text(digest)
+    return lib
+
+
+INCLUDE = PKG.parent / "include"
 HYBRID_SRC = CSRC / "hybrid"
 HYBRID_LIB = PKG / "libmb200_hybrid.so"
 
 
 def build_hybrid(force: bool = False) -> Path:
-    """libmb200_hybrid.so: the kernels of layered decoders (csrc/hybrid/), a separate, small library so that a fresh checkout
-    that only serves such a model compiles only them (seconds).  Safe when several processes start at once: the output is
-    written under a private name and renamed."""
-    files = sorted(HYBRID_SRC.glob("*.cu")) + sorted(HYBRID_SRC.glob("*.cuh")) + sorted(HYBRID_SRC.glob("*.h")) + [CSRC / "stream_linear.cuh", CSRC / "device_info.cuh"] + sorted((PKG.parent / "include").glob("mistral_b200_hybrid*.h"))
-    h = hashlib.sha256()
-    for f in files:
-        h.update(f.name.encode())
-        h.update(f.read_bytes())
-    h.update(" ".join(NVCC_FLAGS).encode())
-    digest = h.hexdigest()
-    stamp = HYBRID_SRC / ".build_stamp"
-    if not force and HYBRID_LIB.exists() and stamp.exists() and stamp.read_text().strip() == digest:
-        return HYBRID_LIB
-    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    tmp = PKG / f".libmb200_hybrid.{os.getpid()}.so"
-    cmd = [nvcc, *NVCC_FLAGS, "--threads", "0", "-o", str(tmp)] + [str(f) for f in sorted(HYBRID_SRC.glob("*.cu"))]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError(f"nvcc failed ({proc.returncode}): {' '.join(cmd)}")
-    os.replace(tmp, HYBRID_LIB)
-    stamp.write_text(digest)
-    return HYBRID_LIB
+    """libmb200_hybrid.so: the kernels of layered decoders (csrc/hybrid/)."""
+    return _build_small(HYBRID_SRC, HYBRID_LIB, [CSRC / "stream_linear.cuh", CSRC / "device_info.cuh"] + sorted(INCLUDE.glob("mistral_b200_hybrid*.h")), ("--threads", "0"), force)
 
 
 PAGED_SRC = CSRC / "paged"
@@ -99,29 +104,10 @@ PAGED_LIB = PKG / "libmb200_paged.so"
 
 
 def build_paged(force: bool = False) -> Path:
-    """libmb200_paged.so: pages of 8-bit keys and values and the scores of tokens (csrc/paged/), built like libmb200_hybrid.so."""
+    """libmb200_paged.so: pages of 8-bit keys and values and the scores of tokens (csrc/paged/)."""
     headers = ["common.cuh", "device_info.cuh", "epilogue.cuh", "sigmoid.cuh", "gemm_tcgen05.cuh", "gemm_mma.cuh", "split_schedule.cuh", "decode_megakernel.cuh", "attn_decode.cuh",
                "attn_prompt_tcgen05.cuh"]
-    files = sorted(PAGED_SRC.glob("*.cu")) + sorted(PAGED_SRC.glob("*.cuh")) + [CSRC / h for h in headers] + [PKG.parent / "include" / h for h in ("mistral_b200.h", "mistral_b200_paged.h")]
-    h = hashlib.sha256()
-    for f in files:
-        h.update(f.name.encode())
-        h.update(f.read_bytes())
-    h.update(" ".join(NVCC_FLAGS).encode())
-    digest = h.hexdigest()
-    stamp = PAGED_SRC / ".build_stamp"
-    if not force and PAGED_LIB.exists() and stamp.exists() and stamp.read_text().strip() == digest:
-        return PAGED_LIB
-    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    tmp = PKG / f".libmb200_paged.{os.getpid()}.so"
-    cmd = [nvcc, *NVCC_FLAGS, "-o", str(tmp)] + [str(f) for f in sorted(PAGED_SRC.glob("*.cu"))]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError(f"nvcc failed ({proc.returncode}): {' '.join(cmd)}")
-    os.replace(tmp, PAGED_LIB)
-    stamp.write_text(digest)
-    return PAGED_LIB
+    return _build_small(PAGED_SRC, PAGED_LIB, [CSRC / h for h in headers] + [INCLUDE / h for h in ("mistral_b200.h", "mistral_b200_paged.h")], force=force)
 
 
 if __name__ == "__main__":
