@@ -19,11 +19,13 @@
 //             per dimension, the values' sums of the tile before
 //   producer  TMA: tiles of two pages (8 KB of keys and of values each) into a ring of PA_STAGES x 32 KB
 //   issuer    MMAs: S(0) S(1) | PV(t) S(t + 2) ...
-// What it measured: single tokens of 4 requests with 32500 tokens each, 32 heads over 8: 42.3 us, 5.7 TB/s; of 32 with ~1000 each: 16.2 us, of which the bytes take 10 and launch,
-// the first loads and the merge 6.  A tile of a token's few columns takes 1700 clocks, the last 600 to 1000 of them waiting for the bytes.  (Four warps with eight columns
-// each, half of them empty for groups of four heads: 3200 clocks, 21.0 us.)  A tile of 32 columns takes 3600: scores and maximum 1050, weights 620, sums 470 by 16 warps, whose
-// instructions are the bound: drafts of 5 tokens x 6 heads for 8 requests behind 2100: 21.3 us for 4.9 of bytes.  Keys and values in slots of their own, keys' freed
-// after S(t): no faster (44.8 us for 42.3 with the four long requests): what lies in flight is enough.
+// What it measured, on inputs that L2 does not hold: single tokens of 4 requests with 32500 tokens each, 32 heads over 8: 42.8 us, 5.65 TB/s; of 32 with ~1000 each: 16.2 us, of which
+// the bytes take 10 and launch, the first loads and the merge 6.  A tile of a token's few columns takes 1700 clocks, the last 600 to 1000 of them waiting for the bytes.  (Four warps
+// with eight columns each, half of them empty for groups of four heads: 3200 clocks, 21.0 us.)  A tile of 32 columns takes 3600: scores and maximum 1050, weights 620, sums 470 by 16
+// warps.  Latency bounds those: 1.8 of 4 instructions a clock, one CTA an SM whose warps all wait for a tile's scores, the group's barrier and the sums of the tile before; 96 registers
+// a thread leave 48 bytes of it spilled.  Drafts of 5 tokens x 6 heads for 8 requests behind 2100: 22.4 us for 4.9 of bytes.  The score of weight 1 that goes down costs drafts
+// behind 8400 tokens 56.9 us for 55.5, the four long requests 42.4 for 42.0.  Keys and values in slots of their own, keys' freed after S(t): no faster (44.8 us for 42.3 with the four
+// long requests): what lies in flight is enough.
 #pragma once
 #include <type_traits>
 
@@ -53,7 +55,7 @@ struct PagedAttnParams {
 // NQ query columns, Q of them a group of softmax warps; column c of the MMA: group i has hi parts at i * 2 Q, lo parts at i * 2 Q + Q
 template <int NQ>
 struct PaCfg {
-  static constexpr int G = NQ >= 32 ? 4 : 2, Q = NQ / G;   // (32 columns: two groups 31.1 us for drafts of 8 requests behind 2100, four 25.5; now 21.3)
+  static constexpr int G = NQ >= 32 ? 4 : 2, Q = NQ / G;   // (32 columns: two groups 31.1 us for drafts of 8 requests behind 2100, four 25.5; now 21.2)
   static constexpr int kSoftWarps = 4 * G, kThreads = 32 * (kSoftWarps + 2), kResident = NQ >= 32 ? 1 : 2;
   static constexpr int N = 2 * NQ < 16 ? 16 : 2 * NQ;      // (16 at least; columns that nobody reads hold anything)
   static constexpr int kColBytes = N * 128;                // Q or one P tile: [N columns][128 bytes], 128B-swizzled

@@ -7,7 +7,7 @@
 // Memory: 2 bytes read and 1 written per number.  A page of a head and kind is written by one group of threads alone: a CTA, whose up to 64 rows stay in
 // registers between the maximum and the conversion so that each byte moves once, or, for few tokens a request, a warp.
 // Eight CTAs an SM, 128 KB of rows on their way: 34.7 us for 32000 tokens of 8 heads, 5.7 TB/s; 39.6 us at the five that the compiler's own choice of registers
-// leaves, 44 at ten, which spill.  11.3 us for three prompts of 6900 tokens together, 6.6 of them for the bytes; the rest is the launch and a chain of loads
+// leaves; eight spill 60 bytes a thread, ten more: 44 us.  11.5 us for three prompts of 6900 tokens together, 6.6 of them for the bytes; the rest is the launch and a chain of loads
 // (request, place, slot, scale) ahead of the only rows that a CTA has.
 #pragma once
 #include "paged_common.cuh"

@@ -12,7 +12,7 @@
 // barriers a segment.  A warp a row joins the segments, in a second kernel or, where few rows leave room, behind a cluster's barrier.
 // 1000 x 131072 fp32, 8 alternatives: 104 us, 5.0 TB/s (20 of them 118; bf16 79, whose entries take more of the bound by instructions).  Before: the largest taken off over and
 // over 1540 us; entries in registers, a CTA for 8192 of them 141; longer walks with a list kept up to date 205 (a barrier a slice, and more code than the instruction
-// cache holds); whole segments by one bulk copy each, fetched behind the second barrier 107.  32 rows, 20 alternatives: 14.4 us, 2.6 for the bytes, the rest two launches and
+// cache holds); whole segments by one bulk copy each, fetched behind the second barrier 107.  32 rows, 20 alternatives: 14.4 us (15.7 where L2 does not hold them), 2.6 for the bytes, the rest two launches and
 // two segments' latency; 1 x 32000: 7.6.
 #pragma once
 #include <cfloat>
@@ -389,7 +389,9 @@ __global__ void __launch_bounds__(32) token_scores_join_kernel(TokenScoresParams
 }
 
 
-// Short rows: a warp each, entries in registers, nothing to join.  (4000 x 1003 fp32, 20 alternatives: 11.8 us, 2.5 of them for the bytes; as segments, a CTA and two barriers a row, 47.3.  64 x 2000: 7.5 and 9.8.)
+// Short rows: a warp each, entries in registers, nothing to join.  (4000 x 1003 fp32, 20 alternatives: 12.9 us, 2.5 of them for the
+// bytes; as segments, a CTA and two barriers a row, 47.3.  64 x 2000: 7.0 and 9.8.)  With one alternative 8.7: the other 19 are steps of one ballot and one maximum each, one after the
+// other, and places in a list; 0.2 us each, 26.1 us for 64.
 // The best: the maxima of four parts of each lane's entries; the top-th largest of those 128 is a value that at least `top` entries reach, and few more, which are ranked
 // by counting.  (One maximum a lane: 32 alternatives 89 us, where the least of them lets hundreds pass.)
 constexpr int TS_SHORT = 2048, TS_SHORT_WARPS = 4, TS_SHORT_LIST = 128;
