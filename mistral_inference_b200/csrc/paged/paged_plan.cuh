@@ -8,7 +8,7 @@
 // nothing and says why in `status`.
 //
 // Nothing but latency bounds it: the lengths are a few hundred bytes, and each of the dependent steps (lengths -> prefix sums -> page -> slot) is one trip to L2.  So it is
-// ONE launch (8 requests' step and its truncate 7.7 us together, 64 prompts of 1000 tokens 12.0): every CTA forms the prefix sums of all requests for itself in
+// ONE launch (8 requests' step and its truncate 8.0 us together, 64 prompts of 1000 tokens 12.5): every CTA forms the prefix sums of all requests for itself in
 // shared memory, reads only the state as it was, and the last CTA to be done commits.
 #pragma once
 #include "paged_common.cuh"
