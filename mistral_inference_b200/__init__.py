@@ -13,3 +13,4 @@ from .layered import LayeredTransformer  # noqa: F401
 from .registry import load_model  # noqa: F401
 from .paged import PagedCache, PagePlan, PageTables, attend_pages, write_pages  # noqa: F401
 from .scores import TokenScores, token_scores  # noqa: F401
+from .rows8 import Rows8, gate_rows, multiply_rows, norm_rows, quantise_rows  # noqa: F401

@@ -1,0 +1,221 @@
+"""Rows of 8-bit numbers on the GPU, operator by operator against plain 64-bit restatements (rows8_util)."""
+import math
+
+import pytest
+import torch
+
+import mistral_inference_b200 as mi
+from mistral_inference_b200.rows8 import Rows8
+
+from . import rows8_util as U
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def normal(shape, seed, std=1.0, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device=DEV).normal_(0.0, std, generator=torch.Generator(device=DEV).manual_seed(seed))
+
+
+def uneven(T, K, seed, dtype):
+    """Rows whose entries span many powers of two, zeros among them."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = normal((T, K), seed) * torch.exp2(torch.randint(-9, 10, (T, K), device=DEV, generator=g).float())
+    x[torch.rand((T, K), device=DEV, generator=g) < 0.1] = 0
+    return x.to(dtype)
+
+
+def assert_same_rows(got: Rows8, x: torch.Tensor):
+    codes, scales = U.quantised(x)
+    assert torch.equal(got.scales.view(torch.uint8), scales)
+    same = got.codes.view(torch.uint8) == codes.view(torch.uint8)
+    assert (same | (got.codes.float().isnan() & codes.float().isnan())).all()
+
+
+# ------------------------------------------------------------------------------------------------------------ quantise
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,K", [(1, 1), (1, 4096), (2, 15), (3, 16), (5, 127), (129, 128), (128, 129), (31, 500), (33, 512), (1000, 513), (260, 1003), (7, 5120), (4, 14336)])
+def test_quantise(T, K, dtype):
+    assert_same_rows(mi.quantise_rows(uneven(T, K, 7 * T + K, dtype)), uneven(T, K, 7 * T + K, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantise_at_the_borders(dtype):
+    """Largest magnitudes next to 448 times a power, zeros of both signs, the smallest and largest numbers, numbers half way between codes."""
+    rows = []
+    for top in (448.0, 450.0, 446.0, 896.0, 1.75, 1.0, 3.5, 2.0 ** -120, 2.0 ** -133, 3.3e38, 2.0 ** -100 * 448, 2.0 ** -101 * 448):
+        row = torch.zeros(256)
+        row[0] = -top
+        row[1:100] = torch.linspace(-1, 1, 99) * top / 64
+        row[130], row[131] = -0.0, top / 7
+        rows.append(row)
+    half = torch.zeros(256)
+    half[:128] = torch.arange(128) * 0.25  # (448 as the largest: steps of 0.25 fall half way between codes from 4 on)
+    half[0] = 448
+    rows.append(half)
+    x = torch.stack(rows).to(DEV).to(dtype)
+    assert_same_rows(mi.quantise_rows(x), x)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_blocks_that_hold_no_number(dtype, bad):
+    x = uneven(40, 700, 3, dtype)
+    for r, k in [(0, 0), (3, 127), (3, 128), (20, 699), (39, 512)]:
+        x[r, k] = bad
+    got = mi.quantise_rows(x)
+    assert_same_rows(got, x)
+    nan = got.numbers().isnan()
+    assert nan[0, :128].all() and not nan[0, 128:].any() and nan[3, :256].all() and not nan[3, 256:].any() and nan[20, 640:].all() and not nan[1].any()
+
+
+@pytest.mark.parametrize("offset,ld", [(0, 640), (8, 640), (1, 640), (0, 643), (4, 644)])
+def test_rows_of_wider_matrices(offset, ld):
+    for dtype in (torch.bfloat16, torch.float32):
+        wide = uneven(50, ld, 11, dtype)
+        x = wide[:, offset: offset + 600]
+        assert_same_rows(mi.quantise_rows(x), x)
+
+
+def test_numbers_and_exponents():
+    x = uneven(200, 900, 5, torch.float32)
+    got = mi.quantise_rows(x)
+    assert torch.equal(got.numbers(torch.float64), U.numbers(got.codes, got.scales, 900))
+    assert torch.equal(got.numbers(torch.bfloat16).double(), got.numbers(torch.float64))  # four bits and a power: exact in 16 bits
+    assert torch.equal(got.exponents().long(), U.exponent(U.blocks_of(x).abs().amax(2)))
+
+
+# ---------------------------------------------------------------------------------------------------------------- norm
+def norm_in_64_bits(x, w, eps, add):
+    h = x if add is None else (x.double() + add.double()).to(x.dtype)  # (a sum of two 16-bit numbers has one rounding either way)
+    y = h.double() / torch.sqrt((h.double() ** 2).mean(1, keepdim=True) + eps) * w.double()
+    return h, y
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("with_add", [False, True])
+@pytest.mark.parametrize("T,K", [(1, 1), (1, 4096), (2, 100), (3, 16), (130, 129), (5, 1003), (32, 5120), (300, 6144), (3, 16385), (2, 40000), (1, 65536)])
+def test_norm(T, K, with_add, dtype):
+    x, w = normal((T, K), K, 1.3, dtype), (1 + normal((K,), K + 1, 0.2)).to(dtype)
+    add = normal((T, K), K + 2, 0.7, dtype) if with_add else None
+    rows, h = mi.norm_rows(x, w, 1e-5, add=add)
+    want, y = norm_in_64_bits(x, w, 1e-5, add)
+    if dtype is torch.bfloat16 or not with_add:
+        assert torch.equal(h, want)
+    else:
+        want, y = norm_in_64_bits(h, w, 1e-5, None)
+        assert torch.equal(h, x + add)
+    assert (h is x) == (not with_add)
+    # K products and additions in 32 bits (at most K / 32 one after another, then a tree), a division, a root, two products: each off by 2^-24 of it, the root halves
+    assert_off = y.abs() * (K / 32 + 16) * 2.0 ** -24
+    U.assert_rows_near(rows.codes, rows.scales, y, assert_off)
+
+
+def test_norm_of_zeros_and_of_no_numbers():
+    x, w = normal((6, 600), 1, 1.0, torch.bfloat16), torch.ones(600, dtype=torch.bfloat16, device=DEV)
+    x[1] = 0
+    x[2, 5] = math.nan
+    x[3, 599] = math.inf
+    rows, _ = mi.norm_rows(x, w, 1e-5)
+    assert (rows.numbers()[1] == 0).all() and rows.numbers()[2].isnan().all()
+    y = rows.numbers()[3]
+    assert y[512:].isnan().all() and (y[:512] == 0).all()  # x / infinity, and infinity / infinity in the last block
+    U.assert_rows_near(rows.codes[4:], mi.norm_rows(x[4:], w, 1e-5)[0].scales, norm_in_64_bits(x[4:], w, 1e-5, None)[1], 1e-5)
+
+
+def test_norm_of_rows_of_wider_matrices():
+    for dtype in (torch.bfloat16, torch.float32):
+        for off, ld in [(0, 1000), (8, 1000), (3, 1000), (0, 999)]:
+            x, add = normal((9, ld), 1, 1.0, dtype)[:, off: off + 900], normal((9, ld), 2, 1.0, dtype)[:, off: off + 900]
+            w = normal((1000,), 3, 1.0, dtype)[off: off + 900]
+            a, h = mi.norm_rows(x, w, 1e-5, add=add)
+            b, g = mi.norm_rows(x.contiguous(), w.clone(), 1e-5, add=add.contiguous())
+            assert torch.equal(h, g) and torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales.view(torch.uint8), b.scales.view(torch.uint8))
+
+
+# ------------------------------------------------------------------------------------------------------------ products
+def random_rows(T, K, seed, std=1.0):
+    return mi.quantise_rows(normal((T, K), seed, std) * torch.exp2(torch.randint(-3, 4, (T, -(-K // 128)), device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed))
+                                                                   .float()).repeat_interleave(128, 1)[:, :K])
+
+
+SIZES = [(1, 128, 128), (1, 1, 1), (1, 6144, 4096), (2, 130, 200), (5, 1000, 513), (16, 300, 1003), (17, 256, 640), (32, 5120, 1024), (33, 257, 2000), (64, 4096, 4096), (100, 700, 900),
+         (128, 512, 512), (129, 1001, 1152), (200, 2048, 128), (256, 256, 4096), (300, 4099, 700), (513, 1536, 2048), (777, 6144, 512), (1102, 2048, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,N,K", SIZES)
+def test_multiply(T, N, K, dtype):
+    x, w = random_rows(T, K, T + K), random_rows(N, K, N + K, 0.1)
+    y, off = U.product(U.numbers(x.codes, x.scales, K), U.numbers(w.codes, w.scales, K))
+    got = mi.multiply_rows(x, w, dtype=dtype)
+    assert got.dtype is dtype and got.shape == (T, N)
+    if dtype is torch.bfloat16:
+        off = off + (y.abs() + off) * 2.0 ** -8
+    bad = (got.double() - y).abs() > off
+    assert not bad.any(), f"{int(bad.sum())} off, the first at {bad.nonzero()[0].tolist()}: {got[bad][0]} for {y[bad][0]}"
+
+
+@pytest.mark.parametrize("T,H,K", [(1, 128, 128), (1, 1, 1), (1, 14336, 4096), (3, 100, 200), (16, 700, 513), (32, 1003, 1003), (48, 640, 5120), (64, 2048, 640), (65, 64, 900), (128, 384, 512),
+                                   (129, 500, 1152), (256, 128, 4096), (300, 2050, 700), (1102, 1024, 1000)])
+def test_gate(T, H, K):
+    x, w = random_rows(T, K, T + K), random_rows(2 * H, K, H + K, 1.5 * K ** -0.5)
+    y, off = U.product(U.numbers(x.codes, x.scales, K), U.numbers(w.codes, w.scales, K))
+    gate, up = y[:, 0::2], y[:, 1::2]
+    g = gate * torch.sigmoid(gate) * up
+    # silu's slope is within [-0.1, 1.1]; e^-x is 2^(-x log2 e) of a product that is off by 2^-24 of its magnitude: up to |x| 2^-24, beside a few units of 2^-22 in all
+    far = 1.1 * off[:, 0::2] * (up.abs() + off[:, 1::2]) + gate.abs() * off[:, 1::2] + g.abs() * (8 + gate.abs() / 2) * 2.0 ** -22
+    rows = mi.gate_rows(x, w)
+    assert rows.cols == H and rows.rows == T
+    U.assert_rows_near(rows.codes, rows.scales, g, far)
+
+
+def test_scales_of_every_row_and_block_reach_their_products():
+    """One entry a block: every power is seen by itself."""
+    for T, N in ((4, 260), (40, 130), (300, 260)):
+        K = 128 * 9
+        x, w = torch.zeros(T, K, device=DEV), torch.zeros(N, K, device=DEV)
+        for b in range(9):
+            x[:, 128 * b + 5 * b] = torch.exp2((torch.arange(T, device=DEV) * 7 + b * 3) % 23 - 11.0)
+        for b in range(9):
+            one = torch.zeros_like(w)
+            one[:, 128 * b + 5 * b] = torch.exp2((torch.arange(N, device=DEV) * 5 + b) % 19 - 9.0)
+            got = mi.multiply_rows(mi.quantise_rows(x), mi.quantise_rows(one), dtype=torch.float32)
+            assert torch.equal(got, x[:, 128 * b + 5 * b, None] * one[None, :, 128 * b + 5 * b]), (T, N, b)
+
+
+def test_a_row_of_no_numbers_stays_alone():
+    for T in (3, 40, 200):
+        x, w = normal((T, 700), 1), normal((300, 700), 2)
+        x[1, 600] = math.nan
+        w[7, 3] = math.inf
+        y = mi.multiply_rows(mi.quantise_rows(x), mi.quantise_rows(w))
+        nan = y.isnan()
+        assert nan[1].all() and nan[:, 7].all()
+        nan[1] = False
+        nan[:, 7] = False
+        assert not nan.any()
+        g = mi.gate_rows(mi.quantise_rows(x), mi.quantise_rows(w)).numbers().isnan()
+        assert g[1].all() and g[:, :128].all()  # feature 7 is unit 3: its block of each row
+        g[1] = False
+        assert not g[:, 128:].any()
+
+
+def test_out_may_be_part_of_wider_rows():
+    for T in (2, 60, 300):
+        x, w = random_rows(T, 640, 1), random_rows(500, 640, 2)
+        for dtype in (torch.bfloat16, torch.float32):
+            want = mi.multiply_rows(x, w, dtype=dtype)
+            for off, ld in [(0, 512), (8, 512), (3, 517)]:
+                wide = torch.full((T, ld), 7.0, dtype=dtype, device=DEV)
+                part = wide[:, off: off + 500]
+                assert mi.multiply_rows(x, w, out=part) is part and torch.equal(part, want)
+                assert (wide[:, :off] == 7).all() and (wide[:, off + 500:] == 7).all()
+
+
+def test_no_rows():
+    x = torch.empty(0, 300, dtype=torch.bfloat16, device=DEV)
+    rows = mi.quantise_rows(x)
+    normed, h = mi.norm_rows(x, torch.ones(300, dtype=torch.bfloat16, device=DEV), 1e-5, add=x)
+    w = random_rows(100, 300, 1)
+    assert rows.rows == normed.rows == 0 and h.shape == (0, 300) and mi.multiply_rows(rows, w).shape == (0, 100) and mi.gate_rows(rows, w).rows == 0

@@ -1,0 +1,131 @@
+"""The boundary and refusals of libmb200_rows8, without a GPU: everything here is turned away before a kernel is launched."""
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+import mistral_inference_b200 as mi
+from mistral_inference_b200 import _abi_rows8
+from mistral_inference_b200.build import build_rows8
+from mistral_inference_b200.rows8 import Rows8
+
+from . import rows8_util as U
+
+REPO = Path(__file__).resolve().parents[1]
+HEADER = REPO / "include" / "mistral_b200_rows8.h"
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build_rows8()
+    return _abi_rows8.lib()
+
+
+def test_header_and_binding_name_the_same_symbols(lib):
+    declared = set(re.findall(r"\b(mb8_[a-z0-9_]+)\s*\(", HEADER.read_text()))
+    assert declared == set(_abi_rows8._SIGNATURES)
+    assert lib.mb8_abi_version() == _abi_rows8.ABI_VERSION == int(re.search(r"MB8_ABI_VERSION (\d+)", HEADER.read_text()).group(1))
+
+
+def test_constants_agree_with_the_header():
+    text = HEADER.read_text()
+    assert int(re.search(r"MB8_MAX_NORM (\d+)", text).group(1)) == _abi_rows8.MAX_NORM
+    assert 1 << int(re.search(r"MB8_MAX_ROWS \(1 << (\d+)\)", text).group(1)) == _abi_rows8.MAX_ROWS
+
+
+def last(lib):
+    return lib.mb8_last_error().decode()
+
+
+# Pointers that are never read: every call below is refused by its sizes.
+X = 4096
+BIG = (1 << 24) + 1
+
+
+def test_quantise_is_refused(lib):
+    def call(x=X, ld=256, dtype=0, codes=X, scales=X, T=2, K=256):
+        return lib.mb8_quantise(x, ld, dtype, codes, scales, T, K, None)
+    for kw, why in [(dict(x=None), "null"), (dict(codes=None), "null"), (dict(scales=None), "null"), (dict(codes=X + 8), "16 bytes"), (dict(scales=X + 4), "16 bytes"), (dict(x=X + 1), "aligned"),
+                    (dict(x=X + 2, dtype=1), "aligned"), (dict(dtype=2), "dtype"), (dict(dtype=-1), "dtype"), (dict(ld=255), "apart"), (dict(T=-1), "rows"), (dict(K=0), "entries"),
+                    (dict(T=BIG), "rows"), (dict(K=BIG, ld=BIG), "entries"), (dict(T=1 << 24, K=1 << 24, ld=1 << 24), "rows")]:
+        assert call(**kw) == -1 and why in last(lib), (kw, last(lib))
+    assert call(T=0, x=None) == 0
+
+
+def test_norm_is_refused(lib):
+    def call(x=X, ld=256, add=X, ld_add=256, w=X, dtype=0, out=X, codes=X, scales=X, T=2, K=256):
+        return lib.mb8_norm(x, ld, add, ld_add, w, dtype, out, codes, scales, T, K, 1e-5, None)
+    for kw, why in [(dict(x=None), "null"), (dict(w=None), "null"), (dict(out=None), "null"), (dict(codes=None), "null"), (dict(ld=255), "apart"), (dict(ld_add=255), "apart"),
+                    (dict(add=X + 1), "aligned"), (dict(w=X + 1), "aligned"), (dict(dtype=2), "dtype"), (dict(K=65537, ld=65537, ld_add=65537), "65536"), (dict(T=-1), "rows"), (dict(K=0), "entries")]:
+        assert call(**kw) == -1 and why in last(lib), (kw, last(lib))
+    assert call(T=0, x=None) == 0
+
+
+def test_products_are_refused(lib):
+    def multiply(xc=X, xs=X, wc=X, ws=X, out=X, ld=64, dtype=0, T=2, N=64, K=256):
+        return lib.mb8_multiply(xc, xs, wc, ws, out, ld, dtype, T, N, K, None)
+    for kw, why in [(dict(xc=None), "null"), (dict(xs=None), "null"), (dict(wc=None), "null"), (dict(ws=None), "null"), (dict(out=None), "null"), (dict(xc=X + 8), "16 bytes"), (dict(ws=X + 1), "16 bytes"),
+                    (dict(out=X + 1), "aligned"), (dict(out=X + 2, dtype=1), "aligned"), (dict(dtype=2), "dtype"), (dict(ld=63), "apart"), (dict(T=-1), "rows"), (dict(N=0), "features"), (dict(K=0), "entries"),
+                    (dict(T=BIG), "rows"), (dict(N=BIG, ld=BIG), "features"), (dict(K=BIG), "entries")]:
+        assert multiply(**kw) == -1 and why in last(lib), (kw, last(lib))
+
+    def gate(xc=X, xs=X, wc=X, ws=X, codes=X, scales=X, T=2, H=64, K=256):
+        return lib.mb8_gate(xc, xs, wc, ws, codes, scales, T, H, K, None)
+    for kw, why in [(dict(xc=None), "null"), (dict(codes=None), "null"), (dict(scales=None), "null"), (dict(codes=X + 8), "16 bytes"), (dict(T=-1), "rows"), (dict(H=0), "features"),
+                    (dict(H=(1 << 23) + 1), "features"), (dict(K=0), "entries")]:
+        assert gate(**kw) == -1 and why in last(lib), (kw, last(lib))
+    assert multiply(T=0, out=None, xc=None) == gate(T=0, codes=None, xc=None) == 0
+
+
+def rows(R, K):
+    return Rows8.empty(R, K, "cpu")
+
+
+def test_python_refuses_what_does_not_fit():
+    bf = dict(dtype=torch.bfloat16)
+    for x in [torch.zeros(3, 4, dtype=torch.float16), torch.zeros(4, **bf), torch.zeros(2, 0, **bf), torch.zeros(4, 6, **bf).t(), torch.zeros(1, 6, **bf).expand(3, 6), torch.zeros(4, 6, **bf)]:
+        with pytest.raises(AssertionError):  # (the last one for its device)
+            mi.quantise_rows(x)
+    with pytest.raises(AssertionError):
+        mi.multiply_rows(rows(2, 100), rows(3, 100))
+    with pytest.raises(AssertionError):
+        Rows8.empty(2, 0, "cpu")
+    with pytest.raises(AssertionError):
+        Rows8.empty(2, BIG, "cpu")
+
+
+def test_no_cpu_fallback():
+    for call in (lambda: mi.quantise_rows(torch.zeros(2, 3)), lambda: mi.norm_rows(torch.zeros(2, 3), torch.zeros(3), 1e-5), lambda: mi.multiply_rows(rows(2, 9), rows(3, 9)),
+                 lambda: mi.gate_rows(rows(2, 9), rows(4, 9))):
+        with pytest.raises(AssertionError, match="no fallback"):
+            call()
+
+
+@pytest.mark.parametrize("R,K", [(1, 1), (130, 1003), (128, 512), (33, 4096), (300, 640)])
+def test_numbers_and_exponents(R, K):
+    x = torch.randn(R, K, generator=torch.Generator().manual_seed(R)) * torch.exp2(torch.randint(-20, 20, (R, K), generator=torch.Generator().manual_seed(K)).float())
+    codes, scales = U.quantised(x)
+    r = Rows8(codes, scales.view(torch.float8_e8m0fnu), K)
+    assert torch.equal(r.numbers(torch.float64), U.numbers(codes, scales, K)) and torch.equal(r.exponents().long(), U.exponent(U.blocks_of(x).abs().amax(2)))
+    empty = Rows8.empty(R, K, "cpu")
+    assert empty.codes.shape == codes.shape and empty.scales.shape == scales.shape and empty.rows == R
+    # half a step, 2^-4 of a number, or 2^-10 of the power among the smallest
+    size = U.power(U.exponent(U.blocks_of(x).abs().amax(2))).repeat_interleave(128, 1)[:, :K]
+    assert ((r.numbers(torch.float64) - x.double()).abs() <= torch.maximum(x.double().abs() * 2.0 ** -4, size * 2.0 ** -10)).all()
+
+
+def test_the_restatement_refuses_wrong_rows():
+    """What the GPU tests hold results to, held to mistakes: a code, a power, a place of no row."""
+    x = torch.randn(40, 300, generator=torch.Generator().manual_seed(1)).double()
+    codes, scales = U.quantised(x.float())
+    U.assert_rows_near(codes, scales, x.float().double(), 0.0)
+    wrong = codes.clone().view(torch.uint8)
+    wrong[7, 200] ^= 8
+    with pytest.raises(AssertionError):
+        U.assert_rows_near(wrong.view(torch.float8_e4m3fn), scales, x.float().double(), 0.0)
+    for at in [(0, 0, 3, 0, 1), (0, 0, 20, 1, 0), (0, 0, 0, 0, 3)]:
+        wrong = scales.clone()
+        wrong[at] += 1
+        with pytest.raises(AssertionError):
+            U.assert_rows_near(codes, wrong, x.float().double(), 0.0)
