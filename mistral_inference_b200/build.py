@@ -116,7 +116,7 @@ ROWS8_LIB = PKG / "libmb200_rows8.so"
 
 def build_rows8(force: bool = False) -> Path:
     """libmb200_rows8.so: Linears of 8-bit numbers (csrc/rows8/)."""
-    headers = ["common.cuh", "device_info.cuh", "epilogue.cuh", "sigmoid.cuh", "gemm_tcgen05.cuh", "gemm_mma.cuh", "split_schedule.cuh", "decode_megakernel.cuh", "paged/paged_common.cuh"]
+    headers = ["common.cuh", "device_info.cuh", "epilogue.cuh", "sigmoid.cuh", "gemm_tcgen05.cuh", "gemm_mma.cuh", "split_schedule.cuh", "decode_megakernel.cuh", "gemm_pair.cuh", "paged/paged_common.cuh"]
     return _build_small(ROWS8_SRC, ROWS8_LIB, [CSRC / h for h in headers] + [INCLUDE / h for h in ("mistral_b200.h", "mistral_b200_paged.h", "mistral_b200_rows8.h")], force=force)
 
 

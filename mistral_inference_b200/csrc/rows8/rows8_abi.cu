@@ -1,5 +1,6 @@
 // libmb200_rows8.so -- the C ABI declared in include/mistral_b200_rows8.h.  Argument checking + kernel dispatch only.
 #include "rows8_quantise.cuh"
+#include "rows8_pair.cuh"
 #include "rows8_tile.cuh"
 
 namespace mb200 {
@@ -23,14 +24,18 @@ static int check_numbers(const char* what, const void* x, int dtype, int64_t ld,
   return MB200_OK;
 }
 
+template <int OUT>
+static int product(const ProductParams& p, const void* xc, const void* xs, const void* wc, const void* ws, cudaStream_t st) {
+  return p.T > 128 ? launch_rows8_pair<OUT>(p, xc, xs, wc, ws, st) : launch_rows8_tile<OUT>(p, xc, xs, wc, ws, st);
+}
 static int product(const char* what, int form, ProductParams p, const void* xc, const void* xs, const void* wc, const void* ws, cudaStream_t st) {
   int rc = check_rows(what, xc, xs);
   if (!rc) rc = check_rows(what, wc, ws);
   if (rc) return rc;
   switch (form) {
-    case R8_OUT_BF16: return launch_rows8_tile<R8_OUT_BF16>(p, xc, xs, wc, ws, st);
-    case R8_OUT_F32: return launch_rows8_tile<R8_OUT_F32>(p, xc, xs, wc, ws, st);
-    default: return launch_rows8_tile<R8_OUT_GATE>(p, xc, xs, wc, ws, st);
+    case R8_OUT_BF16: return product<R8_OUT_BF16>(p, xc, xs, wc, ws, st);
+    case R8_OUT_F32: return product<R8_OUT_F32>(p, xc, xs, wc, ws, st);
+    default: return product<R8_OUT_GATE>(p, xc, xs, wc, ws, st);
   }
 }
 }  // namespace mb200

@@ -1,0 +1,257 @@
+// Products of 8-bit rows for prompts: pairs of CTAs share MMAs (cta_group::2), 256 tokens x 256 features a tile, persistent.
+//
+// Bound by the tensor pipe under the power cap.  A k-block of 128 takes the pair 512 clocks; each CTA copies 128 token rows and 128 feature rows of it, 32 KB, where a CTA
+// by itself would copy 48 KB for the same products: L2 gives an SM some 64 bytes a clock.  Tokens are the MMA's rows (lanes), features its columns, so that a thread has a
+// token's features next to one another and, of gated units, half of a block of 128 that share a power.
+//
+// Two accumulators of 256 columns and the scales' 12 do not fit the 512 columns of tensor memory: the second accumulator begins 16 columns inside the first.  An epilogue reads
+// these first and says so (overlap), and the next tile's MMAs begin: some hundred clocks of a tile's 512 k-blocks.
+// Warps: 0 copies, 1 multiplies (in the first CTA, for both), 2-9 epilogue, two to a quarter of the lanes, each 128 columns.  Waits are bounded; results of a tile whose wait ran out are NaN.
+#pragma once
+#include "../gemm_pair.cuh"
+#include "rows8_tile.cuh"
+
+namespace mb200 {
+
+constexpr int RP_ROWS = 256, RP_COLS = 256, RP_EPI_WARPS = 8, RP_THREADS = 64 + 32 * RP_EPI_WARPS;
+constexpr int RP_HALF = 128 * R8_BLOCK, RP_STAGE = 2 * RP_HALF + 2048 /* 3 * R8_TILE of scales; stages start on 1024 bytes */, RP_STAGES = 6;
+constexpr int RP_SMEM = RP_STAGES * RP_STAGE + 1024;
+constexpr uint32_t RP_SECOND = 240, RP_SCALES_X = 496, RP_SCALES_W = 500;
+
+__device__ __forceinline__ void umma_mx8_pair(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b64 da, db;\n"
+      "mov.b64 da, {%1, %7};\n"
+      "mov.b64 db, {%2, %7};\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %3, [%4], [%5], p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "n"(UMMA_DESC_HI)
+      : "memory");
+}
+// copy_scales in both CTAs, each from its own shared memory at this offset
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint32_t smem_addr) {
+  asm volatile(
+      "{\n"
+      ".reg .b64 d;\n"
+      "mov.b64 d, {%1, %2};\n"
+      "tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n"
+      "}\n" ::"r"(taddr),
+      "r"((smem_addr & 0x3ffff) >> 4), "n"(R8_SCALE_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)), "l"(map), "r"(bar),
+               "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+
+template <int OUT>
+__global__ void __launch_bounds__(RP_THREADS, 1) rows8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sx,
+                                                                   const __grid_constant__ CUtensorMap map_sw, const __grid_constant__ ProductParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[RP_STAGES], empty[RP_STAGES], tmem_full[2], tmem_empty[2], overlap;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int gave_up;
+  __shared__ uint32_t meet[2][2][128];  // largest magnitudes of half a block of units
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_ctarank(), cluster = (int)blockIdx.x >> 1, clusters = (int)gridDim.x >> 1;
+  const int num_m = (p.T + RP_ROWS - 1) / RP_ROWS, num_n = (p.N + RP_COLS - 1) / RP_COLS, num_k = (p.K + R8_BLOCK - 1) / R8_BLOCK, tiles = num_m * num_n;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RP_STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&tmem_full[i], 1), mbar_init(&tmem_empty[i], 2 * RP_EPI_WARPS);
+    mbar_init(&overlap, RP_EPI_WARPS);  // the warps of one half of the columns, in both CTAs
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc<2>(&tmem_slot, 512);
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+  TileWalk walk;
+  walk.start(num_m, num_n);
+  int at = 0;
+  auto go_to = [&](int tile) {
+    walk.advance(tile - at, num_m, num_n);
+    at = tile;
+  };
+  auto waited = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bounded_wait(bar, parity, &gave_up)) != 0; };
+
+  if (warp == 0) {
+    const uint32_t full_first = cluster_first(full);
+    uint32_t s = 0, par = 0, issued = 0;
+    bool fine = true;
+    for (int tile = cluster; tile < tiles && fine; tile += clusters) {
+      go_to(tile);
+      const int t0 = walk.m() * RP_ROWS + rank * 128, n0 = walk.n() * RP_COLS;
+      for (int kb = 0; kb < num_k; ++kb) {
+        fine = waited(&empty[s], par ^ 1);
+        if (!fine) break;
+        if (elect_one()) {
+          const bool scales = (kb & 3) == 0;
+          uint8_t* const st = smem + s * RP_STAGE;
+          const uint32_t bar = full_first + s * 8u;
+          // both CTAs' copies count on the first one's barrier (the other's may land before it is armed: the count goes negative)
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (2 * RP_HALF + (scales ? 3 * R8_TILE : 0)));
+          tma_load_2d_pair(st, &map_x, bar, kb * R8_BLOCK, t0);
+          tma_load_2d_pair(st + RP_HALF, &map_w, bar, kb * R8_BLOCK, n0 + rank * 128);
+          if (scales) {
+            tma_load_3d_pair(st + 2 * RP_HALF, &map_sx, bar, 0, kb >> 2, t0 >> 7);
+            tma_load_3d_pair(st + 2 * RP_HALF + R8_TILE, &map_sw, bar, 0, kb >> 2, n0 >> 7);
+          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == RP_STAGES) s = 0, par ^= 1;
+      }
+    }
+    if (gave_up && rank == 0)  // the copies land before the CTAs leave
+      for (uint32_t i = issued > RP_STAGES ? issued - RP_STAGES : 0; i < issued; ++i) {
+        int zero = 0;
+        bounded_wait(&full[i % RP_STAGES], (i / RP_STAGES) & 1, &zero);
+      }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t ring = umma_desc_lo(smem_u32(smem)), sx = tmem + RP_SCALES_X, sw = tmem + RP_SCALES_W;
+      uint32_t s = 0, par = 0, nth = 0;
+      bool fine = true;
+      for (int tile = cluster; tile < tiles && fine; tile += clusters, ++nth) {
+        const uint32_t acc = nth & 1, d = tmem + acc * RP_SECOND;
+        fine = waited(&tmem_empty[acc], ((nth >> 1) & 1) ^ 1) && (nth == 0 || waited(&overlap, (nth - 1) & 1));
+        if (!fine) break;
+        for (int kb = 0; kb < num_k; ++kb) {
+          fine = waited(&full[s], par);
+          if (!fine) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t a = ring + s * (RP_STAGE >> 4), b = a + (RP_HALF >> 4);
+            if ((kb & 3) == 0) {
+              const uint32_t src = smem_u32(smem) + s * RP_STAGE + 2 * RP_HALF;
+              copy_scales_pair(sx, src);
+              copy_scales_pair(sw, src + R8_TILE);
+              copy_scales_pair(sw + 4, src + 2 * R8_TILE);
+            }
+            const uint32_t idesc = r8_idesc(RP_ROWS, RP_COLS, kb & 3);
+            umma_mx8_pair(d, a, b, idesc, sx, sw, kb > 0 ? 1u : 0u);
+#pragma unroll
+            for (int k = 1; k < 4; ++k) umma_mx8_pair(d, a + 2 * k, b + 2 * k, idesc, sx, sw, 1u);
+            umma_commit_pair(&empty[s]);
+            if (kb == num_k - 1) umma_commit_pair(&tmem_full[acc]);
+          }
+          __syncwarp();
+          if (++s == RP_STAGES) s = 0, par ^= 1;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+    uint32_t nth = 0;
+    bool fine = true;
+    for (int tile = cluster; tile < tiles; tile += clusters, ++nth) {
+      go_to(tile);
+      const int64_t t = (int64_t)walk.m() * RP_ROWS + rank * 128 + row;
+      const int n0 = walk.n() * RP_COLS;
+      const uint32_t acc = nth & 1, from = tmem + ((uint32_t)(quarter * 32) << 16) + acc * RP_SECOND;
+      fine = fine && waited(&tmem_full[acc], (nth >> 1) & 1);
+      tc_fence_after();
+      // blocks of 32 columns 0, 1, 2, 3 or 7, 6, 5, 4: the columns that both accumulators have come first
+      auto column = [&](int c) { return half ? 7 - c : c; };
+      auto read = [&](int c, uint32_t(&v)[32]) {
+        if (fine) {
+          tmem_ld_32x32b_x32(from + 32 * column(c), v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0x7fffffffu;
+        }
+        const bool shared = c == 0 && half == (acc ? 0 : 1);
+        if (shared || c == 3) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (shared) mbar_arrive_cluster(cluster_first(&overlap));
+            if (c == 3) mbar_arrive_cluster(cluster_first(&tmem_empty[acc]));
+          }
+        }
+      };
+      if constexpr (OUT != R8_OUT_GATE) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          read(c, v);
+          const int n = n0 + 32 * column(c);
+          if (t < p.T && n < p.N) r8_store32<OUT>(p, t, n, v);
+        }
+      } else {
+        float g[4][16];
+        uint32_t amax = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          read(c, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            g[c][i] = silu_times(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            amax = max(amax, r8_bits(g[c][i]));
+          }
+        }
+        meet[acc][half][row] = amax;
+        asm volatile("bar.sync %0, 64;" ::"r"(4 + quarter) : "memory");
+        amax = max(amax, meet[acc][half ^ 1][row]);
+        const uint32_t byte = r8_byte(amax);
+        const int block = n0 / RP_COLS;
+        if (t < p.T) {
+          uint4* to = reinterpret_cast<uint4*>(p.codes + t * p.width + (int64_t)block * R8_BLOCK);
+          const float inverse = r8_inverse(byte);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) to[column(c)] = r8_codes16(g[c], amax, inverse);
+        }
+        if (half == 0 && t < ((p.T + 127) & ~127)) {
+          uint8_t* sc = p.scales + r8_scale_at(t, block >> 2, p.quads);
+          sc[block & 3] = (uint8_t)(t < p.T ? byte : 127u);
+          if (block == num_n - 1)
+            for (int b = (block & 3) + 1; b < 4; ++b) sc[b] = 127;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // nobody leaves while the other's copies, commits or arrivals may reach it
+  if (warp == 1) tmem_dealloc<2>(tmem, 512);
+}
+
+// ---- host ----
+template <int OUT>
+int launch_rows8_pair(const ProductParams& p, const void* xc, const void* xs, const void* wc, const void* ws, cudaStream_t st) {
+  CUtensorMap mx, mw, msx, msw;
+  const int64_t width = r8_width(p.K), quads = r8_quads(p.K);
+  int rc = r8_code_map(&mx, xc, p.T, width, 128);
+  if (!rc) rc = r8_code_map(&mw, wc, p.N, width, 128);
+  if (!rc) rc = r8_scale_map(&msx, xs, p.T, quads, 1);
+  if (!rc) rc = r8_scale_map(&msw, ws, p.N, quads, 2);
+  if (rc) return rc;
+  const int64_t tiles = (int64_t)((p.N + RP_COLS - 1) / RP_COLS) * ((p.T + RP_ROWS - 1) / RP_ROWS), pairs = device_info::sm_count() / 2;
+  MB_CHECK_ARG(tiles < (1 << 30), "product: %lld tiles", (long long)tiles);
+  MB_CHECK_CUDA(device_info::allow_shared<rows8_pair_kernel<OUT>>(RP_SMEM));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs));
+  cfg.blockDim = dim3(RP_THREADS);
+  cfg.dynamicSmemBytes = RP_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute a[2];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = 2;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  a[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = a;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  MB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, rows8_pair_kernel<OUT>, mx, mw, msx, msw, p));
+  return MB200_OK;
+}
+
+}  // namespace mb200
