@@ -24,8 +24,8 @@ _SIGNATURES = {
     "mb8_last_error": (c_char_p, []),
     "mb8_quantise": (c_int, [P, I, c_int, P, P, I, I, P]),
     "mb8_norm": (c_int, [P, I, P, I, P, c_int, P, P, P, I, I, c_float, P]),
-    "mb8_multiply": (c_int, [P, P, P, P, P, I, c_int, I, I, I, P]),
-    "mb8_gate": (c_int, [P, P, P, P, P, P, I, I, I, P]),
+    "mb8_multiply": (c_int, [P, P, P, P, P, I, c_int, I, I, I, c_int, P]),
+    "mb8_gate": (c_int, [P, P, P, P, P, P, I, I, I, c_int, P]),
 }
 
 

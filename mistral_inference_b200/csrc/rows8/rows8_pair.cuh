@@ -9,7 +9,7 @@
 // Warps: 0 copies, 1 multiplies (in the first CTA, for both), 2-9 epilogue, two to a quarter of the lanes, each 128 columns.  Waits are bounded; results of a tile whose wait ran out are NaN.
 #pragma once
 #include "../gemm_pair.cuh"
-#include "rows8_tile.cuh"
+#include "rows8_product.cuh"
 
 namespace mb200 {
 

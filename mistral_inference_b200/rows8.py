@@ -32,6 +32,7 @@ class Rows8:
     codes: torch.Tensor   # [rows, cols rounded up to 128] float8_e4m3fn, zeros behind a row's end
     scales: torch.Tensor  # [ceil(rows / 128), ceil(cols / 512), 32, 4, 4] float8_e8m0fnu: row 32 j + i and block c of a tile at [i, j, c]; 1 where there is no row or block
     cols: int
+    fixed: bool = False   # everything that ever wrote it has ended (a loaded model's weights): products may read it before their turn on their stream
 
     @property
     def rows(self) -> int:
@@ -112,7 +113,7 @@ def multiply_rows(x: Rows8, w: Rows8, dtype: torch.dtype = torch.bfloat16, out: 
     else:
         assert out.shape == (T, N) and _check_numbers(out, "out") == dev, f"out [{T}, {N}]"
     _abi_rows8.call("mb8_multiply", dev, x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), out.stride(0), 1 if out.dtype is _F32 else 0, T, N,
-                    x.cols)
+                    x.cols, w.fixed)
     return out
 
 
@@ -122,5 +123,5 @@ def gate_rows(x: Rows8, w13: Rows8) -> Rows8:
     assert _check_rows8(w13, "w13") == dev and x.cols == w13.cols and w13.rows >= 2 and w13.rows % 2 == 0, f"pairs of rows of one length on one device, got {x.cols} and {w13.rows} of {w13.cols}"
     T, H = x.rows, w13.rows // 2
     out = Rows8.empty(T, H, x.codes.device)
-    _abi_rows8.call("mb8_gate", dev, x.codes.data_ptr(), x.scales.data_ptr(), w13.codes.data_ptr(), w13.scales.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), T, H, x.cols)
+    _abi_rows8.call("mb8_gate", dev, x.codes.data_ptr(), x.scales.data_ptr(), w13.codes.data_ptr(), w13.scales.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), T, H, x.cols, w13.fixed)
     return out
