@@ -60,12 +60,11 @@ int mb8_quantise(const void* x, int64_t ld, int dtype, void* codes, void* scales
   p.x = x;
   p.codes = (uint8_t*)codes;
   p.scales = (uint8_t*)scales;
-  p.T = T;
-  p.K = K;
+  p.T = (int)T;
+  p.K = (int)K;
   p.ld = ld;
-  p.width = r8_width(K);
+  p.width = (int)r8_width(K);
   p.quads = (int)r8_quads(K);
-  MB_CHECK_ARG(T * p.quads <= (int64_t)0x7fffffff * RQ_WARPS, "quantise: %lld rows of %lld entries", (long long)T, (long long)K);
   return dtype == 0 ? launch_rows8_quantise<bf16>(p, (cudaStream_t)stream) : launch_rows8_quantise<float>(p, (cudaStream_t)stream);
 }
 
@@ -88,11 +87,11 @@ int mb8_norm(const void* x, int64_t ld, const void* add, int64_t ld_add, const v
   p.stream = h_out;
   p.codes = (uint8_t*)codes;
   p.scales = (uint8_t*)scales;
-  p.T = T;
-  p.K = K;
+  p.T = (int)T;
+  p.K = (int)K;
   p.ld = ld;
   p.ld_add = ld_add;
-  p.width = r8_width(K);
+  p.width = (int)r8_width(K);
   p.quads = (int)r8_quads(K);
   p.eps = eps;
   return dtype == 0 ? launch_rows8_norm<bf16>(p, (cudaStream_t)stream) : launch_rows8_norm<float>(p, (cudaStream_t)stream);

@@ -25,14 +25,30 @@ __device__ __forceinline__ uint32_t r8_byte(uint32_t amax_bits) { return amax_bi
 __device__ __forceinline__ float r8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }  // (27 <= byte <= 247)
 
 // 16 numbers, |x| <= 448 after the scale, as codes; all NaN where the block's largest magnitude is no number
-__device__ __forceinline__ uint4 r8_codes16(const float (&v)[16], uint32_t amax_bits, float inverse) {
+__device__ __forceinline__ uint4 r8_codes16(const uint64_t (&v)[8], uint32_t amax_bits) {
+  const float inverse = r8_inverse(r8_byte(amax_bits));
+  const uint64_t scale = pair(inverse, inverse);
   uint32_t c[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    c[j] = to_e4m3x2(v[4 * j] * inverse, v[4 * j + 1] * inverse) | to_e4m3x2(v[4 * j + 2] * inverse, v[4 * j + 3] * inverse) << 16;
+  for (int j = 0; j < 4; ++j) {
+    const float2 x = unpair(mul_pair(v[2 * j], scale)), y = unpair(mul_pair(v[2 * j + 1], scale));
+    c[j] = to_e4m3x2(x.x, x.y) | to_e4m3x2(y.x, y.y) << 16;
+  }
   return amax_bits < 0x7f800000u ? make_uint4(c[0], c[1], c[2], c[3]) : make_uint4(R8_ONES, R8_ONES, R8_ONES, R8_ONES);  // (e4m3's NaN is 0x7f)
 }
+__device__ __forceinline__ uint4 r8_codes16(const float (&v)[16], uint32_t amax_bits) {
+  uint64_t w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = pair(v[2 * j], v[2 * j + 1]);
+  return r8_codes16(w, amax_bits);
+}
 __device__ __forceinline__ uint32_t r8_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }  // (as whole numbers magnitudes order like their values, infinity and NaN above all)
+// the largest of a and two numbers' magnitudes; NaN where one is
+__device__ __forceinline__ float r8_larger(float a, float x, float y) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(x), "f"(y));
+  return r;
+}
 
 // 2-D map of codes [rows][width] with boxes of box_rows x 128, 128-byte swizzle
 inline int r8_code_map(CUtensorMap* map, const void* codes, int64_t rows, int64_t width, int box_rows) {

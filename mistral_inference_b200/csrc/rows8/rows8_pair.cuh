@@ -206,9 +206,8 @@ __global__ void __launch_bounds__(RP_THREADS, 1) rows8_pair_kernel(const __grid_
         const int block = n0 / RP_COLS;
         if (t < p.T) {
           uint4* to = reinterpret_cast<uint4*>(p.codes + t * p.width + (int64_t)block * R8_BLOCK);
-          const float inverse = r8_inverse(byte);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) to[column(c)] = r8_codes16(g[c], amax, inverse);
+          for (int c = 0; c < 4; ++c) to[column(c)] = r8_codes16(g[c], amax);
         }
         if (half == 0 && t < ((p.T + 127) & ~127)) {
           uint8_t* sc = p.scales + r8_scale_at(t, block >> 2, p.quads);

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
           float g[16];
           sixteen(t, g);
           const uint32_t a = most[t];
-          *reinterpret_cast<uint4*>(p.o.codes + (int64_t)t * p.o.width + n0 / 2 + 16 * k) = r8_codes16(g, a, r8_inverse(r8_byte(a)));
+          *reinterpret_cast<uint4*>(p.o.codes + (int64_t)t * p.o.width + n0 / 2 + 16 * k) = r8_codes16(g, a);
         }
         if (part == 0 && !(tile & 1)) {  // a row of the scales' tile a thread
           uint8_t* sc = p.o.scales + r8_scale_at(id, block >> 2, p.o.quads);
