@@ -32,14 +32,17 @@ int mb8_norm(const void* x, int64_t ld, const void* add, int64_t ld_add, const v
              void* stream);
 
 /* Products.  w_fixed: 0, or 1 where everything that ever wrote w has ended (as a loaded model's weights): then w may be read before the call's turn on its stream.
- *
- * out [T, N] (dtype 0 bf16, 1 fp32; rows ld elements apart) = x [T, K] times w [N, K] transposed, summed in fp32. */
+ * scratch: mb8_product_scratch(T, rows of w, K) bytes on 16, for the call alone (0: NULL).
+ */
+int64_t mb8_product_scratch(int64_t T, int64_t N, int64_t K); /* on the current device */
+
+/* out [T, N] (dtype 0 bf16, 1 fp32; rows ld elements apart) = x [T, K] times w [N, K] transposed, summed in fp32. */
 int mb8_multiply(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int64_t ld, int dtype, int64_t T, int64_t N, int64_t K, int w_fixed,
-                 void* stream);
+                 void* scratch, int64_t scratch_bytes, void* stream);
 
 /* Rows [T, H] of silu(y[2 i]) * y[2 i + 1], y = x [T, K] times w [2 H, K] transposed. */
 int mb8_gate(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* codes, void* scales, int64_t T, int64_t H, int64_t K, int w_fixed,
-             void* stream);
+             void* scratch, int64_t scratch_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -4,6 +4,7 @@ Same rules as `_abi`: the only place Python touches this library, and no fallbac
 in-tree by `build.build_rows8()` (a fresh checkout has no binaries), a failing call raises.
 """
 import ctypes
+import functools
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 from typing import Optional
 
@@ -24,8 +25,9 @@ _SIGNATURES = {
     "mb8_last_error": (c_char_p, []),
     "mb8_quantise": (c_int, [P, I, c_int, P, P, I, I, P]),
     "mb8_norm": (c_int, [P, I, P, I, P, c_int, P, P, P, I, I, c_float, P]),
-    "mb8_multiply": (c_int, [P, P, P, P, P, I, c_int, I, I, I, c_int, P]),
-    "mb8_gate": (c_int, [P, P, P, P, P, P, I, I, I, c_int, P]),
+    "mb8_product_scratch": (I, [I, I, I]),
+    "mb8_multiply": (c_int, [P, P, P, P, P, I, c_int, I, I, I, c_int, P, I, P]),
+    "mb8_gate": (c_int, [P, P, P, P, P, P, I, I, I, c_int, P, I, P]),
 }
 
 
@@ -58,3 +60,20 @@ def call(name: str, device: int, *args) -> None:
     if rc != 0:
         msg = lib().mb8_last_error()
         raise Mb200Error(f"{name} failed ({rc}): {msg.decode() if msg else '?'}")
+
+
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(device: int, T: int, N: int, K: int) -> int:
+    """How a product is cut goes by its device's SMs: the same device is asked that the call will run on."""
+    with torch.cuda.device(device):
+        return lib().mb8_product_scratch(T, N, K)
+
+
+STREAM_TOKENS = 128  # up to so many tokens a product needs no scratch
+
+
+def product(name: str, device: int, x, w, out: tuple, T: int, N: int, n: int) -> None:
+    """mb8_multiply or mb8_gate of x [T, K] and w [N, K]; n: what the entry point counts its results by."""
+    need = _scratch_bytes(device, T, N, x.cols) if T > STREAM_TOKENS else 0
+    scratch = x.codes.new_empty(need) if need else None
+    call(name, device, x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), *out, T, n, x.cols, w.fixed, None if scratch is None else scratch.data_ptr(), need)

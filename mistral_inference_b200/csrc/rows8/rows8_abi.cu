@@ -26,19 +26,20 @@ static int check_numbers(const char* what, const void* x, int dtype, int64_t ld,
 }
 
 template <int OUT>
-static int product(const ProductParams& p, const void* xc, const void* xs, const void* wc, const void* ws, bool fixed, cudaStream_t st) {
+static int product(const ProductParams& p, const void* xc, const void* xs, const void* wc, const void* ws, bool fixed, void* scratch, int64_t scratch_bytes, cudaStream_t st) {
   const int sms = device_info::sm_count();
-  MB_CHECK_ARG(sms > 0, "product: the device does not say how many SMs it has");
-  return p.T <= RS_MAX_T ? launch_rows8_stream<OUT>(p, xc, xs, wc, ws, fixed, sms, st) : launch_rows8_pair<OUT>(p, xc, xs, wc, ws, st);
+  MB_CHECK_ARG(sms > 1, "product: the device does not say how many SMs it has");
+  return p.T <= RS_MAX_T ? launch_rows8_stream<OUT>(p, xc, xs, wc, ws, fixed, sms, st) : launch_rows8_pair<OUT>(p, xc, xs, wc, ws, scratch, scratch_bytes, sms, st);
 }
-static int product(const char* what, int form, const ProductParams& p, const void* xc, const void* xs, const void* wc, const void* ws, int fixed, cudaStream_t st) {
+static int product(const char* what, int form, const ProductParams& p, const void* xc, const void* xs, const void* wc, const void* ws, int fixed, void* scratch, int64_t scratch_bytes,
+                   cudaStream_t st) {
   int rc = check_rows(what, xc, xs);
   if (!rc) rc = check_rows(what, wc, ws);
   if (rc) return rc;
   switch (form) {
-    case R8_OUT_BF16: return product<R8_OUT_BF16>(p, xc, xs, wc, ws, fixed != 0, st);
-    case R8_OUT_F32: return product<R8_OUT_F32>(p, xc, xs, wc, ws, fixed != 0, st);
-    default: return product<R8_OUT_GATE>(p, xc, xs, wc, ws, fixed != 0, st);
+    case R8_OUT_BF16: return product<R8_OUT_BF16>(p, xc, xs, wc, ws, fixed != 0, scratch, scratch_bytes, st);
+    case R8_OUT_F32: return product<R8_OUT_F32>(p, xc, xs, wc, ws, fixed != 0, scratch, scratch_bytes, st);
+    default: return product<R8_OUT_GATE>(p, xc, xs, wc, ws, fixed != 0, scratch, scratch_bytes, st);
   }
 }
 }  // namespace mb200
@@ -97,8 +98,13 @@ int mb8_norm(const void* x, int64_t ld, const void* add, int64_t ld_add, const v
   return dtype == 0 ? launch_rows8_norm<bf16>(p, (cudaStream_t)stream) : launch_rows8_norm<float>(p, (cudaStream_t)stream);
 }
 
+int64_t mb8_product_scratch(int64_t T, int64_t N, int64_t K) {
+  const int sms = device_info::sm_count();
+  return T <= RS_MAX_T || N < 1 || K < 1 || sms < 2 ? 0 : rows8_pair_scratch(T, N, K, sms);
+}
+
 int mb8_multiply(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int64_t ld, int dtype, int64_t T, int64_t N, int64_t K, int w_fixed,
-                 void* stream) {
+                 void* scratch, int64_t scratch_bytes, void* stream) {
   int rc = check_sizes("multiply", T, N, K);
   if (rc || T == 0) return rc;
   rc = check_numbers("multiply", out, dtype, ld, T, N);
@@ -109,11 +115,11 @@ int mb8_multiply(const void* x_codes, const void* x_scales, const void* w_codes,
   p.K = (int)K;
   p.ld = ld;
   p.out = out;
-  return product("multiply", dtype, p, x_codes, x_scales, w_codes, w_scales, w_fixed, (cudaStream_t)stream);
+  return product("multiply", dtype, p, x_codes, x_scales, w_codes, w_scales, w_fixed, scratch, scratch_bytes, (cudaStream_t)stream);
 }
 
 int mb8_gate(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* codes, void* scales, int64_t T, int64_t H, int64_t K, int w_fixed,
-             void* stream) {
+             void* scratch, int64_t scratch_bytes, void* stream) {
   int rc = check_sizes("gate", T, 2 * H, K);
   if (rc || T == 0) return rc;
   rc = check_rows("gate", codes, scales);
@@ -126,7 +132,7 @@ int mb8_gate(const void* x_codes, const void* x_scales, const void* w_codes, con
   p.scales = (uint8_t*)scales;
   p.width = (int)r8_width(H);
   p.quads = (int)r8_quads(H);
-  return product("gate", R8_OUT_GATE, p, x_codes, x_scales, w_codes, w_scales, w_fixed, (cudaStream_t)stream);
+  return product("gate", R8_OUT_GATE, p, x_codes, x_scales, w_codes, w_scales, w_fixed, scratch, scratch_bytes, (cudaStream_t)stream);
 }
 
 }  // extern "C"

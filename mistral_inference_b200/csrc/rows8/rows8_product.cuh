@@ -56,29 +56,65 @@ __device__ __forceinline__ float silu_times(float gate, float up) {  // within 2
   return gate * r * up;
 }
 
-// 32 features n .. of token t
+// A warp's 32 rows of 64 bytes to memory, lane's row in `own`: turned in `turn` (2 KB of the warp's), so that an instruction writes 8 rows of 64 bytes and not 32 of 16, which took an
+// epilogue of 256 x 256 8000 clocks.  row0: the first lane's row, `rows` of them exist, ld bytes apart.
+__device__ __forceinline__ void r8_store_turned(uint8_t* turn, const uint4 (&own)[4], uint8_t* row0, int64_t ld, int rows) {
+  const int lane = threadIdx.x & 31;
+  uint4* const t = reinterpret_cast<uint4*>(turn);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[lane * 4 + (i ^ ((lane >> 1) & 3))] = own[i];  // (eight lanes' units meet no bank twice)
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2), u = lane & 3;
+    const uint4 v = t[r * 4 + (u ^ ((r >> 1) & 3))];
+    if (r < rows) *reinterpret_cast<uint4*>(row0 + r * ld + u * 16) = v;
+  }
+  __syncwarp();
+}
+// 32 features n .. of a warp's 32 tokens, lane's token t0 + lane
 template <int OUT>
-__device__ __forceinline__ void r8_store32(const ProductParams& p, int64_t t, int n, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void r8_store32(const ProductParams& p, uint8_t* turn, int64_t t0, int n, const uint32_t (&v)[32]) {
   using O = std::conditional_t<OUT == R8_OUT_F32, float, bf16>;
-  O* to = reinterpret_cast<O*>(p.out) + t * p.ld + n;
-  if (n + 32 <= p.N && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+  const int lane = threadIdx.x & 31, rows = (int)min((int64_t)32, p.T - t0);
+  O* const to = reinterpret_cast<O*>(p.out) + t0 * p.ld + n;
+  if (rows <= 0 || n >= p.N) return;
+  if (n + 32 <= p.N && (reinterpret_cast<uintptr_t>(to) & 15) == 0 && (rows == 1 || p.ld * sizeof(O) % 16 == 0)) {
     if constexpr (OUT == R8_OUT_F32) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      for (int h = 0; h < 2; ++h) {
+        uint4 own[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) own[i] = make_uint4(v[16 * h + 4 * i], v[16 * h + 4 * i + 1], v[16 * h + 4 * i + 2], v[16 * h + 4 * i + 3]);
+        r8_store_turned(turn, own, reinterpret_cast<uint8_t*>(to + 16 * h), p.ld * sizeof(O), rows);
+      }
     } else {
+      uint4 own[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(__uint_as_float(v[8 * i + 2 * j]), __uint_as_float(v[8 * i + 2 * j + 1]));
-        reinterpret_cast<uint4*>(to)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 4; ++j) w[j] = pack2_rn(__uint_as_float(v[8 * i + 2 * j]), __uint_as_float(v[8 * i + 2 * j + 1]));
+        own[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      r8_store_turned(turn, own, reinterpret_cast<uint8_t*>(to), p.ld * sizeof(O), rows);
     }
     return;
   }
+  if (lane < rows) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (n + i < p.N) to[i] = (O)__uint_as_float(v[i]);
+    for (int i = 0; i < 32; ++i)
+      if (n + i < p.N) to[lane * p.ld + i] = (O)__uint_as_float(v[i]);
+  }
+}
+
+// The power of token t's block of gated units, `blocks` of them in all; places of no token or block of the scales' tile get 1
+__device__ __forceinline__ void r8_store_unit_scale(const ProductParams& p, int64_t t, int block, int blocks, uint32_t amax_bits) {
+  if (t >= ((p.T + 127) & ~127)) return;
+  uint8_t* sc = p.scales + r8_scale_at(t, block >> 2, p.quads);
+  sc[block & 3] = (uint8_t)(t < p.T ? r8_byte(amax_bits) : 127u);
+  if (block == blocks - 1)
+    for (int b = (block & 3) + 1; b < 4; ++b) sc[b] = 127;
 }
 
 }  // namespace mb200

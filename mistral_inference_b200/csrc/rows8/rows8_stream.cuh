@@ -258,12 +258,7 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
           const uint32_t a = most[t];
           *reinterpret_cast<uint4*>(p.o.codes + (int64_t)t * p.o.width + n0 / 2 + 16 * k) = r8_codes16(g, a);
         }
-        if (part == 0 && !(tile & 1)) {  // a row of the scales' tile a thread
-          uint8_t* sc = p.o.scales + r8_scale_at(id, block >> 2, p.o.quads);
-          sc[block & 3] = (uint8_t)(id < T ? r8_byte(most[id < T ? id : 0]) : 127u);
-          if (block == (p.o.N + 255) / 256 - 1)
-            for (int b = (block & 3) + 1; b < 4; ++b) sc[b] = 127;
-        }
+        if (part == 0 && !(tile & 1)) r8_store_unit_scale(p.o, id, block, (p.o.N + 255) / 256, id < T ? most[id] : 0);  // a row of the scales' tile a thread
       }
     }
   }

@@ -124,7 +124,7 @@ def multiply_rows(x: Rows8, w: Rows8, dtype: torch.dtype = torch.bfloat16, out: 
         out_dev, out_T, out_N, ld = _check_numbers(out, "out")
         assert out_T == T and out_N == N and out_dev == dev, f"out [{T}, {N}] on {x.codes.device}"
         dtype = out.dtype
-    _abi_rows8.call("mb8_multiply", dev, x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ld, 1 if dtype is _F32 else 0, T, N, x.cols, w.fixed)
+    _abi_rows8.product("mb8_multiply", dev, x, w, (out.data_ptr(), ld, 1 if dtype is _F32 else 0), T, N, N)
     return out
 
 
@@ -134,6 +134,5 @@ def gate_rows(x: Rows8, w13: Rows8) -> Rows8:
     w_dev, N = _check_rows8(w13, "w13")
     assert w_dev == dev and x.cols == w13.cols and N >= 2 and N % 2 == 0, f"pairs of rows of one length on one device, got {x.cols} and {N} of {w13.cols}"
     out = Rows8.empty(T, N // 2, x.codes.device)
-    _abi_rows8.call("mb8_gate", dev, x.codes.data_ptr(), x.scales.data_ptr(), w13.codes.data_ptr(), w13.scales.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), T, N // 2, x.cols,
-                    w13.fixed)
+    _abi_rows8.product("mb8_gate", dev, x, w13, (out.codes.data_ptr(), out.scales.data_ptr()), T, N, N // 2)
     return out

@@ -140,7 +140,7 @@ def random_rows(T, K, seed, std=1.0):
 
 
 SIZES = [(1, 128, 128), (1, 1, 1), (1, 6144, 4096), (2, 130, 200), (5, 1000, 513), (16, 300, 1003), (17, 256, 640), (32, 5120, 1024), (33, 257, 2000), (64, 4096, 4096), (100, 700, 900),
-         (128, 512, 512), (129, 1001, 1152), (200, 2048, 128), (256, 256, 4096), (300, 4099, 700), (513, 1536, 2048), (777, 6144, 512), (1102, 2048, 1000)]
+         (128, 512, 512), (129, 1001, 1152), (200, 2048, 128), (256, 256, 4096), (300, 4099, 700), (513, 1536, 2048), (777, 6144, 512), (1102, 2048, 1000), (777, 6144, 4096), (129, 4096, 14336), (1500, 5000, 2700)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -157,7 +157,7 @@ def test_multiply(T, N, K, dtype):
 
 
 @pytest.mark.parametrize("T,H,K", [(1, 128, 128), (1, 1, 1), (1, 14336, 4096), (3, 100, 200), (16, 700, 513), (32, 1003, 1003), (48, 640, 5120), (64, 2048, 640), (65, 64, 900), (128, 384, 512),
-                                   (129, 500, 1152), (256, 128, 4096), (300, 2050, 700), (1102, 1024, 1000)])
+                                   (129, 500, 1152), (256, 128, 4096), (300, 2050, 700), (1102, 1024, 1000), (777, 3001, 4096), (140, 14336, 2560)])
 def test_gate(T, H, K):
     x, w = random_rows(T, K, T + K), random_rows(2 * H, K, H + K, 1.5 * K ** -0.5)
     y, off = U.product(U.numbers(x.codes, x.scales, K), U.numbers(w.codes, w.scales, K))

@@ -64,14 +64,14 @@ def test_norm_is_refused(lib):
 
 def test_products_are_refused(lib):
     def multiply(xc=X, xs=X, wc=X, ws=X, out=X, ld=64, dtype=0, T=2, N=64, K=256):
-        return lib.mb8_multiply(xc, xs, wc, ws, out, ld, dtype, T, N, K, 0, None)
+        return lib.mb8_multiply(xc, xs, wc, ws, out, ld, dtype, T, N, K, 0, None, 0, None)
     for kw, why in [(dict(xc=None), "null"), (dict(xs=None), "null"), (dict(wc=None), "null"), (dict(ws=None), "null"), (dict(out=None), "null"), (dict(xc=X + 8), "16 bytes"), (dict(ws=X + 1), "16 bytes"),
                     (dict(out=X + 1), "aligned"), (dict(out=X + 2, dtype=1), "aligned"), (dict(dtype=2), "dtype"), (dict(ld=63), "apart"), (dict(T=-1), "rows"), (dict(N=0), "features"), (dict(K=0), "entries"),
                     (dict(T=BIG), "rows"), (dict(N=BIG, ld=BIG), "features"), (dict(K=BIG), "entries")]:
         assert multiply(**kw) == -1 and why in last(lib), (kw, last(lib))
 
     def gate(xc=X, xs=X, wc=X, ws=X, codes=X, scales=X, T=2, H=64, K=256):
-        return lib.mb8_gate(xc, xs, wc, ws, codes, scales, T, H, K, 0, None)
+        return lib.mb8_gate(xc, xs, wc, ws, codes, scales, T, H, K, 0, None, 0, None)
     for kw, why in [(dict(xc=None), "null"), (dict(codes=None), "null"), (dict(scales=None), "null"), (dict(codes=X + 8), "16 bytes"), (dict(T=-1), "rows"), (dict(H=0), "features"),
                     (dict(H=(1 << 23) + 1), "features"), (dict(K=0), "entries")]:
         assert gate(**kw) == -1 and why in last(lib), (kw, last(lib))
