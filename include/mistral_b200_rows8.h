@@ -44,6 +44,11 @@ int mb8_multiply(const void* x_codes, const void* x_scales, const void* w_codes,
 int mb8_gate(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* codes, void* scales, int64_t T, int64_t H, int64_t K, int w_fixed,
              void* scratch, int64_t scratch_bytes, void* stream);
 
+/* Queries and keys of qkv [T, (n_heads + 2 n_kv_heads) * 128] bf16, rotated by rope [positions, 64, 2] fp32 (cosine, sine of a pair) at positions [T], and its values: q [T, n_heads * 128],
+ * k, v [.., n_kv_heads * 128], token t in row rows[t] of them (-1: nowhere), or in row t (rows NULL). */
+int mb8_rotate(const void* qkv, const float* rope, const int32_t* positions, const int32_t* rows, void* q, void* k, void* v, int64_t T, int64_t n_heads, int64_t n_kv_heads,
+               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

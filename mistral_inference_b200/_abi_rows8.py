@@ -25,6 +25,7 @@ _SIGNATURES = {
     "mb8_last_error": (c_char_p, []),
     "mb8_quantise": (c_int, [P, I, c_int, P, P, I, I, P]),
     "mb8_norm": (c_int, [P, I, P, I, P, c_int, P, P, P, I, I, c_float, P]),
+    "mb8_rotate": (c_int, [P, P, P, P, P, P, P, I, I, I, P]),
     "mb8_product_scratch": (I, [I, I, I]),
     "mb8_multiply": (c_int, [P, P, P, P, P, I, c_int, I, I, I, c_int, P, I, P]),
     "mb8_gate": (c_int, [P, P, P, P, P, P, I, I, I, c_int, P, I, P]),
@@ -77,3 +78,12 @@ def product(name: str, device: int, x, w, out: tuple, T: int, N: int, n: int) ->
     need = _scratch_bytes(device, T, N, x.cols) if T > STREAM_TOKENS else 0
     scratch = x.codes.new_empty(need) if need else None
     call(name, device, x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), *out, T, n, x.cols, w.fixed, None if scratch is None else scratch.data_ptr(), need)
+
+
+def rotate(qkv, rope, positions, rows, q, k, v, n_heads: int, n_kv_heads: int) -> None:
+    """Behind the model's own product: tensors as the model makes them, contiguous and of one device."""
+    for t in (qkv, rope, positions, q, k, v):
+        assert t.get_device() == qkv.get_device() and t.is_contiguous(), "contiguous tensors of one device"
+    assert rows is None or (rows.get_device() == qkv.get_device() and rows.is_contiguous())
+    call("mb8_rotate", qkv.get_device(), qkv.data_ptr(), rope.data_ptr(), positions.data_ptr(), None if rows is None else rows.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), qkv.shape[0],
+         n_heads, n_kv_heads)

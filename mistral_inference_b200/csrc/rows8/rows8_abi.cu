@@ -1,6 +1,7 @@
 // libmb200_rows8.so -- the C ABI declared in include/mistral_b200_rows8.h.  Argument checking + kernel dispatch only.
 #include "rows8_quantise.cuh"
 #include "rows8_pair.cuh"
+#include "rows8_rotate.cuh"
 #include "rows8_stream.cuh"
 #include "rows8_product.cuh"
 
@@ -133,6 +134,29 @@ int mb8_gate(const void* x_codes, const void* x_scales, const void* w_codes, con
   p.width = (int)r8_width(H);
   p.quads = (int)r8_quads(H);
   return product("gate", R8_OUT_GATE, p, x_codes, x_scales, w_codes, w_scales, w_fixed, scratch, scratch_bytes, (cudaStream_t)stream);
+}
+
+int mb8_rotate(const void* qkv, const float* rope, const int32_t* positions, const int32_t* rows, void* q, void* k, void* v, int64_t T, int64_t n_heads, int64_t n_kv_heads,
+               void* stream) {
+  MB_CHECK_ARG(T >= 0 && T <= MB8_MAX_ROWS && n_heads >= 1 && n_kv_heads >= 1 && n_heads + 2 * n_kv_heads <= 65536, "rotate: %lld tokens, %lld + 2 * %lld heads", (long long)T,
+               (long long)n_heads, (long long)n_kv_heads);
+  if (T == 0) return MB200_OK;
+  MB_CHECK_ARG(qkv && rope && positions && q && k && v, "rotate: null pointer");
+  MB_CHECK_ARG(((uintptr_t)qkv | (uintptr_t)rope | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "rotate: matrices start on 16 bytes");
+  RotateParams p;
+  p.qkv = (const uint4*)qkv;
+  p.rope = (const float4*)rope;
+  p.positions = positions;
+  p.rows = rows;
+  p.q = (uint4*)q;
+  p.k = (uint4*)k;
+  p.v = (uint4*)v;
+  p.T = (int)T;
+  p.H = (int)n_heads;
+  p.KV = (int)n_kv_heads;
+  const int threads = (p.H + 2 * p.KV) * 16;
+  MB_CHECK_CUDA(launch_pdl(rows8_rotate_kernel, dim3((unsigned)T, (unsigned)((threads + RR_THREADS - 1) / RR_THREADS)), dim3(RR_THREADS), 0, (cudaStream_t)stream, p));
+  return MB200_OK;
 }
 
 }  // extern "C"

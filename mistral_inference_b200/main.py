@@ -20,6 +20,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     g.add_argument("--chunk-size", type=int, default=None)
     g.add_argument("--dtype", choices=["bfloat16", "float32"], default=None)
     g.add_argument("--kv-cache", choices=["ring", "pages"], default="ring", help="keys and values in 16-bit rings, or in 8-bit pages (reference-format checkpoints)")
+    g.add_argument("--weights", choices=["checkpoint", "e4m3"], default="checkpoint", help="keep the layers' matrices as the checkpoint has them, or in 8 bits (dense reference-format checkpoints)")
     g.add_argument("--alternatives", type=int, default=0, help="print that many of the most likely tokens at every generated one, with its log-probability and entropy")
     a = ap.parse_args(argv)
 
@@ -29,7 +30,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     from .registry import load_model
 
     prompts = [[int(t) for t in p.split()] for p in a.prompt]
-    model = load_model(a.model, max_batch_size=len(prompts), dtype=getattr(torch, a.dtype) if a.dtype else None)
+    more = {} if a.weights == "checkpoint" else {"weights": a.weights}
+    model = load_model(a.model, max_batch_size=len(prompts), dtype=getattr(torch, a.dtype) if a.dtype else None, **more)
     out = generate(prompts, model, max_tokens=a.max_tokens, temperature=a.temperature, chunk_size=a.chunk_size, kv_cache=a.kv_cache, alternatives=a.alternatives)
     for b, row in enumerate(out[0]):
         print(" ".join(str(t) for t in row))

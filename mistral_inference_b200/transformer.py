@@ -15,7 +15,7 @@ from typing import Any, Dict, List, Mapping, Optional, Tuple, Union
 import torch
 from torch import nn
 
-from . import _abi
+from . import _abi, rows8
 from .args import TransformerArgs
 from .cache import BufferCache, CacheInputMetadata, upload
 from .paged import PagedCache
@@ -96,6 +96,8 @@ class Transformer(nn.Module):
         for j, blk in enumerate(self.layers.values()):  # consecutive MoE layers alternate the expert-parallel exchange buffer
             if hasattr(blk.feed_forward, "layer_parity"):
                 blk.feed_forward.layer_parity = j & 1
+        self.weights8 = False                            # the Linears are 8-bit rows (quantise_weights)
+        self._output8: Optional[rows8.Rows8] = None      # ... the lm head as well
         self._ws: Optional[_abi.Workspace] = None
         self._ws_tokens = 0
         self.last_argmax: Optional[torch.Tensor] = None  # device token id(s) written by the last fused-argmax decode step
@@ -182,10 +184,7 @@ class Transformer(nn.Module):
             h = torch.empty(num_toks, self.args.dim, device=self.device, dtype=self.dtype)
             torch.distributed.recv(h, src=self.pipeline_rank - 1)
 
-        rope = self.rope_table
-        for local_layer_id, layer in enumerate(self.layers.values()):
-            view = cache.get_view(local_layer_id, input_metadata[local_layer_id]) if cache is not None else None
-            h = layer(h, rope, positions, view, ws)
+        h = self._run_layers(h, positions, cache, input_metadata, ws)
 
         if cache is not None:
             cache.update_seqlens(seqlens)
@@ -211,8 +210,7 @@ class Transformer(nn.Module):
             if cache is not None:
                 cache.update_seqlens(seqlens)
             outs32 = torch.empty(h.shape[0], self.vocab_size, device=h.device, dtype=torch.float32)
-            assert self.norm is not None and self.output_weight is not None
-            _abi.lm_head(h, self.norm.weight, self.output_weight, outs32, self.args.norm_eps, self.workspace(h.shape[0]))
+            self._head(h, outs32)
             return outs32 if self.softmax_fp32 else outs32.to(self.dtype)
         h = self.forward_partial(input_ids, seqlens, cache=cache)
         if not last:
@@ -240,12 +238,27 @@ class Transformer(nn.Module):
             positions = upload(torch.cat([torch.arange(0, s, dtype=torch.int32) for s in seqlens]), self.device)
         assert self.tok_embeddings is not None
         h = self.tok_embeddings(input_ids)
-        rope = self.rope_table
         with _nvtx(f"mb200.layers[T={num_toks}]"):
-            for local_layer_id, layer in enumerate(self.layers.values()):
-                view = cache.get_view(local_layer_id, input_metadata[local_layer_id]) if cache is not None else None
+            return self._run_layers(h, positions, cache, input_metadata, ws)
+
+    def _run_layers(self, h: torch.Tensor, positions: torch.Tensor, cache: Optional[BufferCache], input_metadata: Optional[List[CacheInputMetadata]], ws: "_abi.Workspace") -> torch.Tensor:
+        rope = self.rope_table
+        add: Optional[torch.Tensor] = None  # 8-bit weights: a layer's last addition to the stream is made by the next norm
+        for local_layer_id, layer in enumerate(self.layers.values()):
+            view = cache.get_view(local_layer_id, input_metadata[local_layer_id]) if cache is not None else None
+            if self.weights8:
+                h, add = layer.forward8(h, add, rope, positions, view, ws)
+            else:
                 h = layer(h, rope, positions, view, ws)
-        return h
+        return h if add is None else h + add
+
+    def _head(self, h: torch.Tensor, out: torch.Tensor) -> None:
+        """Final norm and lm head of rows h: fp32 logits into `out`."""
+        assert self.norm is not None and self.output_weight is not None
+        if self._output8 is not None:
+            rows8.multiply_rows(rows8.norm_rows(h, self.norm.weight, self.args.norm_eps)[0], self._output8, out=out)
+        else:
+            _abi.lm_head(h, self.norm.weight, self.output_weight, out, self.args.norm_eps, self.workspace(max(h.shape[0], 1)))
 
     def _check_positions(self, cache: BufferCache, seqlens: List[int]) -> None:
         """The reference indexes freqs_cis[positions] and raises past the table (transformer.py:199); the kernels would read out of bounds."""
@@ -265,7 +278,7 @@ class Transformer(nn.Module):
                 and len(set(cache.cache_sizes)) <= 8)
 
     def _megakernel_ok(self, B: int) -> bool:
-        return (B == 1 and self.num_pipeline_ranks == 1 and self.expert_parallel[1] == 1 and self.args.n_kv_heads <= 8
+        return (B == 1 and not self.weights8 and self.num_pipeline_ranks == 1 and self.expert_parallel[1] == 1 and self.args.n_kv_heads <= 8
                 and os.environ.get("MB200_MEGAKERNEL", "1") != "0"
                 and (self.args.moe is None or (self.args.moe.num_experts <= 32 and self.args.moe.num_experts_per_tok <= 4)))
 
@@ -275,10 +288,11 @@ class Transformer(nn.Module):
         reallocated since (a captured graph holds the old pointer)."""
         states = cache.__dict__.setdefault("_mb200_decode_states", {})
         ws_ptr = self._ws.ptr if self._ws is not None else 0
-        st = states.get((id(self), key))
+        key = (id(self), self.weights8, key)  # (a graph captured before quantise_weights reads matrices that are gone)
+        st = states.get(key)
         if st is None or st["ws_ptr"] != ws_ptr or st["device"] != self.device:
             st = {"ws_ptr": ws_ptr, "device": self.device}
-            states[(id(self), key)] = st
+            states[key] = st
         return st
 
     @torch.inference_mode()
@@ -379,7 +393,7 @@ class Transformer(nn.Module):
                 md = cache.metadata_from_block(st["meta"], layout, seqlens)
                 _abi.decode_meta(st["seqpos"], st["meta"], distinct)
             h = self._hidden_no_norm(st["tokens"], seqlens, cache, md)
-            _abi.lm_head(h, self.norm.weight, self.output_weight, st["logits"], self.args.norm_eps, self.workspace(B))
+            self._head(h, st["logits"])
             _abi.argmax_rows(st["logits"], st["next"])  # greedy pick on the device (generate.py:156): feeds the next step
 
         if st["graph"] is None and not st["warmed"]:
@@ -439,8 +453,8 @@ class Transformer(nn.Module):
             cache.update_seqlens(seqlens)
         assert self.norm is not None and self.output_weight is not None
         ws = self.workspace(max(T, 1))
-        if not _abi.lm_head_logprobs_ok(T, self.args.dim, V):
-            return self._logprobs_of_written_logits(h, targets, ends, lp, ws)
+        if self._output8 is not None or not _abi.lm_head_logprobs_ok(T, self.args.dim, V):
+            return self._logprobs_of_written_logits(h, targets, ends, lp)
         keep = torch.full((T,), -1, dtype=torch.int32)
         keep[torch.tensor(ends) - 1] = torch.arange(len(ends), dtype=torch.int32)
         keep = upload(keep, h.device)
@@ -470,30 +484,27 @@ class Transformer(nn.Module):
         h = self._hidden_no_norm(input_ids, seqlens, cache)
         if cache is not None:
             cache.update_seqlens(seqlens)
-        assert self.norm is not None and self.output_weight is not None
-        ws = self.workspace(max(T, 1))
         rows = max(128, (256 << 20) // (4 * V))
         block = torch.empty(min(rows, T), V, dtype=torch.float32, device=h.device)
         last_logits = torch.empty(len(ends), V, dtype=torch.float32, device=h.device)
         out = empty_scores(T, top, True, h.device)
         for r0 in range(0, T, rows):
             r1 = min(T, r0 + rows)
-            _abi.lm_head(h[r0:r1], self.norm.weight, self.output_weight, block[: r1 - r0], self.args.norm_eps, ws)
+            self._head(h[r0:r1], block[: r1 - r0])
             token_scores(block[: r1 - r0], targets[r0:r1], top=top, out=out.rows(r0, r1))
             for b, e in enumerate(ends):
                 if r0 < e <= r1:
                     last_logits[b].copy_(block[e - 1 - r0])
         return out, last_logits
 
-    def _logprobs_of_written_logits(self, h: torch.Tensor, targets: torch.Tensor, ends: List[int], lp: torch.Tensor, ws: "_abi.Workspace"
-                                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    def _logprobs_of_written_logits(self, h: torch.Tensor, targets: torch.Tensor, ends: List[int], lp: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         T, V = h.shape[0], self.vocab_size
         rows = max(128, (256 << 20) // (4 * V))
         block = torch.empty(min(rows, T), V, dtype=torch.float32, device=h.device)
         last_logits = torch.empty(len(ends), V, dtype=torch.float32, device=h.device)
         for r0 in range(0, T, rows):
             r1 = min(T, r0 + rows)
-            _abi.lm_head(h[r0:r1], self.norm.weight, self.output_weight, block[: r1 - r0], self.args.norm_eps, ws)
+            self._head(h[r0:r1], block[: r1 - r0])
             _abi.logprob_gather(block[: r1 - r0], targets[r0:r1], out=lp[r0:r1])
             for b, e in enumerate(ends):
                 if r0 < e <= r1:
@@ -579,6 +590,7 @@ class Transformer(nn.Module):
     def load_state_dict(self, state_dict: Mapping[str, Any], strict: bool = True, assign: bool = False) -> None:  # type: ignore[override]
         """Takes a REFERENCE-keyed state dict (transformer.py:244-295), filters by pipeline rank and packs."""
         del assign  # tensors are copied into the packed buffers
+        self._check_16_bit("load_state_dict")
         loaded = set()
         with torch.no_grad():
             for k, v in state_dict.items():
@@ -595,6 +607,7 @@ class Transformer(nn.Module):
 
     def state_dict(self, *args: Any, **kwargs: Any) -> Dict[str, torch.Tensor]:  # type: ignore[override]
         """Reference-keyed views of the packed parameters."""
+        self._check_16_bit("state_dict")
         out: Dict[str, torch.Tensor] = {}
         if self.tok_embeddings is not None:
             out["tok_embeddings.weight"] = self.tok_embeddings.weight
@@ -621,6 +634,34 @@ class Transformer(nn.Module):
             out["output.weight"] = self.output_weight
         return out
 
+    # ------------------------------------------------------------------ 8-bit weights
+    @torch.no_grad()
+    def quantise_weights(self, head: bool = False) -> "Transformer":
+        """Keeps every layer's matrices as 8-bit rows (rows8.py: e4m3 with a power of two for each 128 entries of a row), with `head` the lm head too, and runs the Linears on 8-bit
+        activations.  The 16-bit matrices are given up: no state dict, loading or merging afterwards.  Dense models on one pipeline stage."""
+        self._check_runnable()
+        if self.args.moe is not None or self.num_pipeline_ranks != 1:
+            raise _abi.Mb200Error("8-bit weights: dense models on one pipeline stage only")
+        if self.weights8:
+            raise _abi.Mb200Error("the weights are in 8 bits already")
+        for layer in self.layers.values():
+            layer.quantise()
+        kept = [r for layer in self.layers.values() for r in (layer.attention.wqkv8, layer.attention.wo8, layer.feed_forward.w13_8, layer.feed_forward.w2_8)]
+        if head:
+            assert self.output_weight is not None
+            self._output8 = rows8.quantise_rows(self.output_weight.data)
+            kept.append(self._output8)
+            self.output_weight.data = self.output_weight.data.new_empty(0)
+        torch.cuda.synchronize(self.device)
+        for r in kept:
+            r.fixed = True  # what wrote it has ended
+        self.weights8 = True
+        return self
+
+    def _check_16_bit(self, what: str) -> None:
+        if self.weights8:
+            raise _abi.Mb200Error(f"{what}: the weights are in 8 bits (quantise_weights)")
+
     # ------------------------------------------------------------------ LoRA, merged path (lora.py:92-155 with args.lora is None)
     def load_lora(self, lora_path: Union[Path, str], scaling: float = 2.0) -> None:
         """Loads a LoRA checkpoint and MERGES it into the packed weights (lora.py:93-101,120-139): the forward path is unchanged."""
@@ -638,6 +679,7 @@ class Transformer(nn.Module):
         lora_dtype = lora_dtypes.pop()
         assert lora_dtype == self.dtype, f"LoRA weights dtype differs from model's dtype {lora_dtype} != {self.dtype}"
         assert all("lora" in key for key in lora_state_dict.keys())
+        self._check_16_bit("load_lora")
         assert self.args.lora is None, "un-merged LoRA adapters are outside the accelerated hot path: merge them (args.lora = None)"
         lora_state_dict = {k: v.to(self.device) for k, v in lora_state_dict.items()}
         with torch.no_grad():
@@ -664,12 +706,17 @@ class Transformer(nn.Module):
     @staticmethod
     def from_folder(folder: Union[Path, str], max_batch_size: int = 1, num_pipeline_ranks: int = 1,
                     device: Union[torch.device, str] = "cuda", dtype: Optional[torch.dtype] = None,
-                    softmax_fp32: bool = True, expert_parallel: Optional[Tuple[int, int]] = None, expert_group: Any = None) -> "Transformer":
+                    softmax_fp32: bool = True, expert_parallel: Optional[Tuple[int, int]] = None, expert_group: Any = None,
+                    weights: str = "checkpoint") -> "Transformer":
         """transformer.py:297-338.  Tensors stream from disk straight into the packed device buffers; with `expert_parallel`
-        the experts of other ranks are skipped (never read into device memory)."""
+        the experts of other ranks are skipped (never read into device memory).  weights "e4m3": the layers' matrices are kept in 8 bits afterwards (quantise_weights)."""
+        if weights not in ("checkpoint", "e4m3"):
+            raise ValueError(f"weights {weights!r} (checkpoint, or e4m3)")
         with open(Path(folder) / "params.json", "r") as f:
             model_args = TransformerArgs.from_dict(json.load(f))
         model_args.max_batch_size = max_batch_size
+        if weights == "e4m3" and (model_args.moe is not None or num_pipeline_ranks != 1):
+            raise _abi.Mb200Error("8-bit weights: dense models on one pipeline stage only")
         pipeline_rank = torch.distributed.get_rank() if num_pipeline_ranks > 1 else 0
 
         pt_model_file = Path(folder) / "consolidated.00.pth"
@@ -705,4 +752,6 @@ class Transformer(nn.Module):
                             loaded_keys.add(k)
                 missing = set(model.reference_keys()) - loaded_keys
                 assert not missing, f"missing keys: {sorted(missing)[:8]}"
+        if weights == "e4m3":
+            model.quantise_weights()
         return model.eval()

@@ -11,7 +11,7 @@ from typing import List, Optional, Tuple
 import torch
 from torch import nn
 
-from . import _abi
+from . import _abi, _abi_rows8, rows8
 from .args import LoraArgs, MoeArgs
 from .cache import CacheView
 from .moe import MoeLayer
@@ -56,6 +56,8 @@ class Attention(nn.Module):
         self.kv_dim = n_kv_heads * head_dim
         self.wqkv = nn.Parameter(torch.empty(self.q_dim + 2 * self.kv_dim, dim), requires_grad=False)
         self.wo_weight = nn.Parameter(torch.empty(dim, self.q_dim), requires_grad=False)
+        self.wqkv8: Optional[rows8.Rows8] = None  # 8-bit weights (TransformerBlock.quantise), in the place of the two above
+        self.wo8: Optional[rows8.Rows8] = None
 
     # state-dict compatible views
     @property
@@ -75,23 +77,30 @@ class Attention(nn.Module):
         return _WeightView(lambda: self.wo_weight)
 
     def attend(self, x: torch.Tensor, norm_w: torch.Tensor, eps: float, rope: torch.Tensor, positions: torch.Tensor,
-               cache: Optional[CacheView], ws: "_abi.Workspace") -> torch.Tensor:
-        """RMSNorm + QKV + RoPE + cache phase + attention core.  Returns the pre-`wo` output [T, H*hd]."""
+               cache: Optional[CacheView], ws: "_abi.Workspace", rows: Optional[rows8.Rows8] = None) -> torch.Tensor:
+        """RMSNorm + QKV + RoPE + cache phase + attention core.  Returns the pre-`wo` output [T, H*hd].  `rows`, with 8-bit weights: x's norm, already there."""
         T = x.shape[0]
         q = torch.empty(T, self.q_dim, dtype=x.dtype, device=x.device)
         k = torch.empty(T, self.kv_dim, dtype=x.dtype, device=x.device)
         v = torch.empty(T, self.kv_dim, dtype=x.dtype, device=x.device)
         out = torch.empty(T, self.q_dim, dtype=x.dtype, device=x.device)
         H, KV, hd = self.n_heads, self.n_kv_heads, self.head_dim
+
+        def project(cache_k: Optional[torch.Tensor] = None, cache_v: Optional[torch.Tensor] = None, cache_rows: Optional[torch.Tensor] = None) -> None:
+            if rows is None:
+                _abi.attn_qkv(x, norm_w, self.wqkv, rope, positions, q, k, v, cache_k, cache_v, cache_rows, H, KV, hd, eps, ws)
+            else:
+                _abi_rows8.rotate(rows8.multiply_rows(rows, self.wqkv8), rope, positions, cache_rows, q, k if cache_k is None else cache_k, v if cache_v is None else cache_v, H, KV)
+
         if cache is None:
             # cache-less forward: unmasked over the whole flattened batch
-            _abi.attn_qkv(x, norm_w, self.wqkv, rope, positions, q, k, v, None, None, None, H, KV, hd, eps, ws)
+            project()
             _abi.attn_prefill(q, k, v, None, None, None, None, out, 1, T, 0, H, KV, hd, causal=False)
             return out
         md = cache.metadata
         if cache.paged:
             # write, THEN read the pages; a batch's first tokens attend over their own rows as they are
-            _abi.attn_qkv(x, norm_w, self.wqkv, rope, positions, q, k, v, None, None, None, H, KV, hd, eps, ws)
+            project()
             cache.write(k, v)
             if md.first_prefill:
                 _abi.attn_prefill(q, k, v, k, v, md.q_start, md.seqpos, out, len(md.seqlens), md.max_seqlen, md.window, H, KV, hd, causal=True, first_prefill=True)
@@ -100,13 +109,13 @@ class Attention(nn.Module):
             return out
         if md.prefill:
             # read the old ring, THEN write (transformer_layers.py:75-76)
-            _abi.attn_qkv(x, norm_w, self.wqkv, rope, positions, q, k, v, None, None, None, H, KV, hd, eps, ws)
+            project()
             _abi.attn_prefill(q, k, v, cache.cache_k, cache.cache_v, md.q_start, md.seqpos, out, len(md.seqlens), md.max_seqlen,
                               md.window, H, KV, hd, causal=True, first_prefill=md.first_prefill)
             _abi.kv_ring_write(k, v, cache.cache_k, cache.cache_v, md.cache_rows, KV, hd)
         else:
             # write, THEN read the ring (transformer_layers.py:78-81); the scatter is the QKV kernel's epilogue
-            _abi.attn_qkv(x, norm_w, self.wqkv, rope, positions, q, k, v, cache.cache_k, cache.cache_v, md.cache_rows, H, KV, hd, eps, ws)
+            project(cache.cache_k, cache.cache_v, md.cache_rows)
             B = len(md.seqlens)
             _abi.attn_decode(q, cache.cache_k, cache.cache_v, md.kv_len, out, H, KV, hd, decode_splits(B, KV, md.window), ws)
         return out
@@ -130,6 +139,8 @@ class FeedForward(nn.Module):
         self.hidden_dim = hidden_dim
         self.w13 = nn.Parameter(torch.empty(2 * hidden_dim, dim), requires_grad=False)
         self.w2_weight = nn.Parameter(torch.empty(dim, hidden_dim), requires_grad=False)
+        self.w13_8: Optional[rows8.Rows8] = None  # 8-bit weights (TransformerBlock.quantise), in the place of the two above
+        self.w2_8: Optional[rows8.Rows8] = None
 
     @property
     def w1(self) -> _WeightView:
@@ -190,6 +201,24 @@ class TransformerBlock(nn.Module):
             hn = _abi.rmsnorm(h, self.ffn_norm.weight, self.norm_eps)
             return self.feed_forward.run(hn, h, ws)  # router + grouped experts + ordered combine + residual, no host sync
         return self.feed_forward.run(h, self.ffn_norm.weight, self.norm_eps, h, ws)
+
+    # ------------------------------------------------------------------ 8-bit weights
+    def quantise(self) -> None:
+        """Keeps the block's matrices as 8-bit rows and gives their 16-bit memory back."""
+        att, ff = self.attention, self.feed_forward
+        assert isinstance(ff, FeedForward), "a mixture's experts have no 8-bit form"
+        att.wqkv8, att.wo8, ff.w13_8, ff.w2_8 = (rows8.quantise_rows(w.data) for w in (att.wqkv, att.wo_weight, ff.w13, ff.w2_weight))
+        for p in (att.wqkv, att.wo_weight, ff.w13, ff.w2_weight):
+            p.data = p.data.new_empty(0)
+
+    def forward8(self, x: torch.Tensor, add: Optional[torch.Tensor], rope: torch.Tensor, positions: torch.Tensor, cache: Optional[CacheView],
+                 ws: "_abi.Workspace") -> Tuple[torch.Tensor, torch.Tensor]:
+        """`forward` with 8-bit weights, of the stream x + add: (the stream ahead of the feed-forward's addition, that addition)."""
+        att, ff = self.attention, self.feed_forward
+        rows, h = rows8.norm_rows(x, self.attention_norm.weight, self.norm_eps, add=add)
+        a = att.attend(h, self.attention_norm.weight, self.norm_eps, rope, positions, cache, ws, rows)
+        rows, h = rows8.norm_rows(h, self.ffn_norm.weight, self.norm_eps, add=rows8.multiply_rows(rows8.quantise_rows(a), att.wo8))
+        return h, rows8.multiply_rows(rows8.gate_rows(rows, ff.w13_8), ff.w2_8)
 
 
 # ============================================================================= layered decoders
