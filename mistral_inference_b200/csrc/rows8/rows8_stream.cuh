@@ -38,6 +38,7 @@ __device__ __forceinline__ void max_in_cluster(uint32_t* p, int rank, uint32_t v
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+MB_HD constexpr int R8_UNITS_PITCH(int units) { return units + 4; }  // floats of a token's units
 struct StreamParams {
   ProductParams o;
   int split;    // CTAs of 128 features
@@ -178,10 +179,15 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
         for (int i = 0; i < 16; i += 4)
           if (c + i < T)
             asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c + i) * 4), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]) : "memory");
-      } else if (GATE) {
+      } else if (GATE) {  // lanes 2 i and 2 i + 1 have a unit's gate and up: the even one takes the first eight tokens, the odd one the others
+        const bool odd = lane & 1;
+        float* const at = reinterpret_cast<float*>(smem + p.units_at) + (c + (odd ? 8 : 0)) * R8_UNITS_PITCH(64) + (f >> 1);
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          if (c + i < T) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c + i) * 4), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]) : "memory");
+        for (int i = 0; i < 8; ++i) {
+          const float own = __uint_as_float(odd ? v[i + 8] : v[i]), other = __uint_as_float(__shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 8], 1));
+          const float g = silu_times(odd ? other : own, odd ? own : other);
+          if (c + i + (odd ? 8 : 0) < T) at[i * R8_UNITS_PITCH(64)] = g;
+        }
       } else if (there) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -192,8 +198,6 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
       __syncwarp();
       cluster_arrive();
       cluster_wait();
-    } else if (GATE) {
-      asm volatile("bar.sync 2, 128;" ::: "memory");
     }
     if (sends || GATE) {
       const int n0 = tile * 128 + part * p.share;  // the first feature that this CTA finishes
@@ -223,9 +227,9 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
               if (4 * q + j < T) at[j * p.o.ld] = (O)x[j];
           }
       } else {
-        const int block = tile >> 1, pitch = per + 4;  // (64, 32 or 16 units)
+        const int block = tile >> 1, pitch = R8_UNITS_PITCH(per);  // (64, 32 or 16 units)
         float* const units = reinterpret_cast<float*>(smem + p.units_at);
-        for (int q = id / lanes; q < quads; q += groups)
+        for (int q = sends ? id / lanes : quads; q < quads; q += groups)
           for (int u = id % lanes; u < per; u += lanes) {
             const float4 x = total(2 * u, q), y = total(2 * u + 1, q);
             float* const at = units + 4 * q * pitch + u;
@@ -300,8 +304,8 @@ inline size_t rows8_stream_layout(StreamParams& s, int64_t T, int64_t N, int64_t
   s.x_bytes = cols * R8_BLOCK;
   s.stage_bytes = RS_W + s.x_bytes + 2 * R8_TILE;
   const int64_t ctas = (N + 127) / 128 * s.split, blocks = ((K + 127) / 128 + s.split - 1) / s.split;
-  const int sums = gate || s.split > 1 ? s.split * s.share * s.pitch * 4 : 0, units = gate ? rs_up((int)T, 4) * (s.share / 2 + 4) * 4 : 0;
-  const int beside = T <= 32 && sums > 0 ? sums + units : 0, room = (ctas <= sms ? RS_SMEM : RS_SMEM_TWO) - 1024 - beside;
+  const int sums = s.split > 1 ? s.split * s.share * s.pitch * 4 : 0, units = gate ? rs_up((int)T, 4) * R8_UNITS_PITCH(s.share / 2) * 4 : 0;
+  const int beside = T <= 32 ? sums + units : 0, room = (ctas <= sms ? RS_SMEM : RS_SMEM_TWO) - 1024 - beside;
   s.stages = room / s.stage_bytes;
   if (s.stages > RS_MAX_STAGES) s.stages = RS_MAX_STAGES;
   if (s.stages > blocks) s.stages = (int)blocks;
