@@ -27,9 +27,11 @@ def main(argv: Optional[List[str]] = None) -> int:
     import torch
 
     from .generate import generate
-    from .registry import load_model
+    from .registry import architecture_of, load_model
 
     prompts = [[int(t) for t in p.split()] for p in a.prompt]
+    if a.weights != "checkpoint" and architecture_of(a.model) != "transformer":
+        ap.error(f"--weights {a.weights}: reference-format checkpoints only")
     more = {} if a.weights == "checkpoint" else {"weights": a.weights}
     model = load_model(a.model, max_batch_size=len(prompts), dtype=getattr(torch, a.dtype) if a.dtype else None, **more)
     out = generate(prompts, model, max_tokens=a.max_tokens, temperature=a.temperature, chunk_size=a.chunk_size, kv_cache=a.kv_cache, alternatives=a.alternatives)

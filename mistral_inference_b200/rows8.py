@@ -48,15 +48,18 @@ class Rows8:
         width, tiles = _width(cols), _tiles(rows, cols)
         return Rows8(_empty((rows, width), (width, 1), dtype=_E4M3, device=device), _empty(tiles, (tiles[1] * 512, 512, 16, 4, 1), dtype=_E8M0, device=device), cols)
 
+    def _blocks(self, tiles: torch.Tensor) -> torch.Tensor:
+        """Bytes in tiles as [rows, blocks]."""
+        n, quads = tiles.shape[:2]
+        return tiles.permute(0, 3, 2, 1, 4).reshape(n * 128, quads * 4)[: self.rows, : self.codes.shape[1] // BLOCK]
+
     def exponents(self) -> torch.Tensor:
         """[rows, ceil(cols / 128)] int32: the power of two of each block."""
-        tiles, quads = self.scales.shape[:2]
-        flat = self.scales.view(torch.uint8).permute(0, 3, 2, 1, 4).reshape(tiles * 128, quads * 4)
-        return flat[: self.rows, : self.codes.shape[1] // BLOCK].int() - 127
+        return self._blocks(self.scales.view(torch.uint8)).int() - 127
 
     def numbers(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """[rows, cols]: what the codes stand for (exact in 16 bits as well)."""
-        power = ((self.exponents() + 127) << 23).view(torch.float32)
+        power = self._blocks(self.scales.view(torch.uint8)).contiguous().view(_E8M0).float()
         return (self.codes.float().view(self.rows, -1, BLOCK) * power[:, :, None]).view(self.rows, -1)[:, : self.cols].to(dtype)
 
 

@@ -219,3 +219,140 @@ def test_no_rows():
     normed, h = mi.norm_rows(x, torch.ones(300, dtype=torch.bfloat16, device=DEV), 1e-5, add=x)
     w = random_rows(100, 300, 1)
     assert rows.rows == normed.rows == 0 and h.shape == (0, 300) and mi.multiply_rows(rows, w).shape == (0, 100) and mi.gate_rows(rows, w).rows == 0
+
+
+# ------------------------------------------------------------------------------------------------------------ how calls are made
+def same(a, b):
+    if isinstance(a, Rows8):
+        return torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales.view(torch.uint8), b.scales.view(torch.uint8))
+    return torch.equal(a, b)
+
+
+def chain(x, weight, wqkv, w13, w2):
+    """A sublayer and the next as a layer runs them."""
+    rows, h = mi.norm_rows(x, weight, 1e-5)
+    a = mi.multiply_rows(rows, wqkv)
+    rows, h = mi.norm_rows(h, weight, 1e-5, add=a[:, : x.shape[1]])
+    g = mi.gate_rows(rows, w13)
+    return h, mi.multiply_rows(mi.quantise_rows(a), wqkv, dtype=torch.float32), g, mi.multiply_rows(g, w2)
+
+
+def chain_inputs(T, K, H, seed):
+    return (normal((T, K), seed, 1.0, torch.bfloat16), (1 + normal((K,), seed + 1, 0.1)).to(torch.bfloat16), random_rows(K, K, seed + 2, K ** -0.5), random_rows(2 * H, K, seed + 3, K ** -0.5),
+            random_rows(K, H, seed + 4, H ** -0.5))
+
+
+@pytest.mark.parametrize("T", [1, 20, 128, 129, 600])
+def test_a_run_of_them_against_64_bits(T):
+    """Each operator on what the one before it gave: rounded where that is rounded, by the bounds of each."""
+    K, H = 640, 1100
+    x, weight, wqkv, w13, w2 = chain_inputs(T, K, H, 3 * T)
+    h, again, g, y = chain(x, weight, wqkv, w13, w2)
+    rows, _ = mi.norm_rows(x, weight, 1e-5)
+    want, off = U.product(U.numbers(rows.codes, rows.scales, K), U.numbers(wqkv.codes, wqkv.scales, K))
+    a = mi.multiply_rows(rows, wqkv)
+    assert ((a.double() - want).abs() <= off + (want.abs() + off) * 2.0 ** -8).all() and torch.equal(h, x + a)
+    want, off = U.product(U.numbers(g.codes, g.scales, H), U.numbers(w2.codes, w2.scales, H))
+    assert ((y.double() - want).abs() <= off + (want.abs() + off) * 2.0 ** -8).all()
+    # and the whole against 64 bits without any rounding in between: four roundings to 8 bits (2^-4 at most, some 2^-5.3 on average, of either sign) of each product's terms
+    n = lambda t: t.double() / torch.sqrt((t.double() ** 2).mean(1, keepdim=True) + 1e-5) * weight.double()  # noqa: E731
+    e = n(x) @ U.numbers(wqkv.codes, wqkv.scales, K).t()
+    z = n(x.double() + e) @ U.numbers(w13.codes, w13.scales, K).t()
+    z = (z[:, 0::2] * torch.sigmoid(z[:, 0::2]) * z[:, 1::2]) @ U.numbers(w2.codes, w2.scales, H).t()
+    assert (y.double() - z).norm() <= 2.0 ** -3 * z.norm()
+    assert again.isfinite().all()
+
+
+@pytest.mark.parametrize("T", [1, 40, 129, 300])
+def test_every_call_gives_the_same_bits(T):
+    args = chain_inputs(T, 1000, 1300, T)
+    first = chain(*args)
+    for _ in range(20):
+        assert all(same(a, b) for a, b in zip(first, chain(*args)))
+
+
+@pytest.mark.parametrize("T", [3, 200])
+def test_captured_graphs_on_two_streams_at_once(T):
+    """Two graphs of the same calls share weights and nothing else: replayed at the same time, each has its own results."""
+    x, weight, *ws = chain_inputs(T, 2048, 2304, T)
+    torch.cuda.synchronize()
+    for w in ws:
+        w.fixed = True
+    ins, outs, graphs, want = [], [], [], []
+    for i in range(2):
+        ins.append(normal((T, 2048), 50 + i, 1.0, torch.bfloat16))
+        want.append(chain(ins[i], weight, *ws))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(chain(ins[i], weight, *ws))
+        graphs.append((g, s))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(same(a, b) for a, b in zip(outs[i], want[i]))
+
+
+def test_weights_written_just_before():
+    """Weights that are not fixed are read behind what writes them, whatever runs in between."""
+    for T in (2, 60, 200):
+        x = random_rows(T, 4096, 1)
+        big = normal((6144, 4096), 2)
+        want = mi.multiply_rows(x, mi.quantise_rows(big * 2))
+        torch.cuda.synchronize()
+        for _ in range(10):
+            junk = mi.quantise_rows(big)
+            w = mi.quantise_rows(big * 2)
+            got = mi.multiply_rows(x, w)
+            del junk, w
+            assert torch.equal(got, want)
+
+
+def test_rows_cut_between_tiles():
+    """Rows from a multiple of 128 on are a matrix of their own: no copy is needed."""
+    x, w = random_rows(700, 900, 1), random_rows(300, 900, 2)
+    part, head = Rows8(x.codes[256:], x.scales[2:], 900), Rows8(x.codes[:256], x.scales[:2], 900)
+    assert torch.equal(part.numbers(), x.numbers()[256:]) and torch.equal(head.numbers(), x.numbers()[:256])
+    for a, b in ((part, w), (w, head), (head, part)):
+        y, off = U.product(a.numbers(torch.float64), b.numbers(torch.float64))
+        assert ((mi.multiply_rows(a, b, dtype=torch.float32).double() - y).abs() <= off).all()
+
+
+def test_scales_that_are_no_numbers_and_the_smallest():
+    for T in (4, 200):
+        x, w = random_rows(T, 512, 1), random_rows(140, 512, 2)
+        x.scales.view(torch.uint8)[0, 0, 2, 0, 1] = 255  # row 2, block 1
+        y = mi.multiply_rows(x, w, dtype=torch.float32)
+        nan = y.isnan()
+        assert nan[2].all() and not nan[:2].any() and not nan[3:].any()
+        w.scales.view(torch.uint8)[0, 0, 5, 0, :] = 0     # 2^-127: its products with powers near 1 are 0 or next to it
+        assert (mi.multiply_rows(x, w, dtype=torch.float32)[3:, 5].abs() <= 2.0 ** -90).all()
+
+
+def test_tensors_of_another_stream():
+    x, weight, *ws = chain_inputs(30, 640, 700, 9)
+    want = chain(x, weight, *ws)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = chain(x, weight, *ws)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(same(a, b) for a, b in zip(got, want))
+
+
+def test_results_of_empty_and_refused_calls():
+    x, w = random_rows(3, 200, 1), random_rows(4, 200, 2)
+    bf = torch.bfloat16
+    for call in (lambda: mi.multiply_rows(x, random_rows(4, 201, 1)), lambda: mi.multiply_rows(x, w, dtype=torch.float16), lambda: mi.gate_rows(x, random_rows(3, 200, 1)),
+                 lambda: mi.multiply_rows(x, w, out=torch.empty(3, 5, device=DEV, dtype=bf)), lambda: mi.multiply_rows(x, w, out=torch.empty(4, 3, device=DEV, dtype=bf).t()),
+                 lambda: mi.multiply_rows(x, Rows8(w.codes, w.scales, 100)), lambda: mi.multiply_rows(Rows8(x.codes.view(torch.uint8), x.scales, 200), w),
+                 lambda: mi.multiply_rows(Rows8(x.codes, x.scales.cpu(), 200), w), lambda: mi.multiply_rows(Rows8(x.codes[:, :128], x.scales, 100), w),
+                 lambda: mi.norm_rows(normal((2, 70000), 1, 1.0, bf), normal((70000,), 1, 1.0, bf), 1e-5), lambda: mi.norm_rows(normal((2, 70), 1, 1.0, bf), normal((70,), 1), 1e-5),
+                 lambda: mi.norm_rows(normal((2, 70), 1), normal((70,), 1), 1e-5, add=normal((2, 71), 1)), lambda: mi.quantise_rows(normal((2, 70), 1).half())):
+        with pytest.raises(AssertionError):
+            call()

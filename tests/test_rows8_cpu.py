@@ -129,3 +129,23 @@ def test_the_restatement_refuses_wrong_rows():
         wrong[at] += 1
         with pytest.raises(AssertionError):
             U.assert_rows_near(codes, wrong, x.float().double(), 0.0)
+
+
+def test_powers_of_any_byte():
+    """Scales that another program wrote: 2^-127, the largest, and the byte that is no number."""
+    r = rows(4, 128)
+    r.codes.copy_(torch.full((4, 128), 1.5).to(torch.float8_e4m3fn))
+    bytes_ = r.scales.view(torch.uint8)
+    bytes_.fill_(127)
+    for i, b in enumerate((0, 1, 254, 255)):
+        bytes_[0, 0, i, 0, 0] = b
+    x = r.numbers(torch.float64)
+    assert (x[0] == 1.5 * 2.0 ** -127).all() and (x[1] == 1.5 * 2.0 ** -126).all() and (x[2] == 1.5 * 2.0 ** 127).all() and x[3].isnan().all()
+    assert r.exponents().tolist() == [[-127], [-126], [127], [128]]
+
+
+def test_command_line_refuses_8_bits_of_other_designs(tmp_path):
+    from mistral_inference_b200.main import main
+    (tmp_path / "config.json").write_text('{"architecture": "Fesenex"}')
+    with pytest.raises(SystemExit):
+        main(["generate", str(tmp_path), "--prompt", "1", "--weights", "e4m3"])
