@@ -3,8 +3,8 @@
 // The weights are the MMA's 128 rows, the tokens its columns (16, 32, 64 or 128).  A cluster of `split` CTAs computes 128 features, each CTA a range of k-blocks.  Each sends its fp32 sums to the
 // CTA that finishes them (the r-th takes the r-th part of the features), which adds them in the order of k: the same bits in every run.  What is sent lies over the ring,
 // behind a meeting of the cluster at the end of its MMAs, or for up to 32 tokens beside the ring, without that meeting (0.8 us).
-// Why not fewer features a CTA and all of K: an MMA of this kind takes some 90 clocks however narrow it is, so a CTA of 40 features read 1.3 KB in that time, half of its share of what memory
-// delivers (32 tokens 5120 x 14336: 23 us between the first block and the last), and the scales of rows that do not begin with a tile had to be gathered (4 to 8 us).
+// Why not fewer features a CTA and all of K: an MMA takes 52 clocks however narrow it is, and a CTA of 40 features gets 1.3 KB of weights into one, no more than its share of what memory delivers
+// (32 tokens 5120 x 14336: 23 us between the first block and the last, now 9); and the scales of rows that do not begin with a tile had to be gathered (4 to 8 us).
 // Weights that are fixed (the caller says that nobody writes them any more) are requested before the wait for the predecessor, tokens after it.
 //
 // Gated units: their power is that of 128 units, 256 features, so a cluster holds two such groups; its CTAs exchange their tokens' largest magnitudes.  Units are laid out by tokens in
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
     const bool fine = __all_sync(0xffffffffu, bounded_wait(&done, 0, &gave_up)) != 0;
     tc_fence_after();
     const int f = (warp & 3) * 32 + lane, T = p.o.T, id = threadIdx.x - 64;
-    const int owner = f / p.share, mine = min(p.share, 128 - part * p.share);  // features that this CTA finishes (none where it is <= 0)
+    const int owner = f / p.share, mine = min(p.share, 128 - part * p.share);  // features that this CTA finishes
     const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     using O = std::conditional_t<OUT == R8_OUT_F32, float, bf16>;
     uint32_t to = smem_u32(sums + (size_t)(part * p.share + f % p.share) * p.pitch);
@@ -282,14 +282,14 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
 // ---- host ----
 constexpr int RS_SMEM = 225 * 1024;  // (beside what the kernel names)
 inline int rs_up(int n, int step) { return (n + step - 1) / step * step; }
-constexpr int RS_CTAS = 256;              // that run at once, in clusters of up to eight
+inline int rs_ctas(int sms) { return 7 * sms / 4; }  // that run at once, in clusters of up to eight
 constexpr int RS_SMEM_TWO = 110 * 1024;  // two CTAs an SM
 // CTAs of 128 features: as many as let all CTAs run at once, two an SM (a cluster lies within one GPC, so fewer run than the SMs hold: of 288 CTAs in clusters of six some began
 // when others had ended).  us of a call with cold weights by CTAs of 128 features, 1 token 6144 x 4096: 1 11.5, 2 9.1, 4 7.1, 5 7.4, 6 10.8; 4096 x 14336: 1 35, 2 20, 4 14.4, 6 13.1, 8 12.6; 32 tokens
 // 5120 x 14336: 4 17.9, 5 16.9, 6 16.5, 8 22.5; 8 tokens 32000 x 4096: 1 23.2, 2 28.3.  For gated units a power of two, so that a CTA finishes a multiple of 16 of them.
-inline int rows8_stream_split(int64_t N, int64_t K, bool gate) {
+inline int rows8_stream_split(int64_t N, int64_t K, bool gate, int sms) {
   const int64_t tiles = gate ? (N + 255) / 256 * 2 : (N + 127) / 128, blocks = (K + 127) / 128;
-  int64_t s = RS_CTAS / tiles;
+  int64_t s = rs_ctas(sms) / tiles;
   if (s > RS_MAX_SPLIT) s = RS_MAX_SPLIT;
   if (s > blocks) s = blocks;
   if (gate) s = s >= 4 ? 4 : s >= 2 ? 2 : 1;
@@ -297,7 +297,7 @@ inline int rows8_stream_split(int64_t N, int64_t K, bool gate) {
 }
 // Sizes of a launch, and its dynamic shared memory
 inline size_t rows8_stream_layout(StreamParams& s, int64_t T, int64_t N, int64_t K, bool gate, int sms) {
-  s.split = rows8_stream_split(N, K, gate);
+  s.split = rows8_stream_split(N, K, gate, sms);
   s.share = (128 + s.split - 1) / s.split;
   s.pitch = (int)((T + 15) / 16 * 16 + 4);
   const int cols = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
