@@ -1,11 +1,13 @@
 """ctypes binding of libmb200_rows8.so (C ABI: include/mistral_b200_rows8.h): Linears of 8-bit numbers.
 
 Same rules as `_abi`: the only place Python touches this library, and no fallback -- a missing library is built once
-in-tree by `build.build_rows8()` (a fresh checkout has no binaries), a failing call raises.
+in-tree by `build.build_rows8()` (a fresh checkout has no binaries), a failing call raises.  The operators of rows8.py go
+through a Python extension over the same C ABI (`host()`), which does in C++ what a call needs from the host.
 """
 import ctypes
-import functools
+import importlib.util
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from importlib.machinery import ExtensionFileLoader
 from typing import Optional
 
 import torch
@@ -45,6 +47,23 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The extension (csrc/rows8/rows8_host.cpp), bound to the library's entry points."""
+    global _host
+    if _host is None:
+        handle, path = lib(), str(build.build_rows8_host())
+        loader = ExtensionFileLoader("mb200_rows8_host", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("mb200_rows8_host", path, loader=loader))
+        loader.exec_module(module)
+        entries = ("mb8_last_error", "mb8_quantise", "mb8_norm", "mb8_multiply", "mb8_gate", "mb8_product_scratch")
+        module.bind(Mb200Error, *[ctypes.cast(getattr(handle, n), c_void_p).value for n in entries])
+        _host = module
+    return _host
+
+
 _lazy = {}  # name -> entry point, once the library is loaded
 
 
@@ -61,23 +80,6 @@ def call(name: str, device: int, *args) -> None:
     if rc != 0:
         msg = lib().mb8_last_error()
         raise Mb200Error(f"{name} failed ({rc}): {msg.decode() if msg else '?'}")
-
-
-@functools.lru_cache(maxsize=256)
-def _scratch_bytes(device: int, T: int, N: int, K: int) -> int:
-    """How a product is cut goes by its device's SMs: the same device is asked that the call will run on."""
-    with torch.cuda.device(device):
-        return lib().mb8_product_scratch(T, N, K)
-
-
-STREAM_TOKENS = 128  # up to so many tokens a product needs no scratch
-
-
-def product(name: str, device: int, x, w, out: tuple, T: int, N: int, n: int) -> None:
-    """mb8_multiply or mb8_gate of x [T, K] and w [N, K]; n: what the entry point counts its results by."""
-    need = _scratch_bytes(device, T, N, x.cols) if T > STREAM_TOKENS else 0
-    scratch = x.codes.new_empty(need) if need else None
-    call(name, device, x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), *out, T, n, x.cols, w.fixed, None if scratch is None else scratch.data_ptr(), need)
 
 
 def rotate(qkv, rope, positions, rows, q, k, v, n_heads: int, n_kv_heads: int) -> None:

@@ -120,8 +120,40 @@ def build_rows8(force: bool = False) -> Path:
     return _build_small(ROWS8_SRC, ROWS8_LIB, [CSRC / h for h in headers] + [INCLUDE / h for h in ("mistral_b200.h", "mistral_b200_paged.h", "mistral_b200_rows8.h")], force=force)
 
 
+ROWS8_HOST = PKG / "mb200_rows8_host.so"
+
+
+def build_rows8_host(force: bool = False) -> Path:
+    """mb200_rows8_host.so: the Python extension behind rows8.py (csrc/rows8/rows8_host.cpp, some 10 s), against the torch and the Python that run this."""
+    import sysconfig
+
+    import torch
+
+    src, stamp = ROWS8_SRC / "rows8_host.cpp", ROWS8_SRC / ".build_stamp_host"
+    top = Path(torch.__file__).resolve().parent
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    includes = [str(top / "include"), str(top / "include" / "torch" / "csrc" / "api" / "include"), sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
+    h = hashlib.sha256()
+    for f in (src, INCLUDE / "mistral_b200_rows8.h"):
+        h.update(f.read_bytes())
+    h.update(" ".join(flags + [torch.__version__, sys.version]).encode())
+    digest = h.hexdigest()
+    if not force and ROWS8_HOST.exists() and stamp.exists() and stamp.read_text().strip() == digest:
+        return ROWS8_HOST
+    tmp = PKG / f".{ROWS8_HOST.stem}.{os.getpid()}.so"
+    cmd = [os.environ.get("CXX", "g++"), *flags, *[f"-I{d}" for d in includes], "-o", str(tmp), str(src), f"-L{top / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        sys.stderr.write(proc.stdout + proc.stderr)
+        raise RuntimeError(f"g++ failed ({proc.returncode}): {' '.join(cmd)}")
+    os.replace(tmp, ROWS8_HOST)
+    stamp.write_text(digest)
+    return ROWS8_HOST
+
+
 if __name__ == "__main__":
     print(build_rows8(force="--force" in sys.argv))
+    print(build_rows8_host(force="--force" in sys.argv))
     print(build_paged(force="--force" in sys.argv))
     print(build_hybrid(force="--force" in sys.argv))
     print(build_library(force="--force" in sys.argv, verbose="--verbose" in sys.argv))

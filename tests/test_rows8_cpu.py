@@ -95,6 +95,17 @@ def test_python_refuses_what_does_not_fit():
         Rows8.empty(2, BIG, "cpu")
 
 
+def test_what_is_no_tensor_is_refused():
+    bf = torch.zeros(2, 3, dtype=torch.bfloat16)
+    for call in (lambda: mi.quantise_rows(None), lambda: mi.quantise_rows([[1.0]]), lambda: mi.norm_rows(bf, None, 1e-5), lambda: mi.multiply_rows(Rows8(None, None, 3), rows(3, 9)),
+                 lambda: mi.gate_rows(rows(2, 9), Rows8(rows(4, 9).codes, 7, 9))):
+        with pytest.raises(AssertionError):
+            call()
+    for call in (lambda: mi.multiply_rows(rows(2, 9), Rows8(rows(3, 9).codes, rows(3, 9).scales, "9")), lambda: mi.multiply_rows(None, rows(3, 9))):
+        with pytest.raises((AssertionError, TypeError, AttributeError)):
+            call()
+
+
 def test_no_cpu_fallback():
     for call in (lambda: mi.quantise_rows(torch.zeros(2, 3)), lambda: mi.norm_rows(torch.zeros(2, 3), torch.zeros(3), 1e-5), lambda: mi.multiply_rows(rows(2, 9), rows(3, 9)),
                  lambda: mi.gate_rows(rows(2, 9), rows(4, 9))):
