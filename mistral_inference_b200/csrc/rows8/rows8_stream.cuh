@@ -5,7 +5,8 @@
 // behind a meeting of the cluster at the end of its MMAs, or for up to 32 tokens beside the ring, without that meeting (0.8 us).
 // Why not fewer features a CTA and all of K: an MMA takes 52 clocks however narrow it is, and a CTA of 40 features gets 1.3 KB of weights into one, no more than its share of what memory delivers
 // (32 tokens 5120 x 14336: 23 us between the first block and the last, now 9); and the scales of rows that do not begin with a tile had to be gathered (4 to 8 us).
-// Weights that are fixed (the caller says that nobody writes them any more) are requested before the wait for the predecessor, tokens after it.
+// Weights that are fixed (the caller says that nobody writes them any more) are requested before the wait for the predecessor, tokens after it; others are asked into L2 before it,
+// where whatever is still written to them arrives as well (us, 1 token: 6144 x 4096 8.5 without, 8.1 with, 4096 x 14336 13.8, 13.0; fixed 7.4, 12.6).
 //
 // Gated units: their power is that of 128 units, 256 features, so a cluster holds two such groups; its CTAs exchange their tokens' largest magnitudes.  Units are laid out by tokens in
 // shared memory, so that a thread has 16 of a token's next to one another.
@@ -81,7 +82,13 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
   const uint32_t tmem = tmem_slot;
   if (meetings > 0 && !(sends && over)) cluster_arrive();  // this CTA has begun: others may write to it
   pdl_trigger();
-  if (!p.ahead) pdl_wait();
+  if (!p.ahead) {
+    if (warp == 0 && elect_one())
+      for (int kb = kb0; kb < min(kb1, kb0 + p.stages); ++kb)
+        asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(&map_w), "r"(kb * R8_BLOCK), "r"(tile * 128) : "memory");
+    __syncwarp();
+    pdl_wait();
+  }
 
   if (warp == 0) {
     // ================= copies =================
