@@ -122,9 +122,14 @@ bool truth(PyObject* o) {
   return v != 0;
 }
 void arguments(Py_ssize_t n, Py_ssize_t want) {
-  if (n == want) return;
-  PyErr_Format(PyExc_TypeError, "%zd arguments, not %zd", want, n);
-  throw python_error();
+  if (n != want) {
+    PyErr_Format(PyExc_TypeError, "%zd arguments, not %zd", want, n);
+    throw python_error();
+  }
+}
+void call_arguments(Py_ssize_t n, Py_ssize_t want) {
+  arguments(n, want);
+  ASSERT(failure != nullptr, "bind() first");
 }
 
 // bind(error class, addresses of last_error, quantise, norm, multiply, gate, product_scratch)
@@ -144,7 +149,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // quantise(x) -> (codes, scales)
 PyObject* quantise(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 1);
+  call_arguments(n, 1);
   const Numbers x = numbers(a[0], "x");
   const Result r = make_rows(x.T, x.K, x.device);
   launch("mb8_quantise", x.device, [&](void* st) { return lib.quantise(x.at, x.ld, x.wide, r.codes.data_ptr(), r.scales.data_ptr(), x.T, x.K, st); });
@@ -155,7 +160,7 @@ PyObject* quantise(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // norm(x, weight, eps, add or None) -> (codes, scales, h or None)
 PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 4);
+  call_arguments(n, 4);
   const Numbers x = numbers(a[0], "x");
   ASSERT(x.K <= MB8_MAX_NORM, "rows of %lld entries (at most %d)", (long long)x.K, MB8_MAX_NORM);
   const at::Tensor& w = tensor(a[1], "weight");
@@ -203,7 +208,7 @@ struct Product {
 // multiply(x codes, scales, columns, w codes, scales, columns, w is fixed, results in fp32, out or None) -> out
 PyObject* multiply(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 9);
+  call_arguments(n, 9);
   const Product p(a);
   const bool fixed = truth(a[6]);
   Numbers out{nullptr, p.x.T, p.w.T, p.w.T, truth(a[7]), p.x.device};
@@ -227,7 +232,7 @@ PyObject* multiply(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // gate(x codes, scales, columns, w codes, scales, columns, w is fixed) -> (codes, scales)
 PyObject* gate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 7);
+  call_arguments(n, 7);
   const Product p(a);
   ASSERT(p.w.T >= 2 && p.w.T % 2 == 0, "pairs of rows, got %lld", (long long)p.w.T);
   const bool fixed = truth(a[6]);

@@ -345,6 +345,30 @@ def test_tensors_of_another_stream():
     assert all(same(a, b) for a, b in zip(got, want))
 
 
+def test_results_behind_32_bit_offsets():
+    """More than 2^31 numbers: the last rows are where they belong."""
+    T, N, K = 70000, 32768, 128
+    x, w = random_rows(T, K, 1), random_rows(N, K, 2)
+    wv = U.numbers(w.codes, w.scales, K)
+    y = mi.multiply_rows(x, w)
+    assert y.numel() > 2 ** 31
+    for r0 in (0, 65500, T - 100):
+        want, off = U.product(x.numbers(torch.float64)[r0: r0 + 100], wv)
+        assert ((y[r0: r0 + 100].double() - want).abs() <= off + (want.abs() + off) * 2.0 ** -8).all()
+    rows = mi.quantise_rows(y)
+    tail = mi.quantise_rows(y[69888:])  # (from a whole tile on)
+    assert torch.equal(rows.codes[69888:].view(torch.uint8), tail.codes.view(torch.uint8)) and torch.equal(rows.scales[546:].view(torch.uint8), tail.scales.view(torch.uint8))
+    weight = torch.ones(N, dtype=torch.bfloat16, device=DEV)
+    normed, h = mi.norm_rows(y, weight, 1e-5, add=y)
+    assert torch.equal(h[-50:], y[-50:] + y[-50:])
+    tail, _ = mi.norm_rows(y[69888:], weight, 1e-5, add=y[69888:])
+    assert torch.equal(normed.codes[69888:].view(torch.uint8), tail.codes.view(torch.uint8)) and torch.equal(normed.scales[546:].view(torch.uint8), tail.scales.view(torch.uint8))
+    del y, rows, normed, h
+    wide = mi.gate_rows(x, random_rows(2 * N, K, 3))
+    part = mi.gate_rows(Rows8(x.codes[69888:], x.scales[546:], K), random_rows(2 * N, K, 3))
+    assert wide.codes.numel() > 2 ** 31 and torch.equal(wide.scales[546:].view(torch.uint8), part.scales.view(torch.uint8)) and torch.equal(wide.codes[69888:].view(torch.uint8), part.codes.view(torch.uint8))
+
+
 def test_results_of_empty_and_refused_calls():
     x, w = random_rows(3, 200, 1), random_rows(4, 200, 2)
     bf = torch.bfloat16
