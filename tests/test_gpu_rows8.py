@@ -298,6 +298,30 @@ def test_captured_graphs_on_two_streams_at_once(T):
         assert all(same(a, b) for a, b in zip(outs[i], want[i]))
 
 
+def test_two_threads_at_once():
+    """Each on a stream of its own: the calls let go of the interpreter while they launch."""
+    import threading
+    args = [chain_inputs(t, 1000, 1200, t) for t in (5, 300)]
+    want = [chain(*a) for a in args]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = chain(*args[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(same(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_weights_written_just_before():
     """Weights that are not fixed are read behind what writes them, whatever runs in between."""
     for T in (2, 60, 200):
