@@ -5,7 +5,11 @@
 // token's features next to one another and, of gated units, half of a block of 128 that share a power.
 //
 // Two accumulators of 256 columns and the scales' 12 do not fit the 512 columns of tensor memory: the second accumulator begins 16 columns inside the first.  An epilogue reads
-// these first and says so (overlap), and the next tile's MMAs begin: some hundred clocks of a tile's 512 k-blocks.
+// these first and says so (overlap), and the next tile's MMAs begin, some hundred clocks behind the last one's.  Tiles begin at multiples of 128 rows: scales of 128 rows fill four
+// columns, and an MMA takes them from a multiple of four.
+//
+// 4096 tokens 28672 x 4096 (gate): 335 us in bursts of milliseconds, 2.87 PFLOP/s, 398 in loops of seconds; a k-block takes some 600 clocks, of which operands out of L2 and a tile's two ends are
+// the rest.  With one accumulator and a tile a CTA of its own (128 tokens, 48 KB a k-block) 756.
 // Tiles are dealt in rounds of the chip's pairs.  A last round that is at most half full is cut along K (pair_cut): its parts leave fp32 sums in scratch memory, which a second kernel, launched
 // programmatically, adds in the order of k and finishes.  Nobody waits for another cluster.
 //
