@@ -18,18 +18,52 @@ constexpr int RQ_WARPS = 8;
 // 16 entries of a row as they lie in memory, 32 or 64 bytes
 template <typename ST>
 struct Entries {
-  static constexpr int WORDS = 4 * sizeof(ST);
+  static constexpr int WORDS = 4 * sizeof(ST), VECTORS = WORDS / 4, PER = 16 / sizeof(ST) /* entries of 16 bytes */;
   uint32_t w[WORDS];
-  // of `row`, K entries in all, from k on; zeros behind the end.  ALIGNED: the row starts on 16 bytes.
+  // word i of what begins `bytes` bytes (even) into x, i + bytes / 4 + 1 <= N - 1 or bytes a multiple of four
+  template <int SKIP, int N>
+  static __device__ __forceinline__ uint32_t shifted(const uint32_t (&x)[N], int i, int bytes) {
+    if constexpr (sizeof(ST) == 4) return x[i + SKIP];
+    else return __funnelshift_r(x[i + SKIP], x[i + SKIP + 1 < N ? i + SKIP + 1 : N - 1], (bytes & 2) * 8);
+  }
+  template <int N, int M>
+  static __device__ __forceinline__ void shift(uint32_t (&to)[M], const uint32_t (&x)[N], int first, int bytes) {  // M words from word `first` on
+    switch (bytes >> 2) {
+#define R8_SHIFT(SKIP)          \
+  case SKIP:                    \
+    _Pragma("unroll") for (int i = 0; i < M; ++i) to[i] = shifted<SKIP>(x, first + i, bytes); \
+    break;
+      R8_SHIFT(0)
+      R8_SHIFT(1)
+      R8_SHIFT(2)
+      R8_SHIFT(3)
+#undef R8_SHIFT
+    }
+  }
+  // Of `row`, K entries in all, from k on; zeros behind the end.  ALIGNED: the row starts on 16 bytes.  Else what lies between two multiples of 16 bytes is loaded as a whole where the
+  // row has all of it, and shifted.
   template <bool ALIGNED>
   __device__ __forceinline__ void load(const ST* row, int k, int K) {
     if (ALIGNED && k + 16 <= K) {
 #pragma unroll
-      for (int i = 0; i < WORDS / 4; ++i) {
+      for (int i = 0; i < VECTORS; ++i) {
         const uint4 u = reinterpret_cast<const uint4*>(row + k)[i];
         w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
       }
       return;
+    }
+    if constexpr (!ALIGNED) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(row + k), base = at & ~(uintptr_t)15;
+      if (base >= reinterpret_cast<uintptr_t>(row) && base + (VECTORS + 1) * 16 <= reinterpret_cast<uintptr_t>(row + K)) {
+        uint32_t x[WORDS + 4];
+#pragma unroll
+        for (int i = 0; i <= VECTORS; ++i) {
+          const uint4 u = reinterpret_cast<const uint4*>(base)[i];
+          x[4 * i] = u.x, x[4 * i + 1] = u.y, x[4 * i + 2] = u.z, x[4 * i + 3] = u.w;
+        }
+        shift(w, x, 0, (int)(at & 15));
+        return;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -42,19 +76,51 @@ struct Entries {
       }
     }
   }
+  // The same places of `row`, by a whole warp whose lanes have 16 entries next to one another.  Not aligned: a lane takes the first entries of the next one and writes from its first multiple of 16
+  // bytes on; what lies before that in lane 0 and behind it in lane 31, or at the row's end, goes entry by entry.
   template <bool ALIGNED>
   __device__ __forceinline__ void store(ST* row, int k, int K) const {
-    if (ALIGNED && k + 16 <= K) {
+    if constexpr (ALIGNED) {
+      if (k + 16 <= K) {
 #pragma unroll
-      for (int i = 0; i < WORDS / 4; ++i) reinterpret_cast<uint4*>(row + k)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-      return;
-    }
+        for (int i = 0; i < VECTORS; ++i) reinterpret_cast<uint4*>(row + k)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (k + i < K) {
-        if constexpr (sizeof(ST) == 2) reinterpret_cast<uint16_t*>(row)[k + i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-        else reinterpret_cast<uint32_t*>(row)[k + i] = w[i];
+        for (int i = 0; i < 16; ++i)
+          if (k + i < K) put(row + k + i, w, i);
       }
+    } else {
+      const int lane = threadIdx.x & 31, skip = (int)(-reinterpret_cast<intptr_t>(row + k) & 15);  // bytes to the next multiple of 16 (the same in all lanes)
+      uint32_t x[WORDS + 4];
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) x[i] = w[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[WORDS + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+      const int limit = min(lane < 31 ? 16 + PER : 16, K - k), first = skip / (int)sizeof(ST);  // entries that this lane may write; its first one in a vector
+      if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < PER - 1; ++i)
+          if (i < first && i < limit) put(row + k + i, w, i);
+      }
+#pragma unroll
+      for (int v = 0; v < VECTORS; ++v) {
+        uint32_t y[4];
+        shift(y, x, 4 * v, skip);
+        const int from = first + v * PER;
+        if (from + PER <= limit) {
+          *reinterpret_cast<uint4*>(row + k + from) = make_uint4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (from + i < limit) put(row + k + from + i, y, i);
+        }
+      }
+    }
+  }
+  template <int N>
+  static __device__ __forceinline__ void put(ST* to, const uint32_t (&x)[N], int i) {
+    if constexpr (sizeof(ST) == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)(x[i / 2] >> (i % 2 * 16));
+    else *reinterpret_cast<uint32_t*>(to) = x[i];
   }
   // entries 2 i and 2 i + 1
   __device__ __forceinline__ uint64_t two(int i) const {
@@ -127,31 +193,36 @@ struct NormParams {
 };
 constexpr int RN8_MAX_STEPS = 4;                          // a warp's steps of a row, which stay in registers
 constexpr int RN8_MAX_K = 32 * RN8_MAX_STEPS * R8_CHUNK;  // entries of a row
-// A CTA a row: its entries are read once and stay in registers behind the sum of their squares.
-template <typename ST, bool ALIGNED, bool ADD, int STEPS>
-__global__ void __launch_bounds__(1024) rows8_norm_kernel(const NormParams p) {
+// A CTA a row: its entries are read once and stay in registers behind the sum of their squares.  ALIGNED: rows start on 16 bytes; W_ALIGNED: the weights do.
+template <typename ST, bool ALIGNED, bool W_ALIGNED, bool ADD, int STEPS, int THREADS>
+__global__ void __launch_bounds__(THREADS) rows8_norm_kernel(const NormParams p) {
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, r = (int)blockIdx.x;
   __shared__ float part[32];
   auto place = [&](int i) { return (i * warps + warp) * R8_CHUNK + lane * 16; };
   pdl_wait();
-  Entries<ST> h[STEPS], add[ADD ? STEPS : 1];
+  Entries<ST> h[STEPS];
+  {
+    Entries<ST> add[ADD ? STEPS : 1];
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) h[i].template load<ALIGNED>(reinterpret_cast<const ST*>(p.x) + r * p.ld, place(i), p.K);
-  if constexpr (ADD) {
+    for (int i = 0; i < STEPS; ++i) h[i].template load<ALIGNED>(reinterpret_cast<const ST*>(p.x) + r * p.ld, place(i), p.K);
+    if constexpr (ADD) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) add[i].template load<ALIGNED>(reinterpret_cast<const ST*>(p.add) + r * p.ld_add, place(i), p.K);
+      for (int i = 0; i < STEPS; ++i) add[i].template load<ALIGNED>(reinterpret_cast<const ST*>(p.add) + r * p.ld_add, place(i), p.K);
+    }
+    if constexpr (ADD) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        h[i].add(add[i]);
+        h[i].template store<ALIGNED>(reinterpret_cast<ST*>(p.stream) + (int64_t)r * p.K, place(i), p.K);
+      }
+    }
   }
   uint64_t sums = pair(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    if constexpr (ADD) {
-      h[i].add(add[i]);
-      h[i].template store<ALIGNED>(reinterpret_cast<ST*>(p.stream) + (int64_t)r * p.K, place(i), p.K);
-    }
+  for (int i = 0; i < STEPS; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) sums = fma_pair(h[i].two(j), h[i].two(j), sums);
-  }
   const float2 two = unpair(sums);
   float sum = warp_sum(two.x + two.y);
   if (lane == 0) part[warp] = sum;
@@ -164,7 +235,7 @@ __global__ void __launch_bounds__(1024) rows8_norm_kernel(const NormParams p) {
     const int q = i * warps + warp;
     if (q >= p.quads) break;
     Entries<ST> w;
-    w.template load<ALIGNED>(reinterpret_cast<const ST*>(p.w), place(i), p.K);
+    w.template load<W_ALIGNED>(reinterpret_cast<const ST*>(p.w), place(i), p.K);
     uint64_t v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = mul_pair(mul_pair(h[i].two(j), scale), w.two(j));
@@ -186,22 +257,27 @@ template <typename ST>
 int launch_rows8_quantise(const QuantiseParams& p, cudaStream_t st) {
   return (uintptr_t)p.x % 16 == 0 && (p.T == 1 || p.ld * sizeof(ST) % 16 == 0) ? launch_rows8_quantise<ST, true>(p, st) : launch_rows8_quantise<ST, false>(p, st);
 }
-template <typename ST, bool ALIGNED, bool ADD>
+template <typename ST, bool ALIGNED, bool W_ALIGNED, bool ADD>
 int launch_rows8_norm(const NormParams& p, cudaStream_t st) {
-  // as many warps as a CTA has, a step each, while a row is no longer than that (8000 x 5120, us: one step a warp 47.2, two 47.1, four 71.9)
-  const int need = (p.quads + 31) / 32, steps = need <= 2 ? need : RN8_MAX_STEPS;
-  const dim3 grid((unsigned)p.T), block(32 * (unsigned)((p.quads + steps - 1) / steps));
-  if (steps == 1) MB_CHECK_CUDA(launch_pdl(rows8_norm_kernel<ST, ALIGNED, ADD, 1>, grid, block, 0, st, p));
-  else if (steps == 2) MB_CHECK_CUDA(launch_pdl(rows8_norm_kernel<ST, ALIGNED, ADD, 2>, grid, block, 0, st, p));
-  else MB_CHECK_CUDA(launch_pdl(rows8_norm_kernel<ST, ALIGNED, ADD, RN8_MAX_STEPS>, grid, block, 0, st, p));
+  // As many warps as a CTA has, a step each, while a row is no longer than that.  What counts is how many rows are on their way: with more steps a warp, or the weights requested ahead of the sum, fewer
+  // CTAs share an SM (16000 x 5000 bf16, us, with addition and without: a step a warp 91, 56; two 96, 64; four 120, 92; weights ahead 106, 66).
+  const int steps = p.quads <= 32 ? 1 : RN8_MAX_STEPS, warps = (p.quads + steps - 1) / steps;
+  const dim3 grid((unsigned)p.T), block(32 * (unsigned)warps);
+  if (steps == 1) MB_CHECK_CUDA((launch_pdl(rows8_norm_kernel<ST, ALIGNED, W_ALIGNED, ADD, 1, 1024>, grid, block, 0, st, p)));
+  else if (warps <= 16) MB_CHECK_CUDA((launch_pdl(rows8_norm_kernel<ST, ALIGNED, W_ALIGNED, ADD, RN8_MAX_STEPS, 512>, grid, block, 0, st, p)));
+  else MB_CHECK_CUDA((launch_pdl(rows8_norm_kernel<ST, ALIGNED, W_ALIGNED, ADD, RN8_MAX_STEPS, 1024>, grid, block, 0, st, p)));
   return MB200_OK;
+}
+template <typename ST, bool ADD>
+int launch_rows8_norm(const NormParams& p, cudaStream_t st) {
+  auto apart = [&](const void* at, int64_t ld) { return (uintptr_t)at % 16 == 0 && (p.T == 1 || ld * sizeof(ST) % 16 == 0); };
+  const bool aligned = apart(p.x, p.ld) && (!ADD || (apart(p.add, p.ld_add) && apart(p.stream, p.K))), w_aligned = (uintptr_t)p.w % 16 == 0;
+  if (aligned && w_aligned) return launch_rows8_norm<ST, true, true, ADD>(p, st);
+  return w_aligned ? launch_rows8_norm<ST, false, true, ADD>(p, st) : launch_rows8_norm<ST, false, false, ADD>(p, st);
 }
 template <typename ST>
 int launch_rows8_norm(const NormParams& p, cudaStream_t st) {
-  auto apart = [&](const void* at, int64_t ld) { return (uintptr_t)at % 16 == 0 && (p.T == 1 || ld * sizeof(ST) % 16 == 0); };
-  const bool aligned = apart(p.x, p.ld) && (uintptr_t)p.w % 16 == 0 && (p.add == nullptr || (apart(p.add, p.ld_add) && apart(p.stream, p.K)));
-  if (p.add == nullptr) return aligned ? launch_rows8_norm<ST, true, false>(p, st) : launch_rows8_norm<ST, false, false>(p, st);
-  return aligned ? launch_rows8_norm<ST, true, true>(p, st) : launch_rows8_norm<ST, false, true>(p, st);
+  return p.add == nullptr ? launch_rows8_norm<ST, false>(p, st) : launch_rows8_norm<ST, true>(p, st);
 }
 
 }  // namespace mb200
