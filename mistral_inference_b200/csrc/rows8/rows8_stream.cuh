@@ -288,31 +288,38 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
 
 // ---- host ----
 constexpr int RS_SMEM = 225 * 1024;  // (beside what the kernel names)
-inline int rs_up(int n, int step) { return (n + step - 1) / step * step; }
-inline int rs_ctas(int sms) { return 7 * sms / 4; }  // that run at once, in clusters of up to eight
 constexpr int RS_SMEM_TWO = 110 * 1024;  // two CTAs an SM
-// CTAs of 128 features: as many as let all CTAs run at once, two an SM (a cluster lies within one GPC, so fewer run than the SMs hold: of 288 CTAs in clusters of six some began
-// when others had ended).  us of a call with cold weights by CTAs of 128 features, 1 token 6144 x 4096: 1 11.5, 2 9.1, 4 7.1, 5 7.4, 6 10.8; 4096 x 14336: 1 35, 2 20, 4 14.4, 6 13.1, 8 12.6; 32 tokens
-// 5120 x 14336: 4 17.9, 5 16.9, 6 16.5, 8 22.5; 8 tokens 32000 x 4096: 1 23.2, 2 28.3.  For gated units a power of two, so that a CTA finishes a multiple of 16 of them.
-inline int rows8_stream_split(int64_t N, int64_t K, bool gate, int sms) {
-  const int64_t tiles = gate ? (N + 255) / 256 * 2 : (N + 127) / 128, blocks = (K + 127) / 128;
-  int64_t s = rs_ctas(sms) / tiles;
-  if (s > RS_MAX_SPLIT) s = RS_MAX_SPLIT;
-  if (s > blocks) s = blocks;
-  if (gate) s = s >= 4 ? 4 : s >= 2 ? 2 : 1;
-  return (int)(s < 1 ? 1 : s);
+inline int rs_up(int n, int step) { return (n + step - 1) / step * step; }
+// CTAs that run at once.  A cluster lies within one GPC, so they are fewer than the SMs hold; of 148 SMs, by the CTAs of a cluster: two an SM 6 270, 7 259, 8 264 (of 288 in clusters of six some
+// began when others had ended); one an SM 2 148, 4 132, 5 130, 7 105, 8 120 (gated units of 4000 x 4096, 1 token, 128 CTAs in clusters of eight: 15.1 us one an SM, two an SM 8.4)
+inline int rs_two(int sms) { return 7 * sms / 4; }
+inline int rs_one(int cluster, int sms) { return cluster > 6 ? 7 * sms / 10 : cluster > 2 ? 7 * sms / 8 : sms; }
+// CTAs of 128 features: as many as let all CTAs run at once, two an SM.  us of a call with cold weights by CTAs of 128 features, 1 token 6144 x 4096: 1 11.5, 2 9.1, 4 7.1, 5 7.4, 6 10.8;
+// 4096 x 14336: 1 35, 2 20, 4 14.4, 6 13.1, 8 12.6; 32 tokens 5120 x 14336: 4 17.9, 5 16.9, 6 16.5, 8 22.5; 8 tokens 32000 x 4096: 1 23.2, 2 28.3.  With more tokens what the CTAs send counts for
+// more, and one CTA an SM is better: always from 65 on (128 tokens 4096 x 2048: 8 21.3, 4 11.3; 5120 x 5120: 6 18.6, 3 17.1; 5120 x 14336: 6 25.9, 3 25.7; 1024 x 4096: 8 9.8, 4 11.5), from 33 on if
+// one an SM uses nearly all SMs (64 tokens 4096 x 4096: 8 12.8, 4 10.5; but 5120 x 14336: 6 19.5, 3 21.1).  For gated units a power of two, so that a CTA finishes a multiple of 16 of them.
+inline int rows8_stream_split(int64_t T, int64_t tiles, int64_t K, bool gate, int sms) {
+  const int64_t blocks = (K + 127) / 128, most = blocks < RS_MAX_SPLIT ? blocks : RS_MAX_SPLIT;
+  int two = 1, one = 1;
+  for (int s = 2; s <= (gate && most > 4 ? 4 : most); s += gate ? s : 1) {
+    if (tiles * s <= rs_two(sms)) two = s;
+    if (tiles * s <= rs_one(gate ? 2 * s : s, sms)) one = s;
+  }
+  return T > 64 || (T > 32 && tiles * one >= 17 * sms / 20) ? one : two;
 }
+inline int64_t rows8_stream_tiles(int64_t N, bool gate) { return gate ? (N + 255) / 256 * 2 : (N + 127) / 128; }
 // Sizes of a launch, and its dynamic shared memory
 inline size_t rows8_stream_layout(StreamParams& s, int64_t T, int64_t N, int64_t K, bool gate, int sms) {
-  s.split = rows8_stream_split(N, K, gate, sms);
+  const int64_t tiles = rows8_stream_tiles(N, gate);
+  s.split = rows8_stream_split(T, tiles, K, gate, sms);
   s.share = (128 + s.split - 1) / s.split;
   s.pitch = (int)((T + 15) / 16 * 16 + 4);
   const int cols = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
   s.x_bytes = cols * R8_BLOCK;
   s.stage_bytes = RS_W + s.x_bytes + 2 * R8_TILE;
-  const int64_t ctas = (N + 127) / 128 * s.split, blocks = ((K + 127) / 128 + s.split - 1) / s.split;
+  const int64_t ctas = tiles * s.split, blocks = ((K + 127) / 128 + s.split - 1) / s.split;
   const int sums = s.split > 1 ? s.split * s.share * s.pitch * 4 : 0, units = gate ? rs_up((int)T, 4) * R8_UNITS_PITCH(s.share / 2) * 4 : 0;
-  const int beside = T <= 32 ? sums + units : 0, room = (ctas <= sms ? RS_SMEM : RS_SMEM_TWO) - 1024 - beside;
+  const int beside = T <= 32 ? sums + units : 0, room = (ctas <= rs_one(gate ? 2 * s.split : s.split, sms) ? RS_SMEM : RS_SMEM_TWO) - 1024 - beside;
   s.stages = room / s.stage_bytes;
   if (s.stages > RS_MAX_STAGES) s.stages = RS_MAX_STAGES;
   if (s.stages > blocks) s.stages = (int)blocks;
@@ -338,7 +345,7 @@ int launch_rows8_stream(const ProductParams& o, const void* xc, const void* xs, 
   if (!rc) rc = r8_scale_map(&msw, ws, o.N, quads, 1);
   if (rc) return rc;
   MB_CHECK_CUDA((device_info::allow_shared<rows8_stream_kernel<OUT, COLS>>(RS_SMEM)));
-  const int64_t tiles = GATE ? (o.N + 255) / 256 * 2 : (o.N + 127) / 128;
+  const int64_t tiles = rows8_stream_tiles(o.N, GATE);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * p.split));
   cfg.blockDim = dim3(RS_THREADS);

@@ -170,6 +170,24 @@ def test_gate(T, H, K):
     U.assert_rows_near(rows.codes, rows.scales, g, far)
 
 
+@pytest.mark.parametrize("T,N,K", [(33, 4096, 1024), (65, 4096, 2048), (100, 2048, 1900), (128, 5120, 2560), (96, 8192, 1024), (48, 2560, 4096), (16, 2048, 4096), (40, 16384, 512)])
+def test_splits_of_few_tokens(T, N, K):
+    """The sizes at which a product for a few tokens changes how many CTAs take its features, and how many of them an SM holds; the same bits each time."""
+    x, w = random_rows(T, K, T + K), random_rows(N, K, N + K, 1.5 * K ** -0.5)
+    y, off = U.product(U.numbers(x.codes, x.scales, K), U.numbers(w.codes, w.scales, K))
+    got = mi.multiply_rows(x, w, dtype=torch.float32)
+    assert ((got.double() - y).abs() <= off).all()
+    gate, up = y[:, 0::2], y[:, 1::2]
+    g = gate * torch.sigmoid(gate) * up
+    far = 1.1 * off[:, 0::2] * (up.abs() + off[:, 1::2]) + gate.abs() * off[:, 1::2] + g.abs() * (8 + gate.abs() / 2) * 2.0 ** -22
+    rows = mi.gate_rows(x, w)
+    U.assert_rows_near(rows.codes, rows.scales, g, far)
+    for _ in range(3):
+        assert torch.equal(mi.multiply_rows(x, w, dtype=torch.float32), got)
+        again = mi.gate_rows(x, w)
+        assert torch.equal(again.codes, rows.codes) and torch.equal(again.scales, rows.scales)
+
+
 def test_scales_of_every_row_and_block_reach_their_products():
     """One entry a block: every power is seen by itself."""
     for T, N in ((4, 260), (40, 130), (300, 260)):
