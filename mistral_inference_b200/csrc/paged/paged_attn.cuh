@@ -206,7 +206,6 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int split = blockIdx.x, splits = gridDim.x, g = blockIdx.y % p.KV, qt = blockIdx.y / p.KV, b = blockIdx.z;
   const int R = p.H / p.KV;
-  pdl_trigger();
   if (tid < kHeadDim) nan_new[tid] = nan_old[tid] = 0;
   if (tid == 0) {
     for (int i = 0; i < PA_STAGES; ++i) {
@@ -227,6 +226,7 @@ __global__ void __launch_bounds__(PaCfg<NQ>::kThreads, PaCfg<NQ>::kResident) pag
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  pdl_trigger();  // behind the columns' allocation: a dependent that takes its own may come onto this SM
   pdl_wait();
 
   const int t_first = p.q_start[b], n_all = p.q_start[b + 1] - t_first, past = p.seqpos[b], row = p.rows[b];

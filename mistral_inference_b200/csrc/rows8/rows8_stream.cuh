@@ -289,6 +289,11 @@ __global__ void __launch_bounds__(RS_THREADS) rows8_stream_kernel(const __grid_c
 // ---- host ----
 constexpr int RS_SMEM = 225 * 1024;  // (beside what the kernel names)
 constexpr int RS_SMEM_TWO = 110 * 1024;  // two CTAs an SM
+// The least a CTA asks for, by columns of tensor memory: 228 KB an SM end before its 512 columns do.  An SM takes CTAs by shared memory alone, and one that found no columns would wait for those of other
+// clusters, whose own CTAs may wait for its cluster's on another SM (gated units of 128 tokens with few k-blocks, or products on several streams).
+constexpr int RS_SMEM_COLUMN = 430;
+static_assert(RS_SMEM_COLUMN * (512 + 32) > 228 * 1024 && RS_SMEM_COLUMN * 2 * RS_MAX_T <= RS_SMEM_TWO, "columns come in multiples of 32");
+inline int rs_larger(int a, int b) { return a > b ? a : b; }
 inline int rs_up(int n, int step) { return (n + step - 1) / step * step; }
 // CTAs that run at once.  A cluster lies within one GPC, so they are fewer than the SMs hold; of 148 SMs, by the CTAs of a cluster: two an SM 6 270, 7 259, 8 264 (of 288 in clusters of six some
 // began when others had ended); one an SM 2 148, 4 132, 5 130, 7 105, 8 120 (gated units of 4000 x 4096, 1 token, 128 CTAs in clusters of eight: 15.1 us one an SM, two an SM 8.4)
@@ -326,8 +331,8 @@ inline size_t rows8_stream_layout(StreamParams& s, int64_t T, int64_t N, int64_t
   const int ring = s.stages * s.stage_bytes;
   s.sums_at = beside > 0 ? ring : 0;
   s.units_at = s.sums_at + sums;
-  const int end = s.units_at + units;
-  return (size_t)(ring > end ? ring : end) + 1024;
+  const int end = s.units_at + units, least = 2 * cols * RS_SMEM_COLUMN;
+  return (size_t)rs_up(rs_larger(rs_larger(ring, end) + 1024, least), 16);
 }
 
 template <int OUT, int COLS>

@@ -188,6 +188,25 @@ def test_splits_of_few_tokens(T, N, K):
         assert torch.equal(again.codes, rows.codes) and torch.equal(again.scales, rows.scales)
 
 
+def test_many_clusters_of_little_shared_memory():
+    """Each token column takes two columns of tensor memory, of which an SM has 512: more CTAs than that come one after another, whatever their shared memory, on one stream and on four."""
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for T, N, K in ((128, 40000, 128), (128, 4096, 1024), (64, 40000, 128), (100, 4096, 512)):
+        x, w = random_rows(T, K, T + K), random_rows(N, K, N + K, 1.5 * K ** -0.5)
+        want, units = mi.multiply_rows(x, w), mi.gate_rows(x, w)
+        torch.cuda.synchronize()
+        got = []
+        for i in range(24):
+            with torch.cuda.stream(streams[i % 4]):
+                got.append(mi.multiply_rows(x, w) if i % 3 == 0 else mi.gate_rows(x, w))
+        torch.cuda.synchronize()
+        for i, g in enumerate(got):
+            if i % 3 == 0:
+                assert torch.equal(g, want), (T, N, K, i)
+            else:
+                assert torch.equal(g.codes, units.codes) and torch.equal(g.scales, units.scales), (T, N, K, i)
+
+
 def test_scales_of_every_row_and_block_reach_their_products():
     """One entry a block: every power is seen by itself."""
     for T, N in ((4, 260), (40, 130), (300, 260)):
