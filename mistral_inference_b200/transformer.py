@@ -97,6 +97,7 @@ class Transformer(nn.Module):
             if hasattr(blk.feed_forward, "layer_parity"):
                 blk.feed_forward.layer_parity = j & 1
         self.weights8 = False                            # the Linears are 8-bit rows (quantise_weights)
+        self._quantising = False                         # ... some of them: a call that did not finish
         self._output8: Optional[rows8.Rows8] = None      # ... the lm head as well
         self._ws: Optional[_abi.Workspace] = None
         self._ws_tokens = 0
@@ -156,6 +157,11 @@ class Transformer(nn.Module):
     def _check_runnable(self) -> None:
         if self.device.type != "cuda" or self.dtype != torch.bfloat16:
             raise _abi.Mb200Error(f"the libmb200 hot path runs bf16 on CUDA only (got {self.dtype} on {self.device}); no fallback exists")
+        self._check_whole()
+
+    def _check_whole(self) -> None:
+        if self._quantising:
+            raise _abi.Mb200Error("quantise_weights did not finish, some matrices are in 8 bits and the others are not: call it again")
 
     @torch.inference_mode()
     def forward_partial(self, input_ids: torch.Tensor, seqlens: List[int], cache: Optional[BufferCache] = None,
@@ -357,6 +363,7 @@ class Transformer(nn.Module):
         needs no host write at all (a pinned staging buffer rewritten by the host while earlier copies are still queued was the
         round-1 design and a race).  Returns the STATIC fp32 logits buffer [B, V] (overwritten by the next step).  The first call
         per (cache, batch) runs eagerly (warm-up: loads modules, sets function attributes), the second captures."""
+        self._check_whole()
         B = tokens.shape[0]
         if self._megakernel_ok(B) and not cache.paged:
             return self._decode_megakernel(tokens, cache)
@@ -638,28 +645,35 @@ class Transformer(nn.Module):
     @torch.no_grad()
     def quantise_weights(self, head: bool = False) -> "Transformer":
         """Keeps every layer's matrices as 8-bit rows (rows8.py: e4m3 with a power of two for each 128 entries of a row), with `head` the lm head too, and runs the Linears on 8-bit
-        activations.  The 16-bit matrices are given up: no state dict, loading or merging afterwards.  Dense models on one pipeline stage."""
-        self._check_runnable()
-        if self.args.moe is not None or self.num_pipeline_ranks != 1:
+        activations.  The 16-bit matrices are given up, layer by layer: no state dict, loading or merging afterwards.  A call that fails on its way (memory) leaves a model that does nothing but
+        go on where it stopped, when it is called again.  Dense models on one pipeline stage."""
+        if self.device.type != "cuda" or self.dtype != torch.bfloat16:
+            raise _abi.Mb200Error(f"8-bit weights: of bf16 models on CUDA only (got {self.dtype} on {self.device})")
+        if self.args.moe is not None or self.num_pipeline_ranks != 1 or self.output_weight is None:
             raise _abi.Mb200Error("8-bit weights: dense models on one pipeline stage only")
         if self.weights8:
             raise _abi.Mb200Error("the weights are in 8 bits already")
-        for layer in self.layers.values():
-            layer.quantise()
+        torch.cuda.synchronize(self.device)  # whatever still reads the 16-bit matrices ends before their memory is given back
+        self._quantising = True
+        try:
+            for layer in self.layers.values():
+                if layer.attention.wqkv8 is None:
+                    layer.quantise()
+            if head and self._output8 is None:
+                self._output8 = rows8.quantise_rows(self.output_weight.data)
+                self.output_weight.data = self.output_weight.data.new_empty(0)
+            torch.cuda.synchronize(self.device)
+        except BaseException:
+            self._quantising = any(layer.attention.wqkv8 is not None for layer in self.layers.values())  # (a layer gives up its matrices together, behind the last one's rows)
+            raise
         kept = [r for layer in self.layers.values() for r in (layer.attention.wqkv8, layer.attention.wo8, layer.feed_forward.w13_8, layer.feed_forward.w2_8)]
-        if head:
-            assert self.output_weight is not None
-            self._output8 = rows8.quantise_rows(self.output_weight.data)
-            kept.append(self._output8)
-            self.output_weight.data = self.output_weight.data.new_empty(0)
-        torch.cuda.synchronize(self.device)
-        for r in kept:
+        for r in kept + ([self._output8] if self._output8 is not None else []):
             r.fixed = True  # what wrote it has ended
-        self.weights8 = True
+        self.weights8, self._quantising = True, False
         return self
 
     def _check_16_bit(self, what: str) -> None:
-        if self.weights8:
+        if self.weights8 or self._quantising:
             raise _abi.Mb200Error(f"{what}: the weights are in 8 bits (quantise_weights)")
 
     # ------------------------------------------------------------------ LoRA, merged path (lora.py:92-155 with args.lora is None)

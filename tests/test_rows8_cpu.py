@@ -1,12 +1,14 @@
 """The boundary and refusals of libmb200_rows8, without a GPU: everything here is turned away before a kernel is launched."""
 import re
+import types
 from pathlib import Path
 
 import pytest
 import torch
 
 import mistral_inference_b200 as mi
-from mistral_inference_b200 import _abi_rows8
+from mistral_inference_b200 import _abi, _abi_rows8
+from mistral_inference_b200 import rows8 as operators
 from mistral_inference_b200.build import build_rows8
 from mistral_inference_b200.rows8 import Rows8
 
@@ -160,3 +162,69 @@ def test_command_line_refuses_8_bits_of_other_designs(tmp_path):
     (tmp_path / "config.json").write_text('{"architecture": "Fesenex"}')
     with pytest.raises(SystemExit):
         main(["generate", str(tmp_path), "--prompt", "1", "--weights", "e4m3"])
+
+
+# ----------------------------------------------------------------------------------------------------- a model's weights
+class Failing:
+    """quantise_rows of a GPU that has memory for `room` matrices; rows that nobody reads."""
+
+    def __init__(self, room):
+        self.room = room
+
+    def __call__(self, x):
+        if self.room == 0:
+            raise torch.OutOfMemoryError("no room")
+        self.room -= 1
+        return rows(x.shape[0], x.shape[1])
+
+
+@pytest.fixture
+def model(monkeypatch):
+    """A model on the CPU that takes itself to be on a GPU: what is tested here ends before anything is launched there."""
+    from mistral_inference_b200.transformer import Transformer
+    args = mi.TransformerArgs(dim=64, n_layers=3, head_dim=16, hidden_dim=96, n_heads=4, n_kv_heads=2, norm_eps=1e-5, vocab_size=80, max_batch_size=2)
+    m = Transformer.empty(args, "cpu", torch.bfloat16)
+    monkeypatch.setattr(Transformer, "device", property(lambda self: torch.device("cuda")))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    return m
+
+
+def refusals(m):
+    cache = types.SimpleNamespace(paged=False, _kv_seqlens_host=[5], cache_sizes=[9])
+    one = torch.zeros(1, dtype=torch.long)
+    return [lambda: m.forward(one, [1]), lambda: m.forward(one, [1], cache), lambda: m.forward_partial(one, [1]), lambda: m.decode_static(one, cache), lambda: m.next_token_logits(one, cache),
+            lambda: m.forward_logprobs(one, [1], None, one), lambda: m.forward_scores(one, [1], None, one, 2), m.state_dict, lambda: m.load_state_dict({}),
+            lambda: m._load_lora_state_dict({"lora": torch.zeros(1, dtype=torch.bfloat16)})]
+
+
+@pytest.mark.parametrize("room", [4, 7, 12])  # at the second layer's first matrix, its last one, and the head
+def test_weights_that_were_quantised_half_way(model, monkeypatch, room):
+    """Memory that ends on the way leaves matrices of both kinds: nothing runs on them, until a second call has gone on behind the first."""
+    monkeypatch.setattr(operators, "quantise_rows", Failing(room))
+    with pytest.raises(torch.OutOfMemoryError):
+        model.quantise_weights(head=True)
+    done = [layer.attention.wqkv8 for layer in model.layers.values()]
+    assert [d is not None for d in done] == [room >= 4, room >= 8, room >= 12] and not model.weights8
+    for call in refusals(model):
+        with pytest.raises(_abi.Mb200Error, match="8 bits"):
+            call()
+    monkeypatch.setattr(operators, "quantise_rows", Failing(13))
+    assert model.quantise_weights(head=True) is model and model.weights8
+    for layer, before in zip(model.layers.values(), done):
+        assert before is None or layer.attention.wqkv8 is before
+        for r, n, k in ((layer.attention.wqkv8, 128, 64), (layer.attention.wo8, 64, 64), (layer.feed_forward.w13_8, 192, 64), (layer.feed_forward.w2_8, 64, 96)):
+            assert r.fixed and (r.rows, r.cols) == (n, k)
+    assert model._output8.fixed and model.output_weight.numel() == 0
+    with pytest.raises(_abi.Mb200Error, match="already"):
+        model.quantise_weights()
+    with pytest.raises(_abi.Mb200Error, match="8 bits"):
+        model.state_dict()
+
+
+def test_weights_of_which_none_was_quantised(model, monkeypatch):
+    """Memory that ends at the first layer has changed nothing."""
+    monkeypatch.setattr(operators, "quantise_rows", Failing(3))
+    with pytest.raises(torch.OutOfMemoryError):
+        model.quantise_weights()
+    model._check_runnable()
+    assert len(model.state_dict()) == 3 + 3 * 9 and all(v.numel() > 0 for v in model.state_dict().values())
