@@ -44,6 +44,11 @@ class Rows8:
         assert 0 <= rows <= MAX_ROWS and 1 <= cols <= MAX_ROWS, f"{rows} rows of {cols} entries (at most {MAX_ROWS})"
         return Rows8(torch.empty(rows, _width(cols), dtype=_E4M3, device=device), torch.empty(_tiles(rows, cols), dtype=_E8M0, device=device), cols)
 
+    def to(self, device) -> "Rows8":
+        """On another device (itself where it is there already)."""
+        codes = self.codes.to(device)
+        return self if codes is self.codes else Rows8(codes, self.scales.to(device), self.cols)
+
     def _blocks(self, tiles: torch.Tensor) -> torch.Tensor:
         """Bytes in tiles as [rows, blocks]."""
         n, quads = tiles.shape[:2]

@@ -99,6 +99,7 @@ class Transformer(nn.Module):
         self.weights8 = False                            # the Linears are 8-bit rows (quantise_weights)
         self._quantising = False                         # ... some of them: a call that did not finish
         self._output8: Optional[rows8.Rows8] = None      # ... the lm head as well
+        self._moves = 0                                  # how often the parameters got other memory
         self._ws: Optional[_abi.Workspace] = None
         self._ws_tokens = 0
         self.last_argmax: Optional[torch.Tensor] = None  # device token id(s) written by the last fused-argmax decode step
@@ -294,7 +295,7 @@ class Transformer(nn.Module):
         reallocated since (a captured graph holds the old pointer)."""
         states = cache.__dict__.setdefault("_mb200_decode_states", {})
         ws_ptr = self._ws.ptr if self._ws is not None else 0
-        key = (id(self), self.weights8, key)  # (a graph captured before quantise_weights reads matrices that are gone)
+        key = (id(self), self.weights8, self._moves, key)  # (a graph captured before quantise_weights, or before a move, reads matrices that are gone)
         st = states.get(key)
         if st is None or st["ws_ptr"] != ws_ptr or st["device"] != self.device:
             st = {"ws_ptr": ws_ptr, "device": self.device}
@@ -666,10 +667,30 @@ class Transformer(nn.Module):
         except BaseException:
             self._quantising = any(layer.attention.wqkv8 is not None for layer in self.layers.values())  # (a layer gives up its matrices together, behind the last one's rows)
             raise
-        kept = [r for layer in self.layers.values() for r in (layer.attention.wqkv8, layer.attention.wo8, layer.feed_forward.w13_8, layer.feed_forward.w2_8)]
-        for r in kept + ([self._output8] if self._output8 is not None else []):
-            r.fixed = True  # what wrote it has ended
+        for owner, name in self._matrices8():
+            getattr(owner, name).fixed = True  # what wrote it has ended
         self.weights8, self._quantising = True, False
+        return self
+
+    def _matrices8(self) -> List[Tuple[nn.Module, str]]:
+        """Where the 8-bit matrices are kept."""
+        places: List[Tuple[nn.Module, str]] = [(self, "_output8")]
+        for layer in self.layers.values():
+            places += [(layer.attention, "wqkv8"), (layer.attention, "wo8"), (layer.feed_forward, "w13_8"), (layer.feed_forward, "w2_8")]
+        return [(owner, name) for owner, name in places if getattr(owner, name, None) is not None]
+
+    def _apply(self, fn: Any, recurse: bool = True) -> "Transformer":
+        """What `to`, `cuda` and `cpu` go through: 8-bit matrices follow the parameters to their device, and stay what they are whatever type those get."""
+        memory = [p.data_ptr() for p in self.parameters()]
+        super()._apply(fn, recurse)
+        moved = [(owner, name) for owner, name in self._matrices8() if getattr(owner, name).codes.device != self.device]
+        for owner, name in moved:
+            setattr(owner, name, getattr(owner, name).to(self.device))
+        if moved and self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+            for owner, name in moved:
+                getattr(owner, name).fixed = True  # (the copies have ended)
+        self._moves += moved != [] or memory != [p.data_ptr() for p in self.parameters()]
         return self
 
     def _check_16_bit(self, what: str) -> None:

@@ -214,3 +214,27 @@ def test_rotation(T, H, KV):
         rest = torch.ones(n, dtype=torch.bool, device="cuda")
         rest[place[there]] = False
         assert (k[rest] == 7).all() and (v[rest] == 7).all()
+
+
+@pytest.mark.parametrize("B", [1, 2])
+@pytest.mark.parametrize("head", [None, True])
+def test_a_model_that_was_moved_goes_on(B, head):
+    """To the host and back between the steps of a cache: what was captured before reads memory that is gone."""
+    m, p = model_of(head=head)
+    still, _ = model_of(head=head)
+    caches = [m.make_cache(B, 100), still.make_cache(B, 100)]
+    ids = (torch.arange(20 * B) % p["vocab_size"]).cuda()
+    nxt = torch.arange(5, 5 + B, device="cuda")
+    for model, cache in zip((m, still), caches):
+        model.forward(ids, [20] * B, cache)
+    for i in range(9):
+        if i == 4:
+            m.cpu()
+            if head:
+                with pytest.raises(Mb200Error):
+                    m.forward(nxt, [1] * B)
+            taken = [torch.full((n,), 0x7f, dtype=torch.uint8, device="cuda") for n in (1 << 20, 1 << 21, 1 << 22)]  # where the matrices were
+            m.cuda()
+            del taken
+        a, b = (model.forward(nxt + i, [1] * B, cache) for model, cache in zip((m, still), caches))
+        assert torch.equal(a, b), i

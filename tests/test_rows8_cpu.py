@@ -228,3 +228,30 @@ def test_weights_of_which_none_was_quantised(model, monkeypatch):
         model.quantise_weights()
     model._check_runnable()
     assert len(model.state_dict()) == 3 + 3 * 9 and all(v.numel() > 0 for v in model.state_dict().values())
+
+
+def test_8_bit_matrices_follow_a_model(model, monkeypatch):
+    """To another device with the parameters; a conversion of these leaves codes and scales as they are."""
+    monkeypatch.setattr(operators, "quantise_rows", Failing(100))
+    model.quantise_weights(head=True)
+    monkeypatch.undo()
+
+    def kept():
+        return [model._output8] + [r for b in model.layers.values() for r in (b.attention.wqkv8, b.attention.wo8, b.feed_forward.w13_8, b.feed_forward.w2_8)]
+    before = kept()
+    model.to("cpu").float().bfloat16()
+    assert all(a is b for a, b in zip(before, kept()))
+    model.to("meta")
+    for a, b in zip(before, kept()):
+        assert b.codes.device.type == b.scales.device.type == "meta" and (b.rows, b.cols) == (a.rows, a.cols) and (b.codes.dtype, b.scales.dtype) == (a.codes.dtype, a.scales.dtype)
+        assert not b.fixed
+
+
+def test_steps_captured_before_a_move_are_not_replayed():
+    from mistral_inference_b200.transformer import Transformer
+    args = mi.TransformerArgs(dim=64, n_layers=1, head_dim=16, hidden_dim=96, n_heads=4, n_kv_heads=2, norm_eps=1e-5, vocab_size=80)
+    m, cache = Transformer.empty(args, "cpu", torch.bfloat16), types.SimpleNamespace()
+    first = m._decode_state(cache, "step")
+    assert m.to("cpu")._decode_state(cache, "step") is first  # (nothing moved)
+    m.float().bfloat16()
+    assert m._decode_state(cache, "step") is not first
