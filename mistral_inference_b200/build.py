@@ -5,6 +5,7 @@ In-tree, so that a copy of the checkout carries its built libraries with it (a J
 """
 import hashlib
 import os
+import re
 import subprocess
 import sys
 from pathlib import Path
@@ -64,12 +65,24 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
-def _build_small(src: Path, lib: Path, others, flags=(), force: bool = False) -> Path:
-    """A library of its own of the sources in `src` (and of `others`, which they include), so that who needs only it compiles only them (seconds).  Safe when several
+_INCLUDE = re.compile(r'^\s*#\s*include\s+"([^"]+)"', re.M)
+
+
+def _with_included(sources) -> list:
+    """The sources and all files of the checkout that they include."""
+    found = todo = {f.resolve() for f in sources}
+    while todo:
+        todo = {f for p in todo for f in ((p.parent / name).resolve() for name in _INCLUDE.findall(p.read_text())) if f.exists()} - found
+        found = found | todo
+    return sorted(found)
+
+
+def _build_small(src: Path, lib: Path, flags=(), force: bool = False) -> Path:
+    """A library of its own of the sources in `src` (and of what they include), so that who needs only it compiles only them (seconds).  Safe when several
     processes start at once: the output is written under a private name and renamed."""
     sources = sorted(src.glob("*.cu"))
     h = hashlib.sha256()
-    for f in sources + sorted(src.glob("*.cuh")) + sorted(src.glob("*.h")) + list(others):
+    for f in _with_included(sources):
         h.update(f.name.encode())
         h.update(f.read_bytes())
     h.update(" ".join(NVCC_FLAGS).encode())
@@ -89,14 +102,13 @@ def _build_small(src: Path, lib: Path, others, flags=(), force: bool = False) ->
     return lib
 
 
-INCLUDE = PKG.parent / "include"
 HYBRID_SRC = CSRC / "hybrid"
 HYBRID_LIB = PKG / "libmb200_hybrid.so"
 
 
 def build_hybrid(force: bool = False) -> Path:
     """libmb200_hybrid.so: the kernels of layered decoders (csrc/hybrid/)."""
-    return _build_small(HYBRID_SRC, HYBRID_LIB, [CSRC / "stream_linear.cuh", CSRC / "device_info.cuh"] + sorted(INCLUDE.glob("mistral_b200_hybrid*.h")), ("--threads", "0"), force)
+    return _build_small(HYBRID_SRC, HYBRID_LIB, ("--threads", "0"), force)
 
 
 PAGED_SRC = CSRC / "paged"
@@ -105,9 +117,7 @@ PAGED_LIB = PKG / "libmb200_paged.so"
 
 def build_paged(force: bool = False) -> Path:
     """libmb200_paged.so: pages of 8-bit keys and values and the scores of tokens (csrc/paged/)."""
-    headers = ["common.cuh", "device_info.cuh", "epilogue.cuh", "sigmoid.cuh", "gemm_tcgen05.cuh", "gemm_mma.cuh", "split_schedule.cuh", "decode_megakernel.cuh", "attn_decode.cuh",
-               "attn_prompt_tcgen05.cuh"]
-    return _build_small(PAGED_SRC, PAGED_LIB, [CSRC / h for h in headers] + [INCLUDE / h for h in ("mistral_b200.h", "mistral_b200_paged.h")], force=force)
+    return _build_small(PAGED_SRC, PAGED_LIB, force=force)
 
 
 ROWS8_SRC = CSRC / "rows8"
@@ -116,8 +126,7 @@ ROWS8_LIB = PKG / "libmb200_rows8.so"
 
 def build_rows8(force: bool = False) -> Path:
     """libmb200_rows8.so: Linears of 8-bit numbers (csrc/rows8/)."""
-    headers = ["common.cuh", "device_info.cuh", "epilogue.cuh", "sigmoid.cuh", "gemm_tcgen05.cuh", "gemm_mma.cuh", "split_schedule.cuh", "decode_megakernel.cuh", "gemm_pair.cuh", "paged/paged_common.cuh"]
-    return _build_small(ROWS8_SRC, ROWS8_LIB, [CSRC / h for h in headers] + [INCLUDE / h for h in ("mistral_b200.h", "mistral_b200_paged.h", "mistral_b200_rows8.h")], force=force)
+    return _build_small(ROWS8_SRC, ROWS8_LIB, force=force)
 
 
 ROWS8_HOST = PKG / "mb200_rows8_host.so"
@@ -134,7 +143,7 @@ def build_rows8_host(force: bool = False) -> Path:
     flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     includes = [str(top / "include"), str(top / "include" / "torch" / "csrc" / "api" / "include"), sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
     h = hashlib.sha256()
-    for f in (src, INCLUDE / "mistral_b200_rows8.h"):
+    for f in _with_included([src]):
         h.update(f.read_bytes())
     h.update(" ".join(flags + [torch.__version__, sys.version]).encode())
     digest = h.hexdigest()

@@ -45,3 +45,23 @@ def test_limits_of_waits_count_from_the_predecessors_end(name, start, wait):
     for role in roles:
         ends = [i for i in (role.find("pdl_wait()"), role.find("griddepcontrol.wait")) if i >= 0]
         assert ends and min(ends) < role.index(wait), role[:300]
+
+
+INCLUDES = re.compile(r'^\s*#\s*include\s+"([^"]+)"', re.M)
+
+
+@pytest.mark.parametrize("name,folder", [("build_library", ""), ("build_hybrid", "hybrid"), ("build_paged", "paged"), ("build_rows8", "rows8"), ("build_rows8_host", "rows8")])
+def test_a_library_is_built_again_when_a_file_that_it_includes_changes(name, folder, monkeypatch):
+    """What decides that is a digest of files: all that its sources include are among them."""
+    from mistral_inference_b200 import build
+    getattr(build, name)()
+    read, whole = set(), Path.read_bytes
+    with monkeypatch.context() as m:
+        m.setattr(Path, "read_bytes", lambda self: read.add(self.resolve()) or whole(self))
+        getattr(build, name)()
+    found = todo = set((CSRC / folder).glob("*.cpp" if name.endswith("host") else "*.cu"))
+    assert found
+    while todo:
+        todo = {f for p in todo for f in ((p.parent / i).resolve() for i in INCLUDES.findall(p.read_text())) if f.exists()} - found
+        found = found | todo
+    assert not {str(p) for p in found} - {str(p) for p in read}
