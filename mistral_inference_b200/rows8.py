@@ -87,9 +87,10 @@ def norm_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, add: Optional[t
     return Rows8(codes, scales, x.shape[1]), x if h is None else h
 
 
-def multiply_rows(x: Rows8, w: Rows8, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x [T, K] times w [N, K] transposed: [T, N] bf16 or fp32, summed in fp32 and rounded once.  `out`: results of the caller's, rows may be part of wider ones."""
-    assert dtype is _BF16 or dtype is _F32, f"bf16 or fp32 results, got {dtype}"
+def multiply_rows(x: Rows8, w: Rows8, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [T, K] times w [N, K] transposed: [T, N] bf16 (without `dtype`) or fp32, summed in fp32 and rounded once.  `out`: results of the caller's, of its type; rows may be part of wider ones."""
+    assert dtype is None or dtype is _BF16 or dtype is _F32, f"bf16 or fp32 results, got {dtype}"
+    assert out is None or dtype is None or getattr(out, "dtype", dtype) is dtype, f"results of type {dtype}, and out of another"
     return (_host or _load()).multiply(x.codes, x.scales, x.cols, w.codes, w.scales, w.cols, w.fixed, dtype is _F32, out)
 
 

@@ -441,3 +441,12 @@ def test_results_of_empty_and_refused_calls():
                  lambda: mi.norm_rows(normal((2, 70), 1), normal((70,), 1), 1e-5, add=normal((2, 71), 1)), lambda: mi.quantise_rows(normal((2, 70), 1).half())):
         with pytest.raises(AssertionError):
             call()
+
+
+def test_results_take_the_type_of_out():
+    x, w = random_rows(5, 300, 1), random_rows(40, 300, 2)
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.empty(5, 40, dtype=dtype, device=DEV)
+        for said in (None, dtype):
+            assert mi.multiply_rows(x, w, dtype=said, out=out) is out and torch.equal(out, mi.multiply_rows(x, w, dtype=dtype))
+    assert mi.multiply_rows(x, w).dtype is torch.bfloat16

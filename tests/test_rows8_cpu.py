@@ -97,6 +97,15 @@ def test_python_refuses_what_does_not_fit():
         Rows8.empty(2, BIG, "cpu")
 
 
+@pytest.mark.parametrize("dtype,other", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_results_of_another_type_than_asked_for_are_refused(dtype, other):
+    with pytest.raises(AssertionError, match="of another"):
+        mi.multiply_rows(rows(2, 9), rows(3, 9), dtype=dtype, out=torch.zeros(2, 3, dtype=other))
+    for said in (None, dtype):
+        with pytest.raises(AssertionError, match="no fallback"):
+            mi.multiply_rows(rows(2, 9), rows(3, 9), dtype=said, out=torch.zeros(2, 3, dtype=dtype))
+
+
 def test_what_is_no_tensor_is_refused():
     bf = torch.zeros(2, 3, dtype=torch.bfloat16)
     for call in (lambda: mi.quantise_rows(None), lambda: mi.quantise_rows([[1.0]]), lambda: mi.norm_rows(bf, None, 1e-5), lambda: mi.multiply_rows(Rows8(None, None, 3), rows(3, 9)),
