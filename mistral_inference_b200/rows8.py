@@ -61,7 +61,7 @@ class Rows8:
     def numbers(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """[rows, cols]: what the codes stand for (exact in 16 bits as well)."""
         power = self._blocks(self.scales.view(torch.uint8)).contiguous().view(_E8M0).float()
-        return (self.codes.float().view(self.rows, -1, BLOCK) * power[:, :, None]).view(self.rows, -1)[:, : self.cols].to(dtype)
+        return (self.codes.float().view(self.rows, power.shape[1], BLOCK) * power[:, :, None]).view(self.codes.shape)[:, : self.cols].to(dtype)
 
 
 _host = None  # the extension that checks, allocates and launches (csrc/rows8/rows8_host.cpp), once a call needed it

@@ -137,6 +137,12 @@ def test_numbers_and_exponents(R, K):
     assert ((r.numbers(torch.float64) - x.double()).abs() <= torch.maximum(x.double().abs() * 2.0 ** -4, size * 2.0 ** -10)).all()
 
 
+@pytest.mark.parametrize("K", [1, 300])
+def test_numbers_and_exponents_of_no_rows(K):
+    r = rows(0, K)
+    assert r.numbers().shape == r.numbers(torch.bfloat16).shape == (0, K) and r.exponents().shape == (0, -(-K // 128))
+
+
 def test_the_restatement_refuses_wrong_rows():
     """What the GPU tests hold results to, held to mistakes: a code, a power, a place of no row."""
     x = torch.randn(40, 300, generator=torch.Generator().manual_seed(1)).double()
