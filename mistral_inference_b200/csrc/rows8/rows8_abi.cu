@@ -101,7 +101,7 @@ int mb8_norm(const void* x, int64_t ld, const void* add, int64_t ld_add, const v
 
 int64_t mb8_product_scratch(int64_t T, int64_t N, int64_t K) {
   const int sms = device_info::sm_count();
-  return T <= RS_MAX_T || N < 1 || K < 1 || sms < 2 ? 0 : rows8_pair_scratch(T, N, K, sms);
+  return T <= RS_MAX_T || T > MB8_MAX_ROWS || N < 1 || N > MB8_MAX_ROWS || K < 1 || K > MB8_MAX_ROWS || sms < 2 ? 0 : rows8_pair_scratch(T, N, K, sms);
 }
 
 int mb8_multiply(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int64_t ld, int dtype, int64_t T, int64_t N, int64_t K, int w_fixed,
@@ -121,7 +121,7 @@ int mb8_multiply(const void* x_codes, const void* x_scales, const void* w_codes,
 
 int mb8_gate(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* codes, void* scales, int64_t T, int64_t H, int64_t K, int w_fixed,
              void* scratch, int64_t scratch_bytes, void* stream) {
-  int rc = check_sizes("gate", T, 2 * H, K);
+  int rc = check_sizes("gate", T, H < 1 || H > MB8_MAX_ROWS ? 0 : 2 * H, K);
   if (rc || T == 0) return rc;
   rc = check_rows("gate", codes, scales);
   if (rc) return rc;
@@ -138,7 +138,7 @@ int mb8_gate(const void* x_codes, const void* x_scales, const void* w_codes, con
 
 int mb8_rotate(const void* qkv, const float* rope, const int32_t* positions, const int32_t* rows, void* q, void* k, void* v, int64_t T, int64_t n_heads, int64_t n_kv_heads,
                void* stream) {
-  MB_CHECK_ARG(T >= 0 && T <= MB8_MAX_ROWS && n_heads >= 1 && n_kv_heads >= 1 && n_heads + 2 * n_kv_heads <= 65536, "rotate: %lld tokens, %lld + 2 * %lld heads", (long long)T,
+  MB_CHECK_ARG(T >= 0 && T <= MB8_MAX_ROWS && n_heads >= 1 && n_kv_heads >= 1 && n_heads <= 65536 && n_kv_heads <= 65536 && n_heads + 2 * n_kv_heads <= 65536, "rotate: %lld tokens, %lld + 2 * %lld heads", (long long)T,
                (long long)n_heads, (long long)n_kv_heads);
   if (T == 0) return MB200_OK;
   MB_CHECK_ARG(qkv && rope && positions && q && k && v, "rotate: null pointer");

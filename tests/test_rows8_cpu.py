@@ -80,6 +80,24 @@ def test_products_are_refused(lib):
     assert multiply(T=0, out=None, xc=None) == gate(T=0, codes=None, xc=None) == 0
 
 
+def test_sizes_whose_doubles_are_no_sizes_are_refused(lib):
+    for H in (-(2 ** 63) + 1, -(2 ** 63) + 64, 2 ** 62 + 1, 2 ** 63 - 1):
+        assert lib.mb8_gate(X, X, X, X, X, X, 2, H, 256, 0, None, 0, None) == -1 and "features" in last(lib), H
+    for heads, kv in ((1, 2 ** 62 + 5), (1, 2 ** 63 - 1), (2 ** 63 - 1, 1), (2 ** 63 - 4, 2 ** 62)):
+        assert lib.mb8_rotate(X, X, X, None, X, X, X, 2, heads, kv, None) == -1 and "heads" in last(lib), (heads, kv)
+    for sizes in ((2 ** 62, 256, 256), (300, 2 ** 62, 256), (300, 256, 2 ** 62), (300, 2 ** 63 - 1, 2 ** 63 - 1)):
+        assert lib.mb8_product_scratch(*sizes) == 0
+
+
+def test_rotate_is_refused(lib):
+    def call(qkv=X, rope=X, positions=X, q=X, k=X, v=X, T=2, heads=4, kv=2):
+        return lib.mb8_rotate(qkv, rope, positions, None, q, k, v, T, heads, kv, None)
+    for kw, why in [(dict(qkv=None), "null"), (dict(rope=None), "null"), (dict(positions=None), "null"), (dict(q=None), "null"), (dict(k=None), "null"), (dict(v=None), "null"), (dict(q=X + 8), "16 bytes"),
+                    (dict(T=-1), "tokens"), (dict(T=BIG), "tokens"), (dict(heads=0), "heads"), (dict(kv=0), "heads"), (dict(heads=65535), "heads")]:
+        assert call(**kw) == -1 and why in last(lib), (kw, last(lib))
+    assert call(T=0, qkv=None) == 0
+
+
 def rows(R, K):
     return Rows8.empty(R, K, "cpu")
 
