@@ -450,3 +450,14 @@ def test_results_take_the_type_of_out():
         for said in (None, dtype):
             assert mi.multiply_rows(x, w, dtype=said, out=out) is out and torch.equal(out, mi.multiply_rows(x, w, dtype=dtype))
     assert mi.multiply_rows(x, w).dtype is torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,K,offset,ld", [(16400, 1003, 0, 1003), (7000, 2561, 0, 2561), (7000, 2561, 1, 2600), (8200, 2049, 0, 2056), (8200, 2049, 3, 2056), (4096, 4096, 0, 4096), (4100, 4000, 4, 4008), (33000, 17, 5, 31)])
+def test_quantise_of_many_rows(T, K, offset, ld, dtype):
+    """From 32768 steps of 512 entries on a warp takes four of them: rows whose steps are no multiple of four, that begin anywhere, and blocks that hold no number, bit for bit."""
+    assert T * -(-K // 512) >= 32768
+    x = uneven(T, ld, T + K, dtype)[:, offset: offset + K]
+    for r, k in [(0, K - 1), (T - 1, 0), (T // 2, K // 2), (T - 130, min(K - 1, 511))]:
+        x[r, k] = math.nan if r % 2 else math.inf
+    assert_same_rows(mi.quantise_rows(x), x)
