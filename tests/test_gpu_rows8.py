@@ -461,3 +461,21 @@ def test_quantise_of_many_rows(T, K, offset, ld, dtype):
     for r, k in [(0, K - 1), (T - 1, 0), (T // 2, K // 2), (T - 130, min(K - 1, 511))]:
         x[r, k] = math.nan if r % 2 else math.inf
     assert_same_rows(mi.quantise_rows(x), x)
+
+
+@pytest.mark.parametrize("T", [100, 250])
+def test_gates_far_from_zero(T):
+    """Units of exact gates from -104 to 104 and ups up to 2^60, each in a block of its own.  Off by (3 + |gate| / 3) 2^-22 of themselves, and below -87, where silu ends, by 2^-119 of the up."""
+    gates = torch.tensor([s * m * 2.0 ** e for e in range(-2, 6) for m in (1.0, 1.125, 1.375, 1.625, 1.75) for s in (-1, 1)] + [s * v for v in (72.0, 80.0, 88.0, 96.0, 104.0) for s in (-1, 1)], device=DEV)
+    x = torch.zeros(T, 256, device=DEV)
+    i = torch.arange(T, device=DEV)
+    x[:, 0] = gates[i * 7 % len(gates)]
+    x[:, 128] = torch.exp2((i * 11 % 61).float()) * torch.where(i % 2 == 0, 1.0, -1.0)
+    w = torch.zeros(2, 256, device=DEV)
+    w[0, 0] = w[1, 128] = 1
+    a = mi.quantise_rows(x)
+    assert torch.equal(a.numbers(), x)
+    rows = mi.gate_rows(a, mi.quantise_rows(w))
+    gate, up = x[:, :1].double(), x[:, 128:129].double()
+    y = gate * torch.sigmoid(gate) * up
+    U.assert_rows_near(rows.codes, rows.scales, y, y.abs() * (3 + gate.abs() / 3) * 2.0 ** -22 + torch.where(gate < -87, 2.0 ** -119, 0.0) * up.abs())
