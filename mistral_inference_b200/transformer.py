@@ -10,7 +10,7 @@ import logging
 import math
 import os
 from pathlib import Path
-from typing import Any, Dict, List, Mapping, Optional, Tuple, Union
+from typing import Any, Dict, List, Mapping, NamedTuple, Optional, Tuple, Union
 
 import torch
 from torch import nn
@@ -50,6 +50,18 @@ class _OutputView:
     @property
     def weight(self) -> torch.Tensor:
         return self._m.output_weight
+
+
+class _Stream(NamedTuple):
+    """The stream behind the layers, h + add: with 8-bit weights the last addition is the next norm's."""
+    h: torch.Tensor
+    add: Optional[torch.Tensor] = None
+
+    def whole(self) -> torch.Tensor:
+        return self.h if self.add is None else self.h + self.add
+
+    def rows(self, r0: int, r1: int) -> "_Stream":
+        return _Stream(self.h[r0:r1], None if self.add is None else self.add[r0:r1])
 
 
 class Transformer(nn.Module):
@@ -191,7 +203,7 @@ class Transformer(nn.Module):
             h = torch.empty(num_toks, self.args.dim, device=self.device, dtype=self.dtype)
             torch.distributed.recv(h, src=self.pipeline_rank - 1)
 
-        h = self._run_layers(h, positions, cache, input_metadata, ws)
+        h = self._run_layers(h, positions, cache, input_metadata, ws).whole()
 
         if cache is not None:
             cache.update_seqlens(seqlens)
@@ -213,11 +225,11 @@ class Transformer(nn.Module):
                 outs32 = self.decode_static(input_ids, cache).clone()
                 return outs32 if self.softmax_fp32 else outs32.to(self.dtype)
             # single stage: final norm + lm head + .float() are one fused call (no [T, dim] normed round trip)
-            h = self._hidden_no_norm(input_ids, seqlens, cache)
+            stream = self._hidden_no_norm(input_ids, seqlens, cache)
             if cache is not None:
                 cache.update_seqlens(seqlens)
-            outs32 = torch.empty(h.shape[0], self.vocab_size, device=h.device, dtype=torch.float32)
-            self._head(h, outs32)
+            outs32 = torch.empty(input_ids.shape[0], self.vocab_size, device=self.device, dtype=torch.float32)
+            self._head(stream, outs32)
             return outs32 if self.softmax_fp32 else outs32.to(self.dtype)
         h = self.forward_partial(input_ids, seqlens, cache=cache)
         if not last:
@@ -231,7 +243,7 @@ class Transformer(nn.Module):
         return outs.float() if self.softmax_fp32 else outs
 
     def _hidden_no_norm(self, input_ids: torch.Tensor, seqlens: List[int], cache: Optional[BufferCache],
-                        input_metadata: Optional[List[CacheInputMetadata]] = None) -> torch.Tensor:
+                        input_metadata: Optional[List[CacheInputMetadata]] = None) -> _Stream:
         assert len(seqlens) <= self.args.max_batch_size, f"Max batch size is {self.args.max_batch_size}, got batch size of {len(seqlens)}"
         (num_toks,) = input_ids.shape
         assert sum(seqlens) == num_toks, (sum(seqlens), num_toks)
@@ -248,23 +260,24 @@ class Transformer(nn.Module):
         with _nvtx(f"mb200.layers[T={num_toks}]"):
             return self._run_layers(h, positions, cache, input_metadata, ws)
 
-    def _run_layers(self, h: torch.Tensor, positions: torch.Tensor, cache: Optional[BufferCache], input_metadata: Optional[List[CacheInputMetadata]], ws: "_abi.Workspace") -> torch.Tensor:
+    def _run_layers(self, h: torch.Tensor, positions: torch.Tensor, cache: Optional[BufferCache], input_metadata: Optional[List[CacheInputMetadata]], ws: "_abi.Workspace") -> _Stream:
         rope = self.rope_table
-        add: Optional[torch.Tensor] = None  # 8-bit weights: a layer's last addition to the stream is made by the next norm
+        add: Optional[torch.Tensor] = None
         for local_layer_id, layer in enumerate(self.layers.values()):
             view = cache.get_view(local_layer_id, input_metadata[local_layer_id]) if cache is not None else None
             if self.weights8:
                 h, add = layer.forward8(h, add, rope, positions, view, ws)
             else:
                 h = layer(h, rope, positions, view, ws)
-        return h if add is None else h + add
+        return _Stream(h, add)
 
-    def _head(self, h: torch.Tensor, out: torch.Tensor) -> None:
-        """Final norm and lm head of rows h: fp32 logits into `out`."""
+    def _head(self, stream: _Stream, out: torch.Tensor) -> None:
+        """Final norm and lm head of a stream's rows: fp32 logits into `out`."""
         assert self.norm is not None and self.output_weight is not None
         if self._output8 is not None:
-            rows8.multiply_rows(rows8.norm_rows(h, self.norm.weight, self.args.norm_eps)[0], self._output8, out=out)
+            rows8.multiply_rows(rows8.norm_rows(stream.h, self.norm.weight, self.args.norm_eps, add=stream.add)[0], self._output8, out=out)
         else:
+            h = stream.whole()
             _abi.lm_head(h, self.norm.weight, self.output_weight, out, self.args.norm_eps, self.workspace(max(h.shape[0], 1)))
 
     def _check_positions(self, cache: BufferCache, seqlens: List[int]) -> None:
@@ -400,8 +413,7 @@ class Transformer(nn.Module):
             else:
                 md = cache.metadata_from_block(st["meta"], layout, seqlens)
                 _abi.decode_meta(st["seqpos"], st["meta"], distinct)
-            h = self._hidden_no_norm(st["tokens"], seqlens, cache, md)
-            self._head(h, st["logits"])
+            self._head(self._hidden_no_norm(st["tokens"], seqlens, cache, md), st["logits"])
             _abi.argmax_rows(st["logits"], st["next"])  # greedy pick on the device (generate.py:156): feeds the next step
 
         if st["graph"] is None and not st["warmed"]:
@@ -456,13 +468,14 @@ class Transformer(nn.Module):
             _abi.logprob_gather(logits, targets, out=lp)
             return lp, logits.index_select(0, torch.tensor([e - 1 for e in ends], device=input_ids.device))
         self._check_runnable()
-        h = self._hidden_no_norm(input_ids, seqlens, cache)
+        stream = self._hidden_no_norm(input_ids, seqlens, cache)
         if cache is not None:
             cache.update_seqlens(seqlens)
         assert self.norm is not None and self.output_weight is not None
         ws = self.workspace(max(T, 1))
         if self._output8 is not None or not _abi.lm_head_logprobs_ok(T, self.args.dim, V):
-            return self._logprobs_of_written_logits(h, targets, ends, lp)
+            return self._logprobs_of_written_logits(stream, targets, ends, lp)
+        h = stream.whole()
         keep = torch.full((T,), -1, dtype=torch.int32)
         keep[torch.tensor(ends) - 1] = torch.arange(len(ends), dtype=torch.int32)
         keep = upload(keep, h.device)
@@ -489,30 +502,30 @@ class Transformer(nn.Module):
             logits = self.forward(input_ids, seqlens, cache).float().contiguous()
             return token_scores(logits, targets, top=top), logits.index_select(0, last_rows)
         self._check_runnable()
-        h = self._hidden_no_norm(input_ids, seqlens, cache)
+        stream = self._hidden_no_norm(input_ids, seqlens, cache)
         if cache is not None:
             cache.update_seqlens(seqlens)
         rows = max(128, (256 << 20) // (4 * V))
-        block = torch.empty(min(rows, T), V, dtype=torch.float32, device=h.device)
-        last_logits = torch.empty(len(ends), V, dtype=torch.float32, device=h.device)
-        out = empty_scores(T, top, True, h.device)
+        block = torch.empty(min(rows, T), V, dtype=torch.float32, device=self.device)
+        last_logits = torch.empty(len(ends), V, dtype=torch.float32, device=self.device)
+        out = empty_scores(T, top, True, self.device)
         for r0 in range(0, T, rows):
             r1 = min(T, r0 + rows)
-            self._head(h[r0:r1], block[: r1 - r0])
+            self._head(stream.rows(r0, r1), block[: r1 - r0])
             token_scores(block[: r1 - r0], targets[r0:r1], top=top, out=out.rows(r0, r1))
             for b, e in enumerate(ends):
                 if r0 < e <= r1:
                     last_logits[b].copy_(block[e - 1 - r0])
         return out, last_logits
 
-    def _logprobs_of_written_logits(self, h: torch.Tensor, targets: torch.Tensor, ends: List[int], lp: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-        T, V = h.shape[0], self.vocab_size
+    def _logprobs_of_written_logits(self, stream: _Stream, targets: torch.Tensor, ends: List[int], lp: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        T, V = lp.shape[0], self.vocab_size
         rows = max(128, (256 << 20) // (4 * V))
-        block = torch.empty(min(rows, T), V, dtype=torch.float32, device=h.device)
-        last_logits = torch.empty(len(ends), V, dtype=torch.float32, device=h.device)
+        block = torch.empty(min(rows, T), V, dtype=torch.float32, device=self.device)
+        last_logits = torch.empty(len(ends), V, dtype=torch.float32, device=self.device)
         for r0 in range(0, T, rows):
             r1 = min(T, r0 + rows)
-            self._head(h[r0:r1], block[: r1 - r0])
+            self._head(stream.rows(r0, r1), block[: r1 - r0])
             _abi.logprob_gather(block[: r1 - r0], targets[r0:r1], out=lp[r0:r1])
             for b, e in enumerate(ends):
                 if r0 < e <= r1:

@@ -238,3 +238,36 @@ def test_a_model_that_was_moved_goes_on(B, head):
             del taken
         a, b = (model.forward(nxt + i, [1] * B, cache) for model, cache in zip((m, still), caches))
         assert torch.equal(a, b), i
+
+
+def test_the_last_addition_is_the_8_bit_heads(monkeypatch):
+    """Every addition to the stream is made by the norm behind it, the head's norm too; the same bits as an addition ahead of it, in every call that has logits or scores."""
+    m, p = model_of(head=True)
+    own, adds = rows8.norm_rows, []
+    ids = (torch.arange(300) * 7 % p["vocab_size"]).cuda()
+    targets = ids.roll(-1)
+    nxt = torch.tensor([5, 6], device="cuda")
+
+    def run():
+        adds.clear()
+        cache, other = m.make_cache(2, 400), m.make_cache(2, 400)
+        first = m.forward(ids, [170, 130], cache)
+        step = m.forward(nxt, [1, 1], cache).clone()
+        scored = m.forward_logprobs(ids, [170, 130], None, targets)
+        scores, last = m.forward_scores(ids, [170, 130], other, targets, 3)
+        return [first, step, *scored, scores.logprob, scores.entropy, scores.top_ids, scores.top_logprobs, last, m.forward_partial(ids[:9], [9])]
+
+    def together(x, weight, eps, add=None):
+        adds.append(add is not None)
+        return own(x, weight, eps, add=add)
+
+    def ahead(x, weight, eps, add=None):
+        h = x if add is None else x + add
+        return own(h, weight, eps)[0], h
+    monkeypatch.setattr(rows8, "norm_rows", together)
+    got = run()
+    layers = [False] + [True] * (2 * p["n_layers"] - 1)
+    assert adds == (layers + [True]) * 4 + layers  # (forward_partial's last norm is in 16 bits)
+    monkeypatch.setattr(rows8, "norm_rows", ahead)
+    for a, b in zip(got, run()):
+        assert torch.equal(a, b)
