@@ -479,3 +479,42 @@ def test_gates_far_from_zero(T):
     gate, up = x[:, :1].double(), x[:, 128:129].double()
     y = gate * torch.sigmoid(gate) * up
     U.assert_rows_near(rows.codes, rows.scales, y, y.abs() * (3 + gate.abs() / 3) * 2.0 ** -22 + torch.where(gate < -87, 2.0 ** -119, 0.0) * up.abs())
+
+
+MOST = 1 << 24
+
+
+def test_as_many_rows_as_there_may_be():
+    """2^24 rows of one entry: every row's code and power, and its products with three features, which are exact."""
+    i = torch.arange(MOST, device=DEV)
+    x = ((1 + i % 8 / 8) * torch.exp2((i // 8 % 20 - 9).float())).to(torch.bfloat16)[:, None]
+    rows = mi.quantise_rows(x)
+    assert torch.equal(rows.codes[:, 0].float() * torch.exp2(rows.exponents()[:, 0].float()), x[:, 0].float())
+    assert int(rows.codes.view(torch.int32)[:, 1:].count_nonzero()) == 0  # (the first four codes of a row are one word)
+    w = mi.quantise_rows(torch.tensor([[1.5], [-1.0], [0.25]], device=DEV))
+    y = mi.multiply_rows(rows, w, dtype=torch.float32)
+    assert torch.equal(y, x.float() * torch.tensor([1.5, -1.0, 0.25], device=DEV))
+    del y
+    one = mi.quantise_rows(torch.ones(1, 1, device=DEV))
+    assert torch.equal(mi.multiply_rows(one, rows, dtype=torch.float32)[0], x[:, 0].float())
+    units = mi.gate_rows(one, rows)
+    gate, up = x[0::2, 0].double()[None], x[1::2, 0].double()[None]
+    y = gate * torch.sigmoid(gate) * up
+    U.assert_rows_near(units.codes, units.scales, y, y.abs() * (3 + gate.abs() / 3) * 2.0 ** -22)
+
+
+@pytest.mark.parametrize("T", [2, 130])
+def test_rows_as_long_as_they_may_be(T):
+    """2^24 entries, a few of which are not zero: sums that are exact."""
+    at = [0, 127, 5_000_000, (1 << 23) + 5, MOST - 129, MOST - 1]
+    x, w = torch.zeros(T, MOST, dtype=torch.bfloat16, device=DEV), torch.zeros(3, MOST, dtype=torch.bfloat16, device=DEV)
+    for j, k in enumerate(at):
+        x[:, k] = (torch.arange(T, device=DEV) * 5 + j * 3) % 15 + 1
+        w[:, k] = torch.tensor([1.0, -2.0, 0.5], device=DEV) * (j + 1)
+    y = x[:, at].float() @ w[:, at].float().t()
+    x = mi.quantise_rows(x)
+    w = mi.quantise_rows(w)
+    for k in at:
+        assert torch.equal(x.exponents()[:, k // 128] > -100, torch.ones(T, dtype=torch.bool, device=DEV))
+    got = mi.multiply_rows(x, w, dtype=torch.float32)
+    assert torch.equal(got, y)
