@@ -271,3 +271,22 @@ def test_the_last_addition_is_the_8_bit_heads(monkeypatch):
     monkeypatch.setattr(rows8, "norm_rows", ahead)
     for a, b in zip(got, run()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kv_cache", ["ring", "pages"])
+def test_decode_steps_of_many_sequences(kv_cache, monkeypatch):
+    """More sequences than the products for a few tokens take: captured steps whose products have parts in memory of their own, of two caches in turn."""
+    m, p = model_of(head=True, max_batch=150, dim=512, n_heads=4, hidden_dim=4096)
+    prompts = [(torch.arange(150 * 3) * k % p["vocab_size"]).cuda() for k in (7, 11)]
+    nxt = torch.arange(150, device="cuda")
+    outs = {}
+    for graph in ("0", "1"):
+        monkeypatch.setenv("MB200_DECODE_GRAPH", graph)
+        caches = [m.make_cache(150, 40, kv_cache=kv_cache) for _ in range(2)]
+        outs[graph] = [[m.forward(ids, [3] * 150, c)] for ids, c in zip(prompts, caches)]
+        for i in range(5):
+            for j, c in enumerate(caches):
+                outs[graph][j].append(m.forward((nxt + i + j) % p["vocab_size"], [1] * 150, c).clone())
+    for a, b in zip(outs["0"], outs["1"]):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
