@@ -697,13 +697,13 @@ class Transformer(nn.Module):
         memory = [p.data_ptr() for p in self.parameters()]
         super()._apply(fn, recurse)
         moved = [(owner, name) for owner, name in self._matrices8() if getattr(owner, name).codes.device != self.device]
+        self._moves += moved != [] or memory != [p.data_ptr() for p in self.parameters()]
         for owner, name in moved:
             setattr(owner, name, getattr(owner, name).to(self.device))
         if moved and self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
-            for owner, name in moved:
-                getattr(owner, name).fixed = True  # (the copies have ended)
-        self._moves += moved != [] or memory != [p.data_ptr() for p in self.parameters()]
+            for owner, name in self._matrices8():
+                getattr(owner, name).fixed = True  # (the copies have ended, those too of a move that failed on its way)
         return self
 
     def _check_16_bit(self, what: str) -> None:

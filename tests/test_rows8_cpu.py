@@ -288,3 +288,27 @@ def test_steps_captured_before_a_move_are_not_replayed():
     assert m.to("cpu")._decode_state(cache, "step") is first  # (nothing moved)
     m.float().bfloat16()
     assert m._decode_state(cache, "step") is not first
+
+
+def test_a_move_that_fails_on_its_way_is_gone_on_with(model, monkeypatch):
+    """Matrices that are left behind move with the next call, and nothing captured before the first one is replayed behind it."""
+    monkeypatch.setattr(operators, "quantise_rows", Failing(100))
+    model.quantise_weights()
+    monkeypatch.undo()
+    own, room = Rows8.to, [5]
+
+    def to(self, device):
+        room[0] -= 1
+        if room[0] < 0:
+            raise torch.OutOfMemoryError("no room")
+        return own(self, device)
+    monkeypatch.setattr(Rows8, "to", to)
+    moves = model._moves
+    with pytest.raises(torch.OutOfMemoryError):
+        model.to("meta")
+    assert model._moves > moves
+    monkeypatch.undo()
+    devices = [getattr(owner, name).codes.device.type for owner, name in model._matrices8()]
+    assert devices == ["meta"] * 5 + ["cpu"] * 7
+    model.to("meta")
+    assert {getattr(owner, name).codes.device.type for owner, name in model._matrices8()} == {"meta"}
