@@ -7,8 +7,8 @@ import pytest
 import torch
 
 import mistral_inference_b200 as mi
-from mistral_inference_b200 import _abi, _abi_rows8
-from mistral_inference_b200 import rows8 as operators
+from mistral_inference_b200 import _abi_rows8
+from mistral_inference_b200 import _abi, rows8 as operators
 from mistral_inference_b200.build import build_rows8
 from mistral_inference_b200.rows8 import Rows8
 
